@@ -212,7 +212,9 @@ def prepare(case, seed):
                      "table": table, "lens": lens, "starts": starts, "mask": mask,
                      "out": torch.zeros(N, H, D, dtype=DTYPES[c["dtype"]], device=DEV)}
     st["start"], st["now"], (st["table"], st["lens"], st["refs"]) = _meta([table, lens, refs])
-    st["told"] = torch.zeros(1, dtype=torch.int32, device=DEV)
+    # what each request came to (0: done), and of the packing the number of pages moved
+    told = {"append": c["seqs"], "fork": c.get("children"), "copy": c.get("children"), "compact": 1, "free": c.get("ends")}[c["kind"]]
+    st["told"] = torch.zeros(told, dtype=torch.int32, device=DEV)
     if c["kind"] == "free":
         return st | {"slots": torch.randperm(c["seqs"], generator=g, device=DEV)[:c["ends"]].to(torch.int32)}
     L, Hkv, D = c["layers"], c["kv_heads"], c["head_dim"]
