@@ -337,6 +337,105 @@ int iron_attention_prefill(const void* q, const void* k, const void* v, void* ou
                            long long o_row_stride, int out_rows, int causal, int q_offset, float scale,
                            void* stream);
 
+/* ------------------------------------------------------ Paged KV cache ---- */
+/* No counterpart in the reference, whose caches are dense and hold one
+ * sequence. State, all of it in device memory:
+ *   k_pages, v_pages (num_layers, num_pages, n_kv_heads, page_size, head_dim)
+ *   page_table (num_seqs, max_pages) int32: position t of sequence s is row
+ *     t % page_size of page page_table[s][t / page_size]; an entry outside
+ *     [0, num_pages) is a hole: its positions have no keys
+ *   seq_lens (num_seqs) int32; entries of a sequence's table row behind its
+ *     last page are never read
+ *   page_refs (num_pages) int32, 16-byte aligned: table entries that hold the
+ *     page; 0 = free. Free pages are given out lowest number first, in the
+ *     order of the requests: results depend on the inputs alone.
+ * page_size is a power of two from 16 to 1024, num_seqs at most 8192. What
+ * device arrays hold cannot be checked before a launch: a request that cannot
+ * be met changes nothing and says so in its status word, and no index read
+ * from them leads out of the arrays. Workspaces need no initialisation and
+ * carry nothing over between calls; calls that share one must be
+ * stream-ordered, as must calls that work on one cache. */
+
+/* What became of a request (status outputs). */
+enum iron_page_status {
+  IRON_PAGE_DONE = 0,
+  IRON_PAGE_INVALID = 1, /* a slot outside the table or named twice, a length outside [0, max_pages * page_size],
+                            a fork onto itself or onto a sequence that is not empty */
+  IRON_PAGE_NO_ROOM = 2, /* too few free pages, or the table row is too short */
+  IRON_PAGE_NOT_OWN = 3  /* append: the partly filled last page is a hole or held by another entry too */
+};
+
+/* Attention of drafted trees over a paged cache. Rows node_starts[s] ..
+ * node_starts[s+1]-1 of q (num_nodes, n_heads, head_dim) and k_new, v_new
+ * (num_nodes, n_kv_heads, head_dim) are the nodes of sequence s; node i sees
+ * every cached position [0, seq_lens[s]) and the nodes j of its own tree whose
+ * bit is set: bit j % 32 of word j / 32 of tree_mask (num_nodes,
+ * ceil(max_nodes / 32)) row i.
+ *   out[i,h] = sum_j softmax_j(scale * q[i,h] . k_j[h/G]) v_j[h/G]   (fp32)
+ * One node that sees itself is an ordinary decode step; the cache is only read
+ * (iron_paged_append adds the accepted rows). A row that sees nothing gets
+ * zeros; rows of out outside every tree, or behind max_nodes of one, are left
+ * as they were. What a row does not see does not reach it, whatever it holds
+ * (infinities, NaN). dtype 0: bf16, 1: fp16 (q, k, v and out). head_dim 64 or
+ * 128; n_heads any multiple of n_kv_heads; max_nodes at most 1024. k_pages and
+ * v_pages are one layer's (num_pages, n_kv_heads, page_size, head_dim).
+ * node_starts must not decrease; each tree is taken as cut to max_nodes nodes
+ * and to num_nodes rows. Lengths outside [0, max_pages * page_size] are cut to
+ * that range. Beside the reference's attention of one token or of a prompt
+ * (iron/applications/llama_3.2_1b/llama_npu.py:486-523, iron/operators/mha/op.py:21-135). */
+long long iron_tree_attention_workspace_bytes(int n_heads, int n_kv_heads, int head_dim, int num_seqs, int num_nodes,
+                                              int max_nodes, int max_pages, int page_size);
+int iron_tree_attention(const void* q, const void* k_new, const void* v_new, const void* k_pages, const void* v_pages,
+                        const int* page_table, const int* seq_lens, const int* node_starts, const int* tree_mask,
+                        void* out, int dtype, int n_heads, int n_kv_heads, int head_dim, int num_pages, int page_size,
+                        int num_seqs, int max_pages, int num_nodes, int max_nodes, float scale, void* workspace,
+                        long long workspace_bytes, void* stream);
+
+/* Rows rows[row_starts[s]] .. rows[row_starts[s+1]-1] of k_new and v_new
+ * (num_layers, num_nodes, n_kv_heads, head_dim) go, in order, to positions
+ * seq_lens[s], seq_lens[s] + 1, .. of sequence s in every layer, on new pages
+ * where its last one is full; seq_lens[s] grows by their number. A row number
+ * outside [0, num_nodes) appends zeros. Elements of any type: row_bytes is
+ * head_dim times their size, a multiple of 16. status (num_seqs). A sequence
+ * that cannot grow by all its rows is left as it was; where the free pages run
+ * out, so are all later ones that need any. row_starts (num_seqs + 1) must not
+ * decrease. num_rows at most 2^20. The paged form of the KV-cache append
+ * (StridedCopy of iron/applications/llama_3.2_1b/llama_npu.py:311-323). */
+long long iron_paged_append_workspace_bytes(int num_seqs, int num_rows, int page_size);
+int iron_paged_append(const void* k_new, const void* v_new, const int* rows, const int* row_starts, void* k_pages,
+                      void* v_pages, int* page_table, int* seq_lens, int* page_refs, int* status, int num_layers,
+                      int n_kv_heads, int row_bytes, int num_pages, int page_size, int num_seqs, int max_pages,
+                      int num_nodes, int num_rows, void* workspace, long long workspace_bytes, void* stream);
+
+/* For each pair forks[i] = (parent, child), child an empty sequence of the
+ * table: the child becomes a sequence with the parent's positions. share != 0:
+ * it holds the parent's full pages too (page_refs count it) and a new page
+ * with a copy of the rows of the last, partly filled one, so that either can
+ * grow. share == 0: new pages with copies of everything. Holes stay holes.
+ * Rows of a new page behind the child's last position are left as they were.
+ * Parents are taken as they are before the call. status (num_forks <= 8192);
+ * of pairs that name one child the first counts. */
+long long iron_page_fork_workspace_bytes(int num_forks, int num_seqs, int max_pages, int num_pages, int share);
+int iron_page_fork(const int* forks, void* k_pages, void* v_pages, int* page_table, int* seq_lens, int* page_refs,
+                   int* status, int num_layers, int n_kv_heads, int row_bytes, int num_pages, int page_size,
+                   int num_seqs, int max_pages, int num_forks, int share, void* workspace, long long workspace_bytes,
+                   void* stream);
+
+/* Packs the pool: with L pages in use, those at or above page L move to the
+ * free ones below it (both in ascending order), in every layer, and page_table
+ * (within seq_lens) and page_refs follow. moved[0] = their number. Afterwards
+ * the pages in use are 0 .. L-1. */
+long long iron_page_compact_workspace_bytes(int num_pages);
+int iron_page_compact(void* k_pages, void* v_pages, int* page_table, int* seq_lens, int* page_refs, int* moved,
+                      int num_layers, int n_kv_heads, int row_bytes, int num_pages, int page_size, int num_seqs,
+                      int max_pages, void* workspace, long long workspace_bytes, void* stream);
+
+/* The sequences slots[0 .. num_slots) give their pages back: page_refs of each
+ * drops by one (never below 0), the table entries become -1, the length 0.
+ * status (num_slots <= 8192); of entries that name one slot the first counts. */
+int iron_page_free(const int* slots, int* page_table, int* seq_lens, int* page_refs, int* status, int num_pages,
+                   int page_size, int num_seqs, int max_pages, int num_slots, void* stream);
+
 /* ---------------------------------------------------------------- GEMM ---- */
 
 /* C = clamp(act(bf16(A . B^T))) on bf16 MFMA, fp32 accumulation:

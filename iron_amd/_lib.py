@@ -58,6 +58,11 @@ SIGNATURES: dict[str, list] = {
     "iron_embedding": [_P, _P, _P, _I, _I, _I, _P],
     "iron_argmax_bf16": [_P, _I, _P, _P, _P, _I, _P],
     "iron_argmax_select": [_P, _I, _P, _I, _I, _P, _P, _P, _P, _I, _P],
+    "iron_tree_attention": [_P] * 10 + [_I] * 10 + [_F, _P, _LL, _P],
+    "iron_paged_append": [_P] * 10 + [_I] * 9 + [_P, _LL, _P],
+    "iron_page_fork": [_P] * 7 + [_I] * 9 + [_P, _LL, _P],
+    "iron_page_compact": [_P] * 6 + [_I] * 7 + [_P, _LL, _P],
+    "iron_page_free": [_P] * 5 + [_I] * 5 + [_P],
     "iron_qkv_rope_scatter": [_P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P],
     "iron_qkv_rope_scatter_splitk": [_P, _I, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P],
     "iron_rmsnorm_splitk": [_P, _P, _I, _P, _P, _P, _I, _I, _F, _P],
@@ -81,6 +86,10 @@ QUERIES: dict[str, tuple] = {
     "iron_llama_decode_fused_exchange_bytes": (_LL, [_I]),
     "iron_swiglu_decode_i4g32_workspace_bytes": (_LL, [_I, _I]),
     "iron_xcd_round_robin": (_I, [_P]),
+    "iron_tree_attention_workspace_bytes": (_LL, [_I] * 8),
+    "iron_paged_append_workspace_bytes": (_LL, [_I] * 3),
+    "iron_page_fork_workspace_bytes": (_LL, [_I] * 5),
+    "iron_page_compact_workspace_bytes": (_LL, [_I]),
     "iron_gemm_splitk_choose": (_I, [_I, _I, _I]),
     "iron_gemm_i4g32_splitk_choose": (_I, [_I, _I, _I]),
     "iron_gemm_splitk_workspace_bytes": (_LL, [_I, _I, _I]),
@@ -161,6 +170,13 @@ def gemm_split(policy: str, rows: int, cols: int, K: int) -> tuple[int, int]:
     gives a GEMM: a function of the shape alone, so asked once per shape."""
     splits = int(query(policy, rows, cols, K))
     return splits, int(query("iron_gemm_splitk_workspace_bytes", rows, cols, splits)) if splits > 1 else 0
+
+
+@functools.lru_cache(maxsize=4096)
+def workspace_bytes(name: str, *numbers: int) -> int:
+    """Bytes that workspace query ``name`` gives for a shape: a function of the
+    shape alone, so asked once per shape."""
+    return int(query(name, *numbers))
 
 
 def ptr(t) -> int | None:

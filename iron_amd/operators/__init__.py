@@ -18,6 +18,10 @@ _OPERATOR_MODULES = {
     "GEMVInt4": "gemv_int4",
     "GQADecode": "gqa_decode",
     "MHA": "mha",
+    "PageCompact": "page_compact",
+    "PageFork": "page_fork",
+    "PageFree": "page_free",
+    "PagedAppend": "paged_append",
     "RMSNorm": "rms_norm",
     "RoPE": "rope",
     "SiLU": "silu",
@@ -25,6 +29,7 @@ _OPERATOR_MODULES = {
     "SwiGLUDecode": "swiglu_decode",
     "SwiGLUPrefill": "swiglu_prefill",
     "Transpose": "transpose",
+    "TreeAttention": "tree_attention",
     "StridedCopy": "strided_copy",
     "Repeat": "repeat",
 }
