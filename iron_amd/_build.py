@@ -50,6 +50,7 @@ HIP_FLAGS = [
 # -fno-honor-nans: max(a, b) of finite scores then needs no NaN-quieting
 # v_max_f32 per operand (finite inputs give identical results).
 # decode_fused.hip runs the same decode attention body, so it takes the same flags.
+# tree_attention.hip rescales its accumulators the same way (but NaN and infinity have a meaning there).
 # gemv.hip, attention.hip, llama.hip: the dispatch preloads a kernel's leading
 # scalar and pointer arguments into SGPRs (up to 14 SGPRs; a struct argument
 # ends the preloaded run), so the GEMVs, the decode attention and the token
@@ -62,6 +63,7 @@ FILE_FLAGS = {
     "probe.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=3"],
     "attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-honor-nans", "-mllvm", "-amdgpu-kernarg-preload-count=9"],
     "decode_fused.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-honor-nans"],
+    "tree_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

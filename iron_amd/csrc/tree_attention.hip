@@ -5,6 +5,8 @@
 #include "iron_common.hpp"
 #include "../../include/iron_hip.h"
 
+#include <algorithm>
+
 namespace iron {
 namespace {
 
@@ -19,7 +21,10 @@ struct TreeArgs {
   const int* starts;  // (num_seqs + 1)
   const int* mask;    // (num_nodes, words)
   uint16_t* out;      // (num_nodes, H, D)
-  int H, Hkv, num_pages, page_shift, num_seqs, max_pages, num_nodes, max_nodes, words;
+  float* part_o;      // workspace (2 x workgroups, R, D): sum(p v) of the parts of split tiles
+  float2* part_ml;    // workspace (2 x workgroups, R): their maximum and sum(p)
+  long long* prefix;  // workspace (num_seqs + 1): units before each sequence; units of a workgroup
+  int H, Hkv, num_pages, page_shift, num_seqs, max_pages, num_nodes, max_nodes, words, workgroups;
   float scale_log2;
 };
 
@@ -40,65 +45,580 @@ __device__ __forceinline__ void tree_of(const TreeArgs& a, int s, int& first, in
   nodes = min(min(max(a.starts[s + 1], first), a.num_nodes) - first, a.max_nodes);
 }
 
-// One workgroup of 4 waves per (node of a tree, head): each wave takes every
-// fourth key, a lane D / 64 dims.
-template <int D, bool F16>
-__global__ __launch_bounds__(256) void tree_attention_kernel(TreeArgs a) {
-  __shared__ float part[4][D + 2];
-  constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int s = blockIdx.z, h = blockIdx.y, hk = h / (a.H / a.Hkv);
-  int first, nodes;
-  tree_of(a, s, first, nodes);
-  if (static_cast<int>(blockIdx.x) >= nodes) return;
-  const long long row = first + blockIdx.x;
-  const int ps = 1 << a.page_shift;
-  const int len = min(max(a.lens[s], 0), a.max_pages * ps);
-  float q[E], o[E], m = -INFINITY, l = 0.f;
-  for (int e = 0; e < E; ++e) {
-    q[e] = widen<F16>(a.q[(row * a.H + h) * D + lane * E + e]);
-    o[e] = 0.f;
-  }
-  for (int j = w; j < len + nodes; j += 4) {
-    const uint16_t *k, *v;
-    if (j < len) {
-      const int page = a.table[static_cast<long long>(s) * a.max_pages + (j >> a.page_shift)];
-      if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.num_pages)) continue;
-      const long long at = ((static_cast<long long>(page) * a.Hkv + hk) * ps + (j & (ps - 1))) * D;
-      k = a.k_pages + at;
-      v = a.v_pages + at;
-    } else {
-      const int n = j - len;
-      if (!(a.mask[row * a.words + (n >> 5)] >> (n & 31) & 1)) continue;
-      const long long at = (static_cast<long long>(first + n) * a.Hkv + hk) * D;
-      k = a.k_new + at;
-      v = a.v_new + at;
+typedef __bf16 ta_bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 ta_f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 ta_f16x2 __attribute__((ext_vector_type(2)));
+typedef float ta_f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned ta_u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned ta_u32x4 __attribute__((ext_vector_type(4)));
+typedef short ta_i16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kBlock = 64;   // keys of a block: 16 for each of the 4 waves
+constexpr int kStages = 4;   // blocks resident in a wave's ring
+
+template <bool F16>
+__device__ __forceinline__ ta_f32x4 mfma(ta_u32x4 a, ta_u32x4 b, ta_f32x4 c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ta_f16x8, a), __builtin_bit_cast(ta_f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(ta_bf16x8, a), __builtin_bit_cast(ta_bf16x8, b), c, 0, 0, 0);
+}
+
+// Four weights as 16-bit pairs hi + lo: {hi0, hi1, hi2, hi3, lo0, lo1, lo2, lo3}.
+// A weight keeps ~16 bits (bf16) or ~21 (fp16) that way: rounded to one 16-bit
+// value it would add an error of the size of the output's own rounding.
+template <bool F16>
+__device__ __forceinline__ ta_u32x4 split4(const float (&p)[4]) {
+  ta_u32x4 r;
+  if constexpr (F16) {  // both parts truncate: what the first leaves off is never negative
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const auto hi = __builtin_amdgcn_cvt_pkrtz(p[2 * i], p[2 * i + 1]);
+      const auto lo = __builtin_amdgcn_cvt_pkrtz(p[2 * i] - static_cast<float>(hi[0]), p[2 * i + 1] - static_cast<float>(hi[1]));
+      r[i] = __builtin_bit_cast(unsigned, hi);
+      r[2 + i] = __builtin_bit_cast(unsigned, lo);
     }
-    float x = 0.f;
-    for (int e = 0; e < E; ++e) x += q[e] * widen<F16>(k[lane * E + e]);
-    x = wave_sum(x) * a.scale_log2;
-    const float top = fmaxf(m, x);
-    const float off = top == -INFINITY ? 0.f : top;
-    const float alpha = exp2f(m - off), p = exp2f(x - off);
-    m = top;
-    l = l * alpha + p;
-    for (int e = 0; e < E; ++e) o[e] = o[e] * alpha + p * widen<F16>(v[lane * E + e]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const unsigned hi = cvt_pk_bf16(p[2 * i], p[2 * i + 1]);
+      r[i] = hi;
+      r[2 + i] = cvt_pk_bf16(p[2 * i] - lo_bf16(hi), p[2 * i + 1] - hi_bf16(hi));
+    }
   }
-  for (int e = 0; e < E; ++e) part[w][lane * E + e] = o[e];
-  if (lane == 0) {
-    part[w][D] = m;
-    part[w][D + 1] = l;
+  return r;
+}
+
+// x[l], y[l] = a[l % 32], a[l % 32 + 32] (swap32), or a of the even and odd
+// 16-lane row of l's pair (swap16): op(x, y) joins the lanes that hold one
+// row's other keys. The s_nop covers the VALU-write to permlane-read hazard.
+__device__ __forceinline__ void swap32(float a, float& x, float& y) {
+  unsigned u = __builtin_bit_cast(unsigned, a), v = u;
+  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(u), "+v"(v));
+  x = __builtin_bit_cast(float, u);
+  y = __builtin_bit_cast(float, v);
+}
+__device__ __forceinline__ void swap16(float a, float& x, float& y) {
+  unsigned u = __builtin_bit_cast(unsigned, a), v = u;
+  asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(u), "+v"(v));
+  x = __builtin_bit_cast(float, u);
+  y = __builtin_bit_cast(float, v);
+}
+__device__ __forceinline__ float row_max(float a) {
+  float x, y;
+  swap32(a, x, y);
+  a = fmaxf(x, y);
+  swap16(a, x, y);
+  return fmaxf(x, y);
+}
+__device__ __forceinline__ float row_sum(float a) {
+  float x, y;
+  swap32(a, x, y);
+  a = x + y;
+  swap16(a, x, y);
+  return x + y;
+}
+
+// A word of memory that does not change during the launch, at a uniform
+// address: a scalar load, which does not wait for the loads in flight.
+__device__ __forceinline__ int uniform_word(const int* p, long long i) {
+  return reinterpret_cast<const __attribute__((address_space(4))) int*>(reinterpret_cast<uintptr_t>(p))[i];
+}
+
+// The same value in every lane, in a scalar register.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ long long uniform(long long x) {
+  const unsigned lo = uniform(static_cast<int>(x)), hi = uniform(static_cast<int>(x >> 32));
+  return static_cast<long long>(hi) << 32 | lo;
+}
+
+// Where the work is cut. A tile is R rows (node, head of the KV head's group)
+// of one sequence and KV head; a unit is one block of 64 keys of a tile:
+// first the blocks of the cache, then those of the tree. Units are numbered
+// sequence by sequence, and workgroup b takes units [b * chunk, (b + 1) * chunk).
+struct Tiles {
+  int first, nodes, len, cached, blocks, row_tiles;
+  long long units;
+};
+
+template <int R>
+__device__ __forceinline__ Tiles tiles_of(const TreeArgs& a, int s) {
+  Tiles t;
+  tree_of(a, s, t.first, t.nodes);
+  t.len = min(max(a.lens[s], 0), a.max_pages << a.page_shift);
+  t.cached = (t.len + kBlock - 1) / kBlock;
+  t.blocks = t.cached + (t.nodes + kBlock - 1) / kBlock;
+  t.row_tiles = (t.nodes * (a.H / a.Hkv) + R - 1) / R;
+  t.units = static_cast<long long>(t.row_tiles) * a.Hkv * t.blocks;
+  return t;
+}
+
+__device__ __forceinline__ Tiles uniform(const Tiles& t) {
+  return {uniform(t.first), uniform(t.nodes), uniform(t.len), uniform(t.cached), uniform(t.blocks), uniform(t.row_tiles), uniform(t.units)};
+}
+
+__device__ __forceinline__ long long chunk_of(const TreeArgs& a, long long total) {
+  return max((total + a.workgroups - 1) / a.workgroups, 1LL);
+}
+
+template <int D>
+__device__ __forceinline__ int k_slot(int row, int c) {  // 16 rows of a 16-byte read on different banks
+  return D == 64 ? c ^ ((row >> 1) & 7) : c ^ row;
+}
+template <int D>
+__device__ __forceinline__ int v_slot(int row, int c) {  // the 8 rows of half a transposed read on different banks
+  return D == 64 ? c ^ (((row >> 1) & 3) << 1) : c ^ ((row & 7) << 1);
+}
+
+// A wave waits until at most N of its loads are in flight and its LDS reads
+// are done: a stage has landed, and the one before it may be overwritten.
+template <int N>
+__device__ __forceinline__ void wait_stage() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+
+template <int D, bool F16, int RT>
+__global__ __launch_bounds__(256) void tree_attention_kernel(TreeArgs a) {
+  constexpr int R = 16 * RT, kRow = D * 2, kHalf = 16 * kRow, kStage = 2 * kHalf, kRing = kStages * kStage;
+  constexpr int kLoads = kStage / 1024;  // 1 KiB loads of a stage, the first half of them K
+  constexpr int NK = D / 32, ND = D / 16;
+  static_assert(R * D * 4 <= kRing, "a wave's output goes through its ring");
+  __shared__ __attribute__((aligned(16))) unsigned char lds[4 * kRing];
+  __shared__ float stat_m[4][R], stat_l[4][R];
+  __shared__ long long scan[5];
+  __shared__ int found;
+  __shared__ long long found_at;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = uniform(tid >> 6);
+  const int c = lane & 15, quad = lane >> 4;
+  const int G = a.H / a.Hkv, ps = 1 << a.page_shift;
+
+  // The units of all sequences before each thread's own ones, the workgroup's
+  // first unit and its sequence.
+  const int per = (a.num_seqs + 255) / 256;
+  long long mine = 0;
+  for (int i = 0; i < per; ++i)
+    if (tid * per + i < a.num_seqs) mine += tiles_of<R>(a, tid * per + i).units;
+  long long incl = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const long long y = __shfl_up(incl, d, 64);
+    if (lane >= d) incl += y;
+  }
+  if (lane == 63) scan[w] = incl;
+  __syncthreads();
+  long long before = incl - mine, total = 0;
+  for (int i = 0; i < 4; ++i) {
+    before += i < w ? scan[i] : 0;
+    total += scan[i];
+  }
+  total = uniform(total);
+  const long long chunk = chunk_of(a, total);
+  long long u = blockIdx.x * chunk;
+  const long long end = min(u + chunk, total);
+  if (blockIdx.x == 0) {  // for the launch that joins the parts
+    long long at = before;
+    for (int i = 0; i < per; ++i)
+      if (tid * per + i < a.num_seqs) {
+        a.prefix[tid * per + i] = at;
+        at += tiles_of<R>(a, tid * per + i).units;
+      }
+    if (tid == 0) a.prefix[a.num_seqs] = chunk;
+  }
+  if (u >= end) return;
+  if (before <= u && u < before + mine) {
+    long long at = before;
+    for (int i = 0; i < per; ++i) {
+      const long long n = tiles_of<R>(a, tid * per + i).units;
+      if (u < at + n) {
+        found = tid * per + i;
+        found_at = at;
+        break;
+      }
+      at += n;
+    }
   }
   __syncthreads();
-  if (w) return;
-  float top = -INFINITY, sum = 0.f, r[E] = {};
-  for (int i = 0; i < 4; ++i) top = fmaxf(top, part[i][D]);
-  for (int i = 0; i < 4; ++i) {
-    const float f = top == -INFINITY ? 0.f : exp2f(part[i][D] - top);
-    sum += f * part[i][D + 1];
-    for (int e = 0; e < E; ++e) r[e] += f * part[i][lane * E + e];
+  int s = uniform(found);
+  long long base = uniform(found_at);
+  Tiles t = uniform(tiles_of<R>(a, s));
+
+  // This lane's part of a stage's loads: load i puts 1024 bytes, 16 from each
+  // lane in order, so lane l fetches the chunk that belongs at its slot.
+  int lrow[kLoads / 2];
+  unsigned kchunk[kLoads / 2], vchunk[kLoads / 2];
+#pragma unroll
+  for (int i = 0; i < kLoads / 2; ++i) {
+    const int slot = lane % (kRow / 16), row = i * (1024 / kRow) + lane / (kRow / 16);
+    lrow[i] = row;
+    kchunk[i] = k_slot<D>(row, slot) * 16;
+    vchunk[i] = v_slot<D>(row, slot) * 16;
   }
-  for (int e = 0; e < E; ++e) a.out[(row * a.H + h) * D + lane * E + e] = narrow<F16>(sum > 0.f || sum != sum ? r[e] / sum : 0.f);
+  unsigned char* ring = lds + w * kRing;
+  const int trow = 4 * quad + (c >> 2), tcol = 4 * (c & 3);  // this lane's address of a transposed V read
+
+  while (u < end) {
+    const int tile = static_cast<int>((u - base) / t.blocks), blk0 = static_cast<int>((u - base) - static_cast<long long>(tile) * t.blocks);
+    const int n = static_cast<int>(min(static_cast<long long>(t.blocks - blk0), end - u));
+    const int hk = tile / t.row_tiles, row0 = (tile - hk * t.row_tiles) * R;
+    const int rows = min(R, t.nodes * G - row0);
+    // Q: the B operand of S^T = K Q^T (column: row 16 rt + c; dims 32 kk + 8 quad .. + 8)
+    ta_u32x4 qf[RT][NK];
+    int node[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = min(row0 + 16 * rt + c, t.nodes * G - 1);
+      node[rt] = t.first + r / G;
+      const uint16_t* qp = a.q + (static_cast<long long>(node[rt]) * a.H + hk * G + r % G) * D + 8 * quad;
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) qf[rt][kk] = *reinterpret_cast<const ta_u32x4*>(qp + 32 * kk);
+    }
+    ta_f32x4 o[RT][ND];
+    float m[RT], off[RT], l[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      m[rt] = -INFINITY;
+      off[rt] = l[rt] = 0.f;
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt) o[rt][dt] = ta_f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)  // Q has arrived before the first load of the ring is issued
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) asm volatile("" ::"v"(qf[rt][kk]));
+
+    const long long table = static_cast<long long>(s) * a.max_pages;
+    const unsigned new_row = static_cast<unsigned>(a.Hkv) * kRow;
+    unsigned holes = 0;  // bit i % kStages: block i's page of this wave is none
+    auto page_of = [&](int i) {
+      const int blk = min(blk0 + i, t.cached - 1);
+      return t.cached ? uniform_word(a.table, table + (min(blk * kBlock + 16 * w, t.len - 1) >> a.page_shift)) : 0;
+    };
+    int page = page_of(0);
+    auto issue = [&](int i) {
+      unsigned char* st = ring + (i % kStages) * kStage;
+      const int blk = blk0 + i;
+      if (blk < t.cached) {
+        const bool real = static_cast<unsigned>(page) < static_cast<unsigned>(a.num_pages);
+        holes = (holes & ~(1u << (i % kStages))) | (real ? 0u : 1u << (i % kStages));
+        const long long at = ((static_cast<long long>(real ? page : 0) * a.Hkv + hk) * ps + ((blk * kBlock + 16 * w) & (ps - 1))) * D;
+        const i32x4v rk = buffer_rsrc(a.k_pages + at), rv = buffer_rsrc(a.v_pages + at);
+#pragma unroll
+        for (int j = 0; j < kLoads / 2; ++j) {
+          load_lds16(rk, lrow[j] * kRow + kchunk[j], st + j * 1024);
+          load_lds16(rv, lrow[j] * kRow + vchunk[j], st + kHalf + j * 1024);
+        }
+        page = page_of(i + 1);
+      } else {
+        const int j0 = (blk - t.cached) * kBlock + 16 * w;
+        const long long at = (static_cast<long long>(t.first) * a.Hkv + hk) * D;
+        const i32x4v rk = buffer_rsrc(a.k_new + at), rv = buffer_rsrc(a.v_new + at);
+#pragma unroll
+        for (int j = 0; j < kLoads / 2; ++j) {
+          const unsigned r = min(j0 + lrow[j], t.nodes - 1) * new_row;
+          load_lds16(rk, r + kchunk[j], st + j * 1024);
+          load_lds16(rv, r + vchunk[j], st + kHalf + j * 1024);
+        }
+      }
+    };
+
+    auto step = [&](int i) {
+      const int blk = blk0 + i;
+      const bool cache = blk < t.cached;
+      const int j0 = (cache ? blk : blk - t.cached) * kBlock + 16 * w;
+      const int valid = cache && (holes >> (i % kStages) & 1) ? 0 : min((cache ? t.len : t.nodes) - j0, 16);
+      if (valid <= 0) return;
+      const unsigned char* ks = ring + (i % kStages) * kStage;
+      const unsigned char* vs = ks + kHalf;
+      ta_u32x4 kf[NK];
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) kf[kk] = *reinterpret_cast<const ta_u32x4*>(ks + c * kRow + k_slot<D>(c, 4 * kk + quad) * 16);
+      ta_u32x2 vt[ND];
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt) {
+        const int dim = 16 * dt + tcol;
+        vt[dt] = __builtin_bit_cast(ta_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) ta_i16x4*)(vs + trow * kRow + v_slot<D>(trow, dim >> 3) * 16 + (dim & 7) * 2)));
+      }
+      ta_f32x4 sc[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        sc[rt] = ta_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) sc[rt] = mfma<F16>(kf[kk], qf[rt][kk], sc[rt]);
+      }
+      if (valid < 16) {  // keys behind the last one: no score, and values that cannot do harm
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) sc[rt][e] = 4 * quad + e < valid ? sc[rt][e] : -INFINITY;
+        const unsigned k0 = 4 * quad;
+        const unsigned m01 = (k0 < static_cast<unsigned>(valid) ? 0xffffu : 0u) | (k0 + 1 < static_cast<unsigned>(valid) ? 0xffff0000u : 0u);
+        const unsigned m23 = (k0 + 2 < static_cast<unsigned>(valid) ? 0xffffu : 0u) | (k0 + 3 < static_cast<unsigned>(valid) ? 0xffff0000u : 0u);
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) {
+          vt[dt].x &= m01;
+          vt[dt].y &= m23;
+        }
+      }
+      if (!cache) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const int word = a.mask[static_cast<long long>(node[rt]) * a.words + (j0 >> 5)] >> ((j0 & 31) + 4 * quad);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[rt][e] = word >> e & 1 ? sc[rt][e] : -INFINITY;
+        }
+      }
+      // Softmax in the log2 domain, p = 2^(s c - m). The row's maximum m moves only
+      // when a score passes it by more than 8, so p <= 2^8 and O is rarely
+      // rescaled; sum(p v) / sum(p) does not depend on which m is used.
+      const float cs = a.scale_log2;
+      bool grow = false;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+        grow |= fmaxf(fmaxf(sc[rt][0], sc[rt][1]), fmaxf(sc[rt][2], sc[rt][3])) * cs > m[rt] + 8.f;
+      if (__builtin_amdgcn_ballot_w64(grow)) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const float top = row_max(fmaxf(fmaxf(sc[rt][0], sc[rt][1]), fmaxf(sc[rt][2], sc[rt][3]))) * cs;
+          if (top > m[rt] + 8.f) {
+            const float alpha = __builtin_amdgcn_exp2f(m[rt] - top);  // 0 from m = -inf
+            m[rt] = off[rt] = top;
+            l[rt] *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt) o[rt][dt] *= alpha;
+          }
+        }
+      }
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(sc[rt][e], cs, -off[rt]));
+        l[rt] += (p[0] + p[1]) + (p[2] + p[3]);
+        const ta_u32x4 pf = split4<F16>(p);
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) o[rt][dt] = mfma<F16>(ta_u32x4{vt[dt].x, vt[dt].y, vt[dt].x, vt[dt].y}, pf, o[rt][dt]);
+      }
+    };
+
+    static_assert(kStages == 4, "the waits below count three stages in flight");
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i)
+      if (i < n) issue(i);
+    for (int i = 0; i < n; ++i) {
+      const int left = n - 1 - i;  // stages in flight behind block i
+      if (left >= 2)
+        wait_stage<2 * kLoads>();
+      else if (left == 1)
+        wait_stage<kLoads>();
+      else
+        wait_stage<0>();
+      if (i + kStages - 1 < n) issue(i + kStages - 1);  // into the stage of block i - 1, which every read has left
+      step(i);
+    }
+
+    // The four waves' parts of the tile meet in LDS.
+    const bool whole = n == t.blocks;
+    const long long slot = 2LL * blockIdx.x + (blk0 == 0 ? 1 : 0);
+    wait_stage<0>();
+    float* mine_o = reinterpret_cast<float*>(ring);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = 16 * rt + c;
+      const float sum = row_sum(l[rt]);
+      if (quad == 0) {
+        stat_m[w][r] = m[rt];
+        stat_l[w][r] = sum;
+      }
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt)
+        *reinterpret_cast<ta_f32x4*>(mine_o + r * D + (((4 * dt + quad) ^ c) * 4)) = o[rt][dt];
+    }
+    __syncthreads();
+    for (int x = tid; x < rows * (D / 4); x += 256) {
+      const int r = x / (D / 4), c4 = x % (D / 4);
+      float top = stat_m[0][r];
+#pragma unroll
+      for (int i = 1; i < 4; ++i) top = fmaxf(top, stat_m[i][r]);
+      float sum = 0.f;
+      ta_f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (stat_l[i][r] == 0.f) continue;  // saw nothing
+        const float f = __builtin_amdgcn_exp2f(stat_m[i][r] - top);
+        sum += f * stat_l[i][r];
+        v += f * *reinterpret_cast<const ta_f32x4*>(reinterpret_cast<const float*>(lds + i * kRing) + r * D + ((c4 ^ (r & 15)) * 4));
+      }
+      if (whole) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        ta_u32x2 y;
+        if (sum == 0.f) v = ta_f32x4{0.f, 0.f, 0.f, 0.f};
+        y.x = narrow<F16>(v[0] * inv) | static_cast<unsigned>(narrow<F16>(v[1] * inv)) << 16;
+        y.y = narrow<F16>(v[2] * inv) | static_cast<unsigned>(narrow<F16>(v[3] * inv)) << 16;
+        const int row = row0 + r;
+        *reinterpret_cast<ta_u32x2*>(a.out + (static_cast<long long>(t.first + row / G) * a.H + hk * G + row % G) * D + c4 * 4) = y;
+      } else {
+        *reinterpret_cast<ta_f32x4*>(a.part_o + (slot * R + r) * D + c4 * 4) = v;
+        if (c4 == 0) a.part_ml[slot * R + r] = make_float2(top, sum);
+      }
+    }
+    __syncthreads();  // the rings are free again
+
+    u += n;
+    if (u < end && u == base + t.units) {
+      base += t.units;
+      do t = uniform(tiles_of<R>(a, ++s));
+      while (t.units == 0);
+    }
+  }
+}
+
+// One workgroup per node and 4 heads, a wave for each row: joins the parts of
+// rows whose keys were shared out, and does over the rows that came out
+// infinite or NaN, one key at a time and only the keys that the row sees (a
+// product with a weight of zero lets what is not seen through).
+template <int D, bool F16, int R>
+__global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
+  constexpr int E = D / 64, V4 = D / 4, NP = 64 / V4;  // parts added at a time
+  __shared__ int owner;
+  const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
+  const int n = blockIdx.x, h = blockIdx.y * 4 + w;
+  if (tid == 0) owner = -1;
+  __syncthreads();
+  for (int s = tid; s < a.num_seqs; s += 256) {
+    int first, nodes;
+    tree_of(a, s, first, nodes);
+    if (first <= n && n < first + nodes) atomicMax(&owner, s);
+  }
+  __syncthreads();
+  const int s = uniform(owner);
+  if (s < 0 || h >= a.H) return;
+  const Tiles t = tiles_of<R>(a, s);
+  const int G = a.H / a.Hkv, hk = h / G, row = (n - t.first) * G + h % G;
+  const long long chunk = a.prefix[a.num_seqs];
+  const long long u0 = a.prefix[s] + static_cast<long long>(hk * t.row_tiles + row / R) * t.blocks, u1 = u0 + t.blocks - 1;
+  const long long b0 = u0 / chunk, b1 = u1 / chunk;
+  uint16_t* out = a.out + (static_cast<long long>(n) * a.H + h) * D;
+  bool again = false;
+  if (b0 == b1) {  // one workgroup had all its keys
+    for (int e = 0; e < E; ++e) again |= !__builtin_isfinite(widen<F16>(out[lane * E + e]));
+  } else {
+    const int parts = static_cast<int>(b1 - b0) + 1;
+    const long long r = row % R;
+    auto slot = [&](int i) { return 2 * (b0 + i) + (i == 0); };
+    float top = -INFINITY;
+    for (int i = lane; i < parts; i += 64) top = fmaxf(top, a.part_ml[slot(i) * R + r].x);
+    top = wave_max(top);
+    float sum = 0.f;
+    ta_f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int i = lane / V4; i < parts; i += NP) {
+      const float2 ml = a.part_ml[slot(i) * R + r];
+      if (ml.y == 0.f) continue;
+      const float f = __builtin_amdgcn_exp2f(ml.x - top);
+      sum += f * ml.y;
+      v += f * *reinterpret_cast<const ta_f32x4*>(a.part_o + (slot(i) * R + r) * D + (lane % V4) * 4);
+    }
+#pragma unroll
+    for (int d = V4; d < 64; d *= 2) {
+      sum += __shfl_xor(sum, d, 64);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += __shfl_xor(v[e], d, 64);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (sum == 0.f) v = ta_f32x4{0.f, 0.f, 0.f, 0.f};
+    ta_u32x2 y;
+    for (int e = 0; e < 4; ++e) again |= !__builtin_isfinite(v[e] * inv);
+    y.x = narrow<F16>(v[0] * inv) | static_cast<unsigned>(narrow<F16>(v[1] * inv)) << 16;
+    y.y = narrow<F16>(v[2] * inv) | static_cast<unsigned>(narrow<F16>(v[3] * inv)) << 16;
+    if (lane < V4) *reinterpret_cast<ta_u32x2*>(out + lane * 4) = y;
+  }
+  if (!__builtin_amdgcn_ballot_w64(again)) return;
+
+  const uint16_t* q = a.q + (static_cast<long long>(n) * a.H + h) * D;
+  const int ps = 1 << a.page_shift;
+  // the key and value of position or node j, null where the row does not see it
+  auto key = [&](int j, const uint16_t*& v) -> const uint16_t* {
+    if (j < t.len) {
+      const int page = a.table[static_cast<long long>(s) * a.max_pages + (j >> a.page_shift)];
+      if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.num_pages)) return nullptr;
+      const long long at = ((static_cast<long long>(page) * a.Hkv + hk) * ps + (j & (ps - 1))) * D;
+      v = a.v_pages + at;
+      return a.k_pages + at;
+    }
+    j -= t.len;
+    if (j >= t.nodes || !(a.mask[static_cast<long long>(n) * a.words + (j >> 5)] >> (j & 31) & 1)) return nullptr;
+    const long long at = (static_cast<long long>(t.first + j) * a.Hkv + hk) * D;
+    v = a.v_new + at;
+    return a.k_new + at;
+  };
+  const int keys = t.len + t.nodes;
+  auto score = [&](int j, const uint16_t*& v) {  // one key a lane
+    const uint16_t* k = j < keys ? key(j, v) : (v = nullptr, nullptr);
+    if (!k) {
+      v = nullptr;
+      return -INFINITY;
+    }
+    float x = 0.f;
+    for (int d = 0; d < D; ++d) x += widen<F16>(q[d]) * widen<F16>(k[d]);
+    return x * a.scale_log2;
+  };
+  float top = -INFINITY, sum = 0.f, o[E] = {};
+  for (int j = 0; j < keys; j += 64) {
+    const uint16_t* v;
+    top = fmaxf(top, score(j + lane, v));
+  }
+  top = wave_max(top);
+  for (int j = 0; j < keys; j += 64) {
+    const uint16_t* v;
+    const float x = score(j + lane, v);
+    // a weight too small for fp32 is still not zero: it keeps an infinity one
+    const float p = !v ? 0.f : x != x || top == INFINITY ? NAN : fmaxf(__builtin_amdgcn_exp2f(x - top), 1.17549435e-38f);
+    sum += p;
+    const unsigned long long seen = __ballot(v != nullptr);
+    for (unsigned long long left = seen; left; left &= left - 1) {
+      const int i = __ffsll(static_cast<unsigned long long>(left)) - 1;
+      const float pi = __shfl(p, i, 64);
+      const uintptr_t vi = static_cast<uintptr_t>(__shfl(static_cast<unsigned long long>(reinterpret_cast<uintptr_t>(v)), i, 64));
+      for (int e = 0; e < E; ++e) o[e] += pi * widen<F16>(reinterpret_cast<const uint16_t*>(vi)[lane * E + e]);
+    }
+  }
+  sum = wave_sum(sum);
+  for (int e = 0; e < E; ++e) out[lane * E + e] = narrow<F16>(sum == 0.f ? 0.f : o[e] / sum);
+}
+
+// Workgroups that fit the 256 CUs at once: LDS holds two rings of head_dim 64, one of 128.
+constexpr int resident(int D) { return D == 64 ? 512 : 256; }
+
+// Row tiles of 16, 32 or 64 rows.
+int rows_of_tile(int n_heads, int n_kv_heads, int max_nodes) {
+  const int rows = max_nodes * (n_heads / n_kv_heads);
+  return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+}
+
+// The workgroups of a launch: no more than there can be units of work.
+int workgroups_of(int n_heads, int n_kv_heads, int head_dim, int num_seqs, int max_nodes, int max_pages, int page_size) {
+  const int R = rows_of_tile(n_heads, n_kv_heads, max_nodes);
+  const long long blocks = (static_cast<long long>(max_pages) * page_size + kBlock - 1) / kBlock + (max_nodes + kBlock - 1) / kBlock;
+  const long long tiles = static_cast<long long>(max_nodes * (n_heads / n_kv_heads) + R - 1) / R * n_kv_heads * num_seqs;
+  return blocks > resident(head_dim) || tiles > resident(head_dim) ? resident(head_dim)
+                                                                   : static_cast<int>(std::min<long long>(blocks * tiles, resident(head_dim)));
+}
+
+template <int D, bool F16, int RT>
+void launch_tree(const TreeArgs& a, hipStream_t s) {
+  IRON_LAUNCH((tree_attention_kernel<D, F16, RT>), dim3(a.workgroups), dim3(256), 0, s, a);
+  IRON_LAUNCH((tree_join_kernel<D, F16, 16 * RT>), dim3(a.num_nodes, (a.H + 3) / 4), dim3(256), 0, s, a);
+}
+
+template <int D, bool F16>
+void launch_rows(const TreeArgs& a, int R, hipStream_t s) {
+  if (R == 16)
+    launch_tree<D, F16, 1>(a, s);
+  else if (R == 32)
+    launch_tree<D, F16, 2>(a, s);
+  else
+    launch_tree<D, F16, 4>(a, s);
 }
 
 constexpr int kMaxNodes = 1024;
@@ -126,7 +646,9 @@ using namespace iron;
 extern "C" long long iron_tree_attention_workspace_bytes(int n_heads, int n_kv_heads, int head_dim, int num_seqs,
                                                          int num_nodes, int max_nodes, int max_pages, int page_size) {
   if (check_shape(n_heads, n_kv_heads, head_dim, num_seqs, num_nodes, max_nodes, max_pages, page_size)) return -1;
-  return 16;
+  const long long slots = 2LL * workgroups_of(n_heads, n_kv_heads, head_dim, num_seqs, max_nodes, max_pages, page_size) *
+                          rows_of_tile(n_heads, n_kv_heads, max_nodes);
+  return slots * head_dim * 4 + slots * 8 + (num_seqs + 1) * 8;
 }
 
 extern "C" int iron_tree_attention(const void* q, const void* k_new, const void* v_new, const void* k_pages,
@@ -171,18 +693,16 @@ extern "C" int iron_tree_attention(const void* q, const void* k_new, const void*
   a.max_nodes = max_nodes;
   a.words = (max_nodes + 31) / 32;
   a.scale_log2 = scale * 1.4426950408889634f;
+  const int R = rows_of_tile(n_heads, n_kv_heads, max_nodes);
+  a.workgroups = workgroups_of(n_heads, n_kv_heads, head_dim, num_seqs, max_nodes, max_pages, page_size);
+  const long long slots = 2LL * a.workgroups * R;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + slots * head_dim);
+  a.prefix = reinterpret_cast<long long*>(a.part_ml + slots);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid(max_nodes, n_heads, num_seqs), block(256);
-  if (head_dim == 64) {
-    if (dtype)
-      IRON_LAUNCH((tree_attention_kernel<64, true>), grid, block, 0, s, a);
-    else
-      IRON_LAUNCH((tree_attention_kernel<64, false>), grid, block, 0, s, a);
-  } else {
-    if (dtype)
-      IRON_LAUNCH((tree_attention_kernel<128, true>), grid, block, 0, s, a);
-    else
-      IRON_LAUNCH((tree_attention_kernel<128, false>), grid, block, 0, s, a);
-  }
+  if (head_dim == 64)
+    dtype ? launch_rows<64, true>(a, R, s) : launch_rows<64, false>(a, R, s);
+  else
+    dtype ? launch_rows<128, true>(a, R, s) : launch_rows<128, false>(a, R, s);
   return check_launch("tree_attention");
 }
