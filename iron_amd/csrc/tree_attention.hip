@@ -23,8 +23,8 @@ struct TreeArgs {
   uint16_t* out;      // (num_nodes, H, D)
   float* part_o;      // workspace (2 x workgroups, R, D): sum(p v) of the parts of split tiles
   float2* part_ml;    // workspace (2 x workgroups, R): their maximum and sum(p)
-  long long* prefix;  // workspace (num_seqs + 1): units before each sequence; units of a workgroup
-  int H, Hkv, num_pages, page_shift, num_seqs, max_pages, num_nodes, max_nodes, words, workgroups;
+  int* prefix;        // workspace (num_seqs + 1): units before each sequence; units of a workgroup
+  int H, Hkv, G, num_pages, page_shift, num_seqs, max_pages, num_nodes, max_nodes, words, workgroups;
   float scale_log2;
 };
 
@@ -127,38 +127,101 @@ __device__ __forceinline__ int uniform_word(const int* p, long long i) {
 
 // The same value in every lane, in a scalar register.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ long long uniform(long long x) {
-  const unsigned lo = uniform(static_cast<int>(x)), hi = uniform(static_cast<int>(x >> 32));
-  return static_cast<long long>(hi) << 32 | lo;
+
+// Inclusive prefix sum over the wave's lanes by DPP row shifts and broadcasts.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return x;
 }
 
 // Where the work is cut. A tile is R rows (node, head of the KV head's group)
-// of one sequence and KV head; a unit is one block of 64 keys of a tile:
-// first the blocks of the cache, then those of the tree. Units are numbered
-// sequence by sequence, and workgroup b takes units [b * chunk, (b + 1) * chunk).
+// of one sequence and KV head; its units are kOver of them for starting and
+// ending it, then one for each block of 64 keys: the cache's, then the tree's.
+// Units are numbered sequence by sequence, and workgroup b takes units
+// [b * chunk, (b + 1) * chunk): every workgroup gets the same share, however
+// ragged the lengths. The host sees to it that all units count in 31 bits.
+constexpr int kOver = 3;
+
 struct Tiles {
-  int first, nodes, len, cached, blocks, row_tiles;
-  long long units;
+  int first, nodes, len, cached, blocks, row_tiles, units;
+  __device__ __forceinline__ int tile_units() const { return blocks + kOver; }
 };
 
 template <int R>
-__device__ __forceinline__ Tiles tiles_of(const TreeArgs& a, int s) {
+__device__ __forceinline__ Tiles tiles_from(const TreeArgs& a, int start, int stop, int len) {
   Tiles t;
-  tree_of(a, s, t.first, t.nodes);
-  t.len = min(max(a.lens[s], 0), a.max_pages << a.page_shift);
+  t.first = min(max(start, 0), a.num_nodes);
+  t.nodes = min(min(max(stop, t.first), a.num_nodes) - t.first, a.max_nodes);
+  t.len = min(max(len, 0), a.max_pages << a.page_shift);
   t.cached = (t.len + kBlock - 1) / kBlock;
   t.blocks = t.cached + (t.nodes + kBlock - 1) / kBlock;
-  t.row_tiles = (t.nodes * (a.H / a.Hkv) + R - 1) / R;
-  t.units = static_cast<long long>(t.row_tiles) * a.Hkv * t.blocks;
+  t.row_tiles = (t.nodes * a.G + R - 1) / R;
+  t.units = t.row_tiles * a.Hkv * t.tile_units();
   return t;
 }
-
-__device__ __forceinline__ Tiles uniform(const Tiles& t) {
-  return {uniform(t.first), uniform(t.nodes), uniform(t.len), uniform(t.cached), uniform(t.blocks), uniform(t.row_tiles), uniform(t.units)};
+template <int R>
+__device__ __forceinline__ Tiles tiles_of(const TreeArgs& a, int s) {
+  return tiles_from<R>(a, a.starts[s], a.starts[s + 1], a.lens[s]);
+}
+// The same of a sequence that is one for the whole wave, by scalar loads.
+template <int R>
+__device__ __forceinline__ Tiles uniform_tiles_of(const TreeArgs& a, int s) {
+  return tiles_from<R>(a, uniform_word(a.starts, s), uniform_word(a.starts, s + 1), uniform_word(a.lens, s));
 }
 
-__device__ __forceinline__ long long chunk_of(const TreeArgs& a, long long total) {
-  return max((total + a.workgroups - 1) / a.workgroups, 1LL);
+// The share of workgroup b: its units, the sequence of the first one and the
+// units before that sequence. Every wave finds it by itself, without a barrier.
+struct Share {
+  int at, end, s, base;
+  Tiles t;
+};
+
+template <int R>
+__device__ __forceinline__ bool share_of(const TreeArgs& a, int b, Share& sh) {
+  const int lane = threadIdx.x & 63, per = (a.num_seqs + 63) / 64, s0 = lane * per;
+  Tiles t = {};
+  int mine = 0;
+  for (int i = 0; i < per; ++i)
+    if (s0 + i < a.num_seqs) {
+      t = tiles_of<R>(a, s0 + i);
+      mine += t.units;
+    }
+  const int incl = wave_scan(mine), total = __builtin_amdgcn_readlane(incl, 63);
+  const int chunk = max(static_cast<int>((static_cast<unsigned>(total) + a.workgroups - 1) / a.workgroups), 1);
+  int at = incl - mine;
+  if (b == 0 && threadIdx.x < 64) {  // for the launch that joins the parts
+    int before = at;
+    for (int i = 0; i < per; ++i)
+      if (s0 + i < a.num_seqs) {
+        a.prefix[s0 + i] = before;
+        if (per > 1) before += tiles_of<R>(a, s0 + i).units;
+      }
+    if (lane == 0) a.prefix[a.num_seqs] = chunk;
+  }
+  const long long first = static_cast<long long>(b) * chunk;
+  if (first >= total) return false;
+  const int u = static_cast<int>(first);
+  const bool has = at <= u && u < incl;
+  int s = s0;
+  if (has && per > 1)
+    for (;; ++s) {
+      t = tiles_of<R>(a, s);
+      if (u < at + t.units) break;
+      at += t.units;
+    }
+  const int who = __ffsll(static_cast<unsigned long long>(__ballot(has))) - 1;
+  auto pick = [&](int x) { return __builtin_amdgcn_readlane(x, who); };
+  sh.at = u;
+  sh.end = static_cast<int>(min(first + chunk, static_cast<long long>(total)));
+  sh.s = pick(s);
+  sh.base = pick(at);
+  sh.t = {pick(t.first), pick(t.nodes), pick(t.len), pick(t.cached), pick(t.blocks), pick(t.row_tiles), pick(t.units)};
+  return true;
 }
 
 template <int D>
@@ -185,63 +248,15 @@ __global__ __launch_bounds__(256) void tree_attention_kernel(TreeArgs a) {
   static_assert(R * D * 4 <= kRing, "a wave's output goes through its ring");
   __shared__ __attribute__((aligned(16))) unsigned char lds[4 * kRing];
   __shared__ float stat_m[4][R], stat_l[4][R];
-  __shared__ long long scan[5];
-  __shared__ int found;
-  __shared__ long long found_at;
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = uniform(tid >> 6);
   const int c = lane & 15, quad = lane >> 4;
-  const int G = a.H / a.Hkv, ps = 1 << a.page_shift;
-
-  // The units of all sequences before each thread's own ones, the workgroup's
-  // first unit and its sequence.
-  const int per = (a.num_seqs + 255) / 256;
-  long long mine = 0;
-  for (int i = 0; i < per; ++i)
-    if (tid * per + i < a.num_seqs) mine += tiles_of<R>(a, tid * per + i).units;
-  long long incl = mine;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const long long y = __shfl_up(incl, d, 64);
-    if (lane >= d) incl += y;
-  }
-  if (lane == 63) scan[w] = incl;
-  __syncthreads();
-  long long before = incl - mine, total = 0;
-  for (int i = 0; i < 4; ++i) {
-    before += i < w ? scan[i] : 0;
-    total += scan[i];
-  }
-  total = uniform(total);
-  const long long chunk = chunk_of(a, total);
-  long long u = blockIdx.x * chunk;
-  const long long end = min(u + chunk, total);
-  if (blockIdx.x == 0) {  // for the launch that joins the parts
-    long long at = before;
-    for (int i = 0; i < per; ++i)
-      if (tid * per + i < a.num_seqs) {
-        a.prefix[tid * per + i] = at;
-        at += tiles_of<R>(a, tid * per + i).units;
-      }
-    if (tid == 0) a.prefix[a.num_seqs] = chunk;
-  }
-  if (u >= end) return;
-  if (before <= u && u < before + mine) {
-    long long at = before;
-    for (int i = 0; i < per; ++i) {
-      const long long n = tiles_of<R>(a, tid * per + i).units;
-      if (u < at + n) {
-        found = tid * per + i;
-        found_at = at;
-        break;
-      }
-      at += n;
-    }
-  }
-  __syncthreads();
-  int s = uniform(found);
-  long long base = uniform(found_at);
-  Tiles t = uniform(tiles_of<R>(a, s));
+  const int G = a.G, ps = 1 << a.page_shift;
+  Share sh;
+  if (!share_of<R>(a, blockIdx.x, sh)) return;
+  int u = sh.at, s = sh.s, base = sh.base;
+  const int end = sh.end;
+  Tiles t = sh.t;
 
   // This lane's part of a stage's loads: load i puts 1024 bytes, 16 from each
   // lane in order, so lane l fetches the chunk that belongs at its slot.
@@ -258,21 +273,13 @@ __global__ __launch_bounds__(256) void tree_attention_kernel(TreeArgs a) {
   const int trow = 4 * quad + (c >> 2), tcol = 4 * (c & 3);  // this lane's address of a transposed V read
 
   while (u < end) {
-    const int tile = static_cast<int>((u - base) / t.blocks), blk0 = static_cast<int>((u - base) - static_cast<long long>(tile) * t.blocks);
-    const int n = static_cast<int>(min(static_cast<long long>(t.blocks - blk0), end - u));
+    const int tu = t.tile_units(), tile = (u - base) / tu, in_tile = (u - base) - tile * tu;
+    const int stop = min(tu, in_tile + (end - u)), blk0 = max(in_tile - kOver, 0), n = stop - kOver - blk0;
     const int hk = tile / t.row_tiles, row0 = (tile - hk * t.row_tiles) * R;
     const int rows = min(R, t.nodes * G - row0);
-    // Q: the B operand of S^T = K Q^T (column: row 16 rt + c; dims 32 kk + 8 quad .. + 8)
+    if (n > 0) {
     ta_u32x4 qf[RT][NK];
     int node[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int r = min(row0 + 16 * rt + c, t.nodes * G - 1);
-      node[rt] = t.first + r / G;
-      const uint16_t* qp = a.q + (static_cast<long long>(node[rt]) * a.H + hk * G + r % G) * D + 8 * quad;
-#pragma unroll
-      for (int kk = 0; kk < NK; ++kk) qf[rt][kk] = *reinterpret_cast<const ta_u32x4*>(qp + 32 * kk);
-    }
     ta_f32x4 o[RT][ND];
     float m[RT], off[RT], l[RT];
 #pragma unroll
@@ -282,11 +289,6 @@ __global__ __launch_bounds__(256) void tree_attention_kernel(TreeArgs a) {
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt) o[rt][dt] = ta_f32x4{0.f, 0.f, 0.f, 0.f};
     }
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)  // Q has arrived before the first load of the ring is issued
-#pragma unroll
-      for (int kk = 0; kk < NK; ++kk) asm volatile("" ::"v"(qf[rt][kk]));
-
     const long long table = static_cast<long long>(s) * a.max_pages;
     const unsigned new_row = static_cast<unsigned>(a.Hkv) * kRow;
     unsigned holes = 0;  // bit i % kStages: block i's page of this wave is none
@@ -406,6 +408,21 @@ __global__ __launch_bounds__(256) void tree_attention_kernel(TreeArgs a) {
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i)
       if (i < n) issue(i);
+    // Q: the B operand of S^T = K Q^T (column: row 16 rt + c; dims 32 kk + 8 quad .. + 8).
+    // The compiler's wait for it takes in the ring's first loads, which it does not
+    // count: one round trip for both.
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = min(row0 + 16 * rt + c, t.nodes * G - 1), in_tree = r / G;
+      node[rt] = t.first + in_tree;
+      const uint16_t* qp = a.q + (static_cast<long long>(node[rt]) * a.H + hk * G + (r - in_tree * G)) * D + 8 * quad;
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) qf[rt][kk] = *reinterpret_cast<const ta_u32x4*>(qp + 32 * kk);
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) asm volatile("" ::"v"(qf[rt][kk]));
     for (int i = 0; i < n; ++i) {
       const int left = n - 1 - i;  // stages in flight behind block i
       if (left >= 2)
@@ -445,10 +462,12 @@ __global__ __launch_bounds__(256) void tree_attention_kernel(TreeArgs a) {
       ta_f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (stat_l[i][r] == 0.f) continue;  // saw nothing
+        const float li = stat_l[i][r];
         const float f = __builtin_amdgcn_exp2f(stat_m[i][r] - top);
-        sum += f * stat_l[i][r];
-        v += f * *reinterpret_cast<const ta_f32x4*>(reinterpret_cast<const float*>(lds + i * kRing) + r * D + ((c4 ^ (r & 15)) * 4));
+        const ta_f32x4 part = f * *reinterpret_cast<const ta_f32x4*>(reinterpret_cast<const float*>(lds + i * kRing) + r * D + ((c4 ^ (r & 15)) * 4));
+        sum += li == 0.f ? 0.f : f * li;  // a wave that saw nothing has no maximum either
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += li == 0.f ? 0.f : part[e];
       }
       if (whole) {
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -464,11 +483,11 @@ __global__ __launch_bounds__(256) void tree_attention_kernel(TreeArgs a) {
       }
     }
     __syncthreads();  // the rings are free again
-
-    u += n;
+    }
+    u += stop - in_tile;
     if (u < end && u == base + t.units) {
       base += t.units;
-      do t = uniform(tiles_of<R>(a, ++s));
+      do t = uniform_tiles_of<R>(a, ++s);
       while (t.units == 0);
     }
   }
@@ -494,37 +513,53 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
   __syncthreads();
   const int s = uniform(owner);
   if (s < 0 || h >= a.H) return;
-  const Tiles t = tiles_of<R>(a, s);
-  const int G = a.H / a.Hkv, hk = h / G, row = (n - t.first) * G + h % G;
-  const long long chunk = a.prefix[a.num_seqs];
-  const long long u0 = a.prefix[s] + static_cast<long long>(hk * t.row_tiles + row / R) * t.blocks, u1 = u0 + t.blocks - 1;
-  const long long b0 = u0 / chunk, b1 = u1 / chunk;
+  const Tiles t = uniform_tiles_of<R>(a, s);
+  const int G = a.G, hk = h / G, row = (n - t.first) * G + (h - hk * G);
+  const int chunk = uniform_word(a.prefix, a.num_seqs);
+  const int u0 = uniform_word(a.prefix, s) + (hk * t.row_tiles + row / R) * t.tile_units() + kOver, u1 = u0 + t.blocks - 1;
+  const int b0 = u0 / chunk, b1 = u1 / chunk;
   uint16_t* out = a.out + (static_cast<long long>(n) * a.H + h) * D;
   bool again = false;
   if (b0 == b1) {  // one workgroup had all its keys
     for (int e = 0; e < E; ++e) again |= !__builtin_isfinite(widen<F16>(out[lane * E + e]));
   } else {
-    const int parts = static_cast<int>(b1 - b0) + 1;
+    const int parts = b1 - b0 + 1;
     const long long r = row % R;
-    auto slot = [&](int i) { return 2 * (b0 + i) + (i == 0); };
-    float top = -INFINITY;
-    for (int i = lane; i < parts; i += 64) top = fmaxf(top, a.part_ml[slot(i) * R + r].x);
+    auto slot = [&](int i) { return (2LL * (b0 + i) + (i == 0)) * R + r; };
+    float2 ml = lane < parts ? a.part_ml[slot(lane)] : make_float2(-INFINITY, 0.f);
+    float top = ml.x;
+    for (int i = 64 + lane; i < parts; i += 64) top = fmaxf(top, a.part_ml[slot(i)].x);
     top = wave_max(top);
     float sum = 0.f;
     ta_f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int i = lane / V4; i < parts; i += NP) {
-      const float2 ml = a.part_ml[slot(i) * R + r];
-      if (ml.y == 0.f) continue;
-      const float f = __builtin_amdgcn_exp2f(ml.x - top);
-      sum += f * ml.y;
-      v += f * *reinterpret_cast<const ta_f32x4*>(a.part_o + (slot(i) * R + r) * D + (lane % V4) * 4);
-    }
+    const int g = lane / V4;
+    for (int i0 = 0; i0 < parts; i0 += 64) {
+      if (i0) ml = i0 + lane < parts ? a.part_ml[slot(i0 + lane)] : make_float2(-INFINITY, 0.f);
+      // the weight of part i0 + lane; a part that saw nothing has none
+      const float f = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);
+      sum += ml.y == 0.f ? 0.f : f * ml.y;
+      const unsigned long long some = __ballot(ml.y != 0.f);
+      constexpr int kAhead = 8;  // loads in flight
+      for (int i = 0; i < min(parts - i0, 64); i += kAhead * NP) {
+        ta_f32x4 x[kAhead];
 #pragma unroll
-    for (int d = V4; d < 64; d *= 2) {
-      sum += __shfl_xor(sum, d, 64);
+        for (int k = 0; k < kAhead; ++k)
+          x[k] = *reinterpret_cast<const ta_f32x4*>(a.part_o + slot(min(i0 + i + k * NP + g, parts - 1)) * D + (lane % V4) * 4);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          const int j = i + k * NP + g;
+          const float fj = __shfl(f, j, 64);
+          const bool add = j < 64 && (some >> j & 1);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] += add ? fj * x[k][e] : 0.f;
+        }
+      }
+    }
+    sum = wave_sum(sum);
+#pragma unroll
+    for (int d = V4; d < 64; d *= 2)
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] += __shfl_xor(v[e], d, 64);
-    }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     if (sum == 0.f) v = ta_f32x4{0.f, 0.f, 0.f, 0.f};
     ta_u32x2 y;
@@ -596,13 +631,16 @@ int rows_of_tile(int n_heads, int n_kv_heads, int max_nodes) {
   return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
 
-// The workgroups of a launch: no more than there can be units of work.
-int workgroups_of(int n_heads, int n_kv_heads, int head_dim, int num_seqs, int max_nodes, int max_pages, int page_size) {
+// Units of work that there can be at most.
+long long most_units(int n_heads, int n_kv_heads, int num_seqs, int max_nodes, int max_pages, int page_size) {
   const int R = rows_of_tile(n_heads, n_kv_heads, max_nodes);
   const long long blocks = (static_cast<long long>(max_pages) * page_size + kBlock - 1) / kBlock + (max_nodes + kBlock - 1) / kBlock;
-  const long long tiles = static_cast<long long>(max_nodes * (n_heads / n_kv_heads) + R - 1) / R * n_kv_heads * num_seqs;
-  return blocks > resident(head_dim) || tiles > resident(head_dim) ? resident(head_dim)
-                                                                   : static_cast<int>(std::min<long long>(blocks * tiles, resident(head_dim)));
+  const long long tiles = static_cast<long long>((max_nodes * (n_heads / n_kv_heads) + R - 1) / R) * n_kv_heads * num_seqs;
+  return tiles * (blocks + kOver);
+}
+
+int workgroups_of(int n_heads, int n_kv_heads, int head_dim, int num_seqs, int max_nodes, int max_pages, int page_size) {
+  return static_cast<int>(std::min<long long>(most_units(n_heads, n_kv_heads, num_seqs, max_nodes, max_pages, page_size), resident(head_dim)));
 }
 
 template <int D, bool F16, int RT>
@@ -635,6 +673,8 @@ const char* check_shape(int n_heads, int n_kv_heads, int head_dim, int num_seqs,
     return "page_size is not a power of two from 16 to 1024";
   if (max_pages < 1 || static_cast<long long>(max_pages) * page_size >= (1LL << 31) - (1 << 20))
     return "max_pages: a sequence holds less than 2^31 - 2^20 positions";
+  if (most_units(n_heads, n_kv_heads, num_seqs, max_nodes, max_pages, page_size) >= (1LL << 31))
+    return "num_seqs * max_pages * page_size * row tiles is too large: blocks of 64 keys must count below 2^31";
   return nullptr;
 }
 
@@ -648,7 +688,7 @@ extern "C" long long iron_tree_attention_workspace_bytes(int n_heads, int n_kv_h
   if (check_shape(n_heads, n_kv_heads, head_dim, num_seqs, num_nodes, max_nodes, max_pages, page_size)) return -1;
   const long long slots = 2LL * workgroups_of(n_heads, n_kv_heads, head_dim, num_seqs, max_nodes, max_pages, page_size) *
                           rows_of_tile(n_heads, n_kv_heads, max_nodes);
-  return slots * head_dim * 4 + slots * 8 + (num_seqs + 1) * 8;
+  return slots * head_dim * 4 + slots * 8 + (num_seqs + 1) * 4;
 }
 
 extern "C" int iron_tree_attention(const void* q, const void* k_new, const void* v_new, const void* k_pages,
@@ -685,6 +725,7 @@ extern "C" int iron_tree_attention(const void* q, const void* k_new, const void*
   a.out = static_cast<uint16_t*>(out);
   a.H = n_heads;
   a.Hkv = n_kv_heads;
+  a.G = n_heads / n_kv_heads;
   a.num_pages = num_pages;
   a.page_shift = __builtin_ctz(page_size);
   a.num_seqs = num_seqs;
@@ -698,7 +739,7 @@ extern "C" int iron_tree_attention(const void* q, const void* k_new, const void*
   const long long slots = 2LL * a.workgroups * R;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + slots * head_dim);
-  a.prefix = reinterpret_cast<long long*>(a.part_ml + slots);
+  a.prefix = reinterpret_cast<int*>(a.part_ml + slots);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (head_dim == 64)
     dtype ? launch_rows<64, true>(a, R, s) : launch_rows<64, false>(a, R, s);
