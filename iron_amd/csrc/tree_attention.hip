@@ -233,6 +233,11 @@ __device__ __forceinline__ int v_slot(int row, int c) {  // the 8 rows of half a
   return D == 64 ? c ^ (((row >> 1) & 3) << 1) : c ^ ((row & 7) << 1);
 }
 
+template <int D>
+__device__ __forceinline__ int wide_v_slot(int row, int c) {  // the 4 rows of half a wider transposed read
+  return D == 64 ? c ^ (((row >> 1) & 1) << 2) : c ^ ((row & 3) << 2);
+}
+
 // A wave waits until at most N of its loads are in flight and its LDS reads
 // are done: a stage has landed, and the one before it may be overwritten.
 template <int N>
@@ -493,6 +498,256 @@ __global__ __launch_bounds__(256) void tree_attention_kernel(TreeArgs a) {
   }
 }
 
+typedef float ta_f32x16 __attribute__((ext_vector_type(16)));
+
+template <bool F16>
+__device__ __forceinline__ ta_f32x16 mfma32(ta_u32x4 a, ta_u32x4 b, ta_f32x16 c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(ta_f16x8, a), __builtin_bit_cast(ta_f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(ta_bf16x8, a), __builtin_bit_cast(ta_bf16x8, b), c, 0, 0, 0);
+}
+
+// Many rows: a tile of 128 rows, a workgroup of 8 waves. Wave w has rows
+// 32 (w % 4) .. + 31 and keys 32 (w / 4) .. + 31 of each block of 64, which the
+// waves load together (8 rows of K and of V each) into one ring: every byte
+// read from L2 serves 128 rows. One barrier per block.
+template <int D, bool F16>
+__global__ __launch_bounds__(512) void tree_wide_kernel(TreeArgs a) {
+  constexpr int R = 128, kRow = D * 2, kHalf = kBlock * kRow, kStage = 2 * kHalf;
+  constexpr int kParts = 8 * kRow / 1024, kLoads = 2 * kParts;  // 1 KiB loads of a wave and block: kParts of K, kParts of V
+  constexpr int NK = D / 16, ND = D / 32;
+  __shared__ __attribute__((aligned(16))) unsigned char ring[kStages * kStage];
+  __shared__ __attribute__((aligned(16))) int hole[kStages][8];  // whether the page of a wave's 8 rows of the block is none
+  __shared__ float other_m[4][64], other_l[4][64];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = uniform(tid >> 6), rg = w & 3, kh = w >> 2;
+  const int c = lane & 31, hh = lane >> 5;
+  const int G = a.G, ps = 1 << a.page_shift;
+  Share sh;
+  if (!share_of<R>(a, blockIdx.x, sh)) return;
+  int u = sh.at, s = sh.s, base = sh.base;
+  const int end = sh.end;
+  Tiles t = sh.t;
+
+  int lrow[kParts];
+  unsigned kchunk[kParts], vchunk[kParts];
+#pragma unroll
+  for (int i = 0; i < kParts; ++i) {
+    const int slot = lane % (kRow / 16), row = 8 * w + i * (1024 / kRow) + lane / (kRow / 16);
+    lrow[i] = row;
+    kchunk[i] = k_slot<D>(row & 15, slot) * 16;
+    vchunk[i] = wide_v_slot<D>(row, slot) * 16;
+  }
+  const int trow = 32 * kh + 4 * hh + ((lane & 15) >> 2), tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+
+  while (u < end) {
+    const int tu = t.tile_units(), tile = (u - base) / tu, in_tile = (u - base) - tile * tu;
+    const int stop = min(tu, in_tile + (end - u)), blk0 = max(in_tile - kOver, 0), n = stop - kOver - blk0;
+    const int hk = tile / t.row_tiles, row0 = (tile - hk * t.row_tiles) * R;
+    const int rows = min(R, t.nodes * G - row0);
+    if (n > 0) {
+      const long long table = static_cast<long long>(s) * a.max_pages;
+      const unsigned new_row = static_cast<unsigned>(a.Hkv) * kRow;
+      auto page_of = [&](int i) {
+        const int blk = min(blk0 + i, t.cached - 1);
+        return t.cached ? uniform_word(a.table, table + (min(blk * kBlock + 8 * w, t.len - 1) >> a.page_shift)) : 0;
+      };
+      int page = page_of(0);
+      auto issue = [&](int i) {
+        unsigned char* st = ring + (i % kStages) * kStage + 8 * w * kRow;
+        const int blk = blk0 + i;
+        bool real = true;
+        if (blk < t.cached) {
+          real = static_cast<unsigned>(page) < static_cast<unsigned>(a.num_pages);
+          const int in_page = (blk * kBlock + 8 * w) & (ps - 1);
+          const long long at = ((static_cast<long long>(real ? page : 0) * a.Hkv + hk) * ps + in_page) * D;
+          const i32x4v rk = buffer_rsrc(a.k_pages + at), rv = buffer_rsrc(a.v_pages + at);
+#pragma unroll
+          for (int j = 0; j < kParts; ++j) {
+            load_lds16(rk, (lrow[j] - 8 * w) * kRow + kchunk[j], st + j * 1024);
+            load_lds16(rv, (lrow[j] - 8 * w) * kRow + vchunk[j], st + kHalf + j * 1024);
+          }
+          page = page_of(i + 1);
+        } else {
+          const int j0 = (blk - t.cached) * kBlock;
+          const long long at = (static_cast<long long>(t.first) * a.Hkv + hk) * D;
+          const i32x4v rk = buffer_rsrc(a.k_new + at), rv = buffer_rsrc(a.v_new + at);
+#pragma unroll
+          for (int j = 0; j < kParts; ++j) {
+            const unsigned r = min(j0 + lrow[j], t.nodes - 1) * new_row;
+            load_lds16(rk, r + kchunk[j], st + j * 1024);
+            load_lds16(rv, r + vchunk[j], st + kHalf + j * 1024);
+          }
+        }
+        if (lane == 0) hole[i % kStages][w] = !real;
+      };
+#pragma unroll
+      for (int i = 0; i < kStages - 1; ++i)
+        if (i < n) issue(i);
+      // Q: the B operand of S^T = K Q^T (column: row 32 rg + c; dims 16 kk + 8 hh .. + 8)
+      ta_u32x4 qf[NK];
+      const int r = min(row0 + 32 * rg + c, t.nodes * G - 1), in_tree = r / G;
+      const int node = t.first + in_tree;
+      const long long q_row = static_cast<long long>(node) * a.H + hk * G + (r - in_tree * G);
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) qf[kk] = *reinterpret_cast<const ta_u32x4*>(a.q + q_row * D + 16 * kk + 8 * hh);
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) asm volatile("" ::"v"(qf[kk]));
+      ta_f32x16 o[ND];
+      float m = -INFINITY, off = 0.f, l = 0.f;
+#pragma unroll
+      for (int db = 0; db < ND; ++db)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[db][j] = 0.f;
+      const bool idle = 32 * rg >= rows;  // none of the wave's rows is one
+
+      auto step = [&](int i) {
+        const int blk = blk0 + i;
+        const bool cache = blk < t.cached;
+        const int j0 = (cache ? blk : blk - t.cached) * kBlock + 32 * kh;
+        const int left = (cache ? t.len : t.nodes) - j0;
+        if (left <= 0 || idle) return;
+        unsigned keys = left >= 32 ? ~0u : (1u << left) - 1;  // the wave's keys that there are
+        const int4 none = *reinterpret_cast<const int4*>(&hole[i % kStages][4 * kh]);
+        if (uniform(none.x | none.y | none.z | none.w))
+          keys &= ~((none.x ? 0xffu : 0u) | (none.y ? 0xff00u : 0u) | (none.z ? 0xff0000u : 0u) | (none.w ? 0xff000000u : 0u));
+        keys = uniform(static_cast<int>(keys));
+        if (!keys) return;
+        const unsigned char* ks = ring + (i % kStages) * kStage;
+        const unsigned char* vs = ks + kHalf;
+        ta_f32x16 sc = {};
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) {
+          const ta_u32x4 kf = *reinterpret_cast<const ta_u32x4*>(ks + (32 * kh + c) * kRow + k_slot<D>(c & 15, 2 * kk + hh) * 16);
+          sc = mfma32<F16>(kf, qf[kk], sc);
+        }
+        ta_u32x2 vt[4][ND];  // V^T of keys 8 t + 4 hh .. + 3, dims 32 db + lane % 32
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int db = 0; db < ND; ++db) {
+            const int row = trow + 8 * q, dim = 32 * db + tcol;
+            vt[q][db] = __builtin_bit_cast(ta_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) ta_i16x4*)(vs + row * kRow + wide_v_slot<D>(row, dim >> 3) * 16 + (dim & 7) * 2)));
+          }
+        unsigned seen = keys;
+        if (!cache) seen &= a.mask[static_cast<long long>(node) * a.words + (j0 >> 5)];
+        if (!cache || keys != ~0u) {
+          const unsigned mine = seen >> (4 * hh), real = keys >> (4 * hh);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) sc[j] = mine >> (8 * (j >> 2) + (j & 3)) & 1 ? sc[j] : -INFINITY;
+          if (keys != ~0u) {  // values of keys that are none cannot do harm
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const unsigned b = real >> (8 * q);
+              const unsigned m01 = (b & 1 ? 0xffffu : 0u) | (b & 2 ? 0xffff0000u : 0u), m23 = (b & 4 ? 0xffffu : 0u) | (b & 8 ? 0xffff0000u : 0u);
+#pragma unroll
+              for (int db = 0; db < ND; ++db) {
+                vt[q][db].x &= m01;
+                vt[q][db].y &= m23;
+              }
+            }
+          }
+        }
+        const float cs = a.scale_log2;
+        float mx = fmaxf(fmaxf(sc[0], sc[1]), sc[2]);
+#pragma unroll
+        for (int j = 3; j < 15; j += 2) mx = fmaxf(fmaxf(mx, sc[j]), sc[j + 1]);
+        mx = fmaxf(mx, sc[15]);
+        if (__builtin_amdgcn_ballot_w64(mx * cs > m + 8.f)) {
+          float x, y;
+          swap32(mx, x, y);
+          const float top = fmaxf(x, y) * cs;
+          if (top > m + 8.f) {
+            const float alpha = __builtin_amdgcn_exp2f(m - top);  // 0 from m = -inf
+            m = off = top;
+            l *= alpha;
+#pragma unroll
+            for (int db = 0; db < ND; ++db) o[db] *= alpha;
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float p[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(sc[4 * q + e], cs, -off));
+          l += (p[0] + p[1]) + (p[2] + p[3]);
+          const ta_u32x4 pf = split4<F16>(p);
+#pragma unroll
+          for (int db = 0; db < ND; ++db) o[db] = mfma32<F16>(ta_u32x4{vt[q][db].x, vt[q][db].y, vt[q][db].x, vt[q][db].y}, pf, o[db]);
+        }
+      };
+
+      for (int i = 0; i < n; ++i) {
+        const int left = n - 1 - i;
+        if (left >= 2)
+          wait_stage<2 * kLoads>();
+        else if (left == 1)
+          wait_stage<kLoads>();
+        else
+          wait_stage<0>();
+        __builtin_amdgcn_s_barrier();  // block i is there, and block i - 1's stage read by all
+        asm volatile("" ::: "memory");
+        if (i + kStages - 1 < n) issue(i + kStages - 1);
+        step(i);
+      }
+
+      // The two halves of the keys meet: the upper waves hand theirs over, lane by lane.
+      const bool whole = n == t.blocks;
+      const long long part = 2LL * blockIdx.x + (blk0 == 0 ? 1 : 0);
+      float x, y;
+      swap32(l, x, y);
+      l = x + y;
+      __syncthreads();  // the ring is free
+      ta_f32x4* give = reinterpret_cast<ta_f32x4*>(ring) + rg * ND * 4 * 64 + lane;
+      if (kh == 1) {
+        other_m[rg][lane] = m;
+        other_l[rg][lane] = l;
+#pragma unroll
+        for (int db = 0; db < ND; ++db)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) give[(db * 4 + q) * 64] = ta_f32x4{o[db][4 * q], o[db][4 * q + 1], o[db][4 * q + 2], o[db][4 * q + 3]};
+      }
+      __syncthreads();
+      if (kh == 0 && 32 * rg + c < rows) {
+        const float m1 = other_m[rg][lane], l1 = other_l[rg][lane], top = fmaxf(m, m1);
+        // a half that saw nothing has no maximum, and its sums count for nothing
+        const float f0 = __builtin_amdgcn_exp2f(m - top), f1 = __builtin_amdgcn_exp2f(m1 - top);
+        const float sum = (l == 0.f ? 0.f : f0 * l) + (l1 == 0.f ? 0.f : f1 * l1);
+        const float inv = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
+        const long long pr = part * R + 32 * rg + c;
+        if (!whole && hh == 0) a.part_ml[pr] = make_float2(top, sum);
+#pragma unroll
+        for (int db = 0; db < ND; ++db)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const ta_f32x4 o1 = give[(db * 4 + q) * 64];
+            ta_f32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = ((l == 0.f ? 0.f : f0 * o[db][4 * q + e]) + (l1 == 0.f ? 0.f : f1 * o1[e])) * inv;
+            const int dim = 32 * db + 8 * q + 4 * hh;
+            if (whole) {
+              ta_u32x2 z;
+              z.x = narrow<F16>(v[0]) | static_cast<unsigned>(narrow<F16>(v[1])) << 16;
+              z.y = narrow<F16>(v[2]) | static_cast<unsigned>(narrow<F16>(v[3])) << 16;
+              *reinterpret_cast<ta_u32x2*>(a.out + q_row * D + dim) = z;
+            } else {
+              *reinterpret_cast<ta_f32x4*>(a.part_o + pr * D + dim) = v;
+            }
+          }
+      }
+      __syncthreads();  // the ring is free again
+    }
+    u += stop - in_tile;
+    if (u < end && u == base + t.units) {
+      base += t.units;
+      do t = uniform_tiles_of<R>(a, ++s);
+      while (t.units == 0);
+    }
+  }
+}
+
 // One workgroup per node and 4 heads, a wave for each row: joins the parts of
 // rows whose keys were shared out, and does over the rows that came out
 // infinite or NaN, one key at a time and only the keys that the row sees (a
@@ -623,12 +878,12 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
 }
 
 // Workgroups that fit the 256 CUs at once: LDS holds two rings of head_dim 64, one of 128.
-constexpr int resident(int D) { return D == 64 ? 512 : 256; }
+constexpr int resident(int D, int R) { return D == 64 && R <= 64 ? 512 : 256; }
 
-// Row tiles of 16, 32 or 64 rows.
+// Row tiles of 16, 32, 64 or 128 rows.
 int rows_of_tile(int n_heads, int n_kv_heads, int max_nodes) {
   const int rows = max_nodes * (n_heads / n_kv_heads);
-  return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
 }
 
 // Units of work that there can be at most.
@@ -640,7 +895,7 @@ long long most_units(int n_heads, int n_kv_heads, int num_seqs, int max_nodes, i
 }
 
 int workgroups_of(int n_heads, int n_kv_heads, int head_dim, int num_seqs, int max_nodes, int max_pages, int page_size) {
-  return static_cast<int>(std::min<long long>(most_units(n_heads, n_kv_heads, num_seqs, max_nodes, max_pages, page_size), resident(head_dim)));
+  return static_cast<int>(std::min<long long>(most_units(n_heads, n_kv_heads, num_seqs, max_nodes, max_pages, page_size), resident(head_dim, rows_of_tile(n_heads, n_kv_heads, max_nodes))));
 }
 
 template <int D, bool F16, int RT>
@@ -655,8 +910,12 @@ void launch_rows(const TreeArgs& a, int R, hipStream_t s) {
     launch_tree<D, F16, 1>(a, s);
   else if (R == 32)
     launch_tree<D, F16, 2>(a, s);
-  else
+  else if (R == 64)
     launch_tree<D, F16, 4>(a, s);
+  else {
+    IRON_LAUNCH((tree_wide_kernel<D, F16>), dim3(a.workgroups), dim3(512), 0, s, a);
+    IRON_LAUNCH((tree_join_kernel<D, F16, 128>), dim3(a.num_nodes, (a.H + 3) / 4), dim3(256), 0, s, a);
+  }
 }
 
 constexpr int kMaxNodes = 1024;
