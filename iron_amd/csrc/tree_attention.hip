@@ -6,6 +6,7 @@
 #include "../../include/iron_hip.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace iron {
 namespace {
@@ -54,7 +55,13 @@ typedef unsigned ta_u32x4 __attribute__((ext_vector_type(4)));
 typedef short ta_i16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kBlock = 64;   // keys of a block: 16 for each of the 4 waves
+constexpr int kWideBlock = 32;  // of the kernel of many rows
 constexpr int kStages = 4;   // blocks resident in a wave's ring
+
+// fp16 weights are taken 2^6 times as large (at most 2^14 then), so that small
+// ones stay in fp16's normal range six powers of two longer.
+template <bool F16>
+constexpr float kLift = F16 ? 6.f : 0.f;
 
 template <bool F16>
 __device__ __forceinline__ ta_f32x4 mfma(ta_u32x4 a, ta_u32x4 b, ta_f32x4 c) {
@@ -87,6 +94,18 @@ __device__ __forceinline__ ta_u32x4 split4(const float (&p)[4]) {
     }
   }
   return r;
+}
+
+// Two weights rounded to 16 bits each, and their sum added to l.
+template <bool F16>
+__device__ __forceinline__ unsigned pack2(float a, float b) {
+  if constexpr (F16) return __builtin_bit_cast(unsigned, ta_f16x2{static_cast<_Float16>(a), static_cast<_Float16>(b)});
+  return cvt_pk_bf16(a, b);
+}
+template <bool F16>
+__device__ __forceinline__ float add2(unsigned p, float l) {
+  if constexpr (F16) return __builtin_amdgcn_fdot2(__builtin_bit_cast(ta_f16x2, p), ta_f16x2{1, 1}, l, false);
+  return dot2_bf16(p, 0x3f803f80u, l);
 }
 
 // x[l], y[l] = a[l % 32], a[l % 32 + 32] (swap32), or a of the even and odd
@@ -141,7 +160,7 @@ __device__ __forceinline__ int wave_scan(int x) {
 
 // Where the work is cut. A tile is R rows (node, head of the KV head's group)
 // of one sequence and KV head; its units are kOver of them for starting and
-// ending it, then one for each block of 64 keys: the cache's, then the tree's.
+// ending it, then one for each block of B keys: the cache's, then the tree's.
 // Units are numbered sequence by sequence, and workgroup b takes units
 // [b * chunk, (b + 1) * chunk): every workgroup gets the same share, however
 // ragged the lengths. The host sees to it that all units count in 31 bits.
@@ -152,26 +171,26 @@ struct Tiles {
   __device__ __forceinline__ int tile_units() const { return blocks + kOver; }
 };
 
-template <int R>
+template <int R, int B>
 __device__ __forceinline__ Tiles tiles_from(const TreeArgs& a, int start, int stop, int len) {
   Tiles t;
   t.first = min(max(start, 0), a.num_nodes);
   t.nodes = min(min(max(stop, t.first), a.num_nodes) - t.first, a.max_nodes);
   t.len = min(max(len, 0), a.max_pages << a.page_shift);
-  t.cached = (t.len + kBlock - 1) / kBlock;
-  t.blocks = t.cached + (t.nodes + kBlock - 1) / kBlock;
+  t.cached = (t.len + B - 1) / B;
+  t.blocks = t.cached + (t.nodes + B - 1) / B;
   t.row_tiles = (t.nodes * a.G + R - 1) / R;
   t.units = t.row_tiles * a.Hkv * t.tile_units();
   return t;
 }
-template <int R>
+template <int R, int B>
 __device__ __forceinline__ Tiles tiles_of(const TreeArgs& a, int s) {
-  return tiles_from<R>(a, a.starts[s], a.starts[s + 1], a.lens[s]);
+  return tiles_from<R, B>(a, a.starts[s], a.starts[s + 1], a.lens[s]);
 }
 // The same of a sequence that is one for the whole wave, by scalar loads.
-template <int R>
+template <int R, int B>
 __device__ __forceinline__ Tiles uniform_tiles_of(const TreeArgs& a, int s) {
-  return tiles_from<R>(a, uniform_word(a.starts, s), uniform_word(a.starts, s + 1), uniform_word(a.lens, s));
+  return tiles_from<R, B>(a, uniform_word(a.starts, s), uniform_word(a.starts, s + 1), uniform_word(a.lens, s));
 }
 
 // The share of workgroup b: its units, the sequence of the first one and the
@@ -181,14 +200,14 @@ struct Share {
   Tiles t;
 };
 
-template <int R>
+template <int R, int B>
 __device__ __forceinline__ bool share_of(const TreeArgs& a, int b, Share& sh) {
   const int lane = threadIdx.x & 63, per = (a.num_seqs + 63) / 64, s0 = lane * per;
   Tiles t = {};
   int mine = 0;
   for (int i = 0; i < per; ++i)
     if (s0 + i < a.num_seqs) {
-      t = tiles_of<R>(a, s0 + i);
+      t = tiles_of<R, B>(a, s0 + i);
       mine += t.units;
     }
   const int incl = wave_scan(mine), total = __builtin_amdgcn_readlane(incl, 63);
@@ -199,7 +218,7 @@ __device__ __forceinline__ bool share_of(const TreeArgs& a, int b, Share& sh) {
     for (int i = 0; i < per; ++i)
       if (s0 + i < a.num_seqs) {
         a.prefix[s0 + i] = before;
-        if (per > 1) before += tiles_of<R>(a, s0 + i).units;
+        if (per > 1) before += tiles_of<R, B>(a, s0 + i).units;
       }
     if (lane == 0) a.prefix[a.num_seqs] = chunk;
   }
@@ -210,7 +229,7 @@ __device__ __forceinline__ bool share_of(const TreeArgs& a, int b, Share& sh) {
   int s = s0;
   if (has && per > 1)
     for (;; ++s) {
-      t = tiles_of<R>(a, s);
+      t = tiles_of<R, B>(a, s);
       if (u < at + t.units) break;
       at += t.units;
     }
@@ -247,7 +266,7 @@ __device__ __forceinline__ void wait_stage() {
 
 template <int D, bool F16, int RT>
 __global__ __launch_bounds__(256) void tree_attention_kernel(TreeArgs a) {
-  constexpr int R = 16 * RT, kRow = D * 2, kHalf = 16 * kRow, kStage = 2 * kHalf, kRing = kStages * kStage;
+  constexpr int R = 16 * RT, B = kBlock, kRow = D * 2, kHalf = 16 * kRow, kStage = 2 * kHalf, kRing = kStages * kStage;
   constexpr int kLoads = kStage / 1024;  // 1 KiB loads of a stage, the first half of them K
   constexpr int NK = D / 32, ND = D / 16;
   static_assert(R * D * 4 <= kRing, "a wave's output goes through its ring");
@@ -258,7 +277,7 @@ __global__ __launch_bounds__(256) void tree_attention_kernel(TreeArgs a) {
   const int c = lane & 15, quad = lane >> 4;
   const int G = a.G, ps = 1 << a.page_shift;
   Share sh;
-  if (!share_of<R>(a, blockIdx.x, sh)) return;
+  if (!share_of<R, B>(a, blockIdx.x, sh)) return;
   int u = sh.at, s = sh.s, base = sh.base;
   const int end = sh.end;
   Tiles t = sh.t;
@@ -278,9 +297,9 @@ __global__ __launch_bounds__(256) void tree_attention_kernel(TreeArgs a) {
   const int trow = 4 * quad + (c >> 2), tcol = 4 * (c & 3);  // this lane's address of a transposed V read
 
   while (u < end) {
-    const int tu = t.tile_units(), tile = (u - base) / tu, in_tile = (u - base) - tile * tu;
+    const int tu = t.tile_units(), tile = uniform((u - base) / tu), in_tile = (u - base) - tile * tu;
     const int stop = min(tu, in_tile + (end - u)), blk0 = max(in_tile - kOver, 0), n = stop - kOver - blk0;
-    const int hk = tile / t.row_tiles, row0 = (tile - hk * t.row_tiles) * R;
+    const int hk = uniform(tile / t.row_tiles), row0 = (tile - hk * t.row_tiles) * R;
     const int rows = min(R, t.nodes * G - row0);
     if (n > 0) {
     ta_u32x4 qf[RT][NK];
@@ -390,7 +409,8 @@ __global__ __launch_bounds__(256) void tree_attention_kernel(TreeArgs a) {
           const float top = row_max(fmaxf(fmaxf(sc[rt][0], sc[rt][1]), fmaxf(sc[rt][2], sc[rt][3]))) * cs;
           if (top > m[rt] + 8.f) {
             const float alpha = __builtin_amdgcn_exp2f(m[rt] - top);  // 0 from m = -inf
-            m[rt] = off[rt] = top;
+            m[rt] = top;
+            off[rt] = top - kLift<F16>;
             l[rt] *= alpha;
 #pragma unroll
             for (int dt = 0; dt < ND; ++dt) o[rt][dt] *= alpha;
@@ -450,7 +470,7 @@ __global__ __launch_bounds__(256) void tree_attention_kernel(TreeArgs a) {
       const int r = 16 * rt + c;
       const float sum = row_sum(l[rt]);
       if (quad == 0) {
-        stat_m[w][r] = m[rt];
+        stat_m[w][r] = m[rt] - kLift<F16>;
         stat_l[w][r] = sum;
       }
 #pragma unroll
@@ -492,7 +512,7 @@ __global__ __launch_bounds__(256) void tree_attention_kernel(TreeArgs a) {
     u += stop - in_tile;
     if (u < end && u == base + t.units) {
       base += t.units;
-      do t = uniform_tiles_of<R>(a, ++s);
+      do t = uniform_tiles_of<R, B>(a, ++s);
       while (t.units == 0);
     }
   }
@@ -508,86 +528,101 @@ __device__ __forceinline__ ta_f32x16 mfma32(ta_u32x4 a, ta_u32x4 b, ta_f32x16 c)
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(ta_bf16x8, a), __builtin_bit_cast(ta_bf16x8, b), c, 0, 0, 0);
 }
 
-// Many rows: a tile of 128 rows, a workgroup of 8 waves. Wave w has rows
-// 32 (w % 4) .. + 31 and keys 32 (w / 4) .. + 31 of each block of 64, which the
-// waves load together (8 rows of K and of V each) into one ring: every byte
-// read from L2 serves 128 rows. One barrier per block.
+// Many rows: a tile of 128 rows, a workgroup of 4 waves with 32 rows each. The
+// waves load blocks of 32 keys together (8 rows of K and of V each) into one
+// ring: every byte read from L2 serves 128 rows. One barrier per block; the two
+// waves of a SIMD (four for head_dim 64) are of different workgroups, so that
+// one's softmax runs under another's products: with eight waves on one ring they
+// went through each phase together (wide trees 134 us, so 128).
 template <int D, bool F16>
-__global__ __launch_bounds__(512) void tree_wide_kernel(TreeArgs a) {
-  constexpr int R = 128, kRow = D * 2, kHalf = kBlock * kRow, kStage = 2 * kHalf;
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void tree_wide_kernel(TreeArgs a) {
+  constexpr int R = 128, B = kWideBlock, kRow = D * 2, kHalf = B * kRow, kStage = 2 * kHalf;
   constexpr int kParts = 8 * kRow / 1024, kLoads = 2 * kParts;  // 1 KiB loads of a wave and block: kParts of K, kParts of V
   constexpr int NK = D / 16, ND = D / 32;
   __shared__ __attribute__((aligned(16))) unsigned char ring[kStages * kStage];
-  __shared__ __attribute__((aligned(16))) int hole[kStages][8];  // whether the page of a wave's 8 rows of the block is none
-  __shared__ float other_m[4][64], other_l[4][64];
   const int tid = threadIdx.x, lane = tid & 63;
-  const int w = uniform(tid >> 6), rg = w & 3, kh = w >> 2;
+  const int w = uniform(tid >> 6);
   const int c = lane & 31, hh = lane >> 5;
   const int G = a.G, ps = 1 << a.page_shift;
   Share sh;
-  if (!share_of<R>(a, blockIdx.x, sh)) return;
+  if (!share_of<R, B>(a, blockIdx.x, sh)) return;
   int u = sh.at, s = sh.s, base = sh.base;
   const int end = sh.end;
   Tiles t = sh.t;
 
-  int lrow[kParts];
-  unsigned kchunk[kParts], vchunk[kParts];
+  // This lane's 16 bytes of each of the wave's loads: rows 8 w .. + 7 of a block.
+  unsigned krow[kParts], kat[kParts], vat[kParts];
 #pragma unroll
   for (int i = 0; i < kParts; ++i) {
     const int slot = lane % (kRow / 16), row = 8 * w + i * (1024 / kRow) + lane / (kRow / 16);
-    lrow[i] = row;
-    kchunk[i] = k_slot<D>(row & 15, slot) * 16;
-    vchunk[i] = wide_v_slot<D>(row, slot) * 16;
+    krow[i] = row;
+    kat[i] = k_slot<D>(row & 15, slot) * 16;
+    vat[i] = wide_v_slot<D>(row, slot) * 16;
   }
-  const int trow = 32 * kh + 4 * hh + ((lane & 15) >> 2), tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  const int trow = 4 * hh + ((lane & 15) >> 2), tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  const unsigned page_bytes = static_cast<unsigned>(a.Hkv) << a.page_shift << (D == 64 ? 7 : 8);
 
   while (u < end) {
-    const int tu = t.tile_units(), tile = (u - base) / tu, in_tile = (u - base) - tile * tu;
+    const int tu = t.tile_units(), tile = uniform((u - base) / tu), in_tile = (u - base) - tile * tu;
     const int stop = min(tu, in_tile + (end - u)), blk0 = max(in_tile - kOver, 0), n = stop - kOver - blk0;
-    const int hk = tile / t.row_tiles, row0 = (tile - hk * t.row_tiles) * R;
+    const int hk = uniform(tile / t.row_tiles), row0 = (tile - hk * t.row_tiles) * R;
     const int rows = min(R, t.nodes * G - row0);
     if (n > 0) {
-      const long long table = static_cast<long long>(s) * a.max_pages;
+      const int* table = a.table + static_cast<long long>(s) * a.max_pages;
+      const int cached = t.cached - blk0;                       // blocks of this part that are the cache's (the rest are the tree's)
+      const int whole_blocks = t.len / B - blk0;                // the first ones of them, with no key behind the last
+      const long long head = static_cast<long long>(hk) * ps * kRow;
+      const unsigned char* kc = reinterpret_cast<const unsigned char*>(a.k_pages) + head;
+      const unsigned char* vc = reinterpret_cast<const unsigned char*>(a.v_pages) + head;
+      const long long tree = (static_cast<long long>(t.first) * a.Hkv + hk) * kRow;
       const unsigned new_row = static_cast<unsigned>(a.Hkv) * kRow;
-      auto page_of = [&](int i) {
-        const int blk = min(blk0 + i, t.cached - 1);
-        return t.cached ? uniform_word(a.table, table + (min(blk * kBlock + 8 * w, t.len - 1) >> a.page_shift)) : 0;
+      unsigned holes = 0;  // bits 2 (i % kStages) and + 1: the two pages of block i's 16 rows each are none
+      int page0, page1;    // of the block to be issued next
+      auto pages_of = [&](int i) {
+        if (cached <= 0) return;
+        const int pos = (blk0 + min(i, cached - 1)) * B;
+        page0 = uniform_word(table, min(pos, t.len - 1) >> a.page_shift);
+        page1 = uniform_word(table, min(pos + 16, t.len - 1) >> a.page_shift);
       };
-      int page = page_of(0);
+      page0 = page1 = 0;
+      pages_of(0);
       auto issue = [&](int i) {
-        unsigned char* st = ring + (i % kStages) * kStage + 8 * w * kRow;
-        const int blk = blk0 + i;
-        bool real = true;
-        if (blk < t.cached) {
-          real = static_cast<unsigned>(page) < static_cast<unsigned>(a.num_pages);
-          const int in_page = (blk * kBlock + 8 * w) & (ps - 1);
-          const long long at = ((static_cast<long long>(real ? page : 0) * a.Hkv + hk) * ps + in_page) * D;
-          const i32x4v rk = buffer_rsrc(a.k_pages + at), rv = buffer_rsrc(a.v_pages + at);
+        const int stage = i % kStages;
+        unsigned char* st = ring + stage * kStage + 8 * w * kRow;
+        if (i < cached) {
+          const bool none0 = static_cast<unsigned>(page0) >= static_cast<unsigned>(a.num_pages);
+          const bool none1 = static_cast<unsigned>(page1) >= static_cast<unsigned>(a.num_pages);
+          holes = (holes & ~(3u << (2 * stage))) | ((none0 ? 1u : 0u) | (none1 ? 2u : 0u)) << (2 * stage);
+          const unsigned page = w < 2 ? (none0 ? 0 : page0) : (none1 ? 0 : page1);
+          // from the page's row of the block's first key: row 8 w is in the page, whatever page the first is in
+          const int in_page = (((blk0 + i) * B + 8 * w) & (ps - 1)) - 8 * w;
+          const long long at = static_cast<long long>(static_cast<unsigned long long>(page) * page_bytes) + in_page * kRow;
+          const i32x4v rk = buffer_rsrc(kc + at), rv = buffer_rsrc(vc + at);
 #pragma unroll
           for (int j = 0; j < kParts; ++j) {
-            load_lds16(rk, (lrow[j] - 8 * w) * kRow + kchunk[j], st + j * 1024);
-            load_lds16(rv, (lrow[j] - 8 * w) * kRow + vchunk[j], st + kHalf + j * 1024);
+            load_lds16(rk, krow[j] * kRow + kat[j], st + j * 1024);
+            load_lds16(rv, krow[j] * kRow + vat[j], st + kHalf + j * 1024);
           }
-          page = page_of(i + 1);
+          pages_of(i + 1);
         } else {
-          const int j0 = (blk - t.cached) * kBlock;
-          const long long at = (static_cast<long long>(t.first) * a.Hkv + hk) * D;
-          const i32x4v rk = buffer_rsrc(a.k_new + at), rv = buffer_rsrc(a.v_new + at);
+          const int j0 = (i - cached) * B;
+          holes &= ~(3u << (2 * stage));
+          const i32x4v rk = buffer_rsrc(reinterpret_cast<const unsigned char*>(a.k_new) + tree);
+          const i32x4v rv = buffer_rsrc(reinterpret_cast<const unsigned char*>(a.v_new) + tree);
 #pragma unroll
           for (int j = 0; j < kParts; ++j) {
-            const unsigned r = min(j0 + lrow[j], t.nodes - 1) * new_row;
-            load_lds16(rk, r + kchunk[j], st + j * 1024);
-            load_lds16(rv, r + vchunk[j], st + kHalf + j * 1024);
+            const unsigned r = min(j0 + static_cast<int>(krow[j]), t.nodes - 1) * new_row;
+            load_lds16(rk, r + kat[j], st + j * 1024);
+            load_lds16(rv, r + vat[j], st + kHalf + j * 1024);
           }
         }
-        if (lane == 0) hole[i % kStages][w] = !real;
       };
 #pragma unroll
       for (int i = 0; i < kStages - 1; ++i)
         if (i < n) issue(i);
-      // Q: the B operand of S^T = K Q^T (column: row 32 rg + c; dims 16 kk + 8 hh .. + 8)
+      // Q: the B operand of S^T = K Q^T (column: row 32 w + c; dims 16 kk + 8 hh .. + 8)
       ta_u32x4 qf[NK];
-      const int r = min(row0 + 32 * rg + c, t.nodes * G - 1), in_tree = r / G;
+      const int r = min(row0 + 32 * w + c, t.nodes * G - 1), in_tree = r / G;
       const int node = t.first + in_tree;
       const long long q_row = static_cast<long long>(node) * a.H + hk * G + (r - in_tree * G);
 #pragma unroll
@@ -600,57 +635,23 @@ __global__ __launch_bounds__(512) void tree_wide_kernel(TreeArgs a) {
       for (int db = 0; db < ND; ++db)
 #pragma unroll
         for (int j = 0; j < 16; ++j) o[db][j] = 0.f;
-      const bool idle = 32 * rg >= rows;  // none of the wave's rows is one
+      const bool idle = 32 * w >= rows;  // none of the wave's rows is one
 
-      auto step = [&](int i) {
-        const int blk = blk0 + i;
-        const bool cache = blk < t.cached;
-        const int j0 = (cache ? blk : blk - t.cached) * kBlock + 32 * kh;
-        const int left = (cache ? t.len : t.nodes) - j0;
-        if (left <= 0 || idle) return;
-        unsigned keys = left >= 32 ? ~0u : (1u << left) - 1;  // the wave's keys that there are
-        const int4 none = *reinterpret_cast<const int4*>(&hole[i % kStages][4 * kh]);
-        if (uniform(none.x | none.y | none.z | none.w))
-          keys &= ~((none.x ? 0xffu : 0u) | (none.y ? 0xff00u : 0u) | (none.z ? 0xff0000u : 0u) | (none.w ? 0xff000000u : 0u));
-        keys = uniform(static_cast<int>(keys));
-        if (!keys) return;
-        const unsigned char* ks = ring + (i % kStages) * kStage;
-        const unsigned char* vs = ks + kHalf;
-        ta_f32x16 sc = {};
-#pragma unroll
-        for (int kk = 0; kk < NK; ++kk) {
-          const ta_u32x4 kf = *reinterpret_cast<const ta_u32x4*>(ks + (32 * kh + c) * kRow + k_slot<D>(c & 15, 2 * kk + hh) * 16);
-          sc = mfma32<F16>(kf, qf[kk], sc);
-        }
-        ta_u32x2 vt[4][ND];  // V^T of keys 8 t + 4 hh .. + 3, dims 32 db + lane % 32
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int db = 0; db < ND; ++db) {
-            const int row = trow + 8 * q, dim = 32 * db + tcol;
-            vt[q][db] = __builtin_bit_cast(ta_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) ta_i16x4*)(vs + row * kRow + wide_v_slot<D>(row, dim >> 3) * 16 + (dim & 7) * 2)));
-          }
-        unsigned seen = keys;
-        if (!cache) seen &= a.mask[static_cast<long long>(node) * a.words + (j0 >> 5)];
-        if (!cache || keys != ~0u) {
-          const unsigned mine = seen >> (4 * hh), real = keys >> (4 * hh);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) sc[j] = mine >> (8 * (j >> 2) + (j & 3)) & 1 ? sc[j] : -INFINITY;
-          if (keys != ~0u) {  // values of keys that are none cannot do harm
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const unsigned b = real >> (8 * q);
-              const unsigned m01 = (b & 1 ? 0xffffu : 0u) | (b & 2 ? 0xffff0000u : 0u), m23 = (b & 4 ? 0xffffu : 0u) | (b & 8 ? 0xffff0000u : 0u);
-#pragma unroll
-              for (int db = 0; db < ND; ++db) {
-                vt[q][db].x &= m01;
-                vt[q][db].y &= m23;
-              }
-            }
-          }
-        }
-        const float cs = a.scale_log2;
+      // Both swizzles are exclusive ors, so a fragment's address is the first one's with
+      // the fragment's own bits turned: one register for each operand.
+      const unsigned k_first = c * kRow + k_slot<D>(c & 15, hh) * 16;
+      const unsigned v_first = kHalf + trow * kRow + wide_v_slot<D>(trow, tcol >> 3) * 16 + (tcol & 7) * 2;
+      auto k_frag = [&](int i, int kk) {
+        return *reinterpret_cast<const ta_u32x4*>(ring + (((i % kStages) * kStage + k_first) ^ (32 * kk)));
+      };
+      // V^T of keys 8 q + 4 hh .. + 3 of block i, dims 32 db + lane % 32
+      auto v_frag = [&](int i, int q, int db) {
+        return __builtin_bit_cast(ta_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ta_i16x4*)(
+            ring + (((i % kStages) * kStage + v_first) ^ (64 * db)) + 8 * q * kRow)));
+      };
+      // The row's maximum, when scores pass it by more than 8 (in the log2 domain; cf. tree_attention_kernel).
+      const float cs = a.scale_log2;
+      auto raise = [&](const ta_f32x16& sc) {
         float mx = fmaxf(fmaxf(sc[0], sc[1]), sc[2]);
 #pragma unroll
         for (int j = 3; j < 15; j += 2) mx = fmaxf(fmaxf(mx, sc[j]), sc[j + 1]);
@@ -661,79 +662,121 @@ __global__ __launch_bounds__(512) void tree_wide_kernel(TreeArgs a) {
           const float top = fmaxf(x, y) * cs;
           if (top > m + 8.f) {
             const float alpha = __builtin_amdgcn_exp2f(m - top);  // 0 from m = -inf
-            m = off = top;
+            m = top;
+            off = top - kLift<F16>;
             l *= alpha;
 #pragma unroll
             for (int db = 0; db < ND; ++db) o[db] *= alpha;
           }
         }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float p[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(sc[4 * q + e], cs, -off));
-          l += (p[0] + p[1]) + (p[2] + p[3]);
-          const ta_u32x4 pf = split4<F16>(p);
-#pragma unroll
-          for (int db = 0; db < ND; ++db) o[db] = mfma32<F16>(ta_u32x4{vt[q][db].x, vt[q][db].y, vt[q][db].x, vt[q][db].y}, pf, o[db]);
-        }
       };
-
-      for (int i = 0; i < n; ++i) {
-        const int left = n - 1 - i;
-        if (left >= 2)
-          wait_stage<2 * kLoads>();
-        else if (left == 1)
-          wait_stage<kLoads>();
-        else
-          wait_stage<0>();
-        __builtin_amdgcn_s_barrier();  // block i is there, and block i - 1's stage read by all
-        asm volatile("" ::: "memory");
-        if (i + kStages - 1 < n) issue(i + kStages - 1);
-        step(i);
+      // Weights 2 g and 2 g + 1 of the lane, rounded to 16 bits as the second product takes them; l sums those.
+      auto weights = [&](const ta_f32x16& sc, int g) {
+        const unsigned p = pack2<F16>(__builtin_amdgcn_exp2f(fmaf(sc[2 * g], cs, -off)), __builtin_amdgcn_exp2f(fmaf(sc[2 * g + 1], cs, -off)));
+        l = add2<F16>(p, l);
+        return p;
+      };
+      // Block i from its scores S^T: sc[j] is key 8 (j / 4) + 4 hh + j % 4, row 32 w + c.
+      auto step = [&](int i, ta_f32x16& sc, ta_f32x16& next) {
+        const unsigned none = holes >> (2 * (i % kStages)) & 3u;
+        if (i >= whole_blocks || none) {  // some of its keys are none, or not for every row
+          const bool cache = i < cached;
+          const int j0 = cache ? (blk0 + i) * B : (i - cached) * B, left = (cache ? t.len : t.nodes) - j0;
+          unsigned keys = left >= 32 ? ~0u : (1u << left) - 1;  // those that there are
+          keys &= ~((none & 1 ? 0xffffu : 0u) | (none & 2 ? 0xffff0000u : 0u));
+          unsigned seen = keys;
+          if (!cache) seen &= a.mask[static_cast<long long>(node) * a.words + (j0 >> 5)];
+          seen >>= 4 * hh;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) sc[j] = seen >> (8 * (j >> 2) + (j & 3)) & 1 ? sc[j] : -INFINITY;
+          // The values of the others cannot do harm: every wave clears them before it
+          // reads any (the waves write the same zeros, and none needs another's).
+          for (int e = lane; e < B * (kRow / 16); e += 64)
+            if (!(keys >> (e / (kRow / 16)) & 1))
+              *reinterpret_cast<ta_u32x4*>(ring + (i % kStages) * kStage + kHalf + e * 16) = ta_u32x4{0, 0, 0, 0};
+        }
+        ta_u32x4 kf[NK];  // of block i + 1 (behind the last block: a stage that nothing writes, for scores that go unused)
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) kf[kk] = k_frag(i + 1, kk);
+        raise(sc);
+        // In eight groups, held in this order by the scheduling barriers: two weights,
+        // a part of V^T's reads, a product of the next block's scores, and from the
+        // fifth on the products of the first 16 keys' weights. Left to itself the
+        // compiler waits for each fragment of K before its product and puts the
+        // exponentials behind all of them.
+        ta_u32x4 pf[2];  // P^T of keys 16 g + 4 hh .. + 3 and + 8 .. + 11
+        ta_u32x2 vt[4][ND];
+        auto pv = [&](int g, int db) {
+          o[db] = mfma32<F16>(ta_u32x4{vt[2 * g][db].x, vt[2 * g][db].y, vt[2 * g + 1][db].x, vt[2 * g + 1][db].y}, pf[g], o[db]);
+        };
+        next = ta_f32x16{};
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (g < NK) next = mfma32<F16>(kf[g], qf[g], next);
+          if (g >= 4 && g - 4 < ND) pv(0, g - 4);
+#pragma unroll
+          for (int e = g * ND / 2; e < (g + 1) * ND / 2; ++e) vt[e / ND][e % ND] = v_frag(i, e / ND, e % ND);
+          pf[g / 4][g % 4] = weights(sc, g);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int db = 0; db < ND; ++db) pv(1, db);
+      };
+      // Stages: i (V being read), i + 1 (K being read), i + 2 in flight, i + 3 being
+      // issued into the one that every wave has left.
+      auto turn = [&](int i, ta_f32x16& sc, ta_f32x16& next) {
+        if (i + 1 < n) {
+          if (i + 2 < n)
+            wait_stage<kLoads>();
+          else
+            wait_stage<0>();
+          __builtin_amdgcn_s_barrier();  // block i + 1 is there, and block i - 1's stage read by all
+          asm volatile("" ::: "memory");
+          if (i + kStages - 1 < n) issue(i + kStages - 1);
+        }
+        if (!idle) step(i, sc, next);
+      };
+      if (n >= 3)
+        wait_stage<2 * kLoads>();
+      else if (n == 2)
+        wait_stage<kLoads>();
+      else
+        wait_stage<0>();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      ta_f32x16 sa = {}, sb = {};
+      if (!idle)
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) sa = mfma32<F16>(k_frag(0, kk), qf[kk], sa);
+      for (int i = 0; i < n; i += 2) {
+        turn(i, sa, sb);
+        if (i + 1 < n) turn(i + 1, sb, sa);
       }
 
-      // The two halves of the keys meet: the upper waves hand theirs over, lane by lane.
       const bool whole = n == t.blocks;
-      const long long part = 2LL * blockIdx.x + (blk0 == 0 ? 1 : 0);
-      float x, y;
-      swap32(l, x, y);
-      l = x + y;
-      __syncthreads();  // the ring is free
-      ta_f32x4* give = reinterpret_cast<ta_f32x4*>(ring) + rg * ND * 4 * 64 + lane;
-      if (kh == 1) {
-        other_m[rg][lane] = m;
-        other_l[rg][lane] = l;
-#pragma unroll
-        for (int db = 0; db < ND; ++db)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) give[(db * 4 + q) * 64] = ta_f32x4{o[db][4 * q], o[db][4 * q + 1], o[db][4 * q + 2], o[db][4 * q + 3]};
-      }
-      __syncthreads();
-      if (kh == 0 && 32 * rg + c < rows) {
-        const float m1 = other_m[rg][lane], l1 = other_l[rg][lane], top = fmaxf(m, m1);
-        // a half that saw nothing has no maximum, and its sums count for nothing
-        const float f0 = __builtin_amdgcn_exp2f(m - top), f1 = __builtin_amdgcn_exp2f(m1 - top);
-        const float sum = (l == 0.f ? 0.f : f0 * l) + (l1 == 0.f ? 0.f : f1 * l1);
+      float l0, l1;
+      swap32(l, l0, l1);
+      const float sum = l0 + l1;
+      if (32 * w + c < rows) {
+        const long long part = (2LL * blockIdx.x + (blk0 == 0 ? 1 : 0)) * R + 32 * w + c;
         const float inv = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
-        const long long pr = part * R + 32 * rg + c;
-        if (!whole && hh == 0) a.part_ml[pr] = make_float2(top, sum);
+        if (!whole && hh == 0) a.part_ml[part] = make_float2(m - kLift<F16>, sum);
 #pragma unroll
         for (int db = 0; db < ND; ++db)
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const ta_f32x4 o1 = give[(db * 4 + q) * 64];
+            const int dim = 32 * db + 8 * q + 4 * hh;
             ta_f32x4 v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = ((l == 0.f ? 0.f : f0 * o[db][4 * q + e]) + (l1 == 0.f ? 0.f : f1 * o1[e])) * inv;
-            const int dim = 32 * db + 8 * q + 4 * hh;
+            for (int e = 0; e < 4; ++e) v[e] = sum == 0.f ? 0.f : o[db][4 * q + e] * inv;
             if (whole) {
               ta_u32x2 z;
               z.x = narrow<F16>(v[0]) | static_cast<unsigned>(narrow<F16>(v[1])) << 16;
               z.y = narrow<F16>(v[2]) | static_cast<unsigned>(narrow<F16>(v[3])) << 16;
               *reinterpret_cast<ta_u32x2*>(a.out + q_row * D + dim) = z;
             } else {
-              *reinterpret_cast<ta_f32x4*>(a.part_o + pr * D + dim) = v;
+              *reinterpret_cast<ta_f32x4*>(a.part_o + part * D + dim) = v;
             }
           }
       }
@@ -742,7 +785,7 @@ __global__ __launch_bounds__(512) void tree_wide_kernel(TreeArgs a) {
     u += stop - in_tile;
     if (u < end && u == base + t.units) {
       base += t.units;
-      do t = uniform_tiles_of<R>(a, ++s);
+      do t = uniform_tiles_of<R, B>(a, ++s);
       while (t.units == 0);
     }
   }
@@ -752,7 +795,7 @@ __global__ __launch_bounds__(512) void tree_wide_kernel(TreeArgs a) {
 // rows whose keys were shared out, and does over the rows that came out
 // infinite or NaN, one key at a time and only the keys that the row sees (a
 // product with a weight of zero lets what is not seen through).
-template <int D, bool F16, int R>
+template <int D, bool F16, int R, int B>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
   constexpr int E = D / 64, V4 = D / 4, NP = 64 / V4;  // parts added at a time
   __shared__ int owner;
@@ -768,7 +811,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
   __syncthreads();
   const int s = uniform(owner);
   if (s < 0 || h >= a.H) return;
-  const Tiles t = uniform_tiles_of<R>(a, s);
+  const Tiles t = uniform_tiles_of<R, B>(a, s);
   const int G = a.G, hk = h / G, row = (n - t.first) * G + (h - hk * G);
   const int chunk = uniform_word(a.prefix, a.num_seqs);
   const int u0 = uniform_word(a.prefix, s) + (hk * t.row_tiles + row / R) * t.tile_units() + kOver, u1 = u0 + t.blocks - 1;
@@ -877,8 +920,9 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
   for (int e = 0; e < E; ++e) out[lane * E + e] = narrow<F16>(sum == 0.f ? 0.f : o[e] / sum);
 }
 
-// Workgroups that fit the 256 CUs at once: LDS holds two rings of head_dim 64, one of 128.
-constexpr int resident(int D, int R) { return D == 64 && R <= 64 ? 512 : 256; }
+// Workgroups that fit the 256 CUs at once, by LDS (a ring takes 64 KiB with
+// head_dim 64 and 128 KiB with 128, in the kernel of many rows 32 and 64) and registers.
+constexpr int resident(int D, int R) { return (D == 64 ? 512 : 256) * (R == 128 ? 2 : 1); }
 
 // Row tiles of 16, 32, 64 or 128 rows.
 int rows_of_tile(int n_heads, int n_kv_heads, int max_nodes) {
@@ -889,7 +933,8 @@ int rows_of_tile(int n_heads, int n_kv_heads, int max_nodes) {
 // Units of work that there can be at most.
 long long most_units(int n_heads, int n_kv_heads, int num_seqs, int max_nodes, int max_pages, int page_size) {
   const int R = rows_of_tile(n_heads, n_kv_heads, max_nodes);
-  const long long blocks = (static_cast<long long>(max_pages) * page_size + kBlock - 1) / kBlock + (max_nodes + kBlock - 1) / kBlock;
+  const int B = R == 128 ? kWideBlock : kBlock;
+  const long long blocks = (static_cast<long long>(max_pages) * page_size + B - 1) / B + (max_nodes + B - 1) / B;
   const long long tiles = static_cast<long long>((max_nodes * (n_heads / n_kv_heads) + R - 1) / R) * n_kv_heads * num_seqs;
   return tiles * (blocks + kOver);
 }
@@ -901,7 +946,7 @@ int workgroups_of(int n_heads, int n_kv_heads, int head_dim, int num_seqs, int m
 template <int D, bool F16, int RT>
 void launch_tree(const TreeArgs& a, hipStream_t s) {
   IRON_LAUNCH((tree_attention_kernel<D, F16, RT>), dim3(a.workgroups), dim3(256), 0, s, a);
-  IRON_LAUNCH((tree_join_kernel<D, F16, 16 * RT>), dim3(a.num_nodes, (a.H + 3) / 4), dim3(256), 0, s, a);
+  IRON_LAUNCH((tree_join_kernel<D, F16, 16 * RT, kBlock>), dim3(a.num_nodes, (a.H + 3) / 4), dim3(256), 0, s, a);
 }
 
 template <int D, bool F16>
@@ -913,8 +958,8 @@ void launch_rows(const TreeArgs& a, int R, hipStream_t s) {
   else if (R == 64)
     launch_tree<D, F16, 4>(a, s);
   else {
-    IRON_LAUNCH((tree_wide_kernel<D, F16>), dim3(a.workgroups), dim3(512), 0, s, a);
-    IRON_LAUNCH((tree_join_kernel<D, F16, 128>), dim3(a.num_nodes, (a.H + 3) / 4), dim3(256), 0, s, a);
+    IRON_LAUNCH((tree_wide_kernel<D, F16>), dim3(a.workgroups), dim3(256), 0, s, a);
+    IRON_LAUNCH((tree_join_kernel<D, F16, 128, kWideBlock>), dim3(a.num_nodes, (a.H + 3) / 4), dim3(256), 0, s, a);
   }
 }
 
@@ -933,7 +978,7 @@ const char* check_shape(int n_heads, int n_kv_heads, int head_dim, int num_seqs,
   if (max_pages < 1 || static_cast<long long>(max_pages) * page_size >= (1LL << 31) - (1 << 20))
     return "max_pages: a sequence holds less than 2^31 - 2^20 positions";
   if (most_units(n_heads, n_kv_heads, num_seqs, max_nodes, max_pages, page_size) >= (1LL << 31))
-    return "num_seqs * max_pages * page_size * row tiles is too large: blocks of 64 keys must count below 2^31";
+    return "num_seqs * max_pages * page_size * row tiles is too large: blocks of 32 keys must count below 2^31";
   return nullptr;
 }
 

@@ -178,19 +178,21 @@ def free(cache, slots):
     return status
 
 
-def attention(q, k_new, v_new, k_pages, v_pages, table, lens, starts, sees, scale, prior):
+def attention(q, k_new, v_new, k_pages, v_pages, table, lens, starts, sees, scale, prior, max_nodes):
     """TreeAttention in 64 bits on CPU tensors, with the bound of its rounding: (out, tolerance), both float64.
 
     A score is a dot product of D terms in fp32, in any order: off by at most (D + 2) 2^-24 of the sum of the terms'
     sizes (times scale); its product with log2(e) and the subtraction of a maximum add 2^-22 of the largest score. A
-    weight is off by that, the exponential's 2^-22, and 2^-16 for the two parts that it goes into the second product
-    as; each shows in the sum of the weights too, hence twice. Sums of n terms in fp32 add n 2^-24. In fp16 a weight's
+    weight is off by that, the exponential's 2^-22, and its own rounding before the second product: 2^-16 for the two
+    parts that it goes in as, or, where a KV head has more than 64 rows (max_nodes times the heads of its group), half
+    a step of its type, as MHA rounds it; each shows in the sum of the weights too, hence twice. Sums of n terms in fp32 add n 2^-24. In fp16 a weight's
     lower part may lie under the normal range: n 2^-24 of the largest value. All of it is relative to sum(p |v|).
     The result is then rounded once: half a step of its type.
     """
     out, tol = prior.double().clone(), torch.zeros(prior.shape, dtype=torch.float64)
     D, ps = q.shape[-1], k_pages.shape[2]
     G, half = q.shape[1] // k_new.shape[1], torch.finfo(prior.dtype).eps / 2
+    weight = half if max_nodes * G > 64 else 2.0 ** -16
     for s, n in enumerate(lens):
         a, b = starts[s], starts[s + 1]
         pos = [t for t in range(n) if 0 <= table[s][t // ps] < k_pages.shape[0]]
@@ -209,7 +211,7 @@ def attention(q, k_new, v_new, k_pages, v_pages, table, lens, starts, sees, scal
                 out[i, h] = p @ v
                 size = float((k.abs() @ x.abs()).max()) * scale
                 each = (D + 2) * 2.0 ** -24 * size + 2.0 ** -22 * (1 + float(w.abs().max()) * 1.5)
-                rel = 2 * (each + 2.0 ** -16) + (len(k) + 8) * 2.0 ** -24
+                rel = 2 * (each + weight) + (len(k) + 8) * 2.0 ** -24
                 tol[i, h] = half * out[i, h].abs() + rel * (p @ v.abs()) * (1 + half)
                 if prior.dtype == torch.float16:
                     tol[i, h] += len(k) * 2.0 ** -24 * float(v.abs().max()) + 2.0 ** -25

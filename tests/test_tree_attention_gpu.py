@@ -61,7 +61,8 @@ class Case:
                 words.to(gpu), self.prior.to(gpu)]
 
     def want(self):
-        return ref.attention(self.q, self.kn, self.vn, self.kp, self.vp, self.table, self.lens, self.starts, self.sees, self.scale, self.prior)
+        return ref.attention(self.q, self.kn, self.vn, self.kp, self.vp, self.table, self.lens, self.starts, self.sees, self.scale, self.prior,
+                             self.op.max_nodes)
 
     def check(self, gpu, got=None):
         if got is None:
@@ -379,7 +380,7 @@ def test_a_conversation(gpu):
                     for x in (0, 1):
                         dense[x][s * 20 + t // 16, :, t % 16] = kv[x][l]
             table = [[s * 20 + e for e in range(20)] for s in range(S)]
-            want, tol = ref.attention(q[l], kn[l], vn[l], dense[0], dense[1], table, lens, starts, sees, 1 / math.sqrt(D), prior)
+            want, tol = ref.attention(q[l], kn[l], vn[l], dense[0], dense[1], table, lens, starts, sees, 1 / math.sqrt(D), prior, T)
             assert ((out.cpu().double() - want).abs() <= tol).all(), (l, nodes)
         return kn, vn, starts
 
