@@ -375,7 +375,7 @@ __global__ __launch_bounds__(kPlan) void fork_plan_kernel(ForkArgs a) {
       const int page = e < pages ? from[e] : -1;
       const bool real = e < pages && p.in_pool(page);
       const unsigned long long all = __ballot(real);
-      const int r = at + __popcll(all & ((1ull << lane) - 1));
+      const int r = at + __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(all >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(all), 0));
       if (real) {
         a.src[r] = page;
         a.rows[r] = min(ps, len - e * ps);

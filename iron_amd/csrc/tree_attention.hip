@@ -25,6 +25,7 @@ struct TreeArgs {
   float* part_o;      // workspace (2 x workgroups, R, D): sum(p v) of the parts of split tiles
   float2* part_ml;    // workspace (2 x workgroups, R): their maximum and sum(p)
   int* prefix;        // workspace (num_seqs + 1): units before each sequence; units of a workgroup
+  int* owner;         // workspace (num_nodes): the sequence of each node that is one
   int H, Hkv, G, num_pages, page_shift, num_seqs, max_pages, num_nodes, max_nodes, words, workgroups;
   float scale_log2;
 };
@@ -302,6 +303,8 @@ __global__ __launch_bounds__(256) void tree_attention_kernel(TreeArgs a) {
     const int hk = uniform(tile / t.row_tiles), row0 = (tile - hk * t.row_tiles) * R;
     const int rows = min(R, t.nodes * G - row0);
     if (n > 0) {
+    if (hk == 0 && blk0 == 0)  // for the launch that joins the parts
+      for (int i = row0 / G + tid; i <= (row0 + rows - 1) / G; i += 256) a.owner[t.first + i] = s;
     ta_u32x4 qf[RT][NK];
     int node[RT];
     ta_f32x4 o[RT][ND];
@@ -320,21 +323,26 @@ __global__ __launch_bounds__(256) void tree_attention_kernel(TreeArgs a) {
       const int blk = min(blk0 + i, t.cached - 1);
       return t.cached ? uniform_word(a.table, table + (min(blk * kBlock + 16 * w, t.len - 1) >> a.page_shift)) : 0;
     };
-    int page = page_of(0);
+    // the pages of the blocks that are issued next, read ahead: one round trip for the first ones
+    int page[kStages];
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) page[i] = page_of(i);
     auto issue = [&](int i) {
       unsigned char* st = ring + (i % kStages) * kStage;
       const int blk = blk0 + i;
       if (blk < t.cached) {
-        const bool real = static_cast<unsigned>(page) < static_cast<unsigned>(a.num_pages);
+        const bool real = static_cast<unsigned>(page[0]) < static_cast<unsigned>(a.num_pages);
         holes = (holes & ~(1u << (i % kStages))) | (real ? 0u : 1u << (i % kStages));
-        const long long at = ((static_cast<long long>(real ? page : 0) * a.Hkv + hk) * ps + ((blk * kBlock + 16 * w) & (ps - 1))) * D;
+        const long long at = ((static_cast<long long>(real ? page[0] : 0) * a.Hkv + hk) * ps + ((blk * kBlock + 16 * w) & (ps - 1))) * D;
         const i32x4v rk = buffer_rsrc(a.k_pages + at), rv = buffer_rsrc(a.v_pages + at);
 #pragma unroll
         for (int j = 0; j < kLoads / 2; ++j) {
           load_lds16(rk, lrow[j] * kRow + kchunk[j], st + j * 1024);
           load_lds16(rv, lrow[j] * kRow + vchunk[j], st + kHalf + j * 1024);
         }
-        page = page_of(i + 1);
+#pragma unroll
+        for (int j = 0; j + 1 < kStages; ++j) page[j] = page[j + 1];
+        page[kStages - 1] = page_of(i + kStages);
       } else {
         const int j0 = (blk - t.cached) * kBlock + 16 * w;
         const long long at = (static_cast<long long>(t.first) * a.Hkv + hk) * D;
@@ -568,6 +576,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void tree_wide_kernel(TreeArg
     const int hk = uniform(tile / t.row_tiles), row0 = (tile - hk * t.row_tiles) * R;
     const int rows = min(R, t.nodes * G - row0);
     if (n > 0) {
+      if (hk == 0 && blk0 == 0)  // for the launch that joins the parts
+        for (int i = row0 / G + tid; i <= (row0 + rows - 1) / G; i += 256) a.owner[t.first + i] = s;
       const int* table = a.table + static_cast<long long>(s) * a.max_pages;
       const int cached = t.cached - blk0;                       // blocks of this part that are the cache's (the rest are the tree's)
       const int whole_blocks = t.len / B - blk0;                // the first ones of them, with no key behind the last
@@ -577,23 +587,24 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void tree_wide_kernel(TreeArg
       const long long tree = (static_cast<long long>(t.first) * a.Hkv + hk) * kRow;
       const unsigned new_row = static_cast<unsigned>(a.Hkv) * kRow;
       unsigned holes = 0;  // bits 2 (i % kStages) and + 1: the two pages of block i's 16 rows each are none
-      int page0, page1;    // of the block to be issued next
-      auto pages_of = [&](int i) {
+      // the pages of the blocks that are issued next, read ahead: one round trip for the first ones
+      int page0[kStages] = {}, page1[kStages] = {};
+      auto pages_of = [&](int i, int& p0, int& p1) {
         if (cached <= 0) return;
         const int pos = (blk0 + min(i, cached - 1)) * B;
-        page0 = uniform_word(table, min(pos, t.len - 1) >> a.page_shift);
-        page1 = uniform_word(table, min(pos + 16, t.len - 1) >> a.page_shift);
+        p0 = uniform_word(table, pos >> a.page_shift);
+        p1 = uniform_word(table, min(pos + 16, t.len - 1) >> a.page_shift);
       };
-      page0 = page1 = 0;
-      pages_of(0);
+#pragma unroll
+      for (int i = 0; i < kStages; ++i) pages_of(i, page0[i], page1[i]);
       auto issue = [&](int i) {
         const int stage = i % kStages;
         unsigned char* st = ring + stage * kStage + 8 * w * kRow;
         if (i < cached) {
-          const bool none0 = static_cast<unsigned>(page0) >= static_cast<unsigned>(a.num_pages);
-          const bool none1 = static_cast<unsigned>(page1) >= static_cast<unsigned>(a.num_pages);
+          const bool none0 = static_cast<unsigned>(page0[0]) >= static_cast<unsigned>(a.num_pages);
+          const bool none1 = static_cast<unsigned>(page1[0]) >= static_cast<unsigned>(a.num_pages);
           holes = (holes & ~(3u << (2 * stage))) | ((none0 ? 1u : 0u) | (none1 ? 2u : 0u)) << (2 * stage);
-          const unsigned page = w < 2 ? (none0 ? 0 : page0) : (none1 ? 0 : page1);
+          const unsigned page = w < 2 ? (none0 ? 0 : page0[0]) : (none1 ? 0 : page1[0]);
           // from the page's row of the block's first key: row 8 w is in the page, whatever page the first is in
           const int in_page = (((blk0 + i) * B + 8 * w) & (ps - 1)) - 8 * w;
           const long long at = static_cast<long long>(static_cast<unsigned long long>(page) * page_bytes) + in_page * kRow;
@@ -603,7 +614,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void tree_wide_kernel(TreeArg
             load_lds16(rk, krow[j] * kRow + kat[j], st + j * 1024);
             load_lds16(rv, krow[j] * kRow + vat[j], st + kHalf + j * 1024);
           }
-          pages_of(i + 1);
+#pragma unroll
+          for (int j = 0; j + 1 < kStages; ++j) {
+            page0[j] = page0[j + 1];
+            page1[j] = page1[j + 1];
+          }
+          pages_of(i + kStages, page0[kStages - 1], page1[kStages - 1]);
         } else {
           const int j0 = (i - cached) * B;
           holes &= ~(3u << (2 * stage));
@@ -798,23 +814,15 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void tree_wide_kernel(TreeArg
 template <int D, bool F16, int R, int B>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
   constexpr int E = D / 64, V4 = D / 4, NP = 64 / V4;  // parts added at a time
-  __shared__ int owner;
   const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
   const int n = blockIdx.x, h = blockIdx.y * 4 + w;
-  if (tid == 0) owner = -1;
-  __syncthreads();
-  for (int s = tid; s < a.num_seqs; s += 256) {
-    int first, nodes;
-    tree_of(a, s, first, nodes);
-    if (first <= n && n < first + nodes) atomicMax(&owner, s);
-  }
-  __syncthreads();
-  const int s = uniform(owner);
-  if (s < 0 || h >= a.H) return;
+  const int s = uniform_word(a.owner, n);  // anything where no workgroup wrote it: checked like any number
+  if (static_cast<unsigned>(s) >= static_cast<unsigned>(a.num_seqs) || h >= a.H) return;
   const Tiles t = uniform_tiles_of<R, B>(a, s);
+  const int chunk = uniform_word(a.prefix, a.num_seqs), before = uniform_word(a.prefix, s);
+  if (n < t.first || n >= t.first + t.nodes) return;
   const int G = a.G, hk = h / G, row = (n - t.first) * G + (h - hk * G);
-  const int chunk = uniform_word(a.prefix, a.num_seqs);
-  const int u0 = uniform_word(a.prefix, s) + (hk * t.row_tiles + row / R) * t.tile_units() + kOver, u1 = u0 + t.blocks - 1;
+  const int u0 = before + (hk * t.row_tiles + row / R) * t.tile_units() + kOver, u1 = u0 + t.blocks - 1;
   const int b0 = u0 / chunk, b1 = u1 / chunk;
   uint16_t* out = a.out + (static_cast<long long>(n) * a.H + h) * D;
   bool again = false;
@@ -825,31 +833,33 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
     const long long r = row % R;
     auto slot = [&](int i) { return (2LL * (b0 + i) + (i == 0)) * R + r; };
     float2 ml = lane < parts ? a.part_ml[slot(lane)] : make_float2(-INFINITY, 0.f);
+    const int g = lane / V4;
+    constexpr int kAhead = 8;  // loads in flight
+    ta_f32x4 x[kAhead];
+    auto load = [&](int i) {  // parts i + g, i + g + NP, ..
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) x[k] = *reinterpret_cast<const ta_f32x4*>(a.part_o + slot(min(i + k * NP + g, parts - 1)) * D + (lane % V4) * 4);
+    };
+    load(0);  // with the maxima: one round trip for most rows
     float top = ml.x;
     for (int i = 64 + lane; i < parts; i += 64) top = fmaxf(top, a.part_ml[slot(i)].x);
     top = wave_max(top);
     float sum = 0.f;
     ta_f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    const int g = lane / V4;
     for (int i0 = 0; i0 < parts; i0 += 64) {
       if (i0) ml = i0 + lane < parts ? a.part_ml[slot(i0 + lane)] : make_float2(-INFINITY, 0.f);
-      // the weight of part i0 + lane; a part that saw nothing has none
-      const float f = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);
+      // the weight of part i0 + lane, 0 for a part that saw nothing; one too small
+      // for fp32 is not: it keeps an infinity one
+      const float f = ml.y == 0.f ? 0.f : fmaxf(__builtin_amdgcn_exp2f(ml.x - top), 1.17549435e-38f);
       sum += ml.y == 0.f ? 0.f : f * ml.y;
-      const unsigned long long some = __ballot(ml.y != 0.f);
-      constexpr int kAhead = 8;  // loads in flight
       for (int i = 0; i < min(parts - i0, 64); i += kAhead * NP) {
-        ta_f32x4 x[kAhead];
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k)
-          x[k] = *reinterpret_cast<const ta_f32x4*>(a.part_o + slot(min(i0 + i + k * NP + g, parts - 1)) * D + (lane % V4) * 4);
+        if (i0 + i) load(i0 + i);
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
           const int j = i + k * NP + g;
           const float fj = __shfl(f, j, 64);
-          const bool add = j < 64 && (some >> j & 1);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] += add ? fj * x[k][e] : 0.f;
+          for (int e = 0; e < 4; ++e) v[e] += fj == 0.f ? 0.f : fj * x[k][e];
         }
       }
     }
@@ -921,8 +931,8 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
 }
 
 // Workgroups that fit the 256 CUs at once, by LDS (a ring takes 64 KiB with
-// head_dim 64 and 128 KiB with 128, in the kernel of many rows 32 and 64) and registers.
-constexpr int resident(int D, int R) { return (D == 64 ? 512 : 256) * (R == 128 ? 2 : 1); }
+// head_dim 64 and 128 KiB with 128) and, in the kernel of many rows, by registers.
+constexpr int resident(int D, int R) { return R == 128 ? (D == 64 ? 768 : 512) : (D == 64 ? 512 : 256); }
 
 // Row tiles of 16, 32, 64 or 128 rows.
 int rows_of_tile(int n_heads, int n_kv_heads, int max_nodes) {
@@ -992,7 +1002,7 @@ extern "C" long long iron_tree_attention_workspace_bytes(int n_heads, int n_kv_h
   if (check_shape(n_heads, n_kv_heads, head_dim, num_seqs, num_nodes, max_nodes, max_pages, page_size)) return -1;
   const long long slots = 2LL * workgroups_of(n_heads, n_kv_heads, head_dim, num_seqs, max_nodes, max_pages, page_size) *
                           rows_of_tile(n_heads, n_kv_heads, max_nodes);
-  return slots * head_dim * 4 + slots * 8 + (num_seqs + 1) * 4;
+  return slots * head_dim * 4 + slots * 8 + (num_seqs + 1 + num_nodes) * 4LL;
 }
 
 extern "C" int iron_tree_attention(const void* q, const void* k_new, const void* v_new, const void* k_pages,
@@ -1044,6 +1054,7 @@ extern "C" int iron_tree_attention(const void* q, const void* k_new, const void*
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + slots * head_dim);
   a.prefix = reinterpret_cast<int*>(a.part_ml + slots);
+  a.owner = a.prefix + num_seqs + 1;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (head_dim == 64)
     dtype ? launch_rows<64, true>(a, R, s) : launch_rows<64, false>(a, R, s);
