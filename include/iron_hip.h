@@ -431,7 +431,7 @@ int iron_page_compact(void* k_pages, void* v_pages, int* page_table, int* seq_le
                       int max_pages, void* workspace, long long workspace_bytes, void* stream);
 
 /* The sequences slots[0 .. num_slots) give their pages back: page_refs of each
- * drops by one (never below 0), the table entries become -1, the length 0.
+ * drops by one (0 stays 0), the table entries become -1, the length 0.
  * status (num_slots <= 8192); of entries that name one slot the first counts. */
 int iron_page_free(const int* slots, int* page_table, int* seq_lens, int* page_refs, int* status, int num_pages,
                    int page_size, int num_seqs, int max_pages, int num_slots, void* stream);

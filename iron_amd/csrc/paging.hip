@@ -51,23 +51,23 @@ struct Pool {
 };
 
 // Exclusive prefix sum over the workgroup's NT threads; total to every thread.
-// tmp: NT / 64 ints of LDS. Every thread calls it.
-template <int NT>
-__device__ __forceinline__ int block_scan(int x, int* tmp, int& total) {
+// tmp: NT / 64 values of LDS. Every thread calls it.
+template <int NT, typename T>
+__device__ __forceinline__ T block_scan(T x, T* tmp, T& total) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  int incl = x;
+  T incl = x;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
-    const int y = __shfl_up(incl, d, 64);
+    const T y = __shfl_up(incl, d, 64);
     if (lane >= d) incl += y;
   }
   __syncthreads();  // tmp is free: every thread has left an earlier call
   if (lane == 63) tmp[w] = incl;
   __syncthreads();
-  int base = 0, sum = 0;
+  T base = 0, sum = 0;
 #pragma unroll
   for (int i = 0; i < NT / 64; ++i) {
-    const int y = tmp[i];
+    const T y = tmp[i];
     base += i < w ? y : 0;
     sum += y;
   }
@@ -110,7 +110,7 @@ __device__ int find_free(const int* refs, int num_pages, int want, int* list, in
         if (p0 + j < num_pages && refs[p0 + j] == 0) zeros |= 1u << j;
     }
     int total;
-    int r = found + block_scan<kPlan>(__popc(zeros), tmp, total);
+    int r = found + block_scan<kPlan>(static_cast<int>(__popc(zeros)), tmp, total);
     while (zeros && r < want) {
       const int j = __ffs(zeros) - 1;
       zeros &= zeros - 1;
@@ -423,7 +423,7 @@ struct CompactArgs {
   int* counts;  // workspace (segments): pages in use
   int* src;     // workspace (num_pages / 2 + 1): pages in use at or above their number, ascending
   int* dst;     // workspace (num_pages / 2 + 1): free pages below it, ascending
-  int* rank;    // workspace (num_pages): index into src of a page at or above it, or -1
+  int* rank;    // workspace (num_pages, to a multiple of 4): index into src of a page at or above it, or -1
   int* head;    // workspace (2): pages to move, pages in use
   int segments;
 };
@@ -448,7 +448,7 @@ __device__ __forceinline__ unsigned used_mask(const int* refs, int base, int num
 __global__ __launch_bounds__(256) void compact_count_kernel(CompactArgs a) {
   __shared__ int tmp[4];
   int total;
-  block_scan<256>(__popc(used_mask(a.pool.refs, blockIdx.x * kSegment + threadIdx.x * 16, a.pool.num_pages)), tmp, total);
+  block_scan<256>(static_cast<int>(__popc(used_mask(a.pool.refs, blockIdx.x * kSegment + threadIdx.x * 16, a.pool.num_pages))), tmp, total);
   if (threadIdx.x == 0) a.counts[blockIdx.x] = total;
 }
 
@@ -456,42 +456,46 @@ __global__ __launch_bounds__(256) void compact_count_kernel(CompactArgs a) {
 // both in ascending order: as few moves as there can be, and a source is never
 // a destination.
 __global__ __launch_bounds__(256) void compact_list_kernel(CompactArgs a) {
-  __shared__ int tmp[4];
+  __shared__ long long tmp[4];
   const int P = a.pool.num_pages, seg = blockIdx.x;
-  int mine = 0, all = 0, before, used;
+  const int b = seg * kSegment + threadIdx.x * 16;
+  const unsigned m = used_mask(a.pool.refs, b, P);
+  // two sums at a time, in the halves of one: all pages in use (below 2^28), and those of the segments before this one
+  long long x = 0, sums;
   for (int i = threadIdx.x; i < a.segments; i += 256) {
     const int c = a.counts[i];
-    all += c;
-    mine += i < seg ? c : 0;
+    x += static_cast<long long>(c) << 32 | (i < seg ? c : 0);
   }
-  block_scan<256>(all, tmp, used);
-  block_scan<256>(mine, tmp, before);
+  block_scan<256>(x, tmp, sums);
+  const int used = static_cast<int>(sums >> 32), before = static_cast<int>(sums & 0xffffffff);
   const int cut = used / kSegment;  // the segment of page `used`
-  int under = 0, below;
+  int under = 0;
   for (int i = threadIdx.x; i < cut; i += 256) under += a.counts[i];
   const int cb = cut * kSegment + threadIdx.x * 16;
   const int inside = min(max(used - cb, 0), 16);
   under += __popc(used_mask(a.pool.refs, cb, P) & ((1u << inside) - 1));
-  block_scan<256>(under, tmp, below);  // pages in use below page `used`
+  x = block_scan<256>(static_cast<long long>(under) << 32 | static_cast<long long>(__popc(m)), tmp, sums);
+  const int below = static_cast<int>(sums >> 32);                          // pages in use below page `used`
+  int at = before + static_cast<int>(x & 0xffffffff);                      // pages in use before page b + j
   if (seg == 0 && threadIdx.x == 0) {
     a.head[0] = used - below;
     a.head[1] = used;
     a.moved[0] = used - below;
   }
-  const int b = seg * kSegment + threadIdx.x * 16;
-  const unsigned m = used_mask(a.pool.refs, b, P);
-  int total;
-  int at = before + block_scan<256>(__popc(m), tmp, total);  // pages in use before page b + j
-  for (int j = 0; j < 16 && b + j < P; ++j) {
-    const bool live = m >> j & 1;
-    if (b + j >= used) {
-      a.rank[b + j] = live ? at - below : -1;
-      if (live) a.src[at - below] = b + j;
-    } else if (!live) {
-      a.dst[b + j - at] = b + j;
+  int rank[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const bool live = m >> j & 1, high = b + j >= used;
+    rank[j] = live && high ? at - below : -1;
+    if (b + j < P) {
+      if (live && high) a.src[at - below] = b + j;
+      if (!live && !high) a.dst[b + j - at] = b + j;
     }
     at += live;
   }
+  if (b + 16 > used)  // ranks of lower pages are not asked for
+    for (int j = 0; j < 16; j += 4)
+      if (b + j < P) *reinterpret_cast<int4*>(a.rank + b + j) = make_int4(rank[j], rank[j + 1], rank[j + 2], rank[j + 3]);
 }
 
 // Workgroups [0, copy_blocks) move the pages; the others each rename the pages
@@ -523,33 +527,65 @@ __global__ __launch_bounds__(256) void compact_move_kernel(CompactArgs a, int co
 }
 
 // -------------------------------------------------------------------- free ----
-__global__ __launch_bounds__(kPlan) void free_kernel(Pool p, const int* slots, int* status) {
-  const int i = blockIdx.x, s = slots[i];
-  const bool real = static_cast<unsigned>(s) < static_cast<unsigned>(p.num_seqs);
-  bool again = false;  // an earlier entry of the list names the slot
-  for (int j = threadIdx.x; j < i; j += kPlan) again |= slots[j] == s;
-  if (__syncthreads_or(again) || !real) {
-    if (threadIdx.x == 0) status[i] = PAGE_INVALID;
-    return;
-  }
-  const int len = p.lens[s];
-  __syncthreads();  // everyone has read the length
-  if (!p.len_fits(len)) {
-    if (threadIdx.x == 0) status[i] = PAGE_INVALID;
-    return;
-  }
-  if (threadIdx.x == 0) {
-    status[i] = PAGE_DONE;
-    p.lens[s] = 0;
-  }
+constexpr int kFreeEntries = 2048;  // table entries a workgroup of 256 handles
+
+struct FreeArgs {
+  Pool pool;
+  const int* slots;
+  int* status;
+  int parts;  // workgroups to a slot
+};
+
+// The sequence that entry i of the list ends, or -1: it names none, or one that an earlier entry names.
+__device__ __forceinline__ int ended(const FreeArgs& a, int i, int& len) {
+  const int s = a.slots[i];
+  const bool real = static_cast<unsigned>(s) < static_cast<unsigned>(a.pool.num_seqs);
+  len = real ? a.pool.lens[s] : -1;
+  bool again = false;
+  for (int j = threadIdx.x; j < i; j += 256) again |= a.slots[j] == s;
+  return __syncthreads_or(again) || !a.pool.len_fits(len) ? -1 : s;
+}
+
+__device__ __forceinline__ void end_slot(const FreeArgs& a, int i, int s) {
+  a.status[i] = s < 0 ? PAGE_INVALID : PAGE_DONE;
+  if (s >= 0) a.pool.lens[s] = 0;
+}
+
+// Part y of slot x's table entries. With one part to a slot the length goes to
+// 0 here (the barrier in ended() is behind every read of it); with more a second
+// launch does that, as the other parts may not have read it yet.
+__global__ __launch_bounds__(256) void free_kernel(FreeArgs a) {
+  const Pool& p = a.pool;
+  const int i = blockIdx.x;
+  int len;
+  const int s = ended(a, i, len);
+  if (a.parts == 1 && threadIdx.x == 0) end_slot(a, i, s);
+  if (s < 0) return;
   int* row = p.table + static_cast<long long>(s) * p.max_pages;
-  const int pages = p.pages_of(len);
-  for (int e = threadIdx.x; e < pages; e += kPlan) {
-    const int page = row[e];
-    row[e] = -1;
-    // a count never goes below zero: what is taken off one that is already there is put back
-    if (p.in_pool(page) && atomicSub(p.refs + page, 1) <= 0) atomicAdd(p.refs + page, 1);
+  const int pages = p.pages_of(len), e0 = blockIdx.y * kFreeEntries + threadIdx.x;
+  int page[kFreeEntries / 256], refs[kFreeEntries / 256];
+#pragma unroll
+  for (int k = 0; k < kFreeEntries / 256; ++k) page[k] = e0 + 256 * k < pages ? row[e0 + 256 * k] : -1;
+#pragma unroll
+  for (int k = 0; k < kFreeEntries / 256; ++k) refs[k] = p.in_pool(page[k]) ? p.refs[page[k]] : 0;
+#pragma unroll
+  for (int k = 0; k < kFreeEntries / 256; ++k) {
+    if (e0 + 256 * k < pages) row[e0 + 256 * k] = -1;
+    // A page whose count is 1 is held here alone: nobody else changes it. A count
+    // that was read too early is too high, and the others' are taken off atomically
+    // (a random 4-byte atomic crosses the chip: 355,000 pages, one in six of them
+    // shared, 24 us with an atomic for each, 20 with plain stores where they do).
+    if (refs[k] == 1)
+      p.refs[page[k]] = 0;
+    else if (refs[k] > 1)
+      atomicSub(p.refs + page[k], 1);
   }
+}
+
+__global__ __launch_bounds__(256) void free_lens_kernel(FreeArgs a) {
+  int len;
+  const int s = ended(a, blockIdx.x, len);
+  if (threadIdx.x == 0) end_slot(a, blockIdx.x, s);
 }
 
 // -------------------------------------------------------------------- host ----
@@ -745,7 +781,14 @@ extern "C" int iron_page_free(const int* slots, int* page_table, int* seq_lens, 
   if (int rc = check_pool(who, page_table, seq_lens, page_refs, status, num_pages, page_size, num_seqs, max_pages)) return rc;
   IRON_REQUIRE(slots && (reinterpret_cast<uintptr_t>(slots) & 3u) == 0, "%s: slots must be given and 4-byte aligned", who);
   IRON_REQUIRE(num_slots >= 1 && num_slots <= kMaxRequests, "%s: num_slots=%d outside [1, %d]", who, num_slots, kMaxRequests);
-  const Pool p = make_pool(nullptr, nullptr, page_table, seq_lens, page_refs, 0, 0, 16, num_pages, page_size, num_seqs, max_pages);
-  IRON_LAUNCH(free_kernel, dim3(num_slots), dim3(kPlan), 0, static_cast<hipStream_t>(stream), p, slots, status);
+  FreeArgs a;
+  a.pool = make_pool(nullptr, nullptr, page_table, seq_lens, page_refs, 0, 0, 16, num_pages, page_size, num_seqs, max_pages);
+  a.slots = slots;
+  a.status = status;
+  a.parts = (max_pages + kFreeEntries - 1) / kFreeEntries;
+  IRON_REQUIRE(a.parts <= 65535, "%s: max_pages=%d: at most %d table entries to a sequence", who, max_pages, 65535 * kFreeEntries);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  IRON_LAUNCH(free_kernel, dim3(num_slots, a.parts), dim3(256), 0, s, a);
+  if (a.parts > 1) IRON_LAUNCH(free_lens_kernel, dim3(num_slots), dim3(256), 0, s, a);
   return check_launch("page_free");
 }

@@ -164,7 +164,10 @@ __device__ __forceinline__ int wave_scan(int x) {
 // ending it, then one for each block of B keys: the cache's, then the tree's.
 // Units are numbered sequence by sequence, and workgroup b takes units
 // [b * chunk, (b + 1) * chunk): every workgroup gets the same share, however
-// ragged the lengths. The host sees to it that all units count in 31 bits.
+// ragged the lengths; no fewer than 2 units (6 of the kernel of many rows), as
+// more parts cost the join more than they save (one token behind 2047, smallest
+// share 1, 2, 4, 8: 9.2, 8.6, 9.5, 11.3 us; 240 rows behind 2000 with 1, 4, 6, 8:
+// 22.6, 18.0, 16.7, 18.4). The host sees to it that all units count in 31 bits.
 constexpr int kOver = 3;
 
 struct Tiles {
@@ -212,7 +215,7 @@ __device__ __forceinline__ bool share_of(const TreeArgs& a, int b, Share& sh) {
       mine += t.units;
     }
   const int incl = wave_scan(mine), total = __builtin_amdgcn_readlane(incl, 63);
-  const int chunk = max(static_cast<int>((static_cast<unsigned>(total) + a.workgroups - 1) / a.workgroups), 1);
+  const int chunk = max(static_cast<int>((static_cast<unsigned>(total) + a.workgroups - 1) / a.workgroups), R == 128 ? 6 : 2);
   int at = incl - mine;
   if (b == 0 && threadIdx.x < 64) {  // for the launch that joins the parts
     int before = at;
@@ -934,10 +937,15 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
 // head_dim 64 and 128 KiB with 128) and, in the kernel of many rows, by registers.
 constexpr int resident(int D, int R) { return R == 128 ? (D == 64 ? 768 : 512) : (D == 64 ? 512 : 256); }
 
-// Row tiles of 16, 32, 64 or 128 rows.
+// Row tiles of 16, 32 or 128 rows. The kernel that splits a block's keys over
+// its waves also ran tiles of 64, which lost to the kernel of many rows from 33
+// rows on (40 rows behind 37-3968 positions, 8 sequences: 18.1 against 16.4 us;
+// 64 rows behind 1000-3968, 16 sequences: 32.2 against 28.7; head_dim 128, 40 rows,
+// 4 sequences: 24.5 against 21.1); at 17 to 32 rows the two are equal (23.6 against
+// 24.3, head_dim 128 42.2 against 42.0) and this one keeps the weights' 16 bits.
 int rows_of_tile(int n_heads, int n_kv_heads, int max_nodes) {
   const int rows = max_nodes * (n_heads / n_kv_heads);
-  return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+  return rows <= 16 ? 16 : rows <= 32 ? 32 : 128;
 }
 
 // Units of work that there can be at most.
@@ -965,8 +973,6 @@ void launch_rows(const TreeArgs& a, int R, hipStream_t s) {
     launch_tree<D, F16, 1>(a, s);
   else if (R == 32)
     launch_tree<D, F16, 2>(a, s);
-  else if (R == 64)
-    launch_tree<D, F16, 4>(a, s);
   else {
     IRON_LAUNCH((tree_wide_kernel<D, F16>), dim3(a.workgroups), dim3(256), 0, s, a);
     IRON_LAUNCH((tree_join_kernel<D, F16, 128, kWideBlock>), dim3(a.num_nodes, (a.H + 3) / 4), dim3(256), 0, s, a);

@@ -1,7 +1,7 @@
 """PageFree: sequences of a paged KV cache give their pages back (new operator).
 
-Every page of each listed sequence loses one count in page_refs (never below 0;
-at 0 it is free: pages that a fork shares stay until the last holder lets go),
+Every page of each listed sequence loses one count in page_refs (0 stays 0; at
+0 it is free: pages that a fork shares stay until the last holder lets go),
 its table entries become -1 and its length 0.
 
 Arg spec: slots (num_slots,) int32, page_table (num_seqs, max_pages), seq_lens

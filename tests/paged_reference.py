@@ -184,7 +184,7 @@ def attention(q, k_new, v_new, k_pages, v_pages, table, lens, starts, sees, scal
     A score is a dot product of D terms in fp32, in any order: off by at most (D + 2) 2^-24 of the sum of the terms'
     sizes (times scale); its product with log2(e) and the subtraction of a maximum add 2^-22 of the largest score. A
     weight is off by that, the exponential's 2^-22, and its own rounding before the second product: 2^-16 for the two
-    parts that it goes in as, or, where a KV head has more than 64 rows (max_nodes times the heads of its group), half
+    parts that it goes in as, or, where a KV head has more than 32 rows (max_nodes times the heads of its group), half
     a step of its type, as MHA rounds it; each shows in the sum of the weights too, hence twice. Sums of n terms in fp32 add n 2^-24. In fp16 a weight's
     lower part may lie under the normal range: n 2^-24 of the largest value. All of it is relative to sum(p |v|).
     The result is then rounded once: half a step of its type.
@@ -192,7 +192,7 @@ def attention(q, k_new, v_new, k_pages, v_pages, table, lens, starts, sees, scal
     out, tol = prior.double().clone(), torch.zeros(prior.shape, dtype=torch.float64)
     D, ps = q.shape[-1], k_pages.shape[2]
     G, half = q.shape[1] // k_new.shape[1], torch.finfo(prior.dtype).eps / 2
-    weight = half if max_nodes * G > 64 else 2.0 ** -16
+    weight = half if max_nodes * G > 32 else 2.0 ** -16
     for s, n in enumerate(lens):
         a, b = starts[s], starts[s + 1]
         pos = [t for t in range(n) if 0 <= table[s][t // ps] < k_pages.shape[0]]
