@@ -452,6 +452,25 @@ __global__ __launch_bounds__(256) void compact_count_kernel(CompactArgs a) {
   if (threadIdx.x == 0) a.counts[blockIdx.x] = total;
 }
 
+// Lists pages b .. b + 15 (mask m: those in use; `at`: pages in use before them).
+__device__ __forceinline__ void list_pages(const CompactArgs& a, unsigned m, int b, int at, int used, int below) {
+  const int P = a.pool.num_pages;
+  int rank[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const bool live = m >> j & 1, high = b + j >= used;
+    rank[j] = live && high ? at - below : -1;
+    if (b + j < P) {
+      if (live && high) a.src[at - below] = b + j;
+      if (!live && !high) a.dst[b + j - at] = b + j;
+    }
+    at += live;
+  }
+  if (b + 16 > used)  // ranks of lower pages are not asked for
+    for (int j = 0; j < 16; j += 4)
+      if (b + j < P) *reinterpret_cast<int4*>(a.rank + b + j) = make_int4(rank[j], rank[j + 1], rank[j + 2], rank[j + 3]);
+}
+
 // With L pages in use, those at or above page L go to the free ones below it,
 // both in ascending order: as few moves as there can be, and a source is never
 // a destination.
@@ -482,20 +501,28 @@ __global__ __launch_bounds__(256) void compact_list_kernel(CompactArgs a) {
     a.head[1] = used;
     a.moved[0] = used - below;
   }
-  int rank[16];
-#pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const bool live = m >> j & 1, high = b + j >= used;
-    rank[j] = live && high ? at - below : -1;
-    if (b + j < P) {
-      if (live && high) a.src[at - below] = b + j;
-      if (!live && !high) a.dst[b + j - at] = b + j;
-    }
-    at += live;
+  list_pages(a, m, b, at, used, below);
+}
+
+// Count and list in one launch of one workgroup, 16 pages to a thread: for pools
+// of up to 16384 pages (4,436 pages, few moves, whole call: 11.7 us against 13.7
+// with two launches; four rounds of it at 62,000 pages 21.7 against 15.8).
+constexpr int kPlanPages = kPlan * 16;
+
+__global__ __launch_bounds__(kPlan) void compact_plan_kernel(CompactArgs a) {
+  __shared__ int tmp[kPlan / 64];
+  const int b = threadIdx.x * 16;
+  const unsigned m = used_mask(a.pool.refs, b, a.pool.num_pages);
+  int used, below;
+  const int at = block_scan<kPlan>(static_cast<int>(__popc(m)), tmp, used);
+  const int inside = min(max(used - b, 0), 16);
+  block_scan<kPlan>(static_cast<int>(__popc(m & ((1u << inside) - 1))), tmp, below);  // pages in use below page `used`
+  if (threadIdx.x == 0) {
+    a.head[0] = used - below;
+    a.head[1] = used;
+    a.moved[0] = used - below;
   }
-  if (b + 16 > used)  // ranks of lower pages are not asked for
-    for (int j = 0; j < 16; j += 4)
-      if (b + j < P) *reinterpret_cast<int4*>(a.rank + b + j) = make_int4(rank[j], rank[j + 1], rank[j + 2], rank[j + 3]);
+  if (used > below) list_pages(a, m, b, at, used, below);
 }
 
 // Workgroups [0, copy_blocks) move the pages; the others each rename the pages
@@ -768,8 +795,12 @@ extern "C" int iron_page_compact(void* k_pages, void* v_pages, int* page_table, 
   a.dst = a.src + round4(num_pages / 2 + 1);
   a.rank = a.dst + round4(num_pages / 2 + 1);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  IRON_LAUNCH(compact_count_kernel, dim3(a.segments), dim3(256), 0, s, a);
-  IRON_LAUNCH(compact_list_kernel, dim3(a.segments), dim3(256), 0, s, a);
+  if (num_pages <= kPlanPages) {
+    IRON_LAUNCH(compact_plan_kernel, dim3(1), dim3(kPlan), 0, s, a);
+  } else {
+    IRON_LAUNCH(compact_count_kernel, dim3(a.segments), dim3(256), 0, s, a);
+    IRON_LAUNCH(compact_list_kernel, dim3(a.segments), dim3(256), 0, s, a);
+  }
   const int copy_blocks = static_cast<int>(std::min<long long>(kCopyBlocks, static_cast<long long>(num_pages) * num_layers));
   IRON_LAUNCH(compact_move_kernel, dim3(copy_blocks + num_seqs * parts), dim3(256), 0, s, a, copy_blocks, parts);
   return check_launch("page_compact");

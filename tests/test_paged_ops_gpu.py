@@ -170,7 +170,8 @@ def test_fork_many(gpu):
 @pytest.mark.parametrize("seed,pages,ps,layers,kv_heads,dim,dtype", [
     (0, 60, 16, 2, 2, 64, torch.bfloat16), (1, 1, 16, 1, 1, 64, torch.bfloat16), (2, 4096, 16, 1, 1, 8, torch.int16),
     (3, 4097, 16, 1, 1, 8, torch.int16), (4, 12289, 16, 1, 1, 8, torch.int16), (5, 33, 64, 16, 8, 64, torch.float16),
-    (6, 40, 128, 1, 2, 256, torch.float32),
+    (6, 40, 128, 1, 2, 256, torch.float32), (7, 16384, 16, 1, 1, 8, torch.int16), (8, 16385, 16, 1, 1, 8, torch.int16),
+    (9, 40001, 16, 1, 1, 8, torch.int16),
 ])
 @pytest.mark.parametrize("spare", [0.0, 0.02, 0.4, 0.9, 1.0])
 def test_compact(gpu, seed, pages, ps, layers, kv_heads, dim, dtype, spare):
