@@ -599,13 +599,12 @@ __global__ __launch_bounds__(256) void free_kernel(FreeArgs a) {
   for (int k = 0; k < kFreeEntries / 256; ++k) {
     if (e0 + 256 * k < pages) row[e0 + 256 * k] = -1;
     // A page whose count is 1 is held here alone: nobody else changes it. A count
-    // that was read too early is too high, and the others' are taken off atomically
-    // (a random 4-byte atomic crosses the chip: 355,000 pages, one in six of them
-    // shared, 24 us with an atomic for each, 20 with plain stores where they do).
+    // that was read too early is too high, and the others' are taken off atomically;
+    // one that said too little stays at 0.
     if (refs[k] == 1)
       p.refs[page[k]] = 0;
-    else if (refs[k] > 1)
-      atomicSub(p.refs + page[k], 1);
+    else if (refs[k] > 1 && atomicSub(p.refs + page[k], 1) <= 0)
+      atomicMax(p.refs + page[k], 0);
   }
 }
 
@@ -783,7 +782,8 @@ extern "C" int iron_page_compact(void* k_pages, void* v_pages, int* page_table, 
   if (int rc = check_data(who, k_pages, v_pages, num_layers, n_kv_heads, row_bytes)) return rc;
   if (int rc = check_workspace(who, workspace, workspace_bytes, iron_page_compact_workspace_bytes(num_pages))) return rc;
   const int parts = (max_pages + kEntries - 1) / kEntries;
-  IRON_REQUIRE(static_cast<long long>(num_seqs) * parts < (1LL << 30), "%s: num_seqs * max_pages is too large", who);
+  IRON_REQUIRE(static_cast<long long>(num_seqs) * parts < (1 << 23), "%s: num_seqs=%d with max_pages=%d: a table of up to 2^33 entries", who,
+               num_seqs, max_pages);
   CompactArgs a;
   a.pool = make_pool(k_pages, v_pages, page_table, seq_lens, page_refs, num_layers, n_kv_heads, row_bytes, num_pages,
                      page_size, num_seqs, max_pages);

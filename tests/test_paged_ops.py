@@ -84,13 +84,14 @@ def test_callable_refuses_wrong_tensors():
 P = 1 << 20  # a 16-byte-aligned stand-in address: nothing is launched
 
 
-def _tree(q=P, out=2 * P, dtype=0, H=4, Hkv=2, D=64, pages=8, ps=16, S=2, mp=4, N=6, T=5, scale=0.125, ws=P, size=1 << 30, lens=P):
-    _lib.call("iron_tree_attention", q, P, P, P, P, P, lens, P, P, out, dtype, H, Hkv, D, pages, ps, S, mp, N, T, scale, ws,
+def _tree(q=P, out=2 * P, dtype=0, H=4, Hkv=2, D=64, pages=8, ps=16, S=2, mp=4, N=6, T=5, scale=0.125, ws=P, size=1 << 30, lens=P, vp=P):
+    _lib.call("iron_tree_attention", q, P, P, P, vp, P, lens, P, P, out, dtype, H, Hkv, D, pages, ps, S, mp, N, T, scale, ws,
               size, None)
 
 
 @pytest.mark.parametrize("kw,match", [
     (dict(q=None), "null pointer"), (dict(q=P + 2), "16-byte"), (dict(lens=P + 2), "4-byte"), (dict(out=P), "one of the inputs"),
+    (dict(vp=2 * P), "one of the inputs"),
     (dict(dtype=2), "dtype=2"), (dict(H=3), "multiple"), (dict(D=32), "64 or 128"), (dict(pages=0), "num_pages=0"),
     (dict(ps=24), "power of two"), (dict(S=0), "num_seqs"), (dict(mp=0), "max_pages"), (dict(N=0), "num_nodes"),
     (dict(T=2000), "max_nodes"), (dict(scale=-1.0), "scale"), (dict(ws=None), "workspace"), (dict(size=0), "workspace of 0 bytes"),
@@ -108,8 +109,8 @@ def _fork(forks=P, n=2, mp=4, size=1 << 30, S=2):
     _lib.call("iron_page_fork", forks, P, 2 * P, P, P, P, P, 2, 2, 128, 8, 16, S, mp, n, 1, P, size, None)
 
 
-def _compact(size=1 << 30, L=2, moved=P):
-    _lib.call("iron_page_compact", P, 2 * P, P, P, P, moved, L, 2, 128, 8, 16, 2, 4, P, size, None)
+def _compact(size=1 << 30, L=2, moved=P, S=2, mp=4):
+    _lib.call("iron_page_compact", P, 2 * P, P, P, P, moved, L, 2, 128, 8, 16, S, mp, P, size, None)
 
 
 def _free(slots=P, n=1, ps=16):
@@ -122,7 +123,7 @@ def _free(slots=P, n=1, ps=16):
     (_append, dict(M=(1 << 20) + 1), "num_rows"), (_append, dict(size=16), "workspace of 16"), (_append, dict(L=0), "num_layers"),
     (_append, dict(ps=17), "power of two"), (_append, dict(mp=1 << 28), "2\\^31"), (_append, dict(S=9000), "num_seqs"),
     (_fork, dict(forks=None), "forks"), (_fork, dict(n=0), "num_forks"), (_fork, dict(n=8192, mp=1 << 26), "exceeds"),
-    (_fork, dict(size=0), "workspace"), (_compact, dict(size=0), "workspace"), (_compact, dict(L=5000), "num_layers"),
+    (_fork, dict(size=0), "workspace"), (_compact, dict(size=0), "workspace"), (_compact, dict(L=5000), "num_layers"), (_compact, dict(S=8192, mp=1 << 20), "2\\^33"),
     (_compact, dict(moved=None), "null pointer"), (_free, dict(slots=P + 1), "slots"), (_free, dict(n=9000), "num_slots"),
     (_free, dict(ps=0), "power of two"),
 ])

@@ -214,6 +214,18 @@ def test_free(gpu):
         assert got == want and all(case.same(state)), slots
 
 
+def test_free_of_pages_counted_too_low(gpu):
+    """More entries hold a page than its count says: it ends at 0, free, and never below."""
+    c = _filled(29, pages=64, seqs=12, max_pages=4, layers=1, kv_heads=1, dim=8, lens=[64] * 12)
+    for s in range(1, 12):
+        c.refs[c.table[s, :2]] = 0
+        c.table[s, :2] = c.table[0, :2]
+    c.refs[c.table[0, 0]], c.refs[c.table[0, 1]] = 2, 11
+    state = c.to(gpu)
+    assert _run(ops.PageFree(num_slots=12, **_pool(c)), [_ints(list(range(12)), gpu), *state[2:]], 12) == ref.free(c, list(range(12)))
+    assert all(c.same(state)) and (c.refs == 0).all()
+
+
 def test_large_pools_by_64_bit_offsets(gpu):
     """A pool past 4 GiB: the last pages are written and copied where they are, not 2^32 bytes before."""
     L, P, Hkv, ps, D = 2, 66000, 8, 32, 64  # 2.2 GB of K in each layer
