@@ -376,9 +376,12 @@ enum iron_page_status {
  * (iron_paged_append adds the accepted rows). A row that sees nothing gets
  * zeros; rows of out outside every tree, or behind max_nodes of one, are left
  * as they were. What a row does not see does not reach it, whatever it holds
- * (infinities, NaN). dtype 0: bf16, 1: fp16 (q, k, v and out). head_dim 64 or
- * 128; n_heads any multiple of n_kv_heads; max_nodes at most 1024. k_pages and
- * v_pages are one layer's (num_pages, n_kv_heads, page_size, head_dim).
+ * (infinities, NaN); a row whose scores are all -inf is one that sees nothing.
+ * Where a KV head has more than 32 rows (max_nodes times G), weights are rounded
+ * to dtype before the second product, as iron_attention_prefill does; else they
+ * keep 16 bits. dtype 0: bf16, 1: fp16 (q, k, v and out). head_dim 64 or 128;
+ * n_heads any multiple of n_kv_heads; max_nodes at most 1024. k_pages and v_pages
+ * are one layer's (num_pages, n_kv_heads, page_size, head_dim).
  * node_starts must not decrease; each tree is taken as cut to max_nodes nodes
  * and to num_nodes rows. Lengths outside [0, max_pages * page_size] are cut to
  * that range. Beside the reference's attention of one token or of a prompt

@@ -1,7 +1,26 @@
 // Attention of drafted trees over a paged KV cache.
 //
 // out[i,h] = sum_j softmax_j(scale q[i,h] . k_j) v_j over the cached positions
-// of node i's sequence and the nodes of its tree that it sees.
+// of node i's sequence and the nodes of its tree that it sees. The rows that
+// share a KV head (nodes times heads of its group) make the tiles of a sequence,
+// so that a byte of the cache is read once for all of them.
+//
+// Three launches' worth of code, two of them in a call:
+//  - tree_attention_kernel, tiles of 16 or 32 rows: a decode step, a small tree.
+//    Bound by the cache's bytes. Every wave streams its own keys through its own
+//    LDS ring, without barriers.
+//  - tree_wide_kernel, tiles of 128 rows: bound by the softmax and the products
+//    together. The four waves share a ring.
+//  - tree_join_kernel joins what different workgroups made of one row's keys.
+// The work is cut into equal shares of key blocks whatever the lengths
+// (share_of), from device memory alone: one captured graph serves every step.
+//
+// Measured (32 / 8 heads, whole calls back to back; a large copy moves 4.74 TB/s,
+// a large library product does 1.14-1.17 PFLOP/s): 64 sequences of 150-16384
+// positions, one token each, head_dim 64: 94 us, 5.1 TB/s of cache; the same with
+// a cache that fits L2: 47 us. One token behind 2047: 12.6 us, 8.6 in a graph.
+// 8 trees of 26 nodes behind 37-3968: 18.6 us. 2 trees of 64 nodes behind 20011 and
+// 32768, head_dim 128, fp16: 99-109 us, 530-580 TFLOP/s; 93 with a cache that fits L2.
 #include "iron_common.hpp"
 #include "../../include/iron_hip.h"
 
@@ -55,9 +74,9 @@ typedef unsigned ta_u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned ta_u32x4 __attribute__((ext_vector_type(4)));
 typedef short ta_i16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kBlock = 64;   // keys of a block: 16 for each of the 4 waves
+constexpr int kBlock = 64;      // keys of a block: 16 for each of the 4 waves
 constexpr int kWideBlock = 32;  // of the kernel of many rows
-constexpr int kStages = 4;   // blocks resident in a wave's ring
+constexpr int kStages = 4;      // blocks resident in a ring
 
 // fp16 weights are taken 2^6 times as large (at most 2^14 then), so that small
 // ones stay in fp16's normal range six powers of two longer.
@@ -268,6 +287,13 @@ __device__ __forceinline__ void wait_stage() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
 
+// Few rows: a tile of 16 RT rows, a workgroup of 4 waves. Wave w has keys 16 w ..
+// + 15 of each block of 64 and all rows, so nothing is shared until the end: each
+// wave fills a ring of its own (LDS-direct loads, three blocks in flight, 96 KiB a
+// CU) and waits for its own loads only. S^T = K Q^T on 16x16x32 MFMAs leaves each
+// lane 4 keys of one row; as hi and lo halves (split4) they are the 8 elements of
+// the B operand of O^T += V^T P^T as they stand, with V^T's 4 keys given twice, from
+// one transposed LDS read. The waves' sums meet in LDS once per tile.
 template <int D, bool F16, int RT>
 __global__ __launch_bounds__(256) void tree_attention_kernel(TreeArgs a) {
   constexpr int R = 16 * RT, B = kBlock, kRow = D * 2, kHalf = 16 * kRow, kStage = 2 * kHalf, kRing = kStages * kStage;
@@ -306,219 +332,219 @@ __global__ __launch_bounds__(256) void tree_attention_kernel(TreeArgs a) {
     const int hk = uniform(tile / t.row_tiles), row0 = (tile - hk * t.row_tiles) * R;
     const int rows = min(R, t.nodes * G - row0);
     if (n > 0) {
-    if (hk == 0 && blk0 == 0)  // for the launch that joins the parts
-      for (int i = row0 / G + tid; i <= (row0 + rows - 1) / G; i += 256) a.owner[t.first + i] = s;
-    ta_u32x4 qf[RT][NK];
-    int node[RT];
-    ta_f32x4 o[RT][ND];
-    float m[RT], off[RT], l[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      m[rt] = -INFINITY;
-      off[rt] = l[rt] = 0.f;
-#pragma unroll
-      for (int dt = 0; dt < ND; ++dt) o[rt][dt] = ta_f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    const long long table = static_cast<long long>(s) * a.max_pages;
-    const unsigned new_row = static_cast<unsigned>(a.Hkv) * kRow;
-    unsigned holes = 0;  // bit i % kStages: block i's page of this wave is none
-    auto page_of = [&](int i) {
-      const int blk = min(blk0 + i, t.cached - 1);
-      return t.cached ? uniform_word(a.table, table + (min(blk * kBlock + 16 * w, t.len - 1) >> a.page_shift)) : 0;
-    };
-    // the pages of the blocks that are issued next, read ahead: one round trip for the first ones
-    int page[kStages];
-#pragma unroll
-    for (int i = 0; i < kStages; ++i) page[i] = page_of(i);
-    auto issue = [&](int i) {
-      unsigned char* st = ring + (i % kStages) * kStage;
-      const int blk = blk0 + i;
-      if (blk < t.cached) {
-        const bool real = static_cast<unsigned>(page[0]) < static_cast<unsigned>(a.num_pages);
-        holes = (holes & ~(1u << (i % kStages))) | (real ? 0u : 1u << (i % kStages));
-        const long long at = ((static_cast<long long>(real ? page[0] : 0) * a.Hkv + hk) * ps + ((blk * kBlock + 16 * w) & (ps - 1))) * D;
-        const i32x4v rk = buffer_rsrc(a.k_pages + at), rv = buffer_rsrc(a.v_pages + at);
-#pragma unroll
-        for (int j = 0; j < kLoads / 2; ++j) {
-          load_lds16(rk, lrow[j] * kRow + kchunk[j], st + j * 1024);
-          load_lds16(rv, lrow[j] * kRow + vchunk[j], st + kHalf + j * 1024);
-        }
-#pragma unroll
-        for (int j = 0; j + 1 < kStages; ++j) page[j] = page[j + 1];
-        page[kStages - 1] = page_of(i + kStages);
-      } else {
-        const int j0 = (blk - t.cached) * kBlock + 16 * w;
-        const long long at = (static_cast<long long>(t.first) * a.Hkv + hk) * D;
-        const i32x4v rk = buffer_rsrc(a.k_new + at), rv = buffer_rsrc(a.v_new + at);
-#pragma unroll
-        for (int j = 0; j < kLoads / 2; ++j) {
-          const unsigned r = min(j0 + lrow[j], t.nodes - 1) * new_row;
-          load_lds16(rk, r + kchunk[j], st + j * 1024);
-          load_lds16(rv, r + vchunk[j], st + kHalf + j * 1024);
-        }
-      }
-    };
-
-    auto step = [&](int i) {
-      const int blk = blk0 + i;
-      const bool cache = blk < t.cached;
-      const int j0 = (cache ? blk : blk - t.cached) * kBlock + 16 * w;
-      const int valid = cache && (holes >> (i % kStages) & 1) ? 0 : min((cache ? t.len : t.nodes) - j0, 16);
-      if (valid <= 0) return;
-      const unsigned char* ks = ring + (i % kStages) * kStage;
-      const unsigned char* vs = ks + kHalf;
-      ta_u32x4 kf[NK];
-#pragma unroll
-      for (int kk = 0; kk < NK; ++kk) kf[kk] = *reinterpret_cast<const ta_u32x4*>(ks + c * kRow + k_slot<D>(c, 4 * kk + quad) * 16);
-      ta_u32x2 vt[ND];
-#pragma unroll
-      for (int dt = 0; dt < ND; ++dt) {
-        const int dim = 16 * dt + tcol;
-        vt[dt] = __builtin_bit_cast(ta_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) ta_i16x4*)(vs + trow * kRow + v_slot<D>(trow, dim >> 3) * 16 + (dim & 7) * 2)));
-      }
-      ta_f32x4 sc[RT];
+      if (hk == 0 && blk0 == 0)  // for the launch that joins the parts
+        for (int i = row0 / G + tid; i <= (row0 + rows - 1) / G; i += 256) a.owner[t.first + i] = s;
+      ta_u32x4 qf[RT][NK];
+      int node[RT];
+      ta_f32x4 o[RT][ND];
+      float m[RT], off[RT], l[RT];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        sc[rt] = ta_f32x4{0.f, 0.f, 0.f, 0.f};
+        m[rt] = -INFINITY;
+        off[rt] = l[rt] = 0.f;
 #pragma unroll
-        for (int kk = 0; kk < NK; ++kk) sc[rt] = mfma<F16>(kf[kk], qf[rt][kk], sc[rt]);
+        for (int dt = 0; dt < ND; ++dt) o[rt][dt] = ta_f32x4{0.f, 0.f, 0.f, 0.f};
       }
-      if (valid < 16) {  // keys behind the last one: no score, and values that cannot do harm
+      const long long table = static_cast<long long>(s) * a.max_pages;
+      const unsigned new_row = static_cast<unsigned>(a.Hkv) * kRow;
+      unsigned holes = 0;  // bit i % kStages: block i's page of this wave is none
+      auto page_of = [&](int i) {
+        const int blk = min(blk0 + i, t.cached - 1);
+        return t.cached ? uniform_word(a.table, table + (min(blk * kBlock + 16 * w, t.len - 1) >> a.page_shift)) : 0;
+      };
+      // the pages of the blocks that are issued next, read ahead: one round trip for the first ones
+      int page[kStages];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+      for (int i = 0; i < kStages; ++i) page[i] = page_of(i);
+      auto issue = [&](int i) {
+        unsigned char* st = ring + (i % kStages) * kStage;
+        const int blk = blk0 + i;
+        if (blk < t.cached) {
+          const bool real = static_cast<unsigned>(page[0]) < static_cast<unsigned>(a.num_pages);
+          holes = (holes & ~(1u << (i % kStages))) | (real ? 0u : 1u << (i % kStages));
+          const long long at = ((static_cast<long long>(real ? page[0] : 0) * a.Hkv + hk) * ps + ((blk * kBlock + 16 * w) & (ps - 1))) * D;
+          const i32x4v rk = buffer_rsrc(a.k_pages + at), rv = buffer_rsrc(a.v_pages + at);
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) sc[rt][e] = 4 * quad + e < valid ? sc[rt][e] : -INFINITY;
-        const unsigned k0 = 4 * quad;
-        const unsigned m01 = (k0 < static_cast<unsigned>(valid) ? 0xffffu : 0u) | (k0 + 1 < static_cast<unsigned>(valid) ? 0xffff0000u : 0u);
-        const unsigned m23 = (k0 + 2 < static_cast<unsigned>(valid) ? 0xffffu : 0u) | (k0 + 3 < static_cast<unsigned>(valid) ? 0xffff0000u : 0u);
+          for (int j = 0; j < kLoads / 2; ++j) {
+            load_lds16(rk, lrow[j] * kRow + kchunk[j], st + j * 1024);
+            load_lds16(rv, lrow[j] * kRow + vchunk[j], st + kHalf + j * 1024);
+          }
 #pragma unroll
-        for (int dt = 0; dt < ND; ++dt) {
-          vt[dt].x &= m01;
-          vt[dt].y &= m23;
-        }
-      }
-      if (!cache) {
+          for (int j = 0; j + 1 < kStages; ++j) page[j] = page[j + 1];
+          page[kStages - 1] = page_of(i + kStages);
+        } else {
+          const int j0 = (blk - t.cached) * kBlock + 16 * w;
+          const long long at = (static_cast<long long>(t.first) * a.Hkv + hk) * D;
+          const i32x4v rk = buffer_rsrc(a.k_new + at), rv = buffer_rsrc(a.v_new + at);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          const int word = a.mask[static_cast<long long>(node[rt]) * a.words + (j0 >> 5)] >> ((j0 & 31) + 4 * quad);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[rt][e] = word >> e & 1 ? sc[rt][e] : -INFINITY;
-        }
-      }
-      // Softmax in the log2 domain, p = 2^(s c - m). The row's maximum m moves only
-      // when a score passes it by more than 8, so p <= 2^8 and O is rarely
-      // rescaled; sum(p v) / sum(p) does not depend on which m is used.
-      const float cs = a.scale_log2;
-      bool grow = false;
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-        grow |= fmaxf(fmaxf(sc[rt][0], sc[rt][1]), fmaxf(sc[rt][2], sc[rt][3])) * cs > m[rt] + 8.f;
-      if (__builtin_amdgcn_ballot_w64(grow)) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          const float top = row_max(fmaxf(fmaxf(sc[rt][0], sc[rt][1]), fmaxf(sc[rt][2], sc[rt][3]))) * cs;
-          if (top > m[rt] + 8.f) {
-            const float alpha = __builtin_amdgcn_exp2f(m[rt] - top);  // 0 from m = -inf
-            m[rt] = top;
-            off[rt] = top - kLift<F16>;
-            l[rt] *= alpha;
-#pragma unroll
-            for (int dt = 0; dt < ND; ++dt) o[rt][dt] *= alpha;
+          for (int j = 0; j < kLoads / 2; ++j) {
+            const unsigned r = min(j0 + lrow[j], t.nodes - 1) * new_row;
+            load_lds16(rk, r + kchunk[j], st + j * 1024);
+            load_lds16(rv, r + vchunk[j], st + kHalf + j * 1024);
           }
         }
-      }
+      };
+
+      auto step = [&](int i) {
+        const int blk = blk0 + i;
+        const bool cache = blk < t.cached;
+        const int j0 = (cache ? blk : blk - t.cached) * kBlock + 16 * w;
+        const int valid = cache && (holes >> (i % kStages) & 1) ? 0 : min((cache ? t.len : t.nodes) - j0, 16);
+        if (valid <= 0) return;
+        const unsigned char* ks = ring + (i % kStages) * kStage;
+        const unsigned char* vs = ks + kHalf;
+        ta_u32x4 kf[NK];
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) kf[kk] = *reinterpret_cast<const ta_u32x4*>(ks + c * kRow + k_slot<D>(c, 4 * kk + quad) * 16);
+        ta_u32x2 vt[ND];
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) {
+          const int dim = 16 * dt + tcol;
+          vt[dt] = __builtin_bit_cast(ta_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) ta_i16x4*)(vs + trow * kRow + v_slot<D>(trow, dim >> 3) * 16 + (dim & 7) * 2)));
+        }
+        ta_f32x4 sc[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          sc[rt] = ta_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int kk = 0; kk < NK; ++kk) sc[rt] = mfma<F16>(kf[kk], qf[rt][kk], sc[rt]);
+        }
+        if (valid < 16) {  // keys behind the last one: no score, and values that cannot do harm
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) sc[rt][e] = 4 * quad + e < valid ? sc[rt][e] : -INFINITY;
+          const unsigned k0 = 4 * quad;
+          const unsigned m01 = (k0 < static_cast<unsigned>(valid) ? 0xffffu : 0u) | (k0 + 1 < static_cast<unsigned>(valid) ? 0xffff0000u : 0u);
+          const unsigned m23 = (k0 + 2 < static_cast<unsigned>(valid) ? 0xffffu : 0u) | (k0 + 3 < static_cast<unsigned>(valid) ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt) {
+            vt[dt].x &= m01;
+            vt[dt].y &= m23;
+          }
+        }
+        if (!cache) {
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            const int word = a.mask[static_cast<long long>(node[rt]) * a.words + (j0 >> 5)] >> ((j0 & 31) + 4 * quad);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[rt][e] = word >> e & 1 ? sc[rt][e] : -INFINITY;
+          }
+        }
+        // Softmax in the log2 domain, p = 2^(s c - m). The row's maximum m moves only
+        // when a score passes it by more than 8, so p <= 2^8 and O is rarely
+        // rescaled; sum(p v) / sum(p) does not depend on which m is used.
+        const float cs = a.scale_log2;
+        bool grow = false;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          grow |= fmaxf(fmaxf(sc[rt][0], sc[rt][1]), fmaxf(sc[rt][2], sc[rt][3])) * cs > m[rt] + 8.f;
+        if (__builtin_amdgcn_ballot_w64(grow)) {
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            const float top = row_max(fmaxf(fmaxf(sc[rt][0], sc[rt][1]), fmaxf(sc[rt][2], sc[rt][3]))) * cs;
+            if (top > m[rt] + 8.f) {
+              const float alpha = __builtin_amdgcn_exp2f(m[rt] - top);  // 0 from m = -inf
+              m[rt] = top;
+              off[rt] = top - kLift<F16>;
+              l[rt] *= alpha;
+#pragma unroll
+              for (int dt = 0; dt < ND; ++dt) o[rt][dt] *= alpha;
+            }
+          }
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          float p[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(sc[rt][e], cs, -off[rt]));
+          l[rt] += (p[0] + p[1]) + (p[2] + p[3]);
+          const ta_u32x4 pf = split4<F16>(p);
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt) o[rt][dt] = mfma<F16>(ta_u32x4{vt[dt].x, vt[dt].y, vt[dt].x, vt[dt].y}, pf, o[rt][dt]);
+        }
+      };
+
+      static_assert(kStages == 4, "the waits below count three stages in flight");
+#pragma unroll
+      for (int i = 0; i < kStages - 1; ++i)
+        if (i < n) issue(i);
+      // Q: the B operand of S^T = K Q^T (column: row 16 rt + c; dims 32 kk + 8 quad .. + 8).
+      // The compiler's wait for it takes in the ring's first loads, which it does not
+      // count: one round trip for both.
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        float p[4];
+        const int r = min(row0 + 16 * rt + c, t.nodes * G - 1), in_tree = r / G;
+        node[rt] = t.first + in_tree;
+        const uint16_t* qp = a.q + (static_cast<long long>(node[rt]) * a.H + hk * G + (r - in_tree * G)) * D + 8 * quad;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(sc[rt][e], cs, -off[rt]));
-        l[rt] += (p[0] + p[1]) + (p[2] + p[3]);
-        const ta_u32x4 pf = split4<F16>(p);
-#pragma unroll
-        for (int dt = 0; dt < ND; ++dt) o[rt][dt] = mfma<F16>(ta_u32x4{vt[dt].x, vt[dt].y, vt[dt].x, vt[dt].y}, pf, o[rt][dt]);
+        for (int kk = 0; kk < NK; ++kk) qf[rt][kk] = *reinterpret_cast<const ta_u32x4*>(qp + 32 * kk);
       }
-    };
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) asm volatile("" ::"v"(qf[rt][kk]));
+      for (int i = 0; i < n; ++i) {
+        const int left = n - 1 - i;  // stages in flight behind block i
+        if (left >= 2)
+          wait_stage<2 * kLoads>();
+        else if (left == 1)
+          wait_stage<kLoads>();
+        else
+          wait_stage<0>();
+        if (i + kStages - 1 < n) issue(i + kStages - 1);  // into the stage of block i - 1, which every read has left
+        step(i);
+      }
 
-    static_assert(kStages == 4, "the waits below count three stages in flight");
+      // The four waves' parts of the tile meet in LDS.
+      const bool whole = n == t.blocks;
+      const long long slot = 2LL * blockIdx.x + (blk0 == 0 ? 1 : 0);
+      wait_stage<0>();
+      float* mine_o = reinterpret_cast<float*>(ring);
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i)
-      if (i < n) issue(i);
-    // Q: the B operand of S^T = K Q^T (column: row 16 rt + c; dims 32 kk + 8 quad .. + 8).
-    // The compiler's wait for it takes in the ring's first loads, which it does not
-    // count: one round trip for both.
+      for (int rt = 0; rt < RT; ++rt) {
+        const int r = 16 * rt + c;
+        const float sum = row_sum(l[rt]);
+        if (quad == 0) {
+          stat_m[w][r] = m[rt] - kLift<F16>;
+          stat_l[w][r] = sum;
+        }
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int r = min(row0 + 16 * rt + c, t.nodes * G - 1), in_tree = r / G;
-      node[rt] = t.first + in_tree;
-      const uint16_t* qp = a.q + (static_cast<long long>(node[rt]) * a.H + hk * G + (r - in_tree * G)) * D + 8 * quad;
-#pragma unroll
-      for (int kk = 0; kk < NK; ++kk) qf[rt][kk] = *reinterpret_cast<const ta_u32x4*>(qp + 32 * kk);
-    }
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int kk = 0; kk < NK; ++kk) asm volatile("" ::"v"(qf[rt][kk]));
-    for (int i = 0; i < n; ++i) {
-      const int left = n - 1 - i;  // stages in flight behind block i
-      if (left >= 2)
-        wait_stage<2 * kLoads>();
-      else if (left == 1)
-        wait_stage<kLoads>();
-      else
-        wait_stage<0>();
-      if (i + kStages - 1 < n) issue(i + kStages - 1);  // into the stage of block i - 1, which every read has left
-      step(i);
-    }
-
-    // The four waves' parts of the tile meet in LDS.
-    const bool whole = n == t.blocks;
-    const long long slot = 2LL * blockIdx.x + (blk0 == 0 ? 1 : 0);
-    wait_stage<0>();
-    float* mine_o = reinterpret_cast<float*>(ring);
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int r = 16 * rt + c;
-      const float sum = row_sum(l[rt]);
-      if (quad == 0) {
-        stat_m[w][r] = m[rt] - kLift<F16>;
-        stat_l[w][r] = sum;
+        for (int dt = 0; dt < ND; ++dt)
+          *reinterpret_cast<ta_f32x4*>(mine_o + r * D + (((4 * dt + quad) ^ c) * 4)) = o[rt][dt];
       }
+      __syncthreads();
+      for (int x = tid; x < rows * (D / 4); x += 256) {
+        const int r = x / (D / 4), c4 = x % (D / 4);
+        float top = stat_m[0][r];
 #pragma unroll
-      for (int dt = 0; dt < ND; ++dt)
-        *reinterpret_cast<ta_f32x4*>(mine_o + r * D + (((4 * dt + quad) ^ c) * 4)) = o[rt][dt];
-    }
-    __syncthreads();
-    for (int x = tid; x < rows * (D / 4); x += 256) {
-      const int r = x / (D / 4), c4 = x % (D / 4);
-      float top = stat_m[0][r];
+        for (int i = 1; i < 4; ++i) top = fmaxf(top, stat_m[i][r]);
+        float sum = 0.f;
+        ta_f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 1; i < 4; ++i) top = fmaxf(top, stat_m[i][r]);
-      float sum = 0.f;
-      ta_f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < 4; ++i) {
+          const float li = stat_l[i][r];
+          const float f = __builtin_amdgcn_exp2f(stat_m[i][r] - top);
+          const ta_f32x4 part = f * *reinterpret_cast<const ta_f32x4*>(reinterpret_cast<const float*>(lds + i * kRing) + r * D + ((c4 ^ (r & 15)) * 4));
+          sum += li == 0.f ? 0.f : f * li;  // a wave that saw nothing has no maximum either
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float li = stat_l[i][r];
-        const float f = __builtin_amdgcn_exp2f(stat_m[i][r] - top);
-        const ta_f32x4 part = f * *reinterpret_cast<const ta_f32x4*>(reinterpret_cast<const float*>(lds + i * kRing) + r * D + ((c4 ^ (r & 15)) * 4));
-        sum += li == 0.f ? 0.f : f * li;  // a wave that saw nothing has no maximum either
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += li == 0.f ? 0.f : part[e];
+          for (int e = 0; e < 4; ++e) v[e] += li == 0.f ? 0.f : part[e];
+        }
+        if (whole) {
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          ta_u32x2 y;
+          if (sum == 0.f) v = ta_f32x4{0.f, 0.f, 0.f, 0.f};
+          y.x = narrow<F16>(v[0] * inv) | static_cast<unsigned>(narrow<F16>(v[1] * inv)) << 16;
+          y.y = narrow<F16>(v[2] * inv) | static_cast<unsigned>(narrow<F16>(v[3] * inv)) << 16;
+          const int row = row0 + r;
+          *reinterpret_cast<ta_u32x2*>(a.out + (static_cast<long long>(t.first + row / G) * a.H + hk * G + row % G) * D + c4 * 4) = y;
+        } else {
+          *reinterpret_cast<ta_f32x4*>(a.part_o + (slot * R + r) * D + c4 * 4) = v;
+          if (c4 == 0) a.part_ml[slot * R + r] = make_float2(top, sum);
+        }
       }
-      if (whole) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        ta_u32x2 y;
-        if (sum == 0.f) v = ta_f32x4{0.f, 0.f, 0.f, 0.f};
-        y.x = narrow<F16>(v[0] * inv) | static_cast<unsigned>(narrow<F16>(v[1] * inv)) << 16;
-        y.y = narrow<F16>(v[2] * inv) | static_cast<unsigned>(narrow<F16>(v[3] * inv)) << 16;
-        const int row = row0 + r;
-        *reinterpret_cast<ta_u32x2*>(a.out + (static_cast<long long>(t.first + row / G) * a.H + hk * G + row % G) * D + c4 * 4) = y;
-      } else {
-        *reinterpret_cast<ta_f32x4*>(a.part_o + (slot * R + r) * D + c4 * 4) = v;
-        if (c4 == 0) a.part_ml[slot * R + r] = make_float2(top, sum);
-      }
-    }
-    __syncthreads();  // the rings are free again
+      __syncthreads();  // the rings are free again
     }
     u += stop - in_tile;
     if (u < end && u == base + t.units) {
@@ -541,10 +567,16 @@ __device__ __forceinline__ ta_f32x16 mfma32(ta_u32x4 a, ta_u32x4 b, ta_f32x16 c)
 
 // Many rows: a tile of 128 rows, a workgroup of 4 waves with 32 rows each. The
 // waves load blocks of 32 keys together (8 rows of K and of V each) into one
-// ring: every byte read from L2 serves 128 rows. One barrier per block; the two
-// waves of a SIMD (four for head_dim 64) are of different workgroups, so that
-// one's softmax runs under another's products: with eight waves on one ring they
-// went through each phase together (wide trees 134 us, so 128).
+// ring: every byte read from L2 serves 128 rows. One barrier per block; a SIMD's
+// two waves (three with head_dim 64) are of different workgroups. Weights are
+// rounded once, to the 16 bits of their type, as the prompt's attention (MHA)
+// rounds them, and their sum is that of the rounded ones: as hi and lo they doubled the second
+// product (134 -> 109 us for the wide trees above, with the next block's
+// scores computed among this one's softmax; error against 64 bits 1.2 times that of
+// one rounding of the result). What bounds it: VALU and matrix time of a SIMD's
+// waves add up to the loop's time. Six of eight products of the second GEMM taken
+// out saved 12 of 93 us, half of K's or V's LDS reads nothing, scheduling barriers,
+// wave priorities and accumulators in AGPRs nothing.
 template <int D, bool F16>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void tree_wide_kernel(TreeArgs a) {
   constexpr int R = 128, B = kWideBlock, kRow = D * 2, kHalf = B * kRow, kStage = 2 * kHalf;
@@ -919,7 +951,12 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
     const uint16_t* v;
     const float x = score(j + lane, v);
     // a weight too small for fp32 is still not zero: it keeps an infinity one
-    const float p = !v ? 0.f : x != x || top == INFINITY ? NAN : fmaxf(__builtin_amdgcn_exp2f(x - top), 1.17549435e-38f);
+    float p = fmaxf(__builtin_amdgcn_exp2f(x - top), 1.17549435e-38f);
+    if (x != x || top == INFINITY)
+      p = NAN;
+    else if (top == -INFINITY)
+      p = 0.f;
+    if (!v) p = 0.f;
     sum += p;
     const unsigned long long seen = __ballot(v != nullptr);
     for (unsigned long long left = seen; left; left &= left - 1) {
@@ -1026,7 +1063,7 @@ extern "C" int iron_tree_attention(const void* q, const void* k_new, const void*
     IRON_REQUIRE(p && aligned16(p), "%s: null pointer, or one that is not 16-byte aligned", who);
   for (const void* p : {page_table, seq_lens, node_starts, tree_mask})
     IRON_REQUIRE(p && (reinterpret_cast<uintptr_t>(p) & 3u) == 0, "%s: int32 arrays must be given and 4-byte aligned", who);
-  IRON_REQUIRE(out != q && out != k_new && out != v_new, "%s: out is one of the inputs", who);
+  for (const void* p : {q, k_new, v_new, k_pages, v_pages}) IRON_REQUIRE(out != p, "%s: out is one of the inputs", who);
   IRON_REQUIRE(scale > 0.f && scale < INFINITY, "%s: scale=%g must be positive and finite", who, scale);
   const long long need = iron_tree_attention_workspace_bytes(n_heads, n_kv_heads, head_dim, num_seqs, num_nodes,
                                                              max_nodes, max_pages, page_size);

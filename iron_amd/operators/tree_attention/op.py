@@ -19,7 +19,10 @@ h // (H / Hkv). bf16 or fp16 (``dtype``), D 64 or 128.
 
 A row that sees nothing gets zeros; rows of out behind the last tree are left
 as they were. What a node does not see does not reach its row, whatever it
-holds. Softmax and sums are fp32. Kernel: iron_tree_attention.
+holds; a row whose scores are all -inf is one that sees nothing. Scores, softmax
+and sums are fp32; the weights enter the product with V with 16 bits, or rounded
+to ``dtype`` (as in MHA) where a KV head has more than 32 rows, max_nodes times
+H / Hkv. Kernel: iron_tree_attention.
 """
 
 import math
@@ -71,8 +74,8 @@ class TreeAttention(PagedOperator):
         return (self.max_nodes + 31) // 32
 
     def workspace_bytes(self) -> int:
-        return _lib.workspace_bytes("iron_tree_attention_workspace_bytes", self.num_heads, self.num_kv_heads, self.head_dim, self.num_seqs, self.num_nodes,
-                                self.max_nodes, self.max_pages, self.page_size)
+        return _lib.workspace_bytes("iron_tree_attention_workspace_bytes", self.num_heads, self.num_kv_heads, self.head_dim,
+                                    self.num_seqs, self.num_nodes, self.max_nodes, self.max_pages, self.page_size)
 
     def get_arg_spec(self):
         new = (self.num_nodes, self.num_kv_heads, self.head_dim)

@@ -127,11 +127,12 @@ def test_mask_bits_behind_the_tree_do_not_count(gpu):
 
 @pytest.mark.parametrize("D,dtype", [(64, BF16), (128, FP16)])
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
-def test_what_is_not_seen_does_not_count(gpu, value, D, dtype):
+@pytest.mark.parametrize("nodes", [(12, 20), (4, 8), (4, 4)])  # 80, 32 and 16 rows to a KV head
+def test_what_is_not_seen_does_not_count(gpu, value, D, dtype, nodes):
     """Rows of a page behind the length, other pages, holes, and nodes that a row does not see hold what they like."""
-    c = Case(8, 2, D, 16, [37, 100], [12, 20], dtype, seed=5, mask="chain")
+    c = Case(8, 2, D, 16, [37, 100], nodes, dtype, seed=5, mask="chain")
     c.sees[:] = False
-    for s, t in ((0, 12), (1, 20)):
+    for s, t in enumerate(nodes):
         for i in range(t):
             c.sees[c.starts[s] + i, : i + 1] = True
             c.sees[c.starts[s] + i, 3] = False
@@ -145,7 +146,7 @@ def test_what_is_not_seen_does_not_count(gpu, value, D, dtype):
     c.kp[c.table[1, 6], :, 4:], c.vp[c.table[1, 6], :, 4:] = value, value
     for s in (0, 1):
         c.kn[c.starts[s] + 3], c.vn[c.starts[s] + 3] = value, value
-    c.kn[32:], c.vn[32:] = value, value
+    c.kn[sum(nodes):], c.vn[sum(nodes):] = value, value
     c.check(gpu)
 
 
@@ -186,6 +187,47 @@ def test_cached_values_that_are_not_finite(gpu):
     c.vp[c.table[1, 1], 1, 3, 9] = 0.0
     want, tol = c.want()
     assert ((got - want).abs() <= tol)[~hit].all()
+
+
+@pytest.mark.parametrize("nodes", [3, 30])  # 12 and 120 rows to a KV head
+@pytest.mark.parametrize("behind", [0.0, float("nan")])
+def test_scores_of_minus_infinity(gpu, behind, nodes):
+    """Such a key has no weight; a row that sees no other is a row that sees nothing, also where it is done over."""
+    c = Case(4, 1, 64, 16, [37, 100], [nodes, 1], seed=28)
+    c.q[:] = c.q.abs() + 0.125
+    n = c.starts[1]
+    for p in c.table[0, :3]:
+        c.kp[p] = -float("inf")
+    c.kn[:n] = -float("inf")
+    c.vp[c.table[0, 2], :, 5:] = behind  # behind the last position
+    c.kp[c.table[1, 0], :, 3] = -float("inf")
+    t = c.tensors(gpu)
+    c.op.get_callable()(*t)
+    torch.cuda.synchronize()
+    got = t[-1].cpu().double()
+    assert (got[:n] == 0).all()
+    c.kp[c.table[1, 0], :, 3] = c.q[n:n + 1].mean(1) * -1e4  # a weight of zero in 64 bits too
+    c.kp[c.table[0, :3]], c.kn[:n] = 0.0, 0.0
+    c.vp[c.table[0, 2]] = 0.0
+    want, tol = c.want()
+    assert ((got - want).abs() <= tol)[n].all()
+
+
+@pytest.mark.parametrize("nodes", [3, 30])
+@pytest.mark.parametrize("others", [0.0, -float("inf")])
+def test_a_score_of_nan(gpu, others, nodes):
+    """It makes its rows NaN, whatever the other scores are; a score of plus infinity does too."""
+    c = Case(4, 1, 64, 16, [37, 20, 20], [nodes, nodes, 1], seed=29)
+    c.q[:] = c.q.abs() + 0.125
+    for s, value in ((0, float("nan")), (1, float("inf"))):
+        c.kp[c.table[s, :-(-c.lens[s] // 16)]] = others
+        c.kn[c.starts[s]:c.starts[s + 1]] = others
+        c.kp[c.table[s, 1], :, 2] = value
+    t = c.tensors(gpu)
+    c.op.get_callable()(*t)
+    torch.cuda.synchronize()
+    got = t[-1].cpu().double()
+    assert got[:2 * nodes].isnan().all() and got[2 * nodes:].isfinite().all()
 
 
 @pytest.mark.parametrize("q_scale", [0.0, 1e-3, 60.0])
@@ -244,6 +286,20 @@ def test_many_sequences(gpu):
     Case(4, 2, 64, 16, lens, [int(x) for x in rng.integers(0, 4, 150)], seed=14).check(gpu)
     lens[40] = 5000
     Case(8, 4, 128, 64, lens[:70], [1] * 70, FP16, seed=15).check(gpu)
+
+
+def test_a_thousand_sequences(gpu):
+    """Several sequences to a lane of the wave that shares out the work; most of them without nodes in this call."""
+    rng = np.random.default_rng(23)
+    lens, nodes = [int(x) for x in rng.integers(0, 70, 1000)], [0] * 1000
+    for s in rng.choice(1000, 90, replace=False):
+        nodes[s] = int(rng.integers(1, 4))
+    Case(2, 1, 64, 16, lens, nodes, seed=23).check(gpu)
+
+
+def test_the_largest_trees(gpu):
+    Case(2, 2, 64, 16, [40], [1024], seed=24, mask="random").check(gpu)
+    Case(2, 1, 128, 16, [0, 300], [1000, 24], FP16, seed=25).check(gpu)
 
 
 def test_long_context(gpu):
@@ -332,6 +388,45 @@ def test_two_graphs_and_two_streams_at_once(gpu):
         torch.cuda.synchronize()
         for c, t in zip(cases, sets):
             c.check(gpu, t[-1])
+
+
+@pytest.mark.parametrize("dispatch", ["fused", "separate"])
+def test_in_an_operator_sequence(gpu, dispatch):
+    """Attention and append as one runlist, called three times: the cache that a call leaves is the next one's."""
+    from iron_amd.common import OperatorSequence
+
+    c = Case(8, 2, 64, 16, [30, 5], [3, 2], seed=26, spare=0, max_nodes=4)
+    c.P, c.MP = 16, 6
+    c.table = np.full((2, 6), -1, np.int32)
+    c.table[0, :2], c.table[1, 0] = (3, 9), 4
+    g = torch.Generator().manual_seed(27)
+    c.kp, c.vp = (torch.randn(16, 2, 16, 64, generator=g).to(BF16) for _ in range(2))
+    pool = dict(num_kv_heads=2, head_dim=64, num_pages=16, page_size=16, num_seqs=2, max_pages=6)
+    tree = ops.TreeAttention(num_heads=8, num_nodes=5, max_nodes=4, **pool)
+    append = ops.PagedAppend(num_layers=1, num_nodes=5, num_rows=4, **pool)
+    cache = ("k_pages", "v_pages", "table", "lens")
+    seq = OperatorSequence(name="paged_step", dispatch=dispatch,
+                           runlist=[(tree, "q", "k", "v", *cache, "starts", "mask", "out"),
+                                    (append, "k", "v", "rows", "row_starts", *cache, "refs", "status")],
+                           input_args=["q", "k", "v", "starts", "mask", "rows", "row_starts", *cache, "refs"],
+                           output_args=["out", "status"]).compile()
+    fn = seq.get_callable()
+    refs = torch.zeros(16, dtype=torch.int32)
+    refs[[3, 9, 4]] = 1
+    rows, row_starts = [0, 2, 3, 4], [0, 2, 4]
+    words = tree.pack_mask(torch.from_numpy(c.sees))
+    i32 = lambda v: torch.tensor(np.asarray(v), dtype=torch.int32)
+    for name, value in dict(q=c.q, k=c.kn, v=c.vn, starts=i32(c.starts), mask=words, rows=i32(rows), row_starts=i32(row_starts),
+                            k_pages=c.kp, v_pages=c.vp, table=i32(c.table), lens=i32(c.lens), refs=refs).items():
+        fn.get_buffer(name).torch_view(torch.uint8).copy_(value.contiguous().view(-1).view(torch.uint8))
+    want = ref.Cache(1, 16, 2, 16, 64, 2, 6)
+    want.k, want.v, want.table, want.lens = c.kp[None].clone(), c.vp[None].clone(), c.table.copy(), np.array(c.lens, np.int32)
+    want.refs = refs.numpy().copy()
+    for _ in range(3):
+        fn()
+        c.lens, c.table, c.kp, c.vp = [int(x) for x in want.lens], want.table, want.k[0], want.v[0]
+        c.check(gpu, fn.get_buffer("out").to_torch().view(5, 8, 64))
+        assert ref.append(want, c.kn[None], c.vn[None], rows, row_starts) == [0, 0]
 
 
 def test_a_conversation(gpu):
