@@ -23,7 +23,9 @@ namespace iron {
 namespace {
 
 constexpr int kPlan = 1024;         // threads of the one workgroup that plans a call
-constexpr int kMaxRequests = 8192;  // sequences of an append, pairs of a fork: their prefix sums live in LDS (32 KiB)
+constexpr int kMaxSeqs = 8192;
+constexpr int kMaxRequests = 8192;  // sequences of an append, pairs of a fork: what is known of them lives in LDS
+constexpr int kMaxRows = 1 << 20;   // of one append: the prefix sums stay in 32 bits whatever row_starts holds
 
 // What became of a request (enum iron_page_status).
 constexpr int PAGE_DONE = IRON_PAGE_DONE, PAGE_INVALID = IRON_PAGE_INVALID, PAGE_NO_ROOM = IRON_PAGE_NO_ROOM,
@@ -90,33 +92,50 @@ __device__ int scan_requests(int* need, int n, int* tmp) {
   return carry;
 }
 
+// Bit j: the count of page base + j is 0 (and there is such a page).
+__device__ __forceinline__ unsigned free4(const int4& r, int base, int num_pages) {
+  const unsigned zeros = static_cast<unsigned>(r.x == 0) | static_cast<unsigned>(r.y == 0) << 1 |
+                         static_cast<unsigned>(r.z == 0) << 2 | static_cast<unsigned>(r.w == 0) << 3;
+  const int left = num_pages - base;
+  return zeros & (left >= 4 ? 15u : (1u << max(left, 0)) - 1);
+}
+
+// The counts of pages base .. base + 3 (base a multiple of 4), and of those that there are.
+__device__ __forceinline__ int4 counts4(const int* refs, int base, int num_pages) {
+  if (base + 4 <= num_pages) return *reinterpret_cast<const int4*>(refs + base);
+  int4 r = make_int4(0, 0, 0, 0);
+  if (base < num_pages) r.x = refs[base];
+  if (base + 1 < num_pages) r.y = refs[base + 1];
+  if (base + 2 < num_pages) r.z = refs[base + 2];
+  return r;
+}
+
 // The lowest `want` free pages into list (global), as many as there are;
-// returns how many were found (at most want). Sixteen counts a thread and
-// round, and no further than needed.
-__device__ int find_free(const int* refs, int num_pages, int want, int* list, int* tmp) {
+// returns how many were found (at most want). `first` is counts4 of pages
+// 4 tid .. + 3, which the caller asks for before all else: most calls need no
+// more than those. Then four such reads of each thread at a time, as far as needed.
+__device__ int find_free(const int* refs, int num_pages, int want, int* list, int* tmp, const int4& first) {
+  constexpr int kAhead = 4;
   int found = 0;
-  for (long long b = 0; b < num_pages && found < want; b += kPlan * 16) {
-    const long long p0 = b + threadIdx.x * 16;
-    unsigned zeros = 0;
-    if (p0 + 16 <= num_pages) {
+  int4 r[kAhead] = {first};
+  for (int b = 0, n = 1; b < num_pages && found < want; b += 4 * kPlan * n, n = kAhead) {
+    if (b) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int4 r = *reinterpret_cast<const int4*>(refs + p0 + 4 * j);
-        zeros |= (static_cast<unsigned>(r.x == 0) | static_cast<unsigned>(r.y == 0) << 1 |
-                  static_cast<unsigned>(r.z == 0) << 2 | static_cast<unsigned>(r.w == 0) << 3) << (4 * j);
+      for (int k = 0; k < kAhead; ++k) r[k] = counts4(refs, b + 4 * (k * kPlan + static_cast<int>(threadIdx.x)), num_pages);
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (k >= n || found >= want) break;
+      const int p0 = b + 4 * (k * kPlan + static_cast<int>(threadIdx.x));
+      unsigned zeros = free4(r[k], p0, num_pages);
+      int total;
+      int at = found + block_scan<kPlan>(static_cast<int>(__popc(zeros)), tmp, total);
+      while (zeros && at < want) {
+        list[at++] = p0 + __ffs(zeros) - 1;
+        zeros &= zeros - 1;
       }
-    } else {
-      for (int j = 0; j < 16; ++j)
-        if (p0 + j < num_pages && refs[p0 + j] == 0) zeros |= 1u << j;
+      found += total;
     }
-    int total;
-    int r = found + block_scan<kPlan>(static_cast<int>(__popc(zeros)), tmp, total);
-    while (zeros && r < want) {
-      const int j = __ffs(zeros) - 1;
-      zeros &= zeros - 1;
-      list[r++] = static_cast<int>(p0) + j;
-    }
-    found += total;
   }
   __syncthreads();
   return min(found, want);
@@ -165,11 +184,18 @@ __device__ __forceinline__ void row_range(const AppendArgs& a, int s, int& first
   count = min(max(a.row_starts[s + 1], first), a.num_rows) - first;
 }
 
-// Decides which sequences grow, gives them pages and moves their lengths.
+// Decides which sequences grow, gives them pages and moves their lengths. One
+// workgroup, bound by its chain of dependent reads: the counts that the search
+// for free pages begins with are asked for first, and what was read of the
+// sequences stays in LDS (8 sequences 4.0 -> 2.7 us, four prompts 6.4 -> 4.5).
 __global__ __launch_bounds__(kPlan) void append_plan_kernel(AppendArgs a) {
   __shared__ int need[kMaxRequests];
+  __shared__ int lens[kMaxRequests];
+  __shared__ int grow[kMaxRequests];  // rows to append and, in the lowest two bits, the status
   __shared__ int tmp[kPlan / 64];
+  static_assert(kMaxRows <= 1 << 28 && PAGE_NOT_OWN < 4, "both fit");
   const Pool& p = a.pool;
+  const int4 front = counts4(p.refs, 4 * threadIdx.x, p.num_pages);
   for (int s = threadIdx.x; s < p.num_seqs; s += kPlan) {
     int first, count;
     row_range(a, s, first, count);
@@ -187,31 +213,30 @@ __global__ __launch_bounds__(kPlan) void append_plan_kernel(AppendArgs a) {
       if (st == PAGE_DONE) n = p.pages_of(len + count) - p.pages_of(len);
     }
     need[s] = n;
-    a.status[s] = st;
+    lens[s] = len;
+    grow[s] = count << 2 | st;
   }
   __syncthreads();
   const int want = scan_requests(need, p.num_seqs, tmp);
-  const int have = find_free(p.refs, p.num_pages, min(want, a.list_cap), a.list, tmp);
+  const int have = find_free(p.refs, p.num_pages, min(want, a.list_cap), a.list, tmp, front);
   for (int s = threadIdx.x; s < p.num_seqs; s += kPlan) {
-    int first, count;
-    row_range(a, s, first, count);
-    const int len = p.lens[s];
-    int st = a.status[s];
-    if (st == PAGE_DONE && !granted(need, s, p.num_seqs, want, have)) a.status[s] = st = PAGE_NO_ROOM;
-    a.begin[s] = st == PAGE_DONE ? len : -1;
-    if (st == PAGE_DONE) p.lens[s] = len + count;
+    int st = grow[s] & 3;
+    if (st == PAGE_DONE && !granted(need, s, p.num_seqs, want, have)) st = PAGE_NO_ROOM;
+    a.status[s] = st;
+    a.begin[s] = st == PAGE_DONE ? lens[s] : -1;
+    if (st == PAGE_DONE) p.lens[s] = lens[s] + (grow[s] >> 2);
   }
-  __syncthreads();  // begin is written
   for (int r = threadIdx.x; r < have; r += kPlan) {
     const int s = request_of(need, p.num_seqs, r);
     if (!granted(need, s, p.num_seqs, want, have)) continue;
     const int page = a.list[r];
     p.refs[page] = 1;
-    p.table[static_cast<long long>(s) * p.max_pages + p.pages_of(a.begin[s]) + (r - need[s])] = page;
+    p.table[static_cast<long long>(s) * p.max_pages + p.pages_of(lens[s]) + (r - need[s])] = page;
   }
 }
 
-// One row of the call in `group` layers: K and V of every KV head.
+// One row of the call in `group` layers: K and V of every KV head. Bound by
+// memory: 437 MB (four prompts, 16 layers) in 91 us, 4.8 TB/s.
 __global__ __launch_bounds__(256) void append_rows_kernel(AppendArgs a, int group) {
   __shared__ int owner;
   const Pool& p = a.pool;
@@ -249,7 +274,8 @@ __global__ __launch_bounds__(256) void append_rows_kernel(AppendArgs a, int grou
 // ----------------------------------------------------------- page copies ----
 // Pages to copy: the first rows[i] rows (rows null: all) of every head of page
 // src[i] to page dst[i], K and V, all layers. No page is both a source and a
-// destination.
+// destination. Bound by memory: four whole sequences, 557 MB, in 111 us, and a
+// third of a pool packed, 917 MB, in 183 us: 5.0 TB/s.
 struct Copies {
   const int* src;
   const int* dst;
@@ -283,7 +309,6 @@ struct ForkArgs {
   Pool pool;
   const int* forks;  // (num_forks, 2): parent, child
   int* status;       // (num_forks)
-  int* claim;        // workspace (num_seqs): the first pair that names the child
   int* len;          // workspace (num_forks): the parent's length, or -1 where nothing is done
   int* first;        // workspace (num_forks): where the pair's pages begin in dst
   int* dst;          // workspace (list_cap): pages given out,
@@ -293,33 +318,41 @@ struct ForkArgs {
   int num_forks, list_cap, share;
 };
 
+// One workgroup: which pairs count (each child's first, found in LDS), their
+// pages, and the copies to make. Bound by its chain of dependent reads: 16 pairs
+// 4.4 us (5.8 with the claims in global memory and no counts asked for early),
+// four whole copies 8.4.
 __global__ __launch_bounds__(kPlan) void fork_plan_kernel(ForkArgs a) {
   __shared__ int need[kMaxRequests];
+  __shared__ int claim[kMaxSeqs];  // the first pair that names the child
   __shared__ int tmp[kPlan / 64];
   __shared__ int copies;
   const Pool& p = a.pool;
   const int ps = p.page_size, n = a.num_forks;
+  const int4 front = counts4(p.refs, 4 * threadIdx.x, p.num_pages);
   if (threadIdx.x == 0) copies = 0;
   auto slot = [&](int s) { return static_cast<unsigned>(s) < static_cast<unsigned>(p.num_seqs); };
   auto row = [&](int s) { return p.table + static_cast<long long>(s) * p.max_pages; };
   for (int i = threadIdx.x; i < n; i += kPlan) {
     const int child = a.forks[2 * i + 1];
-    if (slot(child)) __hip_atomic_store(a.claim + child, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (slot(child)) claim[child] = n;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += kPlan) {
     const int child = a.forks[2 * i + 1];
-    if (slot(child)) atomicMin(a.claim + child, i);
+    if (slot(child)) atomicMin(claim + child, i);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += kPlan) {
     const int parent = a.forks[2 * i], child = a.forks[2 * i + 1];
     int st = PAGE_INVALID, len = -1, pages = 0;
-    if (slot(parent) && slot(child) && parent != child && p.lens[child] == 0 && p.len_fits(p.lens[parent]) &&
-        __hip_atomic_load(a.claim + child, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == i) {
-      st = PAGE_DONE;
-      len = p.lens[parent];
-      pages = a.share ? (len % ps != 0 && p.in_pool(row(parent)[len / ps])) : 0;
+    if (slot(parent) && slot(child) && parent != child && claim[child] == i) {
+      const int to = p.lens[child], from = p.lens[parent];
+      if (to == 0 && p.len_fits(from)) {
+        st = PAGE_DONE;
+        len = from;
+        pages = a.share ? (len % ps != 0 && p.in_pool(row(parent)[len / ps])) : 0;
+      }
     }
     a.status[i] = st;
     a.len[i] = len;
@@ -339,7 +372,7 @@ __global__ __launch_bounds__(kPlan) void fork_plan_kernel(ForkArgs a) {
     __syncthreads();
   }
   const int want = scan_requests(need, n, tmp);
-  const int have = find_free(p.refs, p.num_pages, min(want, a.list_cap), a.dst, tmp);
+  const int have = find_free(p.refs, p.num_pages, min(want, a.list_cap), a.dst, tmp, front);
   for (int i = threadIdx.x; i < n; i += kPlan) {
     if (a.len[i] < 0) continue;
     if (!granted(need, i, n, want, have)) {
@@ -578,9 +611,13 @@ __device__ __forceinline__ void end_slot(const FreeArgs& a, int i, int s) {
   if (s >= 0) a.pool.lens[s] = 0;
 }
 
-// Part y of slot x's table entries. With one part to a slot the length goes to
-// 0 here (the barrier in ended() is behind every read of it); with more a second
-// launch does that, as the other parts may not have read it yet.
+// Part y of slot x's table entries: one round trip for the entries and one for
+// their counts. Bound by random 4-byte reads and writes: 355,000 pages all over
+// the pool, one in six of them shared, 15.5 us (with the tables put back, in a
+// graph: 24, 19 without the atomics, 15 without any write of a count).
+// With one part to a slot the length goes to 0 here (the barrier in ended() is
+// behind every read of it); with more a second launch does that, as the other
+// parts may not have read it yet.
 __global__ __launch_bounds__(256) void free_kernel(FreeArgs a) {
   const Pool& p = a.pool;
   const int i = blockIdx.x;
@@ -615,9 +652,7 @@ __global__ __launch_bounds__(256) void free_lens_kernel(FreeArgs a) {
 }
 
 // -------------------------------------------------------------------- host ----
-constexpr int kMaxSeqs = 8192;
 constexpr int kMaxPoolPages = 1 << 27;
-constexpr int kMaxRows = 1 << 20;   // of one append: the prefix sums stay in 32 bits whatever row_starts holds
 constexpr int kCopyBlocks = 2048;
 
 long long round4(long long n) { return (n + 3) / 4 * 4; }
@@ -728,7 +763,7 @@ extern "C" int iron_paged_append(const void* k_new, const void* v_new, const int
 
 extern "C" long long iron_page_fork_workspace_bytes(int num_forks, int num_seqs, int max_pages, int num_pages, int share) {
   if (num_forks < 1 || num_forks > kMaxRequests || num_seqs < 1 || max_pages < 1 || num_pages < 1) return -1;
-  return 4 * (4 + round4(num_seqs) + 2 * round4(num_forks) + 3 * round4(fork_list(num_forks, max_pages, num_pages, share)));
+  return 4 * (4 + 2 * round4(num_forks) + 3 * round4(fork_list(num_forks, max_pages, num_pages, share)));
 }
 
 extern "C" int iron_page_fork(const int* forks, void* k_pages, void* v_pages, int* page_table, int* seq_lens,
@@ -751,8 +786,7 @@ extern "C" int iron_page_fork(const int* forks, void* k_pages, void* v_pages, in
   a.forks = forks;
   a.status = status;
   a.count = static_cast<int*>(workspace);
-  a.claim = a.count + 4;
-  a.len = a.claim + round4(num_seqs);
+  a.len = a.count + 4;
   a.first = a.len + round4(num_forks);
   a.dst = a.first + round4(num_forks);
   a.src = a.dst + round4(cap);

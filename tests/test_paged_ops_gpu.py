@@ -122,6 +122,22 @@ def test_append_batch_sizes(gpu, seqs, max_pages, pages, n):
     assert got == want and all(c.same(state))
 
 
+@pytest.mark.parametrize("pages", [2, 3, 4095, 4097, 4099, 20482, 36871])
+def test_free_pages_are_found_wherever_they_are(gpu, pages):
+    """A nearly full pool: the free pages lie around the edges of what the search looks at together, and at its end."""
+    edges = sorted({e + d for e in (0, 4, 4096, 8192, 20480, 24576, 36864, pages) for d in (-2, -1, 0, 1)} & set(range(pages)))
+    for held in (0, 1, len(edges) // 2, len(edges) - 1, len(edges)):
+        c = ref.Cache(1, pages, 1, 16, 8, 3, 64)
+        c.refs[:] = 1
+        c.refs[edges[held:]] = 0
+        free = len(edges) - held
+        for counts in ([16 * free, 0, 0], [0, 16, 16 * max(0, free - 1)], [16 * (free + 1), 0, 0]):
+            print(f"{pages} pages, {free} free, rows {counts}", flush=True)
+            case = c.copy()
+            got, state, (kn, vn, rows, starts) = _append(gpu, case, counts, pages)
+            assert got == ref.append(case, kn, vn, rows, starts) and all(case.same(state))
+
+
 @pytest.mark.parametrize("share", [True, False])
 @pytest.mark.parametrize("seed,ps,layers,kv_heads,dim,dtype,forks", [
     (0, 16, 2, 2, 64, torch.bfloat16, [(0, 5), (1, 6), (0, 7)]),
