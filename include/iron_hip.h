@@ -376,7 +376,7 @@ enum iron_page_status {
  * (iron_paged_append adds the accepted rows). A row that sees nothing gets
  * zeros; rows of out outside every tree, or behind max_nodes of one, are left
  * as they were. What a row does not see does not reach it, whatever it holds
- * (infinities, NaN); a row whose scores are all -inf is one that sees nothing.
+ * (infinities, NaN); a key whose score is -inf is one that the row does not see.
  * Where a KV head has more than 32 rows (max_nodes times G), weights are rounded
  * to dtype before the second product, as iron_attention_prefill does; else they
  * keep 16 bits. dtype 0: bf16, 1: fp16 (q, k, v and out). head_dim 64 or 128;

@@ -844,7 +844,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void tree_wide_kernel(TreeArg
 
 // One workgroup per node and 4 heads, a wave for each row: joins the parts of
 // rows whose keys were shared out, and does over the rows that came out
-// infinite or NaN, one key at a time and only the keys that the row sees (a
+// infinite or NaN, one key at a time and only the keys that have a weight (a
 // product with a weight of zero lets what is not seen through).
 template <int D, bool F16, int R, int B>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
@@ -931,15 +931,15 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
     return a.k_new + at;
   };
   const int keys = t.len + t.nodes;
-  auto score = [&](int j, const uint16_t*& v) {  // one key a lane
-    const uint16_t* k = j < keys ? key(j, v) : (v = nullptr, nullptr);
-    if (!k) {
-      v = nullptr;
-      return -INFINITY;
-    }
+  auto score = [&](int j, const uint16_t*& v) {  // one key a lane; v null where it has no weight
+    v = nullptr;
+    const uint16_t* k = j < keys ? key(j, v) : nullptr;
+    if (!k) return -INFINITY;
     float x = 0.f;
     for (int d = 0; d < D; ++d) x += widen<F16>(q[d]) * widen<F16>(k[d]);
-    return x * a.scale_log2;
+    x *= a.scale_log2;
+    if (x == -INFINITY) v = nullptr;
+    return x;
   };
   float top = -INFINITY, sum = 0.f, o[E] = {};
   for (int j = 0; j < keys; j += 64) {
@@ -947,27 +947,31 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
     top = fmaxf(top, score(j + lane, v));
   }
   top = wave_max(top);
+  // a weight too small for fp32 is still not zero: it keeps an infinity one
+  auto above_zero = [](float p) { return fmaxf(p, 1.17549435e-38f); };
+  auto weight = [&](float x, const uint16_t* v) {
+    return !v ? 0.f : x != x || top == INFINITY ? NAN : above_zero(__builtin_amdgcn_exp2f(x - top));
+  };
   for (int j = 0; j < keys; j += 64) {
     const uint16_t* v;
     const float x = score(j + lane, v);
-    // a weight too small for fp32 is still not zero: it keeps an infinity one
-    float p = fmaxf(__builtin_amdgcn_exp2f(x - top), 1.17549435e-38f);
-    if (x != x || top == INFINITY)
-      p = NAN;
-    else if (top == -INFINITY)
-      p = 0.f;
-    if (!v) p = 0.f;
-    sum += p;
-    const unsigned long long seen = __ballot(v != nullptr);
-    for (unsigned long long left = seen; left; left &= left - 1) {
-      const int i = __ffsll(static_cast<unsigned long long>(left)) - 1;
-      const float pi = __shfl(p, i, 64);
-      const uintptr_t vi = static_cast<uintptr_t>(__shfl(static_cast<unsigned long long>(reinterpret_cast<uintptr_t>(v)), i, 64));
-      for (int e = 0; e < E; ++e) o[e] += pi * widen<F16>(reinterpret_cast<const uint16_t*>(vi)[lane * E + e]);
-    }
+    sum += weight(x, v);
   }
   sum = wave_sum(sum);
-  for (int e = 0; e < E; ++e) out[lane * E + e] = narrow<F16>(sum == 0.f ? 0.f : o[e] / sum);
+  const float inv = 1.f / sum;
+  if (sum == sum && sum != 0.f)
+    for (int j = 0; j < keys; j += 64) {
+      const uint16_t* v;
+      const float x = score(j + lane, v), p = above_zero(weight(x, v) * inv);  // divided first: sums of the largest values stay finite
+      const unsigned long long seen = __ballot(v != nullptr);
+      for (unsigned long long left = seen; left; left &= left - 1) {
+        const int i = __ffsll(static_cast<unsigned long long>(left)) - 1;
+        const float pi = __shfl(p, i, 64);
+        const uintptr_t vi = static_cast<uintptr_t>(__shfl(static_cast<unsigned long long>(reinterpret_cast<uintptr_t>(v)), i, 64));
+        for (int e = 0; e < E; ++e) o[e] += pi * widen<F16>(reinterpret_cast<const uint16_t*>(vi)[lane * E + e]);
+      }
+    }
+  for (int e = 0; e < E; ++e) out[lane * E + e] = narrow<F16>(sum != sum ? NAN : o[e]);
 }
 
 // Workgroups that fit the 256 CUs at once, by LDS (a ring takes 64 KiB with
@@ -1064,7 +1068,7 @@ extern "C" int iron_tree_attention(const void* q, const void* k_new, const void*
   for (const void* p : {page_table, seq_lens, node_starts, tree_mask})
     IRON_REQUIRE(p && (reinterpret_cast<uintptr_t>(p) & 3u) == 0, "%s: int32 arrays must be given and 4-byte aligned", who);
   for (const void* p : {q, k_new, v_new, k_pages, v_pages}) IRON_REQUIRE(out != p, "%s: out is one of the inputs", who);
-  IRON_REQUIRE(scale > 0.f && scale < INFINITY, "%s: scale=%g must be positive and finite", who, scale);
+  IRON_REQUIRE(scale > 0.f && scale <= 1e30f, "%s: scale=%g must be positive and at most 1e30", who, scale);
   const long long need = iron_tree_attention_workspace_bytes(n_heads, n_kv_heads, head_dim, num_seqs, num_nodes,
                                                              max_nodes, max_pages, page_size);
   IRON_REQUIRE(workspace && aligned16(workspace), "%s: the workspace must be given and 16-byte aligned", who);

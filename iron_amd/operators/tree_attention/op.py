@@ -19,8 +19,8 @@ h // (H / Hkv). bf16 or fp16 (``dtype``), D 64 or 128.
 
 A row that sees nothing gets zeros; rows of out behind the last tree are left
 as they were. What a node does not see does not reach its row, whatever it
-holds; a row whose scores are all -inf is one that sees nothing. Scores, softmax
-and sums are fp32; the weights enter the product with V with 16 bits, or rounded
+holds; a key whose score is -inf counts as one that it does not see. Scores,
+softmax and sums are fp32; the weights enter the product with V with 16 bits, or rounded
 to ``dtype`` (as in MHA) where a KV head has more than 32 rows, max_nodes times
 H / Hkv. Kernel: iron_tree_attention.
 """
@@ -65,8 +65,8 @@ class TreeAttention(PagedOperator):
             raise ValueError(f"dtype must be torch.bfloat16 or torch.float16, got {self.dtype!r}")
         if self.scale is None:
             self.scale = 1.0 / math.sqrt(self.head_dim)
-        if not 0 < self.scale < math.inf:
-            raise ValueError(f"scale must be positive and finite, got {self.scale}")
+        if not 0 < self.scale <= 1e30:
+            raise ValueError(f"scale must be positive and at most 1e30, got {self.scale}")
         PagedOperator.__init__(self, context=self.context)
 
     @property

@@ -23,7 +23,7 @@ TREE = dict(num_heads=4, num_kv_heads=2, head_dim=64, num_nodes=6, max_nodes=5, 
     ("TreeAttention", TREE, dict(num_seqs=8193), "num_seqs"),
     ("TreeAttention", TREE, dict(max_pages=1 << 27), "2\\*\\*31"),
     ("TreeAttention", TREE, dict(scale=0.0), "scale"),
-    ("TreeAttention", TREE, dict(scale=float("nan")), "scale"),
+    ("TreeAttention", TREE, dict(scale=float("nan")), "scale"), ("TreeAttention", TREE, dict(scale=1e31), "scale"),
     ("TreeAttention", TREE, dict(num_pages=2.0), "must be an int"),
     ("PagedAppend", dict(num_nodes=6, num_rows=4, **DATA), dict(num_rows=0), "num_rows"),
     ("PagedAppend", dict(num_nodes=6, num_rows=4, **DATA), dict(head_dim=7), "multiple of 16"),
@@ -94,7 +94,7 @@ def _tree(q=P, out=2 * P, dtype=0, H=4, Hkv=2, D=64, pages=8, ps=16, S=2, mp=4, 
     (dict(vp=2 * P), "one of the inputs"),
     (dict(dtype=2), "dtype=2"), (dict(H=3), "multiple"), (dict(D=32), "64 or 128"), (dict(pages=0), "num_pages=0"),
     (dict(ps=24), "power of two"), (dict(S=0), "num_seqs"), (dict(mp=0), "max_pages"), (dict(N=0), "num_nodes"),
-    (dict(T=2000), "max_nodes"), (dict(scale=-1.0), "scale"), (dict(ws=None), "workspace"), (dict(size=0), "workspace of 0 bytes"),
+    (dict(T=2000), "max_nodes"), (dict(scale=-1.0), "scale"), (dict(scale=1e31), "scale"), (dict(ws=None), "workspace"), (dict(size=0), "workspace of 0 bytes"),
 ])
 def test_tree_attention_entry_point_refuses(kw, match):
     with pytest.raises(_lib.IronHipError, match=match):

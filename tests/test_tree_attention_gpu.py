@@ -190,9 +190,9 @@ def test_cached_values_that_are_not_finite(gpu):
 
 
 @pytest.mark.parametrize("nodes", [3, 30])  # 12 and 120 rows to a KV head
-@pytest.mark.parametrize("behind", [0.0, float("nan")])
+@pytest.mark.parametrize("behind", [0.0, float("nan"), float("inf")])
 def test_scores_of_minus_infinity(gpu, behind, nodes):
-    """Such a key has no weight; a row that sees no other is a row that sees nothing, also where it is done over."""
+    """Such a key has no weight, whatever its value; a row that sees no other is a row that sees nothing."""
     c = Case(4, 1, 64, 16, [37, 100], [nodes, 1], seed=28)
     c.q[:] = c.q.abs() + 0.125
     n = c.starts[1]
@@ -200,17 +200,31 @@ def test_scores_of_minus_infinity(gpu, behind, nodes):
         c.kp[p] = -float("inf")
     c.kn[:n] = -float("inf")
     c.vp[c.table[0, 2], :, 5:] = behind  # behind the last position
-    c.kp[c.table[1, 0], :, 3] = -float("inf")
+    c.kp[c.table[1, 0], :, 3], c.vp[c.table[1, 0], :, 3] = -float("inf"), behind
+    c.vn[:n, :, 7] = behind
     t = c.tensors(gpu)
     c.op.get_callable()(*t)
     torch.cuda.synchronize()
     got = t[-1].cpu().double()
     assert (got[:n] == 0).all()
     c.kp[c.table[1, 0], :, 3] = c.q[n:n + 1].mean(1) * -1e4  # a weight of zero in 64 bits too
-    c.kp[c.table[0, :3]], c.kn[:n] = 0.0, 0.0
-    c.vp[c.table[0, 2]] = 0.0
+    c.kp[c.table[0, :3]], c.kn[:n], c.vn[:n] = 0.0, 0.0, 0.0
+    c.vp[c.table[0, 2]], c.vp[c.table[1, 0], :, 3] = 0.0, 0.0
     want, tol = c.want()
     assert ((got - want).abs() <= tol)[n].all()
+
+
+@pytest.mark.parametrize("D,dtype", [(64, BF16), (128, BF16), (128, FP16)])
+@pytest.mark.parametrize("nodes", [3, 30])
+def test_the_largest_values(gpu, nodes, D, dtype):
+    """A mean of values at the end of the type's range is one: no sum on the way overflows."""
+    c = Case(4, 1, D, 16, [70, 5], [nodes, 1], dtype, seed=30)
+    most = torch.finfo(dtype).max
+    c.vp[:], c.vn[:] = most, -most
+    c.check(gpu)
+    c.vn[:] = most
+    c.q[:] = 0.0
+    assert (c.check(gpu)[:nodes + 1] >= most * (1 - 2 * torch.finfo(dtype).eps)).all()
 
 
 @pytest.mark.parametrize("nodes", [3, 30])
