@@ -92,6 +92,7 @@ class PagedOperator(HIPOperator):
         need = self.workspace_bytes()
         space = ()
         if need:
-            ws = torch.empty(need, dtype=torch.uint8, device=device)
+            # below 0: a shape that the entry point refuses, saying why
+            ws = torch.empty(max(need, 0), dtype=torch.uint8, device=device)
             space = (ws.data_ptr(), need)
         _lib.call(entry, *[t.data_ptr() for t in tensors], *numbers, *space, stream)

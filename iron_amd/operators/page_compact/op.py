@@ -39,6 +39,8 @@ class PageCompact(PagedOperator):
     def __post_init__(self):
         self._check_pool()
         self._check_data()
+        if self.num_seqs * -(-self.max_pages // 1024) >= 1 << 23:
+            raise ValueError(f"num_seqs={self.num_seqs} with max_pages={self.max_pages}: a table of up to 2**33 entries")
         PagedOperator.__init__(self, context=self.context)
 
     def workspace_bytes(self) -> int:

@@ -53,7 +53,8 @@ class PageFork(PagedOperator):
         PagedOperator.__init__(self, context=self.context)
 
     def workspace_bytes(self) -> int:
-        return _lib.workspace_bytes("iron_page_fork_workspace_bytes", self.num_forks, self.num_seqs, self.max_pages, self.num_pages, int(bool(self.share)))
+        return _lib.workspace_bytes("iron_page_fork_workspace_bytes", self.num_forks, self.num_seqs, self.max_pages,
+                                    self.num_pages, int(bool(self.share)))
 
     def get_arg_spec(self):
         return [

@@ -25,6 +25,7 @@ TREE = dict(num_heads=4, num_kv_heads=2, head_dim=64, num_nodes=6, max_nodes=5, 
     ("TreeAttention", TREE, dict(scale=0.0), "scale"),
     ("TreeAttention", TREE, dict(scale=float("nan")), "scale"), ("TreeAttention", TREE, dict(scale=1e31), "scale"),
     ("TreeAttention", TREE, dict(num_pages=2.0), "must be an int"),
+    ("PageCompact", DATA, dict(num_seqs=8192, max_pages=1 << 20), "2\\*\\*33"),
     ("PagedAppend", dict(num_nodes=6, num_rows=4, **DATA), dict(num_rows=0), "num_rows"),
     ("PagedAppend", dict(num_nodes=6, num_rows=4, **DATA), dict(head_dim=7), "multiple of 16"),
     ("PagedAppend", dict(num_nodes=6, num_rows=4, **DATA), dict(dtype="bf16"), "torch dtype"),

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import iron_amd.operators as ops
+from iron_amd import _lib
 from iron_amd.common.graph import capture_graph
 from tests import paged_reference as ref
 
@@ -314,6 +315,14 @@ def test_a_thousand_sequences(gpu):
 def test_the_largest_trees(gpu):
     Case(2, 2, 64, 16, [40], [1024], seed=24, mask="random").check(gpu)
     Case(2, 1, 128, 16, [0, 300], [1000, 24], FP16, seed=25).check(gpu)
+
+
+def test_more_blocks_than_can_be_counted_are_refused(gpu):
+    op = ops.TreeAttention(num_heads=1024, num_kv_heads=1024, head_dim=64, num_pages=1, page_size=16, num_seqs=64, max_pages=8192,
+                           num_nodes=1, max_nodes=1024)
+    args = [torch.zeros(s.shape, dtype=s.dtype, device=gpu) for s in op.get_arg_spec()]
+    with pytest.raises(_lib.IronHipError, match="must count below 2\\^31"):
+        op.get_callable()(*args)
 
 
 def test_long_context(gpu):
