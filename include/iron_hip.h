@@ -360,7 +360,8 @@ int iron_attention_prefill(const void* q, const void* k, const void* v, void* ou
 enum iron_page_status {
   IRON_PAGE_DONE = 0,
   IRON_PAGE_INVALID = 1, /* a slot outside the table or named twice, a length outside [0, max_pages * page_size],
-                            a fork onto itself or onto a sequence that is not empty */
+                            a fork onto itself or onto a sequence that is not empty, a range of rows to append that
+                            leaves the rows, ends before its start or overlaps an earlier one */
   IRON_PAGE_NO_ROOM = 2, /* too few free pages, or the table row is too short */
   IRON_PAGE_NOT_OWN = 3  /* append: the partly filled last page is a hole or held by another entry too */
 };
@@ -401,8 +402,11 @@ int iron_tree_attention(const void* q, const void* k_new, const void* v_new, con
  * outside [0, num_nodes) appends zeros. Elements of any type: row_bytes is
  * head_dim times their size, a multiple of 16. status (num_seqs). A sequence
  * that cannot grow by all its rows is left as it was; where the free pages run
- * out, so are all later ones that need any. row_starts (num_seqs + 1) must not
- * decrease. num_rows at most 2^20. The paged form of the KV-cache append
+ * out, so are all later ones that need any. row_starts (num_seqs + 1) does not
+ * decrease and stays in [0, num_rows]: a sequence whose range has rows and leaves
+ * them, ends before its start or starts below an earlier entry of row_starts gets
+ * IRON_PAGE_INVALID (so does the last one where more rows were accepted than a
+ * captured call has room for). num_rows at most 2^20. The paged form of the KV-cache append
  * (StridedCopy of iron/applications/llama_3.2_1b/llama_npu.py:311-323). */
 long long iron_paged_append_workspace_bytes(int num_seqs, int num_rows, int page_size);
 int iron_paged_append(const void* k_new, const void* v_new, const int* rows, const int* row_starts, void* k_pages,

@@ -18,6 +18,7 @@
 #include "../../include/iron_hip.h"
 
 #include <algorithm>
+#include <climits>
 
 namespace iron {
 namespace {
@@ -176,12 +177,39 @@ struct AppendArgs {
   int num_nodes, num_rows, list_cap;
 };
 
-// Rows [first, first + count) of the call are sequence s's. Ends that lie
-// outside the rows or before their start are moved there: no entry of
-// row_starts can lead out of the arrays.
-__device__ __forceinline__ void row_range(const AppendArgs& a, int s, int& first, int& count) {
-  first = min(max(a.row_starts[s], 0), a.num_rows);
-  count = min(max(a.row_starts[s + 1], first), a.num_rows) - first;
+// Rows [first, stop) of the call are sequence s's, all of them or none: a range
+// that leaves the rows or ends before its start is no range (one without rows is,
+// wherever it lies).
+__device__ __forceinline__ bool range_fits(const AppendArgs& a, int first, int stop) {
+  return first == stop || (0 <= first && first < stop && stop <= a.num_rows);
+}
+
+// row_starts decreases somewhere: a range with rows that starts below an earlier
+// entry would take rows that an earlier range has, so its sequence gets none. The
+// largest entry so far is a running maximum over the workgroup. Every thread calls it.
+__device__ void refuse_overlaps(const AppendArgs& a, int* need, int* grow, int* tmp) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = a.pool.num_seqs;
+  int carry = INT_MIN;
+  for (int b = 0; b < n; b += kPlan) {
+    const int s = b + threadIdx.x, x = s < n ? a.row_starts[s] : INT_MIN;
+    int top = x;
+    for (int d = 1; d < 64; d *= 2) {
+      const int y = __shfl_up(top, d, 64);
+      if (lane >= d) top = max(top, y);
+    }
+    __syncthreads();  // tmp is free
+    if (lane == 63) tmp[w] = top;
+    __syncthreads();
+    top = max(top, carry);
+    for (int i = 0; i < kPlan / 64; ++i) {
+      if (i < w) top = max(top, tmp[i]);
+      carry = max(carry, tmp[i]);
+    }
+    if (s < n && grow[s] >> 2 > 0 && x < top) {
+      need[s] = 0;
+      grow[s] = PAGE_INVALID;
+    }
+  }
 }
 
 // Decides which sequences grow, gives them pages and moves their lengths. One
@@ -196,12 +224,14 @@ __global__ __launch_bounds__(kPlan) void append_plan_kernel(AppendArgs a) {
   static_assert(kMaxRows <= 1 << 28 && PAGE_NOT_OWN < 4, "both fit");
   const Pool& p = a.pool;
   const int4 front = counts4(p.refs, 4 * threadIdx.x, p.num_pages);
+  bool decreases = false;
   for (int s = threadIdx.x; s < p.num_seqs; s += kPlan) {
-    int first, count;
-    row_range(a, s, first, count);
-    const int len = p.lens[s];
+    const int first = a.row_starts[s], stop = a.row_starts[s + 1], len = p.lens[s];
+    const bool fits = range_fits(a, first, stop);
+    const int count = fits ? stop - first : 0;
     int st = PAGE_DONE, n = 0;
-    if (!p.len_fits(len)) {
+    decreases |= stop < first;
+    if (!fits || !p.len_fits(len)) {
       st = PAGE_INVALID;
     } else if (!p.len_fits(static_cast<long long>(len) + count)) {
       st = PAGE_NO_ROOM;
@@ -216,7 +246,7 @@ __global__ __launch_bounds__(kPlan) void append_plan_kernel(AppendArgs a) {
     lens[s] = len;
     grow[s] = count << 2 | st;
   }
-  __syncthreads();
+  if (__syncthreads_or(decreases)) refuse_overlaps(a, need, grow, tmp);
   const int want = scan_requests(need, p.num_seqs, tmp);
   const int have = find_free(p.refs, p.num_pages, min(want, a.list_cap), a.list, tmp, front);
   for (int s = threadIdx.x; s < p.num_seqs; s += kPlan) {
@@ -244,15 +274,11 @@ __global__ __launch_bounds__(256) void append_rows_kernel(AppendArgs a, int grou
   if (threadIdx.x == 0) owner = -1;
   __syncthreads();
   for (int s = threadIdx.x; s < p.num_seqs; s += 256)
-    if (a.row_starts[s] <= r && r < a.row_starts[s + 1]) atomicMax(&owner, s);
+    if (a.row_starts[s] <= r && r < a.row_starts[s + 1] && a.begin[s] >= 0) owner = s;  // one at most: the plan lets no two share a row
   __syncthreads();
   const int s = owner;
   if (s < 0) return;
-  int first, count;
-  row_range(a, s, first, count);
-  const int begin = a.begin[s], src = a.rows[r], i = r - first;
-  if (begin < 0 || i < 0 || i >= count) return;
-  const int pos = begin + i;
+  const int src = a.rows[r], pos = a.begin[s] + (r - a.row_starts[s]);
   const int page = p.table[static_cast<long long>(s) * p.max_pages + pos / p.page_size];
   if (!p.in_pool(page)) return;
   const bool real = static_cast<unsigned>(src) < static_cast<unsigned>(a.num_nodes);

@@ -10,9 +10,11 @@ is full, seq_lens grows. A row number outside [0, num_nodes) appends zeros.
 Arg spec: k_new and v_new (num_layers, num_nodes, Hkv, D), rows (num_rows,),
 row_starts (num_seqs + 1,) int32, the cache (k_pages, v_pages, page_table,
 seq_lens, page_refs; iron_amd.common.paging), status (num_seqs,) int32:
-0 done, 1 the sequence's length is invalid, 2 too few free pages or table
-entries, 3 its partly filled last page is a hole or shared. A sequence with a
-status other than 0 is left as it was. Any dtype whose rows are a multiple of
+0 done, 1 the sequence's length or its range of rows is invalid (the range has
+rows and leaves [0, num_rows], ends before its start or starts below an earlier
+entry of row_starts), 2 too few free pages or table entries, 3 its partly filled
+last page is a hole or shared. A sequence with a status other than 0 is left as
+it was. Any dtype whose rows are a multiple of
 16 bytes. Kernel: iron_paged_append.
 """
 

@@ -78,7 +78,9 @@ def append(cache, k_new, v_new, rows, starts):
     for s in range(len(cache.lens)):
         n, count = int(cache.lens[s]), starts[s + 1] - starts[s]
         st = DONE
-        if not cache.fits(n):
+        if count and not max(0, *starts[:s + 1]) <= starts[s] <= starts[s + 1] <= len(rows):
+            st, count = INVALID, 0  # leaves the rows, ends before its start, or starts before an earlier range did or ended
+        elif not cache.fits(n):
             st = INVALID
         elif not cache.fits(n + count):
             st = NO_ROOM

@@ -319,3 +319,36 @@ def test_other_streams(gpu):
     torch.cuda.synchronize()
     for c, st, t in zip(cases, states, told):
         assert t.tolist() == ref.fork(c, [(0, 6), (3, 7)], False) and all(c.same(st))
+
+
+@pytest.mark.parametrize("starts,status", [
+    ([0, 3, 8, 13, 13, 13], [0, 0, 1, 0, 0]),                    # one row more than there are: the sequence stays whole as it was
+    ([0, 3, 1 << 30, 1 << 30, 1 << 30, 1 << 30], [0, 1, 0, 0, 0]),  # and those that have no rows are done wherever they lie
+    ([-1, 3, 8, 12, 12, 12], [1, 0, 0, 0, 0]),
+    ([2, 3, 8, 8, 8, 12], [0, 0, 0, 0, 0]),                      # rows before the first range are nobody's
+    ([0, 8, 4, 10, 10, 12], [0, 1, 1, 0, 0]),                    # a range that ends before its start, and one on an earlier one's rows
+    ([0, 10, 2, 6, 8, 12], [0, 1, 1, 1, 1]),
+    ([0, 4, 4, 4, 3, 7], [0, 0, 0, 1, 1]),
+    ([9, 5, 5, 7, 12, 12], [1, 0, 1, 1, 0]),
+    ([-(1 << 31), (1 << 31) - 1, 0, 12, 12, 12], [1, 1, 1, 0, 0]),
+    ([12, 0, 0, 0, 0, 0], [1, 0, 0, 0, 0]),
+])
+def test_append_ranges_that_are_none(gpu, starts, status):
+    """A sequence gets all rows of its range or none: ranges that leave the rows, decrease or overlap change nothing, and
+    rows that two ranges name are the first one's."""
+    print(f"append row_starts {starts}", flush=True)
+    c = _filled(31, pages=60, seqs=5, max_pages=6, lens=[5, 20, 33, 0, 16])
+    got, state, (kn, vn, rows, starts) = _append(gpu, c, [3, 3, 3, 2, 1], 31, starts=starts)
+    assert got == status == ref.append(c, kn, vn, rows, starts) and all(c.same(state))
+
+
+def test_append_ranges_of_many_sequences(gpu):
+    """More sequences than threads of the planning workgroup: a range far behind one that it overlaps."""
+    c = _filled(32, pages=3000, seqs=2600, max_pages=2, layers=1, kv_heads=1, dim=8, lens=[s % 17 for s in range(2600)])
+    starts = [0] + list(np.cumsum([1] * 2600))
+    starts[1030] = 1035                   # the ranges after it start before its end, up to that of row 1035
+    starts[2100:2200] = [900] * 100       # one that decreases, then empty ones, then one over all rows from 900 on
+    got, state, (kn, vn, rows, starts) = _append(gpu, c, [1] * 2600, 32, starts=starts)
+    want = ref.append(c, kn, vn, rows, starts)
+    assert got == want and all(c.same(state))
+    assert [s for s in range(2600) if got[s]] == [*range(1030, 1035), 2099, 2199]
