@@ -158,6 +158,14 @@ __device__ __forceinline__ float row_sum(float a) {
   return x + y;
 }
 
+// A weight is 2^(s c - m) with one rounding, while m is the largest s c rounded:
+// the largest weight is 2^d instead of 1, d up to half a step of m. Sums and
+// products carry the same factor, so that it cancels, as long as weights fit their
+// 16 bits: fp16 takes them up to 2^14 lifted, so d may be 1 (m up to 2^24). A row
+// whose maximum lies farther out (or is infinite) is done over by the join, which
+// rounds every s c before it subtracts.
+__device__ __forceinline__ bool far_out(float m) { return fabsf(m) > 0x1p24f && m != -INFINITY; }
+
 // A word of memory that does not change during the launch, at a uniform
 // address: a scalar load, which does not wait for the loads in flight.
 __device__ __forceinline__ int uniform_word(const int* p, long long i) {
@@ -535,6 +543,7 @@ __global__ __launch_bounds__(256) void tree_attention_kernel(TreeArgs a) {
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
           ta_u32x2 y;
           if (sum == 0.f) v = ta_f32x4{0.f, 0.f, 0.f, 0.f};
+          if (far_out(top)) v = ta_f32x4{NAN, NAN, NAN, NAN};  // for the launch that joins the parts
           y.x = narrow<F16>(v[0] * inv) | static_cast<unsigned>(narrow<F16>(v[1] * inv)) << 16;
           y.y = narrow<F16>(v[2] * inv) | static_cast<unsigned>(narrow<F16>(v[3] * inv)) << 16;
           const int row = row0 + r;
@@ -809,6 +818,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void tree_wide_kernel(TreeArg
       float l0, l1;
       swap32(l, l0, l1);
       const float sum = l0 + l1;
+      const bool far = whole && far_out(m);  // NaN, for the launch that joins the parts
       if (32 * w + c < rows) {
         const long long part = (2LL * blockIdx.x + (blk0 == 0 ? 1 : 0)) * R + 32 * w + c;
         const float inv = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
@@ -820,7 +830,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void tree_wide_kernel(TreeArg
             const int dim = 32 * db + 8 * q + 4 * hh;
             ta_f32x4 v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = sum == 0.f ? 0.f : o[db][4 * q + e] * inv;
+            for (int e = 0; e < 4; ++e) v[e] = far ? NAN : sum == 0.f ? 0.f : o[db][4 * q + e] * inv;
             if (whole) {
               ta_u32x2 z;
               z.x = narrow<F16>(v[0]) | static_cast<unsigned>(narrow<F16>(v[1])) << 16;
@@ -844,8 +854,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void tree_wide_kernel(TreeArg
 
 // One workgroup per node and 4 heads, a wave for each row: joins the parts of
 // rows whose keys were shared out, and does over the rows that came out
-// infinite or NaN, one key at a time and only the keys that have a weight (a
-// product with a weight of zero lets what is not seen through).
+// infinite or NaN (or whose scores lie too far out: far_out), one key at a time
+// and only the keys that have a weight (a product with a weight of zero lets what
+// is not seen through).
 template <int D, bool F16, int R, int B>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
   constexpr int E = D / 64, V4 = D / 4, NP = 64 / V4;  // parts added at a time
@@ -879,6 +890,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
     float top = ml.x;
     for (int i = 64 + lane; i < parts; i += 64) top = fmaxf(top, a.part_ml[slot(i)].x);
     top = wave_max(top);
+    again |= far_out(top);
     float sum = 0.f;
     ta_f32x4 v = {0.f, 0.f, 0.f, 0.f};
     for (int i0 = 0; i0 < parts; i0 += 64) {

@@ -524,3 +524,41 @@ def test_a_conversation(gpu):
     kn, vn, starts = verify([1, 5, 6], 5)
     add(kn, vn, list(range(starts[0], starts[3])), starts)
     verify([7, 7, 7], 6)
+
+
+def _one_dim(c, q, rows):
+    """q and keys with one component: a score is one product, exact in 32 bits. rows: (sequence, position) -> key, the rest 0."""
+    c.q[:], c.kp[:], c.kn[:] = 0.0, 0.0, 0.0
+    c.q[:, :, 3] = q
+    for (s, t), k in rows.items():
+        c.kp[c.table[s, t // c.ps], :, t % c.ps, 3] = k
+
+
+@pytest.mark.parametrize("dtype,D,sizes", [(BF16, 64, (2.0 ** 7, 2.0 ** 12, 2.0 ** 17, 2.0 ** 30)), (BF16, 128, (2.0 ** 13, 2.0 ** 25)),
+                                           (FP16, 64, (2.0 ** 7, 2.0 ** 10, 2.0 ** 13, 2.0 ** 15)), (FP16, 128, (2.0 ** 12, 2.0 ** 14))])
+@pytest.mark.parametrize("nodes", [3, 30])  # 12 and 120 rows to a KV head
+@pytest.mark.parametrize("length", [70, 5000])  # keys of one workgroup or two, and of many
+def test_scores_far_from_zero(gpu, dtype, D, sizes, nodes, length):
+    """Scores up to 2^62, far enough apart that all weight is the largest one's, or shared by two that are equal: the row is
+    that value, or the mean of the two, whatever the size and the sign of the scores."""
+    for size in sizes:
+        for sign in (1.0, -1.0):
+            print(f"scores of {size} squared, sign {sign}, {dtype} D {D} nodes {nodes}", flush=True)
+            c = Case(4, 1, D, 16, [length, 33], [nodes, 2], dtype, seed=35, mask="none", scale=1.0)
+            row = torch.arange(c.N * 4, dtype=torch.float32).view(c.N, 4)
+            _one_dim(c, (size * (1 + row % 61 / 64)).to(dtype), {})
+            c.kp[c.table[0, :-(-length // 16)], :, :, 3] = -size * 1.5
+            c.kp[c.table[1, :3], :, :, 3] = -size * 1.5
+            at = [(0, 21), (0, 66), (1, 32)]
+            for s, t in at:
+                c.kp[c.table[s, t // 16], :, t % 16, 3] = sign * size
+            t = c.tensors(gpu)
+            c.op.get_callable()(*t)
+            torch.cuda.synchronize()
+            got = t[-1].cpu().double()
+            v = [c.vp[c.table[s, t // 16], 0, t % 16].double() for s, t in at]
+            want = torch.cat([((v[0] + v[1]) / 2).expand(nodes, 4, D), v[2].expand(2, 4, D)])
+            size_of = torch.cat([((v[0].abs() + v[1].abs()) / 2).expand(nodes, 4, D), v[2].abs().expand(2, 4, D)])
+            tol = want.abs() * torch.finfo(dtype).eps / 2 + size_of * 2.0 ** -15  # equal weights of 16 bits, and their sum's
+            assert ((got[:nodes + 2] - want).abs() <= tol).all(), (size, sign)
+
