@@ -895,9 +895,9 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
     ta_f32x4 v = {0.f, 0.f, 0.f, 0.f};
     for (int i0 = 0; i0 < parts; i0 += 64) {
       if (i0) ml = i0 + lane < parts ? a.part_ml[slot(i0 + lane)] : make_float2(-INFINITY, 0.f);
-      // the weight of part i0 + lane, 0 for a part that saw nothing; one too small
-      // for fp32 is not: it keeps an infinity one
-      const float f = ml.y == 0.f ? 0.f : fmaxf(__builtin_amdgcn_exp2f(ml.x - top), 1.17549435e-38f);
+      // the weight of part i0 + lane, below 0 for a part that saw nothing. One too small
+      // for fp32 is 0, and makes NaN of an infinite sum, which has the row done over.
+      const float f = ml.y == 0.f ? -1.f : __builtin_amdgcn_exp2f(ml.x - top);
       sum += ml.y == 0.f ? 0.f : f * ml.y;
       for (int i = 0; i < min(parts - i0, 64); i += kAhead * NP) {
         if (i0 + i) load(i0 + i);
@@ -906,7 +906,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
           const int j = i + k * NP + g;
           const float fj = __shfl(f, j, 64);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] += fj == 0.f ? 0.f : fj * x[k][e];
+          for (int e = 0; e < 4; ++e) v[e] += fj < 0.f ? 0.f : fj * x[k][e];
         }
       }
     }
@@ -959,10 +959,8 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
     top = fmaxf(top, score(j + lane, v));
   }
   top = wave_max(top);
-  // a weight too small for fp32 is still not zero: it keeps an infinity one
-  auto above_zero = [](float p) { return fmaxf(p, 1.17549435e-38f); };
   auto weight = [&](float x, const uint16_t* v) {
-    return !v ? 0.f : x != x || top == INFINITY ? NAN : above_zero(__builtin_amdgcn_exp2f(x - top));
+    return !v ? 0.f : x != x || top == INFINITY ? NAN : __builtin_amdgcn_exp2f(x - top);
   };
   for (int j = 0; j < keys; j += 64) {
     const uint16_t* v;
@@ -974,13 +972,17 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
   if (sum == sum && sum != 0.f)
     for (int j = 0; j < keys; j += 64) {
       const uint16_t* v;
-      const float x = score(j + lane, v), p = above_zero(weight(x, v) * inv);  // divided first: sums of the largest values stay finite
+      const float x = score(j + lane, v), p = weight(x, v) * inv;  // divided first: sums of the largest values stay finite
       const unsigned long long seen = __ballot(v != nullptr);
       for (unsigned long long left = seen; left; left &= left - 1) {
         const int i = __ffsll(static_cast<unsigned long long>(left)) - 1;
         const float pi = __shfl(p, i, 64);
         const uintptr_t vi = static_cast<uintptr_t>(__shfl(static_cast<unsigned long long>(reinterpret_cast<uintptr_t>(v)), i, 64));
-        for (int e = 0; e < E; ++e) o[e] += pi * widen<F16>(reinterpret_cast<const uint16_t*>(vi)[lane * E + e]);
+        for (int e = 0; e < E; ++e) {
+          const float x = widen<F16>(reinterpret_cast<const uint16_t*>(vi)[lane * E + e]);
+          // a weight too small for fp32 is still not zero: an infinity stays one
+          o[e] += (__builtin_isinf(x) ? fmaxf(pi, 1.17549435e-38f) : pi) * x;
+        }
       }
     }
   for (int e = 0; e < E; ++e) out[lane * E + e] = narrow<F16>(sum != sum ? NAN : o[e]);

@@ -562,3 +562,27 @@ def test_scores_far_from_zero(gpu, dtype, D, sizes, nodes, length):
             tol = want.abs() * torch.finfo(dtype).eps / 2 + size_of * 2.0 ** -15  # equal weights of 16 bits, and their sum's
             assert ((got[:nodes + 2] - want).abs() <= tol).all(), (size, sign)
 
+
+
+@pytest.mark.parametrize("infinity", [False, True])
+@pytest.mark.parametrize("nodes", [3, 30])
+def test_values_behind_far_lower_scores(gpu, nodes, infinity):
+    """Keys whose weight is e^-200: values of 1e36 there do not show in rows of small ones, however many workgroups the keys
+    went to, and not where an infinity in another dimension has the row done over."""
+    c = Case(4, 1, 64, 16, [5000, 20], [nodes, 2], seed=36, mask="none", scale=1.0)
+    _one_dim(c, 8.0, {(0, t): -25.0 if t % 5000 != 4321 else 0.0 for t in range(5000)})
+    c.vp[:] = 1e36
+    c.vp[c.table[0, 4321 // 16], :, 4321 % 16] = torch.randn(64, generator=torch.Generator().manual_seed(37)).to(BF16)
+    c.vp[c.table[1, :2]] = 1.0
+    if infinity:
+        c.vp[c.table[0, 7], :, 9, 40] = float("inf")
+    t = c.tensors(gpu)
+    c.op.get_callable()(*t)
+    torch.cuda.synchronize()
+    got = t[-1].cpu().double()
+    dims = [d for d in range(64) if not infinity or d != 40]
+    want = c.vp[c.table[0, 4321 // 16], 0, 4321 % 16].double()
+    assert ((got[:nodes] - want).abs() <= want.abs() * 2.0 ** -8)[:, :, dims].all(), (got[:nodes] - want).abs()[:, :, dims].max()
+    if infinity:
+        assert (got[:nodes, :, 40] == float("inf")).all()
+    assert (got[nodes:nodes + 2] == 1).all()
