@@ -246,7 +246,13 @@ __global__ __launch_bounds__(kPlan) void append_plan_kernel(AppendArgs a) {
     lens[s] = len;
     grow[s] = count << 2 | st;
   }
-  if (__syncthreads_or(decreases)) refuse_overlaps(a, need, grow, tmp);
+  decreases = __ballot(decreases) != 0;
+  if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = decreases;
+  __syncthreads();
+  int any = 0;
+#pragma unroll
+  for (int i = 0; i < kPlan / 64; ++i) any |= tmp[i];
+  if (__builtin_expect(any, 0)) refuse_overlaps(a, need, grow, tmp);
   const int want = scan_requests(need, p.num_seqs, tmp);
   const int have = find_free(p.refs, p.num_pages, min(want, a.list_cap), a.list, tmp, front);
   for (int s = threadIdx.x; s < p.num_seqs; s += kPlan) {
@@ -268,17 +274,21 @@ __global__ __launch_bounds__(kPlan) void append_plan_kernel(AppendArgs a) {
 // One row of the call in `group` layers: K and V of every KV head. Bound by
 // memory: 437 MB (four prompts, 16 layers) in 91 us, 4.8 TB/s.
 __global__ __launch_bounds__(256) void append_rows_kernel(AppendArgs a, int group) {
-  __shared__ int owner;
+  __shared__ int owner, to_pos;
   const Pool& p = a.pool;
-  const int r = blockIdx.x;
+  const int r = blockIdx.x, src = a.rows[r];
   if (threadIdx.x == 0) owner = -1;
   __syncthreads();
-  for (int s = threadIdx.x; s < p.num_seqs; s += 256)
-    if (a.row_starts[s] <= r && r < a.row_starts[s + 1] && a.begin[s] >= 0) owner = s;  // one at most: the plan lets no two share a row
+  for (int s = threadIdx.x; s < p.num_seqs; s += 256) {
+    const int first = a.row_starts[s], stop = a.row_starts[s + 1], begin = a.begin[s];  // one round trip
+    if (first <= r && r < stop && begin >= 0) {  // one sequence at most: the plan lets no two share a row
+      owner = s;
+      to_pos = begin + (r - first);
+    }
+  }
   __syncthreads();
-  const int s = owner;
+  const int s = owner, pos = to_pos;
   if (s < 0) return;
-  const int src = a.rows[r], pos = a.begin[s] + (r - a.row_starts[s]);
   const int page = p.table[static_cast<long long>(s) * p.max_pages + pos / p.page_size];
   if (!p.in_pool(page)) return;
   const bool real = static_cast<unsigned>(src) < static_cast<unsigned>(a.num_nodes);
