@@ -352,3 +352,29 @@ def test_append_ranges_of_many_sequences(gpu):
     want = ref.append(c, kn, vn, rows, starts)
     assert got == want and all(c.same(state))
     assert [s for s in range(2600) if got[s]] == [*range(1030, 1035), 2099, 2199]
+
+
+@pytest.mark.parametrize("max_pages", [2048, 2049, 5000])
+def test_free_of_long_table_rows(gpu, max_pages):
+    """Several workgroups to a slot: lengths around multiples of a workgroup's 2048 entries and the whole table row, shared
+    pages and holes in every part, one that is short of a count, slots named twice and slots that are none."""
+    ps, at = 16, [2047, 2048, 2049, 4095, 4096, 4097]
+    lens = [max_pages * ps] * 2 + [0, 1] + [min(e, max_pages) * ps - d for e in at for d in (0, 15)] + [max_pages * ps + 1, -1]
+    c = _filled(33, pages=max_pages * 17, ps=ps, seqs=len(lens), max_pages=max_pages, layers=1, kv_heads=1, dim=8, lens=lens[:-2], spare=0.0)
+    c.lens[:] = lens
+    for s in (1, 5, 6, 9, 14):  # entries all along the row are those of sequence 0
+        e = np.arange(s % 3, c.used(int(c.lens[s])), 3)
+        c.refs[c.table[s, e]] -= 1
+        c.table[s, e] = c.table[0, e]
+        c.refs[c.table[0, e]] += 1
+    c.table[1, 2::500] = -1
+    c.table[7, [0, 2047]] = 1 << 30
+    c.refs[c.table[8, [3, 2040]]] = 0
+    S = len(lens)
+    for slots in ([0], [1, 0], [6, 6, 0, 6, S, -1], list(range(S)), [S - 1, S - 2, 14, 3, 2, 14, 1]):
+        print(f"free {slots[:9]} of {max_pages} entries", flush=True)
+        case = c.copy()
+        state = case.to(gpu)
+        got = _run(ops.PageFree(num_slots=len(slots), **_pool(case)), [_ints(slots, gpu), *state[2:]], len(slots))
+        want = ref.free(case, slots)
+        assert got == want and all(case.same(state)), slots
