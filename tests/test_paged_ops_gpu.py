@@ -378,3 +378,22 @@ def test_free_of_long_table_rows(gpu, max_pages):
         got = _run(ops.PageFree(num_slots=len(slots), **_pool(case)), [_ints(slots, gpu), *state[2:]], len(slots))
         want = ref.free(case, slots)
         assert got == want and all(case.same(state)), slots
+
+
+@pytest.mark.parametrize("ps", [256, 512, 1024])
+@pytest.mark.parametrize("layers,kv_heads,dim,dtype", [(1, 8, 128, torch.bfloat16), (3, 2, 64, torch.float16), (2, 1, 24, torch.float32)])
+def test_large_pages(gpu, ps, layers, kv_heads, dim, dtype):
+    """Pages of hundreds of positions: rows appended up to, onto and across their ends, last pages of one row and of all but
+    one forked and copied, a pool packed."""
+    print(f"pages of {ps} {dtype}", flush=True)
+    c = _filled(34, pages=26, ps=ps, seqs=9, max_pages=4, layers=layers, kv_heads=kv_heads, dim=dim, dtype=dtype,
+                lens=[2 * ps - 3, ps, 1, 3 * ps - 1, 5, 0, 0, 0, 0], spare=0.0)
+    got, state, (kn, vn, rows, starts) = _append(gpu, c, [2, 1, ps, 2, 0, ps + 1, 0, 0, 0], 34)
+    assert got == ref.append(c, kn, vn, rows, starts) == [0] * 9 and all(c.same(state))
+    for forks, share in (([(0, 6), (3, 7)], True), ([(2, 8)], False)):
+        got = _run(ops.PageFork(num_forks=len(forks), share=share, **_data(c)), [_ints(forks, gpu), *state], len(forks))
+        assert got == ref.fork(c, forks, share) == [0] * len(forks) and all(c.same(state))
+    got = _run(ops.PageFree(num_slots=2, **_pool(c)), [_ints([0, 1], gpu), *state[2:]], 2)
+    assert got == ref.free(c, [0, 1]) == [0, 0] and all(c.same(state))
+    got = _run(ops.PageCompact(**_data(c)), state, 1)
+    assert got == [ref.compact(c)] and got[0] > 0 and all(c.same(state))
