@@ -586,3 +586,41 @@ def test_values_behind_far_lower_scores(gpu, nodes, infinity):
     if infinity:
         assert (got[:nodes, :, 40] == float("inf")).all()
     assert (got[nodes:nodes + 2] == 1).all()
+
+
+@pytest.mark.parametrize("nodes,ps,infinity", [(30, 64, False), (30, 16, False), (30, 64, True), (4, 16, True)])  # 60 and 8 rows to a KV head
+def test_cache_past_32_bits_wide_and_done_over(gpu, nodes, ps, infinity):
+    """The same for the kernel of many rows, for pages that hold half a block of its keys, and for rows that an infinity
+    has done over key by key."""
+    print(f"{nodes} nodes, pages of {ps}, infinity {infinity}", flush=True)
+    P, Hkv, D = 70000 * 64 // ps, 8, 64  # 4.6 GB each of K and V
+    c = Case(16, Hkv, D, ps, [300], [nodes], seed=38)
+    n = -(-300 // ps)
+    if infinity:
+        c.vp[c.table[0, n - 2], 3, 5, 9] = float("inf")
+    kp, vp = (torch.empty(P, Hkv, ps, D, dtype=BF16, device=gpu) for _ in range(2))
+    t = c.tensors(gpu)
+    ids = [P - 1 - 3 * e for e in range(n)]
+    assert min(ids) * Hkv * ps * D * 2 > 1 << 32
+    kp[ids], vp[ids] = t[3][t[5][0, :n].long()], t[4][t[5][0, :n].long()]
+    t[3], t[4], t[5][0, :n] = kp, vp, torch.tensor(ids, dtype=torch.int32, device=gpu)
+    ops.TreeAttention(num_heads=16, num_kv_heads=Hkv, head_dim=D, num_pages=P, page_size=ps, num_seqs=1, max_pages=c.MP, num_nodes=c.N,
+                      max_nodes=c.T).get_callable()(*t)
+    torch.cuda.synchronize()
+    if not infinity:
+        c.check(gpu, t[-1])
+        return
+    got = t[-1].cpu().double()
+    hit = torch.zeros(got.shape, dtype=torch.bool)
+    hit[:nodes, 6:8, 9] = True
+    assert (got[hit] == float("inf")).all()
+    c.vp[c.table[0, n - 2], 3, 5, 9] = 0.0
+    want, tol = c.want()
+    assert ((got - want).abs() <= tol)[~hit].all()
+
+
+@pytest.mark.parametrize("D,dtype", [(64, BF16), (128, BF16), (128, FP16)])
+def test_a_chunk_beside_single_tokens(gpu, D, dtype):
+    """A prompt's chunk of hundreds of rows and decode steps of other sequences in one call, some of them behind nothing."""
+    lens = [700, 40, 0, 300, 5, 1000, 16, 63, 64, 65, 0, 128]
+    Case(8, 2, D, 16, lens, [300] + [1] * 6 + [0] + [1] * 3 + [2], dtype, seed=39, mask="chain").check(gpu)
