@@ -380,7 +380,8 @@ enum iron_page_status {
  * (infinities, NaN); a key whose score is -inf is one that the row does not see.
  * Where a KV head has more than 32 rows (max_nodes times G), weights are rounded
  * to dtype before the second product, as iron_attention_prefill does; else they
- * keep 16 bits. dtype 0: bf16, 1: fp16 (q, k, v and out). head_dim 64 or 128;
+ * keep 16 bits. That goes by max_nodes, so it holds for every sequence of the call,
+ * those of one node too. fp16 weights are kept to 2^-30 of a row's largest. dtype 0: bf16, 1: fp16 (q, k, v and out). head_dim 64 or 128;
  * n_heads any multiple of n_kv_heads; max_nodes at most 1024. k_pages and v_pages
  * are one layer's (num_pages, n_kv_heads, page_size, head_dim).
  * node_starts must not decrease; each tree is taken as cut to max_nodes nodes

@@ -216,6 +216,8 @@ __device__ void refuse_overlaps(const AppendArgs& a, int* need, int* grow, int* 
 // workgroup, bound by its chain of dependent reads: the counts that the search
 // for free pages begins with are asked for first, and what was read of the
 // sequences stays in LDS (8 sequences 4.0 -> 2.7 us, four prompts 6.4 -> 4.5).
+// Judging row_starts costs 0.2 us: whether it decreases anywhere goes through LDS
+// behind the barrier that was there.
 __global__ __launch_bounds__(kPlan) void append_plan_kernel(AppendArgs a) {
   __shared__ int need[kMaxRequests];
   __shared__ int lens[kMaxRequests];
@@ -310,8 +312,13 @@ __global__ __launch_bounds__(256) void append_rows_kernel(AppendArgs a, int grou
 // ----------------------------------------------------------- page copies ----
 // Pages to copy: the first rows[i] rows (rows null: all) of every head of page
 // src[i] to page dst[i], K and V, all layers. No page is both a source and a
-// destination. Bound by memory: four whole sequences, 557 MB, in 111 us, and a
-// third of a pool packed, 917 MB, in 183 us: 5.0 TB/s.
+// destination. One workgroup copies a page of a layer's K or V, 4 KiB at a time,
+// each waited for. With thousands of pages that is bound by memory (pages of 16
+// positions: four whole sequences, 557 MB, in 111 us, and a third of a pool packed,
+// 917 MB, in 183 us: 5.0 TB/s); with few and large ones by its round trips (whole
+// calls, 8 heads of 128: one fork's last page of 255 of 256 rows, one layer, 28 us
+// for 2 MB, of 1023 of 1024 rows 96 us for 8 MB, 168 us with 16 layers, 134 MB;
+// 12 us at pages of 16).
 struct Copies {
   const int* src;
   const int* dst;

@@ -582,10 +582,13 @@ __device__ __forceinline__ ta_f32x16 mfma32(ta_u32x4 a, ta_u32x4 b, ta_f32x16 c)
 // rounds them, and their sum is that of the rounded ones: as hi and lo they doubled the second
 // product (134 -> 109 us for the wide trees above, with the next block's
 // scores computed among this one's softmax; error against 64 bits 1.2 times that of
-// one rounding of the result). What bounds it: VALU and matrix time of a SIMD's
-// waves add up to the loop's time. Six of eight products of the second GEMM taken
-// out saved 12 of 93 us, half of K's or V's LDS reads nothing, scheduling barriers,
-// wave priorities and accumulators in AGPRs nothing.
+// one rounding of the result). What bounds it, by counters (the wide trees, fp16 and
+// bf16 alike): of its SIMDs' cycles the matrix units are busy in 40 % and VALU
+// instructions take 32 %, 72 % if they never meet; a wave waits for data or a
+// barrier in 27 % of its time and to issue in another 27 %. Neither unit is full and
+// two waves to a SIMD do not keep them both at work. Six of eight products of the
+// second GEMM taken out saved 12 of 93 us, half of K's or V's LDS reads nothing,
+// scheduling barriers, wave priorities and accumulators in AGPRs nothing.
 template <int D, bool F16>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void tree_wide_kernel(TreeArgs a) {
   constexpr int R = 128, B = kWideBlock, kRow = D * 2, kHalf = B * kRow, kStage = 2 * kHalf;

@@ -22,7 +22,9 @@ as they were. What a node does not see does not reach its row, whatever it
 holds; a key whose score is -inf counts as one that it does not see. Scores,
 softmax and sums are fp32; the weights enter the product with V with 16 bits, or rounded
 to ``dtype`` (as in MHA) where a KV head has more than 32 rows, max_nodes times
-H / Hkv. Kernel: iron_tree_attention.
+H / Hkv. That rule goes by max_nodes: a sequence of one node in a call with longer
+trees is rounded as they are; in a call of its own it keeps the 16 bits. fp16
+weights are kept to 2^-30 of a row's largest. Kernel: iron_tree_attention.
 """
 
 import math
