@@ -397,3 +397,45 @@ def test_large_pages(gpu, ps, layers, kv_heads, dim, dtype):
     assert got == ref.free(c, [0, 1]) == [0, 0] and all(c.same(state))
     got = _run(ops.PageCompact(**_data(c)), state, 1)
     assert got == [ref.compact(c)] and got[0] > 0 and all(c.same(state))
+
+
+def test_the_largest_batches(gpu):
+    """8192 sequences and requests, of which a request in ten cannot be met."""
+    S = 8192
+    c = _filled(40, pages=40000, seqs=S, max_pages=3, layers=1, kv_heads=1, dim=8, lens=[(5 * s) % 33 if s < S // 2 else 0 for s in range(S)])
+    c.lens[9:S // 2:10] = 49
+    got, state, (kn, vn, rows, starts) = _append(gpu, c, [s % 3 if s < S // 2 else 0 for s in range(S)], 40)
+    assert got == ref.append(c, kn, vn, rows, starts) and all(c.same(state))
+    forks = [(i % (S // 2), S // 2 + i % (S // 2 - 5)) for i in range(S)]  # the last 4101 name children that earlier pairs name
+    firsts = set(b for _, b in forks)
+    got = _run(ops.PageFork(num_forks=S, **_data(c)), [_ints(forks, gpu), *state], S)
+    assert got == ref.fork(c, forks, True) and all(c.same(state)) and got.count(ref.DONE) > 0.85 * len(firsts)
+    slots = [(i * 7) % S for i in range(S)]
+    got = _run(ops.PageFree(num_slots=S, **_pool(c)), [_ints(slots, gpu), *state[2:]], S)
+    assert got == ref.free(c, slots) and all(c.same(state))
+
+
+def test_the_longest_append(gpu):
+    """2^20 rows to one sequence in one call, copied whole, freed: the pages in order, the rows in their places."""
+    n, ps, MP = 1 << 20, 16, 1 << 16
+    P = 2 * MP + 100
+    pool = dict(num_pages=P, page_size=ps, num_seqs=3, max_pages=MP)
+    data = dict(num_layers=1, num_kv_heads=1, head_dim=8, **pool)
+    i32 = lambda n, v: torch.full((n,), v, dtype=torch.int32, device=gpu)
+    kn = torch.randn(1, n, 1, 8, generator=torch.Generator(gpu).manual_seed(41), device=gpu).to(torch.bfloat16)
+    k, v = (torch.zeros(1, P, 1, ps, 8, dtype=torch.bfloat16, device=gpu) for _ in range(2))
+    table, lens, refs = i32(3 * MP, -1).view(3, MP), i32(3, 0), i32(P, 0)
+    refs[:100] = 1
+    rows = torch.arange(n - 1, -1, -1, dtype=torch.int32, device=gpu)
+    got = _run(ops.PagedAppend(num_nodes=n, num_rows=n, **data), [kn, kn + 1, rows, _ints([0, 0, n, n], gpu), k, v, table, lens, refs], 3)
+    assert got == [0, 0, 0] and lens.tolist() == [0, n, 0]
+    assert torch.equal(table[1], torch.arange(100, 100 + MP, dtype=torch.int32, device=gpu)) and (refs[:100 + MP] == 1).all()
+    assert torch.equal(k[0, 100:100 + MP].reshape(n, 8), kn[0, :, 0].flip(0)) and torch.equal(v[0, 100:100 + MP].reshape(n, 8), (kn + 1)[0, :, 0].flip(0))
+    got = _run(ops.PageFork(num_forks=1, share=False, **data), [_ints([[1, 2]], gpu), k, v, table, lens, refs], 1)
+    assert got == [0] and lens.tolist() == [0, n, n] and (refs == 1).all()
+    assert torch.equal(table[2], table[1] + MP) and torch.equal(k[0, 100 + MP:], k[0, 100:100 + MP]) and torch.equal(v[0, 100 + MP:], v[0, 100:100 + MP])
+    got = _run(ops.PageFree(num_slots=1, **pool), [_ints([1], gpu), table, lens, refs], 1)
+    assert got == [0] and lens.tolist() == [0, 0, n] and (table[1] == -1).all() and int((refs == 0).sum()) == MP
+    got = _run(ops.PageCompact(**data), [k, v, table, lens, refs], 1)
+    assert got == [MP] and torch.equal(table[2], torch.arange(100, 100 + MP, dtype=torch.int32, device=gpu)) and int(refs.sum()) == 100 + MP
+    assert torch.equal(k[0, 100:100 + MP].reshape(n, 8), kn[0, :, 0].flip(0))

@@ -624,3 +624,13 @@ def test_a_chunk_beside_single_tokens(gpu, D, dtype):
     """A prompt's chunk of hundreds of rows and decode steps of other sequences in one call, some of them behind nothing."""
     lens = [700, 40, 0, 300, 5, 1000, 16, 63, 64, 65, 0, 128]
     Case(8, 2, D, 16, lens, [300] + [1] * 6 + [0] + [1] * 3 + [2], dtype, seed=39, mask="chain").check(gpu)
+
+
+def test_as_many_sequences_as_there_can_be(gpu):
+    rng = np.random.default_rng(42)
+    lens, nodes = [int(x) for x in rng.integers(0, 40, 8192)], [0] * 8192
+    for s in [0, 8191, *rng.choice(8192, 700, replace=False)]:
+        nodes[s] = int(rng.integers(1, 4))
+    lens[5000], nodes[5000] = 3000, 1
+    Case(2, 1, 64, 16, lens, nodes, seed=42).check(gpu)
+    Case(2, 1, 64, 16, lens, nodes[:5000] + [30] + nodes[5001:], seed=43).check(gpu)  # 60 rows: the kernel of many rows
