@@ -381,9 +381,10 @@ enum iron_page_status {
  * Where a KV head has more than 32 rows (max_nodes times G), weights are rounded
  * to dtype before the second product, as iron_attention_prefill does; else they
  * keep 16 bits. That goes by max_nodes, so it holds for every sequence of the call,
- * those of one node too. fp16 weights are kept to 2^-30 of a row's largest. dtype 0: bf16, 1: fp16 (q, k, v and out). head_dim 64 or 128;
- * n_heads any multiple of n_kv_heads; max_nodes at most 1024. k_pages and v_pages
- * are one layer's (num_pages, n_kv_heads, page_size, head_dim).
+ * those of one node too. fp16 weights are kept to 2^-30 of a row's largest.
+ * dtype 0: bf16, 1: fp16 (q, k, v and out). head_dim 64 or 128; n_heads any
+ * multiple of n_kv_heads; max_nodes at most 1024. k_pages and v_pages are one
+ * layer's (num_pages, n_kv_heads, page_size, head_dim).
  * node_starts must not decrease; each tree is taken as cut to max_nodes nodes
  * and to num_nodes rows. Lengths outside [0, max_pages * page_size] are cut to
  * that range. Beside the reference's attention of one token or of a prompt
