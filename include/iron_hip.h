@@ -416,6 +416,79 @@ int iron_paged_append(const void* k_new, const void* v_new, const int* rows, con
                       int n_kv_heads, int row_bytes, int num_pages, int page_size, int num_seqs, int max_pages,
                       int num_nodes, int num_rows, void* workspace, long long workspace_bytes, void* stream);
 
+/* iron_tree_attention over pages of 4-bit rows: k_pages and v_pages are one layer's
+ * (num_pages, n_kv_heads, page_size, head_dim / 2 + 16) bytes. A row is head_dim / 2
+ * bytes of codes, then four pairs (s, b) of fp16, one for each quarter of the row:
+ * value = b + s (16 + code). A 32-bit word of codes holds eight consecutive values,
+ * the even ones in the nibbles of its low half from the lowest up, the odd ones in
+ * those of its high half. Rows of pages need no alignment but the pages' own (16
+ * bytes). Values and the weights of cached positions enter the products rounded once
+ * to fp16 (weights kept to 2^-30 of a row's largest); the tree's rows k_new and
+ * v_new are dtype, and so are their weights: in two parts, or one where a KV head
+ * has more than 32 rows (max_nodes times G). Everything else is
+ * iron_tree_attention's. iron_page_fork, iron_page_compact and iron_page_free take
+ * such pages with row_bytes = head_dim / 2 + 16. */
+long long iron_tree_attention_int4_workspace_bytes(int n_heads, int n_kv_heads, int head_dim, int num_seqs,
+                                                   int num_nodes, int max_nodes, int max_pages, int page_size);
+int iron_tree_attention_int4(const void* q, const void* k_new, const void* v_new, const void* k_pages,
+                             const void* v_pages, const int* page_table, const int* seq_lens, const int* node_starts,
+                             const int* tree_mask, void* out, int dtype, int n_heads, int n_kv_heads, int head_dim,
+                             int num_pages, int page_size, int num_seqs, int max_pages, int num_nodes, int max_nodes,
+                             float scale, void* workspace, long long workspace_bytes, void* stream);
+
+/* iron_paged_append into pages of 4-bit rows (num_layers, num_pages, n_kv_heads,
+ * page_size, head_dim / 2 + 16 bytes; iron_tree_attention_int4): requests, pages and
+ * status are iron_paged_append's (and its workspace query). k_new and v_new are bf16
+ * (dtype 0) or fp16 (1), head_dim 64 or 128. Of each quarter of a row, its values cut
+ * to +-20480, lo the least and hi the largest: s = fp16((hi - lo) / 15),
+ * b = fp16(lo - 16 s), and the code of x is the number of k in 0 .. 14 with
+ * x >= b + (k + 16.5) s (0 where s is 0). A quarter with a NaN gets b = NaN. The
+ * paged form of the KV-cache append (llama_npu.py:311-323), quantizing. */
+int iron_paged_append_int4(const void* k_new, const void* v_new, const int* rows, const int* row_starts, void* k_pages,
+                           void* v_pages, int* page_table, int* seq_lens, int* page_refs, int* status, int dtype,
+                           int num_layers, int n_kv_heads, int head_dim, int num_pages, int page_size, int num_seqs,
+                           int max_pages, int num_nodes, int num_rows, void* workspace, long long workspace_bytes,
+                           void* stream);
+
+/* The way back: rows row_starts[s] .. row_starts[s+1]-1 of k_out and v_out
+ * (num_layers, num_rows, n_kv_heads, head_dim), bf16 (dtype 0) or fp16 (1), receive
+ * positions begins[s], begins[s] + 1, .. of sequence s from pages of 4-bit rows:
+ * b + s (16 + code) rounded to dtype, zeros for a position outside [0, seq_lens[s])
+ * or in a hole. Rows in no range are left as they were; a row in several ranges is
+ * the first sequence's. num_rows at most 2^20. */
+int iron_paged_gather_int4(const int* begins, const int* row_starts, const void* k_pages, const void* v_pages,
+                           const int* page_table, const int* seq_lens, void* k_out, void* v_out, int dtype,
+                           int num_layers, int n_kv_heads, int head_dim, int num_pages, int page_size, int num_seqs,
+                           int max_pages, int num_rows, void* stream);
+
+/* Verification of drafted trees: rows node_starts[s] .. node_starts[s+1]-1 of
+ * logits (num_nodes, vocab) are the nodes of sequence s, the first of them its last
+ * token, each other one the token tokens[i] drafted behind its parent, node
+ * parents[i] < i of the tree. p and q are the softmax of logits and draft_logits
+ * divided by temperatures[s]. From the first node on, the children of an accepted
+ * node (max_children at most, further ones are left out) are tried in row order: one
+ * with token x is accepted if accept_draws[i] q(x) < p(x), else p becomes
+ * max(p - q, 0) scaled to a sum of 1. Where none is accepted, next_tokens[s] is the
+ * first token whose cumulative probability passes sample_draws[s] (the last one with
+ * any, if none does). draft_logits null: q is 1 at x. A temperature that is not above
+ * 0 takes the largest logit (the lowest index of equal ones). rows (num_nodes)
+ * receives the accepted rows, sequence by sequence from row_starts[s] on, then -1:
+ * the arguments of iron_paged_append. NaN logits count as -inf, +inf as the largest
+ * fp32; next_tokens[s] is -1 for an empty tree and for a row of -inf. Tokens outside
+ * [0, vocab) are not accepted; where max(p - q, 0) is zero everywhere the next token
+ * is drawn from p. draft_logits of nodes without children are not read. Computed in
+ * 64 bits. dtype 0: bf16, 1: fp16, 2: fp32 logits. vocab at most 2^20, num_nodes 2^20 and
+ * 2^23 / ceil(vocab / 4096), max_nodes 1024, max_children 64. node_starts must not decrease; trees are cut to max_nodes nodes and
+ * to num_nodes rows. In the place of the sampling of
+ * iron/applications/llama_3.2_1b/llama_inference_harness.py:146-169. */
+long long iron_draft_verify_workspace_bytes(int vocab, int num_seqs, int num_nodes, int max_nodes, int max_children,
+                                            int draft);
+int iron_draft_verify(const void* logits, const void* draft_logits, const int* tokens, const int* parents,
+                      const int* node_starts, const float* temperatures, const float* accept_draws,
+                      const float* sample_draws, int* rows, int* row_starts, int* next_tokens, int dtype, int vocab,
+                      int num_seqs, int num_nodes, int max_nodes, int max_children, void* workspace,
+                      long long workspace_bytes, void* stream);
+
 /* For each pair forks[i] = (parent, child), child an empty sequence of the
  * table: the child becomes a sequence with the parent's positions. share != 0:
  * it holds the parent's full pages too (page_refs count it) and a new page

@@ -59,7 +59,11 @@ SIGNATURES: dict[str, list] = {
     "iron_argmax_bf16": [_P, _I, _P, _P, _P, _I, _P],
     "iron_argmax_select": [_P, _I, _P, _I, _I, _P, _P, _P, _P, _I, _P],
     "iron_tree_attention": [_P] * 10 + [_I] * 10 + [_F, _P, _LL, _P],
+    "iron_tree_attention_int4": [_P] * 10 + [_I] * 10 + [_F, _P, _LL, _P],
     "iron_paged_append": [_P] * 10 + [_I] * 9 + [_P, _LL, _P],
+    "iron_paged_append_int4": [_P] * 10 + [_I] * 10 + [_P, _LL, _P],
+    "iron_paged_gather_int4": [_P] * 8 + [_I] * 9 + [_P],
+    "iron_draft_verify": [_P] * 11 + [_I] * 6 + [_P, _LL, _P],
     "iron_page_fork": [_P] * 7 + [_I] * 9 + [_P, _LL, _P],
     "iron_page_compact": [_P] * 6 + [_I] * 7 + [_P, _LL, _P],
     "iron_page_free": [_P] * 5 + [_I] * 5 + [_P],
@@ -87,7 +91,9 @@ QUERIES: dict[str, tuple] = {
     "iron_swiglu_decode_i4g32_workspace_bytes": (_LL, [_I, _I]),
     "iron_xcd_round_robin": (_I, [_P]),
     "iron_tree_attention_workspace_bytes": (_LL, [_I] * 8),
+    "iron_tree_attention_int4_workspace_bytes": (_LL, [_I] * 8),
     "iron_paged_append_workspace_bytes": (_LL, [_I] * 3),
+    "iron_draft_verify_workspace_bytes": (_LL, [_I] * 6),
     "iron_page_fork_workspace_bytes": (_LL, [_I] * 5),
     "iron_page_compact_workspace_bytes": (_LL, [_I]),
     "iron_gemm_splitk_choose": (_I, [_I, _I, _I]),

@@ -10,6 +10,11 @@ A fresh cache has ``seq_lens`` and ``page_refs`` zero and any table. All of it
 lives on the device, so a serving step reads nothing back and can be captured
 whole into a graph. The layout and the rules are those of include/iron_hip.h.
 
+A cache may hold its rows in 4 bits (TreeAttentionInt4, PagedAppendInt4,
+PagedGatherInt4): pages are then uint8 with ``int4_row_bytes(head_dim)`` in the
+place of head_dim, and PageFork, PageCompact and PageFree take them with
+``dtype=torch.uint8, head_dim=int4_row_bytes(head_dim)``.
+
 Calls that work on one cache must be stream-ordered. Each call takes its own
 workspace from torch's allocator (about 2 us of host time), so one operator may
 be called on several streams, for several caches, and captured into several
@@ -24,6 +29,14 @@ from .. import _lib
 from .base import AIERuntimeArgSpec, HIPOperator
 
 INT32 = torch.int32
+
+
+def int4_row_bytes(head_dim: int) -> int:
+    """Bytes of a 4-bit row of head_dim values: the codes, eight to a word (even
+    values in its low half's nibbles, odd ones in its high half's, both from the
+    lowest up), then four fp16 pairs (s, b), one for each quarter of the row. A
+    value is ``b + s * (16 + code)``."""
+    return head_dim // 2 + 16
 
 
 class PagedOperator(HIPOperator):
@@ -69,6 +82,17 @@ class PagedOperator(HIPOperator):
     def row_bytes(self) -> int:
         return self.head_dim * self.dtype.itemsize
 
+    def _check_int4(self) -> None:
+        """Pages of 4-bit rows, and 16-bit rows beside them."""
+        if self.head_dim not in (64, 128):
+            raise ValueError(f"Only head_dim 64 and 128 are supported, got {self.head_dim}")
+        if self.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"dtype must be torch.bfloat16 or torch.float16, got {self.dtype!r}")
+
+    def _int4_specs(self, direction: str, *layers: int) -> list[AIERuntimeArgSpec]:
+        shape = (*layers, self.num_pages, self.num_kv_heads, self.page_size, int4_row_bytes(self.head_dim))
+        return [AIERuntimeArgSpec(direction, shape, dtype=torch.uint8) for _ in range(2)]
+
     def _pool_specs(self) -> list[AIERuntimeArgSpec]:
         shape = (self.num_layers, self.num_pages, self.num_kv_heads, self.page_size, self.head_dim)
         return [AIERuntimeArgSpec("inout", shape, dtype=self.dtype) for _ in range(2)]
@@ -83,8 +107,9 @@ class PagedOperator(HIPOperator):
         return 0
 
     def _call(self, entry: str, tensors, numbers, stream: int) -> None:
-        """Entry point ``entry`` on the tensors' device: their addresses, the
-        numbers, a workspace (if the operator has one) and the stream."""
+        """Entry point ``entry`` on the tensors' device: their addresses (None: an
+        argument that is not given), the numbers, a workspace (if the operator has
+        one) and the stream."""
         device = tensors[0].device
         if device.index != torch.cuda.current_device():
             with torch.cuda.device(device):
@@ -95,4 +120,4 @@ class PagedOperator(HIPOperator):
             # below 0: a shape that the entry point refuses, saying why
             ws = torch.empty(max(need, 0), dtype=torch.uint8, device=device)
             space = (ws.data_ptr(), need)
-        _lib.call(entry, *[t.data_ptr() for t in tensors], *numbers, *space, stream)
+        _lib.call(entry, *[_lib.ptr(t) for t in tensors], *numbers, *space, stream)

@@ -1,0 +1,98 @@
+// Rows of a 4-bit KV cache: a head's D keys or values at one position in
+// D / 2 + 16 bytes. D / 2 bytes of codes, then four pairs (s, b) of fp16, one for
+// each quarter of the row (D / 4 consecutive values): value = b + s (16 + code).
+// A word of codes holds eight consecutive values, the even ones in the nibbles of
+// its low half, the odd ones in those of its high half: two neighbours come out as
+// a packed pair. 16 + code as fp16 is the code in bits 6 .. 9 under the bits of 16,
+// so two values cost a shift, an and-or and one packed fma; with b + s code the
+// conversion would cost a subtraction more.
+#pragma once
+
+#include "iron_common.hpp"
+
+namespace iron {
+
+typedef _Float16 i4_f16x2 __attribute__((ext_vector_type(2)));
+
+template <int D>
+constexpr int kInt4Row = D / 2 + 16;  // bytes
+
+// The fp16 pairs (0, 1), (2, 3), (4, 5), (6, 7) of a word of codes, each value
+// rounded once: half a step of fp16, an eighth of bf16's.
+__device__ __forceinline__ void int4_unpack8(unsigned codes, i4_f16x2 s, i4_f16x2 b, unsigned (&out)[4]) {
+  constexpr unsigned kMask = 0x03c003c0u, kSixteen = 0x4c004c00u;
+  const unsigned x[4] = {codes << 6, codes << 2, codes >> 2, codes >> 6};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    out[i] = __builtin_bit_cast(unsigned, __builtin_elementwise_fma(__builtin_bit_cast(i4_f16x2, (x[i] & kMask) | kSixteen), s, b));
+}
+
+// s and b of a pair, twice each.
+__device__ __forceinline__ i4_f16x2 int4_scale(unsigned pair) {
+  const _Float16 s = __builtin_bit_cast(_Float16, static_cast<uint16_t>(pair & 0xffffu));
+  return i4_f16x2{s, s};
+}
+__device__ __forceinline__ i4_f16x2 int4_base(unsigned pair) {
+  const _Float16 b = __builtin_bit_cast(_Float16, static_cast<uint16_t>(pair >> 16));
+  return i4_f16x2{b, b};
+}
+
+__device__ __forceinline__ int int4_code(unsigned word, int i) { return word >> (4 * (i >> 1) + 16 * (i & 1)) & 15; }
+
+// Value code of a pair in fp32 (the product is exact).
+__device__ __forceinline__ float int4_dequant(unsigned pair, int code) {
+  return fmaf(static_cast<float>(int4_scale(pair)[0]), static_cast<float>(16 + code), static_cast<float>(int4_base(pair)[0]));
+}
+
+// Value d of the row at `row`.
+template <int D>
+__device__ __forceinline__ float int4_value(const void* row, int d) {
+  const unsigned* words = static_cast<const unsigned*>(row);
+  return int4_dequant(words[D / 8 + d / (D / 4)], int4_code(words[d >> 3], d & 7));
+}
+
+// Half the largest range of a quarter whose b stays in fp16: b >= -(1 + 32 / 15) times it.
+constexpr float kInt4Most = 20480.f;
+
+// Quantizes N values (a quarter): the codes of x in words, and the pair. s is the
+// range by 15 and b the least value less 16 s, each rounded to fp16; a code is the
+// nearest for those, of two equally near ones the upper: how many of the borders
+// b + (k + 16.5) s, k = 0 .. 14, lie at or below x. The product is off by less than
+// half a code, and one comparison with the border next to it, which fp32 holds
+// exactly, decides. Values are cut to +-20480; a NaN makes the quarter NaN.
+template <int N>
+__device__ __forceinline__ unsigned int4_quantize(const float (&v)[N], unsigned (&words)[N / 8]) {
+  float x[N];
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    nan |= v[i] != v[i];
+    x[i] = fminf(fmaxf(v[i], -kInt4Most), kInt4Most);
+  }
+  float lo = x[0], hi = x[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) {
+    lo = fminf(lo, x[i]);
+    hi = fmaxf(hi, x[i]);
+  }
+  const _Float16 sh = static_cast<_Float16>((hi - lo) / 15.f);
+  const float s = static_cast<float>(sh);
+  const _Float16 bh = static_cast<_Float16>((lo - 16.f * s) + 0.f);  // of zeros of both signs, +0
+  const float b = static_cast<float>(bh), inv = s > 0.f ? 1.f / s : 0.f;
+#pragma unroll
+  for (int w = 0; w < N / 8; ++w) words[w] = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float k = fminf(fmaxf(floorf((x[i] - b) * inv - 16.f), 0.f), 14.f);  // the border above code k
+    const int code = static_cast<int>(k) + (s > 0.f && x[i] >= fmaf(k + 16.5f, s, b) ? 1 : 0);
+    words[i >> 3] |= static_cast<unsigned>(code) << (4 * ((i & 7) >> 1) + 16 * (i & 1));
+  }
+  if (nan) {
+#pragma unroll
+    for (int w = 0; w < N / 8; ++w) words[w] = 0;
+    return 0x7e000000u;
+  }
+  return __builtin_bit_cast(uint16_t, sh) | static_cast<unsigned>(__builtin_bit_cast(uint16_t, bh)) << 16;
+}
+
+}  // namespace iron

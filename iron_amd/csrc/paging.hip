@@ -15,6 +15,7 @@
 // (a prefix sum over the requests and a search for that many zeros in
 // page_refs); the data then moves in a launch that fills the chip.
 #include "iron_common.hpp"
+#include "int4_rows.hpp"
 #include "../../include/iron_hip.h"
 
 #include <algorithm>
@@ -307,6 +308,155 @@ __global__ __launch_bounds__(256) void append_rows_kernel(AppendArgs a, int grou
     if (real) x = from[(l * a.num_nodes + src) * per_row + c];
     to[(l * p.num_pages + page) * p.page_chunks() + static_cast<long long>(h) * p.page_size * p.row_chunks + to_row + e] = x;
   }
+}
+
+// ------------------------------------------------------- 4-bit rows ----
+// Where 16 rows of a call go or come from: the owner of each (the first sequence
+// whose range holds it, -1 for none), its page and its row there. Every thread
+// calls it; `begin_of(s, begin)` gives the position of the first row of s's range
+// and whether s counts, `end_of(s)` the positions that s has.
+constexpr int kTile = 16;
+
+struct RowPlace {
+  int owner[kTile];
+  int page[kTile];  // -1: none
+  int at[kTile];
+};
+
+template <typename F, typename E>
+__device__ __forceinline__ void place_rows(const Pool& p, const int* row_starts, int num_rows, int r0, RowPlace& place, F begin_of, E end_of) {
+  const int tid = threadIdx.x;
+  if (tid < kTile) place.owner[tid] = INT_MAX;
+  __syncthreads();
+  for (int s = tid; s < p.num_seqs; s += 256) {
+    const int first = row_starts[s], stop = row_starts[s + 1];
+    int begin;
+    if (begin_of(s, begin))
+      for (int r = max(first, r0); r < min(stop, r0 + kTile); ++r) atomicMin(place.owner + (r - r0), s);
+  }
+  __syncthreads();
+  if (tid < kTile) {
+    int s = place.owner[tid], page = -1, at = 0, begin;
+    if (s == INT_MAX || r0 + tid >= num_rows) s = -1;
+    if (s >= 0 && begin_of(s, begin)) {
+      const long long pos = begin + (static_cast<long long>(r0 + tid) - row_starts[s]);
+      if (pos >= 0 && pos < end_of(s) && pos < static_cast<long long>(p.max_pages) * p.page_size) {
+        page = p.table[static_cast<long long>(s) * p.max_pages + pos / p.page_size];
+        at = static_cast<int>(pos % p.page_size);
+      }
+    }
+    place.owner[tid] = s;
+    place.page[tid] = p.in_pool(page) ? page : -1;
+    place.at[tid] = at;
+  }
+  __syncthreads();
+}
+
+template <bool F16>
+__device__ __forceinline__ float wide16(unsigned x) {
+  if constexpr (F16) return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(x)));
+  return __uint_as_float(x << 16);
+}
+
+// 16 rows of the call, `items` of the (layer, K or V, head) planes to a workgroup:
+// a wave takes a plane, four lanes a row of it, so that neighbouring positions of a
+// page are written together.
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void append4_rows_kernel(AppendArgs a, int items) {
+  constexpr int N = D / 4, kRow = kInt4Row<D>;
+  __shared__ RowPlace place;
+  const Pool& p = a.pool;
+  const int r0 = blockIdx.x * kTile, lane = threadIdx.x & 63, i = lane >> 2, part = lane & 3;
+  place_rows(p, a.row_starts, a.num_rows, r0, place, [&](int s, int& begin) { return (begin = a.begin[s]) >= 0; }, [](int) { return INT_MAX; });
+  const int page = place.page[i], at = place.at[i];
+  if (place.owner[i] < 0 || page < 0) return;
+  const int src = a.rows[r0 + i];
+  const bool real = static_cast<unsigned>(src) < static_cast<unsigned>(a.num_nodes);
+  const int H = p.n_kv_heads, planes = p.num_layers * 2 * H, stop = min(planes, (static_cast<int>(blockIdx.y) + 1) * items);
+  for (int x = blockIdx.y * items + (threadIdx.x >> 6); x < stop; x += 4) {
+    const int lk = x / H, h = x - lk * H, l = lk >> 1;
+    float v[N] = {};
+    if (real) {
+      const uint4* from = (lk & 1 ? a.v_new : a.k_new) + ((static_cast<long long>(l) * a.num_nodes + src) * H + h) * (D / 8) + part * (N / 8);
+#pragma unroll
+      for (int e = 0; e < N / 8; ++e) {
+        const uint4 y = from[e];
+        const unsigned w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[8 * e + 2 * j] = wide16<F16>(w[j] & 0xffffu);
+          v[8 * e + 2 * j + 1] = wide16<F16>(w[j] >> 16);
+        }
+      }
+    }
+    unsigned codes[N / 8];
+    const unsigned pair = int4_quantize(v, codes);
+    unsigned char* to = (lk & 1 ? p.v : p.k) + (((static_cast<long long>(l) * p.num_pages + page) * H + h) * p.page_size + at) * kRow;
+    if constexpr (N == 16)
+      *reinterpret_cast<uint2*>(to + part * 8) = make_uint2(codes[0], codes[1]);
+    else
+      *reinterpret_cast<uint4*>(to + part * 16) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+    *reinterpret_cast<unsigned*>(to + D / 2 + part * 4) = pair;
+  }
+}
+
+struct GatherArgs {
+  Pool pool;
+  const int* begins;      // (num_seqs)
+  const int* row_starts;  // (num_seqs + 1)
+  uint4* k_out;           // (layers, num_rows, n_kv_heads, D / 8)
+  uint4* v_out;
+  int num_rows;
+};
+
+// The other way round: 16 rows of the result.
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void gather4_rows_kernel(GatherArgs a, int items) {
+  constexpr int N = D / 4, kRow = kInt4Row<D>;
+  __shared__ RowPlace place;
+  const Pool& p = a.pool;
+  const int r0 = blockIdx.x * kTile, lane = threadIdx.x & 63, i = lane >> 2, part = lane & 3;
+  place_rows(p, a.row_starts, a.num_rows, r0, place, [&](int s, int& begin) { return begin = a.begins[s], true; }, [&](int s) { return p.lens[s]; });
+  if (place.owner[i] < 0) return;
+  const int page = place.page[i], at = place.at[i];
+  const int H = p.n_kv_heads, planes = p.num_layers * 2 * H, stop = min(planes, (static_cast<int>(blockIdx.y) + 1) * items);
+  for (int x = blockIdx.y * items + (threadIdx.x >> 6); x < stop; x += 4) {
+    const int lk = x / H, h = x - lk * H, l = lk >> 1;
+    unsigned words[N / 8], pair = 0;
+    for (int e = 0; e < N / 8; ++e) words[e] = 0;
+    if (page >= 0) {
+      const unsigned char* from = (lk & 1 ? p.v : p.k) + (((static_cast<long long>(l) * p.num_pages + page) * H + h) * p.page_size + at) * kRow;
+      if constexpr (N == 16) {
+        const uint2 y = *reinterpret_cast<const uint2*>(from + part * 8);
+        words[0] = y.x, words[1] = y.y;
+      } else {
+        const uint4 y = *reinterpret_cast<const uint4*>(from + part * 16);
+        words[0] = y.x, words[1] = y.y, words[2] = y.z, words[3] = y.w;
+      }
+      pair = *reinterpret_cast<const unsigned*>(from + D / 2 + part * 4);
+    }
+    uint4* to = (lk & 1 ? a.v_out : a.k_out) + ((static_cast<long long>(l) * a.num_rows + r0 + i) * H + h) * (D / 8) + part * (N / 8);
+#pragma unroll
+    for (int e = 0; e < N / 8; ++e) {
+      unsigned y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float lo = int4_dequant(pair, int4_code(words[e], 2 * j)), hi = int4_dequant(pair, int4_code(words[e], 2 * j + 1));
+        if constexpr (F16)
+          y[j] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(lo)) | static_cast<unsigned>(__builtin_bit_cast(uint16_t, static_cast<_Float16>(hi))) << 16;
+        else
+          y[j] = cvt_pk_bf16(lo, hi);
+      }
+      to[e] = make_uint4(y[0], y[1], y[2], y[3]);
+    }
+  }
+}
+
+// Planes to a workgroup: as many as leave 4096 workgroups, in fours (one to a wave).
+int planes_of(int num_rows, int planes) {
+  const long long all = static_cast<long long>((num_rows + kTile - 1) / kTile) * planes;
+  const long long least = std::max<long long>(4, (planes + 32767) / 32768);  // the grid's second dimension ends at 65535
+  return static_cast<int>(std::max(least, std::min<long long>(planes, all / 4096 / 4 * 4)));
 }
 
 // ----------------------------------------------------------- page copies ----
@@ -700,12 +850,10 @@ constexpr int kCopyBlocks = 2048;
 
 long long round4(long long n) { return (n + 3) / 4 * 4; }
 
-int check_pool(const char* who, const void* table, const void* lens, const void* refs, const void* status, int num_pages,
-               int page_size, int num_seqs, int max_pages) {
-  IRON_REQUIRE(table && lens && refs && status, "%s: null pointer", who);
-  for (const void* q : {table, lens, refs, status})
+int check_table(const char* who, const void* table, const void* lens, int num_pages, int page_size, int num_seqs, int max_pages) {
+  IRON_REQUIRE(table && lens, "%s: null pointer", who);
+  for (const void* q : {table, lens})
     IRON_REQUIRE((reinterpret_cast<uintptr_t>(q) & 3u) == 0, "%s: int32 arrays must be 4-byte aligned", who);
-  IRON_REQUIRE(aligned16(refs), "%s: page_refs must be 16-byte aligned", who);
   IRON_REQUIRE(num_pages >= 1 && num_pages <= kMaxPoolPages, "%s: num_pages=%d outside [1, %d]", who, num_pages, kMaxPoolPages);
   IRON_REQUIRE(page_size >= 16 && page_size <= 1024 && (page_size & (page_size - 1)) == 0,
                "%s: page_size=%d is not a power of two from 16 to 1024", who, page_size);
@@ -713,6 +861,15 @@ int check_pool(const char* who, const void* table, const void* lens, const void*
   IRON_REQUIRE(max_pages >= 1 && static_cast<long long>(max_pages) * page_size < (1LL << 31) - (1 << 20),
                "%s: max_pages=%d: a sequence holds less than 2^31 - 2^20 positions", who, max_pages);
   return 0;
+}
+
+int check_pool(const char* who, const void* table, const void* lens, const void* refs, const void* status, int num_pages,
+               int page_size, int num_seqs, int max_pages) {
+  IRON_REQUIRE(refs && status, "%s: null pointer", who);
+  for (const void* q : {refs, status})
+    IRON_REQUIRE((reinterpret_cast<uintptr_t>(q) & 3u) == 0, "%s: int32 arrays must be 4-byte aligned", who);
+  IRON_REQUIRE(aligned16(refs), "%s: page_refs must be 16-byte aligned", who);
+  return check_table(who, table, lens, num_pages, page_size, num_seqs, max_pages);
 }
 
 int check_data(const char* who, const void* k, const void* v, int num_layers, int n_kv_heads, int row_bytes) {
@@ -752,6 +909,43 @@ Pool make_pool(void* k, void* v, void* table, void* lens, void* refs, int num_la
 
 long long append_list(int num_seqs, int num_rows, int page_size) { return num_rows / page_size + num_seqs; }
 
+// Checks an append and fills its arguments.
+int append_call(const char* who, AppendArgs& a, const void* k_new, const void* v_new, const int* rows, const int* row_starts,
+                void* k_pages, void* v_pages, int* page_table, int* seq_lens, int* page_refs, int* status, int num_layers,
+                int n_kv_heads, int row_bytes, int num_pages, int page_size, int num_seqs, int max_pages, int num_nodes,
+                int num_rows, void* workspace, long long workspace_bytes) {
+  if (int rc = check_pool(who, page_table, seq_lens, page_refs, status, num_pages, page_size, num_seqs, max_pages)) return rc;
+  if (int rc = check_data(who, k_pages, v_pages, num_layers, n_kv_heads, row_bytes)) return rc;
+  IRON_REQUIRE(k_new && v_new && rows && row_starts, "%s: null pointer", who);
+  IRON_REQUIRE(aligned16(k_new) && aligned16(v_new), "%s: k_new and v_new must be 16-byte aligned", who);
+  IRON_REQUIRE(((reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(row_starts)) & 3u) == 0,
+               "%s: int32 arrays must be 4-byte aligned", who);
+  IRON_REQUIRE(num_nodes >= 1, "%s: num_nodes=%d", who, num_nodes);
+  IRON_REQUIRE(num_rows >= 1 && num_rows <= kMaxRows, "%s: num_rows=%d outside [1, %d]", who, num_rows, kMaxRows);
+  if (int rc = check_workspace(who, workspace, workspace_bytes,
+                               iron_paged_append_workspace_bytes(num_seqs, num_rows, page_size)))
+    return rc;
+  a.pool = make_pool(k_pages, v_pages, page_table, seq_lens, page_refs, num_layers, n_kv_heads, row_bytes, num_pages,
+                     page_size, num_seqs, max_pages);
+  a.k_new = static_cast<const uint4*>(k_new);
+  a.v_new = static_cast<const uint4*>(v_new);
+  a.rows = rows;
+  a.row_starts = row_starts;
+  a.status = status;
+  a.begin = static_cast<int*>(workspace);
+  a.list = a.begin + round4(num_seqs);
+  a.num_nodes = num_nodes;
+  a.num_rows = num_rows;
+  a.list_cap = static_cast<int>(append_list(num_seqs, num_rows, page_size));
+  return 0;
+}
+
+int check_int4(const char* who, int dtype, int head_dim) {
+  IRON_REQUIRE(dtype == 0 || dtype == 1, "%s: dtype=%d is neither 0 (bf16) nor 1 (fp16)", who, dtype);
+  IRON_REQUIRE(head_dim == 64 || head_dim == 128, "%s: head_dim must be 64 or 128", who);
+  return 0;
+}
+
 long long fork_list(int num_forks, int max_pages, int num_pages, int share) {
   return share ? num_forks : std::min<long long>(static_cast<long long>(num_forks) * max_pages, num_pages);
 }
@@ -771,37 +965,80 @@ extern "C" int iron_paged_append(const void* k_new, const void* v_new, const int
                                  int* status, int num_layers, int n_kv_heads, int row_bytes, int num_pages,
                                  int page_size, int num_seqs, int max_pages, int num_nodes, int num_rows,
                                  void* workspace, long long workspace_bytes, void* stream) {
-  const char* who = "iron_paged_append";
-  if (int rc = check_pool(who, page_table, seq_lens, page_refs, status, num_pages, page_size, num_seqs, max_pages)) return rc;
-  if (int rc = check_data(who, k_pages, v_pages, num_layers, n_kv_heads, row_bytes)) return rc;
-  IRON_REQUIRE(k_new && v_new && rows && row_starts, "%s: null pointer", who);
-  IRON_REQUIRE(aligned16(k_new) && aligned16(v_new), "%s: k_new and v_new must be 16-byte aligned", who);
-  IRON_REQUIRE(((reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(row_starts)) & 3u) == 0,
-               "%s: int32 arrays must be 4-byte aligned", who);
-  IRON_REQUIRE(num_nodes >= 1, "%s: num_nodes=%d", who, num_nodes);
-  IRON_REQUIRE(num_rows >= 1 && num_rows <= kMaxRows, "%s: num_rows=%d outside [1, %d]", who, num_rows, kMaxRows);
-  if (int rc = check_workspace(who, workspace, workspace_bytes,
-                               iron_paged_append_workspace_bytes(num_seqs, num_rows, page_size)))
-    return rc;
   AppendArgs a;
-  a.pool = make_pool(k_pages, v_pages, page_table, seq_lens, page_refs, num_layers, n_kv_heads, row_bytes, num_pages,
-                     page_size, num_seqs, max_pages);
-  a.k_new = static_cast<const uint4*>(k_new);
-  a.v_new = static_cast<const uint4*>(v_new);
-  a.rows = rows;
-  a.row_starts = row_starts;
-  a.status = status;
-  a.begin = static_cast<int*>(workspace);
-  a.list = a.begin + round4(num_seqs);
-  a.num_nodes = num_nodes;
-  a.num_rows = num_rows;
-  a.list_cap = static_cast<int>(append_list(num_seqs, num_rows, page_size));
+  if (int rc = append_call("iron_paged_append", a, k_new, v_new, rows, row_starts, k_pages, v_pages, page_table, seq_lens,
+                           page_refs, status, num_layers, n_kv_heads, row_bytes, num_pages, page_size, num_seqs, max_pages,
+                           num_nodes, num_rows, workspace, workspace_bytes))
+    return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
   IRON_LAUNCH(append_plan_kernel, dim3(1), dim3(kPlan), 0, s, a);
   // as many layers to a workgroup as leave 4096 of them
   const int group = std::min(num_layers, std::max(1, static_cast<int>(static_cast<long long>(num_rows) * num_layers / 4096)));
   IRON_LAUNCH(append_rows_kernel, dim3(num_rows, (num_layers + group - 1) / group), dim3(256), 0, s, a, group);
   return check_launch("paged_append");
+}
+
+extern "C" int iron_paged_append_int4(const void* k_new, const void* v_new, const int* rows, const int* row_starts,
+                                      void* k_pages, void* v_pages, int* page_table, int* seq_lens, int* page_refs,
+                                      int* status, int dtype, int num_layers, int n_kv_heads, int head_dim, int num_pages,
+                                      int page_size, int num_seqs, int max_pages, int num_nodes, int num_rows,
+                                      void* workspace, long long workspace_bytes, void* stream) {
+  const char* who = "iron_paged_append_int4";
+  if (int rc = check_int4(who, dtype, head_dim)) return rc;
+  AppendArgs a;
+  if (int rc = append_call(who, a, k_new, v_new, rows, row_starts, k_pages, v_pages, page_table, seq_lens, page_refs, status,
+                           num_layers, n_kv_heads, head_dim / 2 + 16, num_pages, page_size, num_seqs, max_pages, num_nodes,
+                           num_rows, workspace, workspace_bytes))
+    return rc;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  IRON_LAUNCH(append_plan_kernel, dim3(1), dim3(kPlan), 0, s, a);
+  const int planes = num_layers * 2 * n_kv_heads, items = planes_of(num_rows, planes);
+  const dim3 grid((num_rows + kTile - 1) / kTile, (planes + items - 1) / items);
+  if (head_dim == 64 && dtype)
+    IRON_LAUNCH((append4_rows_kernel<64, true>), grid, dim3(256), 0, s, a, items);
+  else if (head_dim == 64)
+    IRON_LAUNCH((append4_rows_kernel<64, false>), grid, dim3(256), 0, s, a, items);
+  else if (dtype)
+    IRON_LAUNCH((append4_rows_kernel<128, true>), grid, dim3(256), 0, s, a, items);
+  else
+    IRON_LAUNCH((append4_rows_kernel<128, false>), grid, dim3(256), 0, s, a, items);
+  return check_launch("paged_append_int4");
+}
+
+extern "C" int iron_paged_gather_int4(const int* begins, const int* row_starts, const void* k_pages, const void* v_pages,
+                                      const int* page_table, const int* seq_lens, void* k_out, void* v_out, int dtype,
+                                      int num_layers, int n_kv_heads, int head_dim, int num_pages, int page_size,
+                                      int num_seqs, int max_pages, int num_rows, void* stream) {
+  const char* who = "iron_paged_gather_int4";
+  if (int rc = check_int4(who, dtype, head_dim)) return rc;
+  if (int rc = check_table(who, page_table, seq_lens, num_pages, page_size, num_seqs, max_pages)) return rc;
+  if (int rc = check_data(who, k_pages, v_pages, num_layers, n_kv_heads, head_dim / 2 + 16)) return rc;
+  for (const int* p : {begins, row_starts})
+    IRON_REQUIRE(p && (reinterpret_cast<uintptr_t>(p) & 3u) == 0, "%s: int32 arrays must be given and 4-byte aligned", who);
+  IRON_REQUIRE(k_out && v_out && aligned16(k_out) && aligned16(v_out), "%s: k_out and v_out must be given and 16-byte aligned", who);
+  for (const void* p : {k_pages, v_pages}) IRON_REQUIRE(k_out != p && v_out != p, "%s: k_out or v_out is one of the inputs", who);
+  IRON_REQUIRE(k_out != v_out, "%s: k_out and v_out are the same buffer", who);
+  IRON_REQUIRE(num_rows >= 1 && num_rows <= kMaxRows, "%s: num_rows=%d outside [1, %d]", who, num_rows, kMaxRows);
+  GatherArgs a;
+  a.pool = make_pool(const_cast<void*>(k_pages), const_cast<void*>(v_pages), const_cast<int*>(page_table), const_cast<int*>(seq_lens),
+                     nullptr, num_layers, n_kv_heads, head_dim / 2 + 16, num_pages, page_size, num_seqs, max_pages);
+  a.begins = begins;
+  a.row_starts = row_starts;
+  a.k_out = static_cast<uint4*>(k_out);
+  a.v_out = static_cast<uint4*>(v_out);
+  a.num_rows = num_rows;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int planes = num_layers * 2 * n_kv_heads, items = planes_of(num_rows, planes);
+  const dim3 grid((num_rows + kTile - 1) / kTile, (planes + items - 1) / items);
+  if (head_dim == 64 && dtype)
+    IRON_LAUNCH((gather4_rows_kernel<64, true>), grid, dim3(256), 0, s, a, items);
+  else if (head_dim == 64)
+    IRON_LAUNCH((gather4_rows_kernel<64, false>), grid, dim3(256), 0, s, a, items);
+  else if (dtype)
+    IRON_LAUNCH((gather4_rows_kernel<128, true>), grid, dim3(256), 0, s, a, items);
+  else
+    IRON_LAUNCH((gather4_rows_kernel<128, false>), grid, dim3(256), 0, s, a, items);
+  return check_launch("paged_gather_int4");
 }
 
 extern "C" long long iron_page_fork_workspace_bytes(int num_forks, int num_seqs, int max_pages, int num_pages, int share) {

@@ -9,6 +9,7 @@ import importlib
 
 _OPERATOR_MODULES = {
     "Dequant": "dequant",
+    "DraftVerify": "draft_verify",
     "ElementwiseAdd": "elementwise_add",
     "ElementwiseMul": "elementwise_mul",
     "GELU": "gelu",
@@ -22,6 +23,8 @@ _OPERATOR_MODULES = {
     "PageFork": "page_fork",
     "PageFree": "page_free",
     "PagedAppend": "paged_append",
+    "PagedAppendInt4": "paged_append_int4",
+    "PagedGatherInt4": "paged_gather_int4",
     "RMSNorm": "rms_norm",
     "RoPE": "rope",
     "SiLU": "silu",
@@ -30,6 +33,7 @@ _OPERATOR_MODULES = {
     "SwiGLUPrefill": "swiglu_prefill",
     "Transpose": "transpose",
     "TreeAttention": "tree_attention",
+    "TreeAttentionInt4": "tree_attention_int4",
     "StridedCopy": "strided_copy",
     "Repeat": "repeat",
 }

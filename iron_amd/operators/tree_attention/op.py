@@ -55,6 +55,7 @@ class TreeAttention(PagedOperator):
 
     _spec_fields: ClassVar[tuple] = ("num_heads", "num_kv_heads", "head_dim", "num_pages", "page_size", "num_seqs",
                                      "max_pages", "num_nodes", "max_nodes", "dtype")
+    _entry: ClassVar[str] = "iron_tree_attention"
 
     def __post_init__(self):
         self._check_counts(num_heads=1024, num_kv_heads=1024, num_nodes=1 << 20, max_nodes=1024)
@@ -76,19 +77,21 @@ class TreeAttention(PagedOperator):
         return (self.max_nodes + 31) // 32
 
     def workspace_bytes(self) -> int:
-        return _lib.workspace_bytes("iron_tree_attention_workspace_bytes", self.num_heads, self.num_kv_heads, self.head_dim,
+        return _lib.workspace_bytes(self._entry + "_workspace_bytes", self.num_heads, self.num_kv_heads, self.head_dim,
                                     self.num_seqs, self.num_nodes, self.max_nodes, self.max_pages, self.page_size)
+
+    def _page_specs(self):
+        pages = (self.num_pages, self.num_kv_heads, self.page_size, self.head_dim)
+        return [AIERuntimeArgSpec("in", pages, dtype=self.dtype) for _ in range(2)]
 
     def get_arg_spec(self):
         new = (self.num_nodes, self.num_kv_heads, self.head_dim)
-        pages = (self.num_pages, self.num_kv_heads, self.page_size, self.head_dim)
         rows = (self.num_nodes, self.num_heads, self.head_dim)
         return [
             AIERuntimeArgSpec("in", rows, dtype=self.dtype),
             AIERuntimeArgSpec("in", new, dtype=self.dtype),
             AIERuntimeArgSpec("in", new, dtype=self.dtype),
-            AIERuntimeArgSpec("in", pages, dtype=self.dtype),
-            AIERuntimeArgSpec("in", pages, dtype=self.dtype),
+            *self._page_specs(),
             AIERuntimeArgSpec("in", (self.num_seqs, self.max_pages), dtype=INT32),
             AIERuntimeArgSpec("in", (self.num_seqs,), dtype=INT32),
             AIERuntimeArgSpec("in", (self.num_seqs + 1,), dtype=INT32),
@@ -97,7 +100,7 @@ class TreeAttention(PagedOperator):
         ]
 
     def _launch(self, *tensors, stream):
-        self._call("iron_tree_attention", tensors,
+        self._call(self._entry, tensors,
                    (int(self.dtype == torch.float16), self.num_heads, self.num_kv_heads, self.head_dim,
                     self.num_pages, self.page_size, self.num_seqs, self.max_pages, self.num_nodes, self.max_nodes,
                     float(self.scale)), stream)
