@@ -6,6 +6,366 @@
 namespace iron {
 namespace {
 
+// A wave's loads of a block: its 16 keys' codes and pairs, K's and V's. Lane
+// (key c, quad) has quarter `quad` of key c's row.
+template <int D>
+struct Quarter {
+  unsigned codes[D / 32];
+  unsigned pair;
+};
+
+template <int D>
+__device__ __forceinline__ Quarter<D> load_quarter(const unsigned char* rows, unsigned at_codes, unsigned at_pair) {
+  Quarter<D> x;
+  if constexpr (D == 64) {
+    const ta_u32x2 v = *reinterpret_cast<const ta_u32x2*>(rows + at_codes);
+    x.codes[0] = v.x, x.codes[1] = v.y;
+  } else {
+    const ta_u32x4 v = *reinterpret_cast<const ta_u32x4*>(rows + at_codes);
+    x.codes[0] = v.x, x.codes[1] = v.y, x.codes[2] = v.z, x.codes[3] = v.w;
+  }
+  x.pair = *reinterpret_cast<const unsigned*>(rows + at_pair);
+  return x;
+}
+
+// Eight values of a quarter (word kk) as the fp16 operand of a product.
+template <int D>
+__device__ __forceinline__ ta_u32x4 unpack(const Quarter<D>& x, int kk) {
+  unsigned w[4];
+  int4_unpack8(x.codes[kk], int4_scale(x.pair), int4_base(x.pair), w);
+  return ta_u32x4{w[0], w[1], w[2], w[3]};
+}
+
+// A row of q as the fp16 operand beside cached keys: bf16 rows are scaled by a power
+// of two that puts their largest element into [2^14, 2^15), so that none is cut and
+// those of 2^-29 of it and more stay exact; the scores get the inverse (factor).
+// A row with an infinity or NaN comes out with one, and is done over by the join.
+template <bool F16, int NK>
+__device__ __forceinline__ float to_fp16(ta_u32x4 (&q)[NK], float scale) {
+  if constexpr (F16) return scale;
+  float top = 0.f;
+#pragma unroll
+  for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(lo_bf16(q[kk][i])), fabsf(hi_bf16(q[kk][i]))));
+  const int e = 15 - __builtin_amdgcn_frexp_expf(row_max(top));
+#pragma unroll
+  for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      q[kk][i] = pack2<true>(__builtin_amdgcn_ldexpf(lo_bf16(q[kk][i]), e), __builtin_amdgcn_ldexpf(hi_bf16(q[kk][i]), e));
+  const float factor = __builtin_amdgcn_ldexpf(scale, -e);
+  return factor == INFINITY ? NAN : factor;  // done over, too
+}
+
+// Few rows: a tile of 16 RT rows, a workgroup of 4 waves. Wave w has keys 16 w ..
+// + 15 of each block of 64 and all rows, so that nothing is shared until the end.
+// A lane has a quarter of a key's row, which it loads (kAhead blocks ahead, into
+// registers) and dequantizes itself. K's quarters are the A operand of S^T = K Q^T as
+// they stand, with Q's dims in the same order; V's go through the wave's own LDS,
+// 16-bit rows in, V^T out by transposed reads. Two blocks make a step: the weights of
+// 2 x 4 keys, rounded to fp16, are the 8 elements of the B operand of O^T += V^T P^T.
+template <int D, bool F16, int RT>
+__global__ __launch_bounds__(256) void tree4_kernel(TreeArgs a) {
+  constexpr int R = 16 * RT, B = kBlock, kRow = kInt4Row<D>, kWide = D * 2;
+  constexpr int NK = D / 32, ND = D / 16, kAhead = D == 64 ? 8 : 4;
+  constexpr int kOwn = 32 * kWide > R * D * 4 ? 32 * kWide : R * D * 4;  // LDS of a wave: V of two blocks, at the end its output
+  __shared__ __attribute__((aligned(16))) unsigned char lds[4 * kOwn];
+  __shared__ float stat_m[4][R], stat_l[4][R];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = uniform(tid >> 6);
+  const int c = lane & 15, quad = lane >> 4;
+  const int G = a.G, ps = 1 << a.page_shift;
+  Share sh;
+  if (!share_of<R, B>(a, blockIdx.x, sh)) return;
+  int u = sh.at, s = sh.s, base = sh.base;
+  const int end = sh.end;
+  Tiles t = sh.t;
+  unsigned char* own = lds + w * kOwn;
+  const unsigned at_codes = c * kRow + quad * (D / 8), at_pair = c * kRow + D / 2 + quad * 4;
+  const int trow = 4 * quad + (c >> 2), tcol = 4 * (c & 3);  // this lane's address of a transposed V read
+  const unsigned char* k_pages = reinterpret_cast<const unsigned char*>(a.k_pages);
+  const unsigned char* v_pages = reinterpret_cast<const unsigned char*>(a.v_pages);
+
+  // V rows of 16 keys: this lane's quarter in, four keys of dims 16 dt + c out.
+  auto put_v = [&](int half, int kk, ta_u32x4 x) {
+    *reinterpret_cast<ta_u32x4*>(own + half * 16 * kWide + c * kWide + v_slot<D>(c, quad * NK + kk) * 16) = x;
+  };
+  auto get_v = [&](int half, int dt) {
+    const int dim = 16 * dt + tcol;
+    return __builtin_bit_cast(ta_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ta_i16x4*)(
+        own + half * 16 * kWide + trow * kWide + v_slot<D>(trow, dim >> 3) * 16 + (dim & 7) * 2)));
+  };
+  // bits of V^T's four keys that count: of `valid` keys
+  auto keep01 = [&](int valid) { return (4 * quad < valid ? 0xffffu : 0u) | (4 * quad + 1 < valid ? 0xffff0000u : 0u); };
+  auto keep23 = [&](int valid) { return (4 * quad + 2 < valid ? 0xffffu : 0u) | (4 * quad + 3 < valid ? 0xffff0000u : 0u); };
+
+  while (u < end) {
+    const int tu = t.tile_units(), tile = uniform((u - base) / tu), in_tile = (u - base) - tile * tu;
+    const int stop = min(tu, in_tile + (end - u)), blk0 = max(in_tile - kOver, 0), n = stop - kOver - blk0;
+    const int hk = uniform(tile / t.row_tiles), row0 = (tile - hk * t.row_tiles) * R;
+    const int rows = min(R, t.nodes * G - row0);
+    if (n > 0) {
+      if (hk == 0 && blk0 == 0)  // for the launch that joins the parts
+        for (int i = row0 / G + tid; i <= (row0 + rows - 1) / G; i += 256) a.owner[t.first + i] = s;
+      const int* table = a.table + static_cast<long long>(s) * a.max_pages;
+      const int cached = min(n, t.cached - blk0);  // blocks of this part that are the cache's (the rest are the tree's)
+      const long long head = static_cast<long long>(hk) * ps * kRow, page_bytes = static_cast<long long>(a.Hkv) * ps * kRow;
+
+      // A block of the cache: where this wave's keys lie, and how many of them count.
+      auto page_of = [&](int i) { return uniform_word(table, min((blk0 + min(i, cached - 1)) * B + 16 * w, t.len - 1) >> a.page_shift); };
+      auto rows_of = [&](int i, int page) {
+        const bool real = static_cast<unsigned>(page) < static_cast<unsigned>(a.num_pages);
+        return (real ? page : 0) * page_bytes + head + (((blk0 + min(i, cached - 1)) * B + 16 * w) & (ps - 1)) * kRow;
+      };
+      auto valid_of = [&](int i, int page) {
+        const bool real = static_cast<unsigned>(page) < static_cast<unsigned>(a.num_pages);
+        return real && i < cached ? max(min(t.len - ((blk0 + i) * B + 16 * w), 16), 0) : 0;
+      };
+      Quarter<D> kq[kAhead], vq[kAhead];
+      int valid[kAhead], page[2] = {0, 0};
+      auto issue = [&](int i, int j) {  // block i into place j
+        const long long at = rows_of(i, page[j & 1]);
+        valid[j] = valid_of(i, page[j & 1]);
+        kq[j] = load_quarter<D>(k_pages + at, at_codes, at_pair);
+        vq[j] = load_quarter<D>(v_pages + at, at_codes, at_pair);
+      };
+      if (cached > 0) {
+        int first[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) first[j] = page_of(j);
+        page[0] = page_of(kAhead);
+        page[1] = page_of(kAhead + 1);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          const int keep = page[j & 1];
+          page[j & 1] = first[j];
+          issue(j, j);
+          page[j & 1] = keep;
+        }
+      }
+      // Q: the B operand of S^T = K Q^T (column: row 16 rt + c; dims D / 4 quad + 8 kk .. + 8)
+      ta_u32x4 qf[RT][NK];
+      int node[RT];
+      float cs[RT];
+      auto load_q = [&](int rt) {
+        const int r = min(row0 + 16 * rt + c, t.nodes * G - 1), in_tree = r / G;
+        node[rt] = t.first + in_tree;
+        const uint16_t* qp = a.q + (static_cast<long long>(node[rt]) * a.H + hk * G + (r - in_tree * G)) * D + quad * (D / 4);
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) qf[rt][kk] = *reinterpret_cast<const ta_u32x4*>(qp + 8 * kk);
+      };
+      ta_f32x4 o[RT][ND];
+      float m[RT], off[RT], l[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        load_q(rt);
+        cs[rt] = to_fp16<F16>(qf[rt], a.scale_log2);
+        m[rt] = -INFINITY;
+        off[rt] = l[rt] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) o[rt][dt] = ta_f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+
+      // Softmax in the log2 domain, p = 2^(s c - m). The row's maximum m moves only
+      // when a score passes it by more than 8, so p <= 2^8 and O is rarely
+      // rescaled; sum(p v) / sum(p) does not depend on which m is used.
+      auto raise = [&](const float (&top)[RT]) {  // of the lane's scores, times c
+        bool grow = false;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) grow |= top[rt] > m[rt] + 8.f;
+        if (__builtin_amdgcn_ballot_w64(grow)) {
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            const float all = row_max(top[rt]);
+            if (all > m[rt] + 8.f) {
+              const float alpha = __builtin_amdgcn_exp2f(m[rt] - all);  // 0 from m = -inf
+              m[rt] = all;
+              off[rt] = all - kLift<true>;
+              l[rt] *= alpha;
+#pragma unroll
+              for (int dt = 0; dt < ND; ++dt) o[rt][dt] *= alpha;
+            }
+          }
+        }
+      };
+      auto step = [&](int j) {  // the blocks in places j and j + 1
+        if (valid[j] + valid[j + 1] == 0) return;
+        ta_f32x4 sc[2][RT];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+#pragma unroll
+          for (int kk = 0; kk < NK; ++kk) put_v(b, kk, unpack<D>(vq[j + b], kk));
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) sc[b][rt] = ta_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int kk = 0; kk < NK; ++kk) {
+            const ta_u32x4 kf = unpack<D>(kq[j + b], kk);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) sc[b][rt] = mfma<true>(kf, qf[rt][kk], sc[b][rt]);
+          }
+        }
+        asm volatile("" ::: "memory");
+        ta_u32x2 vt[2][ND];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt) vt[b][dt] = get_v(b, dt);
+        if (valid[j] + valid[j + 1] < 32) {  // keys that are none: no score, and values that cannot do harm
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const int have = valid[j + b];
+            const unsigned m01 = keep01(have), m23 = keep23(have);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int rt = 0; rt < RT; ++rt) sc[b][rt][e] = 4 * quad + e < have ? sc[b][rt][e] : -INFINITY;
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt) {
+              vt[b][dt].x &= m01;
+              vt[b][dt].y &= m23;
+            }
+          }
+        }
+        float top[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const ta_f32x4 x = sc[0][rt], y = sc[1][rt];
+          top[rt] = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]))) * cs[rt];
+        }
+        raise(top);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          ta_u32x4 pf;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const ta_f32x4 x = sc[i >> 1][rt];
+            pf[i] = pack2<true>(__builtin_amdgcn_exp2f(fmaf(x[2 * (i & 1)], cs[rt], -off[rt])), __builtin_amdgcn_exp2f(fmaf(x[2 * (i & 1) + 1], cs[rt], -off[rt])));
+            l[rt] = add2<true>(pf[i], l[rt]);
+          }
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt) o[rt][dt] = mfma<true>(ta_u32x4{vt[0][dt].x, vt[0][dt].y, vt[1][dt].x, vt[1][dt].y}, pf, o[rt][dt]);
+        }
+        asm volatile("" ::: "memory");
+      };
+      for (int i = 0; i < cached; i += kAhead) {
+#pragma unroll
+        for (int j = 0; j < kAhead; j += 2) {
+          step(j);
+          issue(i + j + kAhead, j);
+          issue(i + j + 1 + kAhead, j + 1);
+          page[0] = page_of(i + j + 2 + kAhead);
+          page[1] = page_of(i + j + 3 + kAhead);
+        }
+      }
+
+      // The tree's own keys, 16-bit rows: weights in two parts (split4), V^T's 4 keys given twice.
+      for (int i = max(cached, 0); i < n; ++i) {
+        const int j0 = (blk0 + i - t.cached) * B + 16 * w, have = min(t.nodes - j0, 16);
+        if (have <= 0) continue;
+        const long long key = (static_cast<long long>(t.first + min(j0 + c, t.nodes - 1)) * a.Hkv + hk) * D + quad * (D / 4);
+        ta_f32x4 sc[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          sc[rt] = ta_f32x4{0.f, 0.f, 0.f, 0.f};
+          load_q(rt);
+        }
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) {
+          const ta_u32x4 kf = *reinterpret_cast<const ta_u32x4*>(a.k_new + key + 8 * kk);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) sc[rt] = mfma<F16>(kf, qf[rt][kk], sc[rt]);
+          put_v(0, kk, *reinterpret_cast<const ta_u32x4*>(a.v_new + key + 8 * kk));
+        }
+        asm volatile("" ::: "memory");
+        float top[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const int word = a.mask[static_cast<long long>(node[rt]) * a.words + (j0 >> 5)] >> ((j0 & 31) + 4 * quad);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[rt][e] = 4 * quad + e < have && (word >> e & 1) ? sc[rt][e] : -INFINITY;
+          top[rt] = fmaxf(fmaxf(sc[rt][0], sc[rt][1]), fmaxf(sc[rt][2], sc[rt][3])) * a.scale_log2;
+        }
+        raise(top);
+        const unsigned m01 = keep01(have), m23 = keep23(have);
+        ta_u32x4 pf[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          float p[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(sc[rt][e], a.scale_log2, -off[rt]));
+          l[rt] += (p[0] + p[1]) + (p[2] + p[3]);
+          pf[rt] = split4<F16>(p);
+        }
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) {
+          ta_u32x2 vt = get_v(0, dt);
+          vt.x &= m01;
+          vt.y &= m23;
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) o[rt][dt] = mfma<F16>(ta_u32x4{vt.x, vt.y, vt.x, vt.y}, pf[rt], o[rt][dt]);
+        }
+        asm volatile("" ::: "memory");
+      }
+
+      // The four waves' parts of the tile meet in LDS.
+      const bool whole = n == t.blocks;
+      const long long slot = 2LL * blockIdx.x + (blk0 == 0 ? 1 : 0);
+      float* mine_o = reinterpret_cast<float*>(own);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const int r = 16 * rt + c;
+        const float sum = row_sum(l[rt]);
+        if (quad == 0) {
+          stat_m[w][r] = m[rt] - kLift<true>;
+          stat_l[w][r] = sum;
+        }
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt)
+          *reinterpret_cast<ta_f32x4*>(mine_o + r * D + (((4 * dt + quad) ^ c) * 4)) = o[rt][dt];
+      }
+      __syncthreads();
+      for (int x = tid; x < rows * (D / 4); x += 256) {
+        const int r = x / (D / 4), c4 = x % (D / 4);
+        float top = stat_m[0][r];
+#pragma unroll
+        for (int i = 1; i < 4; ++i) top = fmaxf(top, stat_m[i][r]);
+        float sum = 0.f;
+        ta_f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float li = stat_l[i][r];
+          const float f = __builtin_amdgcn_exp2f(stat_m[i][r] - top);
+          const ta_f32x4 part = f * *reinterpret_cast<const ta_f32x4*>(reinterpret_cast<const float*>(lds + i * kOwn) + r * D + ((c4 ^ (r & 15)) * 4));
+          sum += li == 0.f ? 0.f : f * li;  // a wave that saw nothing has no maximum either
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] += li == 0.f ? 0.f : part[e];
+        }
+        if (whole) {
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          ta_u32x2 y;
+          if (sum == 0.f) v = ta_f32x4{0.f, 0.f, 0.f, 0.f};
+          if (far_out(top)) v = ta_f32x4{NAN, NAN, NAN, NAN};  // for the launch that joins the parts
+          y.x = narrow<F16>(v[0] * inv) | static_cast<unsigned>(narrow<F16>(v[1] * inv)) << 16;
+          y.y = narrow<F16>(v[2] * inv) | static_cast<unsigned>(narrow<F16>(v[3] * inv)) << 16;
+          const int row = row0 + r;
+          *reinterpret_cast<ta_u32x2*>(a.out + (static_cast<long long>(t.first + row / G) * a.H + hk * G + row % G) * D + c4 * 4) = y;
+        } else {
+          *reinterpret_cast<ta_f32x4*>(a.part_o + (slot * R + r) * D + c4 * 4) = v;
+          if (c4 == 0) a.part_ml[slot * R + r] = make_float2(top, sum);
+        }
+      }
+      __syncthreads();  // the waves' LDS is free again
+    }
+    u += stop - in_tile;
+    if (u < end && u == base + t.units) {
+      base += t.units;
+      do t = uniform_tiles_of<R, B>(a, ++s);
+      while (t.units == 0);
+    }
+  }
+}
+
 // One workgroup per node and 4 heads, a wave for each row, one key at a time.
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void tree4_rows_kernel(TreeArgs a) {
@@ -23,11 +383,23 @@ __global__ __launch_bounds__(256) void tree4_rows_kernel(TreeArgs a) {
   }
 }
 
-int resident(int D, int R) { return 512; }
+// Workgroups that fit the 256 CUs at once.
+int resident(int D, int R) { return D == 64 && R == 16 ? 768 : 512; }
+
+template <int D, bool F16, int RT>
+void launch_few(const TreeArgs& a, hipStream_t s) {
+  IRON_LAUNCH((tree4_kernel<D, F16, RT>), dim3(a.workgroups), dim3(256), 0, s, a);
+  IRON_LAUNCH((tree_join_kernel<D, F16, 16 * RT, kBlock, true>), dim3(a.num_nodes, (a.H + 3) / 4), dim3(256), 0, s, a);
+}
 
 template <int D, bool F16>
-void launch_rows(const TreeArgs& a, hipStream_t s) {
-  IRON_LAUNCH((tree4_rows_kernel<D, F16>), dim3(a.num_nodes, (a.H + 3) / 4), dim3(256), 0, s, a);
+void launch_rows(const TreeArgs& a, int R, hipStream_t s) {
+  if (R == 16)
+    launch_few<D, F16, 1>(a, s);
+  else if (R == 32)
+    launch_few<D, F16, 2>(a, s);
+  else
+    IRON_LAUNCH((tree4_rows_kernel<D, F16>), dim3(a.num_nodes, (a.H + 3) / 4), dim3(256), 0, s, a);
 }
 
 }  // namespace
@@ -51,10 +423,11 @@ extern "C" int iron_tree_attention_int4(const void* q, const void* k_new, const 
                          node_starts, tree_mask, out, dtype, n_heads, n_kv_heads, head_dim, num_pages, page_size, num_seqs,
                          max_pages, num_nodes, max_nodes, scale, workspace, workspace_bytes))
     return rc;
+  const int R = rows_of_tile(n_heads, n_kv_heads, max_nodes);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (head_dim == 64)
-    dtype ? launch_rows<64, true>(a, s) : launch_rows<64, false>(a, s);
+    dtype ? launch_rows<64, true>(a, R, s) : launch_rows<64, false>(a, R, s);
   else
-    dtype ? launch_rows<128, true>(a, s) : launch_rows<128, false>(a, s);
+    dtype ? launch_rows<128, true>(a, R, s) : launch_rows<128, false>(a, R, s);
   return check_launch("tree_attention_int4");
 }

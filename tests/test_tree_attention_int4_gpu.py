@@ -143,8 +143,8 @@ def test_what_is_not_seen_does_not_matter(gpu, dtype, counts):
     c = case(gpu, 4, 2, 64, dtype, [37, 70], counts, seed=8)
     c["sees"][:, 1] = False
     c["table"][1, 1] = -1
-    want = run(gpu, c).clone()
-    check(c, want)
+    clean = {**c, **{k: c[k].clone() for k in ("k", "v", "k_new", "v_new")}}
+    check(clean, run(gpu, clean))
     nan_row = torch.full((int4_row_bytes(64),), 0xff, dtype=torch.uint8, device=gpu)  # s and b are NaN
     inf_row = nan_row.clone()
     inf_row[32:] = torch.tensor([0x00, 0x7c] * 8, dtype=torch.uint8, device=gpu)
@@ -158,9 +158,7 @@ def test_what_is_not_seen_does_not_matter(gpu, dtype, counts):
         c["v"][unused] = row
         c["k_new"][1] = math.nan
         c["v_new"][1] = math.inf
-        got = run(gpu, c)
-        keep = [i for i in range(sum(counts)) if i != 1]
-        assert torch.equal(got[keep], want[keep])
+        check(clean, run(gpu, c))  # rows may be done over for it, with other roundings
 
 
 @pytest.mark.parametrize("counts", [[2, 1], [40, 3]])
