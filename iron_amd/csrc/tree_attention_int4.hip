@@ -40,7 +40,7 @@ __device__ __forceinline__ ta_u32x4 unpack(const Quarter<D>& x, int kk) {
 // of two that puts their largest element into [2^14, 2^15), so that none is cut and
 // those of 2^-29 of it and more stay exact; the scores get the inverse (factor).
 // A row with an infinity or NaN comes out with one, and is done over by the join.
-template <bool F16, int NK>
+template <bool F16, bool WIDE, int NK>
 __device__ __forceinline__ float to_fp16(ta_u32x4 (&q)[NK], float scale) {
   if constexpr (F16) return scale;
   float top = 0.f;
@@ -48,7 +48,14 @@ __device__ __forceinline__ float to_fp16(ta_u32x4 (&q)[NK], float scale) {
   for (int kk = 0; kk < NK; ++kk)
 #pragma unroll
     for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(lo_bf16(q[kk][i])), fabsf(hi_bf16(q[kk][i]))));
-  const int e = 15 - __builtin_amdgcn_frexp_expf(row_max(top));
+  if constexpr (WIDE) {  // two lanes have a row, or four
+    float x, y;
+    swap32(top, x, y);
+    top = fmaxf(x, y);
+  } else {
+    top = row_max(top);
+  }
+  const int e = 15 - __builtin_amdgcn_frexp_expf(top);
 #pragma unroll
   for (int kk = 0; kk < NK; ++kk)
 #pragma unroll
@@ -160,7 +167,7 @@ __global__ __launch_bounds__(256) void tree4_kernel(TreeArgs a) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         load_q(rt);
-        cs[rt] = to_fp16<F16>(qf[rt], a.scale_log2);
+        cs[rt] = to_fp16<F16, false>(qf[rt], a.scale_log2);
         m[rt] = -INFINITY;
         off[rt] = l[rt] = 0.f;
 #pragma unroll
@@ -366,25 +373,282 @@ __global__ __launch_bounds__(256) void tree4_kernel(TreeArgs a) {
   }
 }
 
-// One workgroup per node and 4 heads, a wave for each row, one key at a time.
+// Many rows: a tile of 128 rows, a workgroup of 4 waves with 32 rows each. The waves
+// dequantize blocks of 32 keys together (8 rows of K and of V each) into a ring of
+// 16-bit rows in LDS, two blocks ahead of their use and four ahead of it into
+// registers; a block is dequantized once for 128 rows. From there on it is
+// tree_wide_kernel: scores of the next block among this one's softmax, one barrier a
+// block. The cache's blocks come first, with fp16 products, then the tree's, with
+// those of its type; a row's maximum, sum and output go on through both.
 template <int D, bool F16>
-__global__ __launch_bounds__(256) void tree4_rows_kernel(TreeArgs a) {
-  const int n = blockIdx.x, h = blockIdx.y * 4 + uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (h >= a.H) return;
-  for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
-    const int s = min(s0 + lane, a.num_seqs - 1);
-    int first, nodes;
-    tree_of(a, s, first, nodes);
-    const unsigned long long has = __ballot(s0 + lane < a.num_seqs && first <= n && n < first + nodes);
-    if (!has) continue;
-    const int who = s0 + __ffsll(has) - 1;
-    attend_row<D, F16, true>(a, uniform_tiles_of<16, kBlock>(a, who), who, n, h);
-    return;
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void tree4_wide_kernel(TreeArgs a) {
+  constexpr int R = 128, B = kWideBlock, kRow = D * 2, kHalf = B * kRow, kStage = 2 * kHalf, kRing = 3;
+  constexpr int kRow4 = kInt4Row<D>, NW = D / 64;  // words of codes (16-byte chunks of 16-bit rows) of a lane and block
+  constexpr int NK = D / 16, ND = D / 32;
+  __shared__ __attribute__((aligned(16))) unsigned char ring[kRing * kStage];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = uniform(tid >> 6);
+  const int c = lane & 31, hh = lane >> 5;
+  const int G = a.G, ps = 1 << a.page_shift;
+  Share sh;
+  if (!share_of<R, B>(a, blockIdx.x, sh)) return;
+  int u = sh.at, s = sh.s, base = sh.base;
+  const int end = sh.end;
+  Tiles t = sh.t;
+
+  // This lane's part of a block: NW chunks from chunk0 on of row srow.
+  const int srow = 8 * w + (lane >> 3), chunk0 = NW * (lane & 7);
+  const unsigned at_codes = (lane >> 3) * kRow4 + chunk0 * 4, at_pair = (lane >> 3) * kRow4 + D / 2 + (lane & 7) / 2 * 4;
+  const int trow = 4 * hh + ((lane & 15) >> 2), tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  // Both swizzles are exclusive ors, so a fragment's address is the first one's with
+  // the fragment's own bits turned: one register for each operand.
+  const unsigned k_first = c * kRow + k_slot<D>(c & 15, hh) * 16;
+  const unsigned v_first = kHalf + trow * kRow + wide_v_slot<D>(trow, tcol >> 3) * 16 + (tcol & 7) * 2;
+  const unsigned char* k_pages = reinterpret_cast<const unsigned char*>(a.k_pages);
+  const unsigned char* v_pages = reinterpret_cast<const unsigned char*>(a.v_pages);
+
+  while (u < end) {
+    const int tu = t.tile_units(), tile = uniform((u - base) / tu), in_tile = (u - base) - tile * tu;
+    const int stop = min(tu, in_tile + (end - u)), blk0 = max(in_tile - kOver, 0), n = stop - kOver - blk0;
+    const int hk = uniform(tile / t.row_tiles), row0 = (tile - hk * t.row_tiles) * R;
+    const int rows = min(R, t.nodes * G - row0);
+    if (n > 0) {
+      if (hk == 0 && blk0 == 0)  // for the launch that joins the parts
+        for (int i = row0 / G + tid; i <= (row0 + rows - 1) / G; i += 256) a.owner[t.first + i] = s;
+      const int r = min(row0 + 32 * w + c, t.nodes * G - 1), in_tree = r / G;
+      const int node = t.first + in_tree;
+      const long long q_row = static_cast<long long>(node) * a.H + hk * G + (r - in_tree * G);
+      ta_f32x16 o[ND];
+      float m = -INFINITY, off = 0.f, l = 0.f;
+#pragma unroll
+      for (int db = 0; db < ND; ++db)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[db][j] = 0.f;
+      const bool idle = 32 * w >= rows;  // none of the wave's rows is one
+
+      // Blocks blk0 .. of the cache (CACHE) or of the tree.
+      auto phase = [&](auto cache) {
+        constexpr bool CACHE = decltype(cache)::value, T16 = CACHE || F16;  // fp16 operands
+        const int nb = CACHE ? min(n, t.cached - blk0) : n - max(min(n, t.cached - blk0), 0);
+        if (nb <= 0) return;
+        const int first = CACHE ? blk0 : max(blk0 - t.cached, 0), have = CACHE ? t.len : t.nodes;
+        const int whole_blocks = have / B - first;  // the first ones of them, with no key behind the last
+        // Q: the B operand of S^T = K Q^T (column: row 32 w + c; dims 16 kk + 8 hh .. + 8)
+        ta_u32x4 qf[NK];
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) qf[kk] = *reinterpret_cast<const ta_u32x4*>(a.q + q_row * D + 16 * kk + 8 * hh);
+        const float cs = CACHE ? to_fp16<F16, true>(qf, a.scale_log2) : a.scale_log2;
+
+        // A block's rows on their way: codes and pairs, or 16-bit chunks.
+        struct Ahead {
+          ta_u32x4 k[CACHE ? 1 : NW], v[CACHE ? 1 : NW];
+          unsigned kp, vp;
+        };
+        constexpr int kDeep = !CACHE && D == 128 ? 1 : 2;  // blocks on their way (16-bit rows of 128 take too many registers for two)
+        Ahead ahead[2];
+        unsigned holes = 0;  // bits 2 (i % 8) and + 1: the two pages of block i's 16 rows each are none
+        const int* table = a.table + static_cast<long long>(s) * a.max_pages;
+        const long long head = static_cast<long long>(hk) * ps * kRow4, page_bytes = static_cast<long long>(a.Hkv) * ps * kRow4;
+        int page0 = 0, page1 = 0;
+        auto pages_of = [&](int i) {
+          if constexpr (CACHE) {
+            const int pos = (first + min(i, nb - 1)) * B;
+            page0 = uniform_word(table, pos >> a.page_shift);
+            page1 = uniform_word(table, min(pos + 16, t.len - 1) >> a.page_shift);
+          }
+        };
+        auto issue = [&](int i, Ahead& x) {  // block i, or the last one again
+          const int blk = first + min(i, nb - 1);
+          if constexpr (CACHE) {
+            const bool none0 = static_cast<unsigned>(page0) >= static_cast<unsigned>(a.num_pages);
+            const bool none1 = static_cast<unsigned>(page1) >= static_cast<unsigned>(a.num_pages);
+            holes = (holes & ~(3u << (2 * (i & 7)))) | ((none0 ? 1u : 0u) | (none1 ? 2u : 0u)) << (2 * (i & 7));
+            const int page = w < 2 ? (none0 ? 0 : page0) : (none1 ? 0 : page1);
+            const long long at = page * page_bytes + head + ((blk * B + 8 * w) & (ps - 1)) * kRow4;
+            if constexpr (NW == 1) {
+              x.k[0].x = *reinterpret_cast<const unsigned*>(k_pages + at + at_codes);
+              x.v[0].x = *reinterpret_cast<const unsigned*>(v_pages + at + at_codes);
+            } else {
+              const ta_u32x2 k = *reinterpret_cast<const ta_u32x2*>(k_pages + at + at_codes), v = *reinterpret_cast<const ta_u32x2*>(v_pages + at + at_codes);
+              x.k[0].x = k.x, x.k[0].y = k.y, x.v[0].x = v.x, x.v[0].y = v.y;
+            }
+            x.kp = *reinterpret_cast<const unsigned*>(k_pages + at + at_pair);
+            x.vp = *reinterpret_cast<const unsigned*>(v_pages + at + at_pair);
+            pages_of(i + 1);
+          } else {
+            const long long at = (static_cast<long long>(t.first + min(blk * B + srow, t.nodes - 1)) * a.Hkv + hk) * D + chunk0 * 8;
+#pragma unroll
+            for (int e = 0; e < NW; ++e) {
+              x.k[e] = *reinterpret_cast<const ta_u32x4*>(a.k_new + at + 8 * e);
+              x.v[e] = *reinterpret_cast<const ta_u32x4*>(a.v_new + at + 8 * e);
+            }
+          }
+        };
+        // Block i's rows into their stage; values of keys that are none become zeros, which cannot do harm.
+        auto stage = [&](int i, const Ahead& x) {
+          unsigned char* st = ring + i % kRing * kStage;
+          const unsigned none = holes >> (2 * (i & 7)) & 3u;
+          const bool gone = (i >= whole_blocks && (first + i) * B + srow >= have) || (none >> (w >> 1) & 1);
+#pragma unroll
+          for (int e = 0; e < NW; ++e) {
+            ta_u32x4 k, v;
+            if constexpr (CACHE) {
+              unsigned y[4];
+              int4_unpack8(e ? x.k[0].y : x.k[0].x, int4_scale(x.kp), int4_base(x.kp), y);
+              k = ta_u32x4{y[0], y[1], y[2], y[3]};
+              int4_unpack8(e ? x.v[0].y : x.v[0].x, int4_scale(x.vp), int4_base(x.vp), y);
+              v = ta_u32x4{y[0], y[1], y[2], y[3]};
+            } else {
+              k = x.k[e], v = x.v[e];
+            }
+            if (gone) v = ta_u32x4{0, 0, 0, 0};
+            *reinterpret_cast<ta_u32x4*>(st + srow * kRow + k_slot<D>(srow & 15, chunk0 + e) * 16) = k;
+            *reinterpret_cast<ta_u32x4*>(st + kHalf + srow * kRow + wide_v_slot<D>(srow, chunk0 + e) * 16) = v;
+          }
+        };
+        auto k_frag = [&](int i, int kk) {
+          return *reinterpret_cast<const ta_u32x4*>(ring + ((i % kRing * kStage + k_first) ^ (32 * kk)));
+        };
+        // V^T of keys 8 q + 4 hh .. + 3 of block i, dims 32 db + lane % 32
+        auto v_frag = [&](int i, int q, int db) {
+          return __builtin_bit_cast(ta_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ta_i16x4*)(
+              ring + ((i % kRing * kStage + v_first) ^ (64 * db)) + 8 * q * kRow)));
+        };
+        // The row's maximum, when scores pass it by more than 8 (in the log2 domain; cf. tree4_kernel).
+        auto raise = [&](const ta_f32x16& sc) {
+          float mx = fmaxf(fmaxf(sc[0], sc[1]), sc[2]);
+#pragma unroll
+          for (int j = 3; j < 15; j += 2) mx = fmaxf(fmaxf(mx, sc[j]), sc[j + 1]);
+          mx = fmaxf(mx, sc[15]);
+          if (__builtin_amdgcn_ballot_w64(mx * cs > m + 8.f)) {
+            float x, y;
+            swap32(mx, x, y);
+            const float top = fmaxf(x, y) * cs;
+            if (top > m + 8.f) {
+              const float alpha = __builtin_amdgcn_exp2f(m - top);  // 0 from m = -inf
+              m = top;
+              off = top - kLift<true>;
+              l *= alpha;
+#pragma unroll
+              for (int db = 0; db < ND; ++db) o[db] *= alpha;
+            }
+          }
+        };
+        // Weights 2 g and 2 g + 1 of the lane, rounded to 16 bits as the second product takes them; l sums those.
+        auto weights = [&](const ta_f32x16& sc, int g) {
+          const unsigned p = pack2<T16>(__builtin_amdgcn_exp2f(fmaf(sc[2 * g], cs, -off)), __builtin_amdgcn_exp2f(fmaf(sc[2 * g + 1], cs, -off)));
+          l = add2<T16>(p, l);
+          return p;
+        };
+        // Block i from its scores S^T: sc[j] is key 8 (j / 4) + 4 hh + j % 4, row 32 w + c.
+        auto step = [&](int i, ta_f32x16& sc, ta_f32x16& next) {
+          const unsigned none = holes >> (2 * (i & 7)) & 3u;
+          if (!CACHE || i >= whole_blocks || none) {  // some of its keys are none, or not for every row
+            const int j0 = (first + i) * B, left = have - j0;
+            unsigned seen = left >= 32 ? ~0u : (1u << left) - 1;  // those that there are
+            seen &= ~((none & 1 ? 0xffffu : 0u) | (none & 2 ? 0xffff0000u : 0u));
+            if (!CACHE) seen &= a.mask[static_cast<long long>(node) * a.words + (j0 >> 5)];
+            seen >>= 4 * hh;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sc[j] = seen >> (8 * (j >> 2) + (j & 3)) & 1 ? sc[j] : -INFINITY;
+          }
+          ta_u32x4 kf[NK];  // of block i + 1 (behind the last block: a stage that nothing writes, for scores that go unused)
+#pragma unroll
+          for (int kk = 0; kk < NK; ++kk) kf[kk] = k_frag(i + 1, kk);
+          raise(sc);
+          // In eight groups, held in this order by the scheduling barriers (cf. tree_wide_kernel).
+          ta_u32x4 pf[2];  // P^T of keys 16 g + 4 hh .. + 3 and + 8 .. + 11
+          ta_u32x2 vt[4][ND];
+          auto pv = [&](int g, int db) {
+            o[db] = mfma32<T16>(ta_u32x4{vt[2 * g][db].x, vt[2 * g][db].y, vt[2 * g + 1][db].x, vt[2 * g + 1][db].y}, pf[g], o[db]);
+          };
+          next = ta_f32x16{};
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (g < NK) next = mfma32<T16>(kf[g], qf[g], next);
+            if (g >= 4 && g - 4 < ND) pv(0, g - 4);
+#pragma unroll
+            for (int e = g * ND / 2; e < (g + 1) * ND / 2; ++e) vt[e / ND][e % ND] = v_frag(i, e / ND, e % ND);
+            pf[g / 4][g % 4] = weights(sc, g);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int db = 0; db < ND; ++db) pv(1, db);
+        };
+        auto meet = [&] {  // every wave's LDS accesses so far are done
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+        };
+        // Stages: i (V being read), i + 1 (K being read), i + 2 being written, which every wave has left.
+        auto turn = [&](int i, ta_f32x16& sc, ta_f32x16& next, Ahead& x) {
+          meet();  // block i + 1 is there, and block i - 1's stage read by all
+          if (i + 2 < nb) stage(i + 2, x);
+          issue(i + 2 + kDeep, x);
+          if (!idle) step(i, sc, next);
+        };
+        pages_of(0);
+        issue(0, ahead[0]);
+        if (kDeep == 2) issue(1, ahead[1]);
+        stage(0, ahead[0]);
+        issue(kDeep, ahead[0]);
+        if (nb > 1) stage(1, ahead[kDeep - 1]);
+        issue(kDeep + 1, ahead[kDeep - 1]);
+        meet();
+        ta_f32x16 sa = {}, sb = {};
+        if (!idle)
+#pragma unroll
+          for (int kk = 0; kk < NK; ++kk) sa = mfma32<T16>(k_frag(0, kk), qf[kk], sa);
+        for (int i = 0; i < nb; i += 2) {
+          turn(i, sa, sb, ahead[0]);
+          if (i + 1 < nb) turn(i + 1, sb, sa, ahead[kDeep - 1]);
+        }
+        meet();  // the ring is free again
+      };
+      phase(std::true_type{});
+      phase(std::false_type{});
+
+      const bool whole = n == t.blocks;
+      float l0, l1;
+      swap32(l, l0, l1);
+      const float sum = l0 + l1;
+      const bool far = whole && far_out(m);  // NaN, for the launch that joins the parts
+      if (32 * w + c < rows) {
+        const long long part = (2LL * blockIdx.x + (blk0 == 0 ? 1 : 0)) * R + 32 * w + c;
+        const float inv = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
+        if (!whole && hh == 0) a.part_ml[part] = make_float2(m - kLift<true>, sum);
+#pragma unroll
+        for (int db = 0; db < ND; ++db)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int dim = 32 * db + 8 * q + 4 * hh;
+            ta_f32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = far ? NAN : sum == 0.f ? 0.f : o[db][4 * q + e] * inv;
+            if (whole) {
+              ta_u32x2 z;
+              z.x = narrow<F16>(v[0]) | static_cast<unsigned>(narrow<F16>(v[1])) << 16;
+              z.y = narrow<F16>(v[2]) | static_cast<unsigned>(narrow<F16>(v[3])) << 16;
+              *reinterpret_cast<ta_u32x2*>(a.out + q_row * D + dim) = z;
+            } else {
+              *reinterpret_cast<ta_f32x4*>(a.part_o + part * D + dim) = v;
+            }
+          }
+      }
+      __syncthreads();  // the ring is free again
+    }
+    u += stop - in_tile;
+    if (u < end && u == base + t.units) {
+      base += t.units;
+      do t = uniform_tiles_of<R, B>(a, ++s);
+      while (t.units == 0);
+    }
   }
 }
 
 // Workgroups that fit the 256 CUs at once.
-int resident(int D, int R) { return D == 64 && R == 16 ? 768 : 512; }
+int resident(int D, int R) { return D == 64 && R != 32 ? 768 : 512; }
 
 template <int D, bool F16, int RT>
 void launch_few(const TreeArgs& a, hipStream_t s) {
@@ -398,8 +662,10 @@ void launch_rows(const TreeArgs& a, int R, hipStream_t s) {
     launch_few<D, F16, 1>(a, s);
   else if (R == 32)
     launch_few<D, F16, 2>(a, s);
-  else
-    IRON_LAUNCH((tree4_rows_kernel<D, F16>), dim3(a.num_nodes, (a.H + 3) / 4), dim3(256), 0, s, a);
+  else {
+    IRON_LAUNCH((tree4_wide_kernel<D, F16>), dim3(a.workgroups), dim3(256), 0, s, a);
+    IRON_LAUNCH((tree_join_kernel<D, F16, 128, kWideBlock, true>), dim3(a.num_nodes, (a.H + 3) / 4), dim3(256), 0, s, a);
+  }
 }
 
 }  // namespace
