@@ -27,6 +27,21 @@ __device__ __forceinline__ void int4_unpack8(unsigned codes, i4_f16x2 s, i4_f16x
     out[i] = __builtin_bit_cast(unsigned, __builtin_elementwise_fma(__builtin_bit_cast(i4_f16x2, (x[i] & kMask) | kSixteen), s, b));
 }
 
+// The same as sums of two fp16 numbers and b, without rounding: s has 11 bits and
+// 16 + code has 5, so s is cut behind its sixth, and (16 + code) / 2 times either part
+// fits fp16 (halved, the largest s does too; below 2^-13 the lower part may lose
+// its last bit, 2^-25). high + low + b / 2 is half the value.
+__device__ __forceinline__ void int4_split8(unsigned codes, i4_f16x2 s_high, i4_f16x2 s_low, unsigned (&high)[4], unsigned (&low)[4]) {
+  constexpr unsigned kMask = 0x03c003c0u, kEight = 0x48004800u;
+  const unsigned x[4] = {codes << 6, codes << 2, codes >> 2, codes >> 6};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const i4_f16x2 y = __builtin_bit_cast(i4_f16x2, (x[i] & kMask) | kEight);
+    high[i] = __builtin_bit_cast(unsigned, y * s_high);
+    low[i] = __builtin_bit_cast(unsigned, y * s_low);
+  }
+}
+
 // s and b of a pair, twice each.
 __device__ __forceinline__ i4_f16x2 int4_scale(unsigned pair) {
   const _Float16 s = __builtin_bit_cast(_Float16, static_cast<uint16_t>(pair & 0xffffu));

@@ -36,6 +36,22 @@ __device__ __forceinline__ ta_u32x4 unpack(const Quarter<D>& x, int kk) {
   return ta_u32x4{w[0], w[1], w[2], w[3]};
 }
 
+// The same without rounding: half a value is high + low + b / 2 (int4_split8).
+template <int D>
+__device__ __forceinline__ void unpack(const Quarter<D>& x, int kk, ta_u32x4& high, ta_u32x4& low) {
+  const i4_f16x2 s = int4_scale(x.pair), s_high = int4_scale(x.pair & 0xffe0u);
+  unsigned a[4], b[4];
+  int4_split8(x.codes[kk], s_high, s - s_high, a, b);
+  high = ta_u32x4{a[0], a[1], a[2], a[3]};
+  low = ta_u32x4{b[0], b[1], b[2], b[3]};
+}
+
+// A number as two fp16 ones, the upper in the low half.
+__device__ __forceinline__ unsigned split_fp16(float x) {
+  const _Float16 high = static_cast<_Float16>(x), low = static_cast<_Float16>(x - static_cast<float>(high));
+  return __builtin_bit_cast(unsigned, ta_f16x2{high, low});
+}
+
 // A row of q as the fp16 operand beside cached keys: bf16 rows are scaled by a power
 // of two that puts their largest element into [2^14, 2^15), so that none is cut and
 // those of 2^-29 of it and more stay exact; the scores get the inverse (factor).
@@ -73,9 +89,9 @@ __device__ __forceinline__ float to_fp16(ta_u32x4 (&q)[NK], float scale) {
 // 16-bit rows in, V^T out by transposed reads. Two blocks make a step: the weights of
 // 2 x 4 keys, rounded to fp16, are the 8 elements of the B operand of O^T += V^T P^T.
 template <int D, bool F16, int RT>
-__global__ __launch_bounds__(256) void tree4_kernel(TreeArgs a) {
+__global__ __launch_bounds__(256, 2) void tree4_kernel(TreeArgs a) {
   constexpr int R = 16 * RT, B = kBlock, kRow = kInt4Row<D>, kWide = D * 2;
-  constexpr int NK = D / 32, ND = D / 16, kAhead = D == 64 ? 8 : 4;
+  constexpr int NK = D / 32, ND = D / 16, kAhead = D == 64 ? 8 : RT == 2 ? 2 : 4;
   constexpr int kOwn = 32 * kWide > R * D * 4 ? 32 * kWide : R * D * 4;  // LDS of a wave: V of two blocks, at the end its output
   __shared__ __attribute__((aligned(16))) unsigned char lds[4 * kOwn];
   __shared__ float stat_m[4][R], stat_l[4][R];
@@ -153,6 +169,7 @@ __global__ __launch_bounds__(256) void tree4_kernel(TreeArgs a) {
       }
       // Q: the B operand of S^T = K Q^T (column: row 16 rt + c; dims D / 4 quad + 8 kk .. + 8)
       ta_u32x4 qf[RT][NK];
+      unsigned q_half[RT];  // fp16: half the sum of the lane's dims, in two parts, b's factor
       int node[RT];
       float cs[RT];
       auto load_q = [&](int rt) {
@@ -168,6 +185,15 @@ __global__ __launch_bounds__(256) void tree4_kernel(TreeArgs a) {
       for (int rt = 0; rt < RT; ++rt) {
         load_q(rt);
         cs[rt] = to_fp16<F16, false>(qf[rt], a.scale_log2);
+        if constexpr (F16) {
+          float sum = 0.f;
+#pragma unroll
+          for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum = add2<true>(qf[rt][kk][i], sum);
+          q_half[rt] = split_fp16(sum * 0.5f);
+          cs[rt] *= 2.f;
+        }
         m[rt] = -INFINITY;
         off[rt] = l[rt] = 0.f;
 #pragma unroll
@@ -207,32 +233,49 @@ __global__ __launch_bounds__(256) void tree4_kernel(TreeArgs a) {
           for (int rt = 0; rt < RT; ++rt) sc[b][rt] = ta_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int kk = 0; kk < NK; ++kk) {
-            const ta_u32x4 kf = unpack<D>(kq[j + b], kk);
+            if constexpr (F16) {
+              ta_u32x4 high, low;
+              unpack<D>(kq[j + b], kk, high, low);
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) sc[b][rt] = mfma<true>(kf, qf[rt][kk], sc[b][rt]);
+              for (int rt = 0; rt < RT; ++rt) sc[b][rt] = mfma<true>(low, qf[rt][kk], mfma<true>(high, qf[rt][kk], sc[b][rt]));
+            } else {
+              const ta_u32x4 kf = unpack<D>(kq[j + b], kk);
+#pragma unroll
+              for (int rt = 0; rt < RT; ++rt) sc[b][rt] = mfma<true>(kf, qf[rt][kk], sc[b][rt]);
+            }
+          }
+          if constexpr (F16) {  // b, twice, times the two parts of the sum of the quarter's dims
+            const unsigned bb = __builtin_bit_cast(unsigned, int4_base(kq[j + b].pair));
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) sc[b][rt] = mfma<true>(ta_u32x4{bb, 0, 0, 0}, ta_u32x4{q_half[rt], 0, 0, 0}, sc[b][rt]);
           }
         }
         asm volatile("" ::: "memory");
-        ta_u32x2 vt[2][ND];
+        const bool some = valid[j] + valid[j + 1] < 32;  // keys that are none: no score, and values that cannot do harm
+        if (some) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int dt = 0; dt < ND; ++dt) vt[b][dt] = get_v(b, dt);
-        if (valid[j] + valid[j + 1] < 32) {  // keys that are none: no score, and values that cannot do harm
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const int have = valid[j + b];
-            const unsigned m01 = keep01(have), m23 = keep23(have);
+          for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
-              for (int rt = 0; rt < RT; ++rt) sc[b][rt][e] = 4 * quad + e < have ? sc[b][rt][e] : -INFINITY;
+              for (int rt = 0; rt < RT; ++rt) sc[b][rt][e] = 4 * quad + e < valid[j + b] ? sc[b][rt][e] : -INFINITY;
+        }
+        ta_u32x2 vt[2][ND];
+        auto get = [&](int b) {
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt) vt[b][dt] = get_v(b, dt);
+          if (some) {
+            const unsigned m01 = keep01(valid[j + b]), m23 = keep23(valid[j + b]);
 #pragma unroll
             for (int dt = 0; dt < ND; ++dt) {
               vt[b][dt].x &= m01;
               vt[b][dt].y &= m23;
             }
           }
+        };
+        if constexpr (!F16) {
+          get(0);
+          get(1);
         }
         float top[RT];
 #pragma unroll
@@ -241,17 +284,35 @@ __global__ __launch_bounds__(256) void tree4_kernel(TreeArgs a) {
           top[rt] = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]))) * cs[rt];
         }
         raise(top);
+        if constexpr (F16) {  // weights in two parts (split4), V^T's 4 keys given twice
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          ta_u32x4 pf;
+          for (int b = 0; b < 2; ++b) {
+            get(b);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const ta_f32x4 x = sc[i >> 1][rt];
-            pf[i] = pack2<true>(__builtin_amdgcn_exp2f(fmaf(x[2 * (i & 1)], cs[rt], -off[rt])), __builtin_amdgcn_exp2f(fmaf(x[2 * (i & 1) + 1], cs[rt], -off[rt])));
-            l[rt] = add2<true>(pf[i], l[rt]);
+            for (int rt = 0; rt < RT; ++rt) {
+              float p[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(sc[b][rt][e], cs[rt], -off[rt]));
+              l[rt] += (p[0] + p[1]) + (p[2] + p[3]);
+              const ta_u32x4 pf = split4<true>(p);
+#pragma unroll
+              for (int dt = 0; dt < ND; ++dt) o[rt][dt] = mfma<true>(ta_u32x4{vt[b][dt].x, vt[b][dt].y, vt[b][dt].x, vt[b][dt].y}, pf, o[rt][dt]);
+            }
+            asm volatile("" ::: "memory");
           }
+        } else {
 #pragma unroll
-          for (int dt = 0; dt < ND; ++dt) o[rt][dt] = mfma<true>(ta_u32x4{vt[0][dt].x, vt[0][dt].y, vt[1][dt].x, vt[1][dt].y}, pf, o[rt][dt]);
+          for (int rt = 0; rt < RT; ++rt) {
+            ta_u32x4 pf;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const ta_f32x4 x = sc[i >> 1][rt];
+              pf[i] = pack2<true>(__builtin_amdgcn_exp2f(fmaf(x[2 * (i & 1)], cs[rt], -off[rt])), __builtin_amdgcn_exp2f(fmaf(x[2 * (i & 1) + 1], cs[rt], -off[rt])));
+              l[rt] = add2<true>(pf[i], l[rt]);
+            }
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt) o[rt][dt] = mfma<true>(ta_u32x4{vt[0][dt].x, vt[0][dt].y, vt[1][dt].x, vt[1][dt].y}, pf, o[rt][dt]);
+          }
         }
         asm volatile("" ::: "memory");
       };
@@ -381,11 +442,12 @@ __global__ __launch_bounds__(256) void tree4_kernel(TreeArgs a) {
 // block. The cache's blocks come first, with fp16 products, then the tree's, with
 // those of its type; a row's maximum, sum and output go on through both.
 template <int D, bool F16>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void tree4_wide_kernel(TreeArgs a) {
-  constexpr int R = 128, B = kWideBlock, kRow = D * 2, kHalf = B * kRow, kStage = 2 * kHalf, kRing = 3;
+__global__ __launch_bounds__(256, D == 64 && !F16 ? 3 : 2) void tree4_wide_kernel(TreeArgs a) {
+  constexpr int R = 128, B = kWideBlock, kRow = D * 2, kHalf = B * kRow, kRing = 3;
+  constexpr int kStage = F16 ? 3 * kHalf : 2 * kHalf;  // K, V and, with fp16, K's lower parts; b's behind the ring
   constexpr int kRow4 = kInt4Row<D>, NW = D / 64;  // words of codes (16-byte chunks of 16-bit rows) of a lane and block
   constexpr int NK = D / 16, ND = D / 32;
-  __shared__ __attribute__((aligned(16))) unsigned char ring[kRing * kStage];
+  __shared__ __attribute__((aligned(16))) unsigned char ring[kRing * kStage + (F16 ? kRing * B * 16 : 0)];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = uniform(tid >> 6);
   const int c = lane & 31, hh = lane >> 5;
@@ -399,6 +461,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void tree4_wide_kernel(TreeAr
   // This lane's part of a block: NW chunks from chunk0 on of row srow.
   const int srow = 8 * w + (lane >> 3), chunk0 = NW * (lane & 7);
   const unsigned at_codes = (lane >> 3) * kRow4 + chunk0 * 4, at_pair = (lane >> 3) * kRow4 + D / 2 + (lane & 7) / 2 * 4;
+  const unsigned k_store = srow * kRow + k_slot<D>(srow & 15, chunk0) * 16, v_store = kHalf + srow * kRow + wide_v_slot<D>(srow, chunk0) * 16;
   const int trow = 4 * hh + ((lane & 15) >> 2), tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
   // Both swizzles are exclusive ors, so a fragment's address is the first one's with
   // the fragment's own bits turned: one register for each operand.
@@ -428,7 +491,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void tree4_wide_kernel(TreeAr
 
       // Blocks blk0 .. of the cache (CACHE) or of the tree.
       auto phase = [&](auto cache) {
-        constexpr bool CACHE = decltype(cache)::value, T16 = CACHE || F16;  // fp16 operands
+        constexpr bool CACHE = decltype(cache)::value, T16 = CACHE || F16, EXACT = CACHE && F16;  // T16: fp16 operands
         const int nb = CACHE ? min(n, t.cached - blk0) : n - max(min(n, t.cached - blk0), 0);
         if (nb <= 0) return;
         const int first = CACHE ? blk0 : max(blk0 - t.cached, 0), have = CACHE ? t.len : t.nodes;
@@ -437,14 +500,28 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void tree4_wide_kernel(TreeAr
         ta_u32x4 qf[NK];
 #pragma unroll
         for (int kk = 0; kk < NK; ++kk) qf[kk] = *reinterpret_cast<const ta_u32x4*>(a.q + q_row * D + 16 * kk + 8 * hh);
-        const float cs = CACHE ? to_fp16<F16, true>(qf, a.scale_log2) : a.scale_log2;
+        float cs = CACHE ? to_fp16<F16, true>(qf, a.scale_log2) : a.scale_log2;
+        ta_u32x4 q_half = {0, 0, 0, 0};  // half the sums of the quarters' dims, each in two parts: b's factors (the upper lanes' are 0)
+        if constexpr (EXACT) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            float sum = 0.f, x, y;
+#pragma unroll
+            for (int kk = g * NK / 4; kk < (g + 1) * NK / 4; ++kk)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) sum = add2<true>(qf[kk][i], sum);
+            swap32(sum, x, y);
+            q_half[g] = hh ? 0 : split_fp16((x + y) * 0.5f);
+          }
+          cs *= 2.f;
+        }
 
         // A block's rows on their way: codes and pairs, or 16-bit chunks.
         struct Ahead {
           ta_u32x4 k[CACHE ? 1 : NW], v[CACHE ? 1 : NW];
           unsigned kp, vp;
         };
-        constexpr int kDeep = !CACHE && D == 128 ? 1 : 2;  // blocks on their way (16-bit rows of 128 take too many registers for two)
+        constexpr int kDeep = D == 128 && (EXACT || !CACHE) ? 1 : 2;  // blocks on their way: what registers there are
         Ahead ahead[2];
         unsigned holes = 0;  // bits 2 (i % 8) and + 1: the two pages of block i's 16 rows each are none
         const int* table = a.table + static_cast<long long>(s) * a.max_pages;
@@ -494,7 +571,15 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void tree4_wide_kernel(TreeAr
             ta_u32x4 k, v;
             if constexpr (CACHE) {
               unsigned y[4];
-              int4_unpack8(e ? x.k[0].y : x.k[0].x, int4_scale(x.kp), int4_base(x.kp), y);
+              if constexpr (EXACT) {
+                const i4_f16x2 sk = int4_scale(x.kp), s_high = int4_scale(x.kp & 0xffe0u);
+                unsigned z[4];
+                int4_split8(e ? x.k[0].y : x.k[0].x, s_high, sk - s_high, y, z);
+                *reinterpret_cast<ta_u32x4*>(st + 2 * kHalf + (k_store ^ 16 * e)) = ta_u32x4{z[0], z[1], z[2], z[3]};
+                if (e == 0 && !(lane & 1)) *reinterpret_cast<unsigned*>(ring + kRing * kStage + i % kRing * B * 16 + srow * 16 + (lane & 7) * 2) = __builtin_bit_cast(unsigned, int4_base(x.kp));
+              } else {
+                int4_unpack8(e ? x.k[0].y : x.k[0].x, int4_scale(x.kp), int4_base(x.kp), y);
+              }
               k = ta_u32x4{y[0], y[1], y[2], y[3]};
               int4_unpack8(e ? x.v[0].y : x.v[0].x, int4_scale(x.vp), int4_base(x.vp), y);
               v = ta_u32x4{y[0], y[1], y[2], y[3]};
@@ -502,13 +587,17 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void tree4_wide_kernel(TreeAr
               k = x.k[e], v = x.v[e];
             }
             if (gone) v = ta_u32x4{0, 0, 0, 0};
-            *reinterpret_cast<ta_u32x4*>(st + srow * kRow + k_slot<D>(srow & 15, chunk0 + e) * 16) = k;
-            *reinterpret_cast<ta_u32x4*>(st + kHalf + srow * kRow + wide_v_slot<D>(srow, chunk0 + e) * 16) = v;
+            *reinterpret_cast<ta_u32x4*>(st + (k_store ^ 16 * e)) = k;
+            *reinterpret_cast<ta_u32x4*>(st + (v_store ^ 16 * e)) = v;
           }
         };
         auto k_frag = [&](int i, int kk) {
           return *reinterpret_cast<const ta_u32x4*>(ring + ((i % kRing * kStage + k_first) ^ (32 * kk)));
         };
+        auto low_frag = [&](int i, int kk) {
+          return *reinterpret_cast<const ta_u32x4*>(ring + ((i % kRing * kStage + 2 * kHalf + k_first) ^ (32 * kk)));
+        };
+        auto base_frag = [&](int i) { return *reinterpret_cast<const ta_u32x4*>(ring + kRing * kStage + i % kRing * B * 16 + c * 16); };
         // V^T of keys 8 q + 4 hh .. + 3 of block i, dims 32 db + lane % 32
         auto v_frag = [&](int i, int q, int db) {
           return __builtin_bit_cast(ta_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ta_i16x4*)(
@@ -534,6 +623,14 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void tree4_wide_kernel(TreeAr
             }
           }
         };
+        // Weights 2 g and 2 g + 1 of the lane in two parts (cf. split4), where the cached values are exact.
+        auto weights2 = [&](const ta_f32x16& sc, int g, unsigned& low) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(sc[2 * g], cs, -off)), q = __builtin_amdgcn_exp2f(fmaf(sc[2 * g + 1], cs, -off));
+          const auto x = __builtin_amdgcn_cvt_pkrtz(p, q);
+          low = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(p - static_cast<float>(x[0]), q - static_cast<float>(x[1])));
+          l += p + q;
+          return __builtin_bit_cast(unsigned, x);
+        };
         // Weights 2 g and 2 g + 1 of the lane, rounded to 16 bits as the second product takes them; l sums those.
         auto weights = [&](const ta_f32x16& sc, int g) {
           const unsigned p = pack2<T16>(__builtin_amdgcn_exp2f(fmaf(sc[2 * g], cs, -off)), __builtin_amdgcn_exp2f(fmaf(sc[2 * g + 1], cs, -off)));
@@ -552,25 +649,46 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void tree4_wide_kernel(TreeAr
 #pragma unroll
             for (int j = 0; j < 16; ++j) sc[j] = seen >> (8 * (j >> 2) + (j & 3)) & 1 ? sc[j] : -INFINITY;
           }
-          ta_u32x4 kf[NK];  // of block i + 1 (behind the last block: a stage that nothing writes, for scores that go unused)
+          // K's fragments of block i + 1 (behind the last block: a stage that nothing writes, for scores that go unused)
+          ta_u32x4 kf[NK], low[NK], bf;
+          if constexpr (EXACT) {
+            bf = base_frag(i + 1);
+            kf[0] = k_frag(i + 1, 0);
+          } else {
 #pragma unroll
-          for (int kk = 0; kk < NK; ++kk) kf[kk] = k_frag(i + 1, kk);
+            for (int kk = 0; kk < NK; ++kk) kf[kk] = k_frag(i + 1, kk);
+          }
           raise(sc);
           // In eight groups, held in this order by the scheduling barriers (cf. tree_wide_kernel).
-          ta_u32x4 pf[2];  // P^T of keys 16 g + 4 hh .. + 3 and + 8 .. + 11
+          ta_u32x4 pf[2], pl[2];  // P^T of keys 16 g + 4 hh .. + 3 and + 8 .. + 11, its lower part
           ta_u32x2 vt[4][ND];
           auto pv = [&](int g, int db) {
-            o[db] = mfma32<T16>(ta_u32x4{vt[2 * g][db].x, vt[2 * g][db].y, vt[2 * g + 1][db].x, vt[2 * g + 1][db].y}, pf[g], o[db]);
+            const ta_u32x4 v = {vt[2 * g][db].x, vt[2 * g][db].y, vt[2 * g + 1][db].x, vt[2 * g + 1][db].y};
+            o[db] = mfma32<T16>(v, pf[g], o[db]);
+            if constexpr (EXACT) o[db] = mfma32<T16>(v, pl[g], o[db]);
           };
           next = ta_f32x16{};
 #pragma unroll
           for (int g = 0; g < 8; ++g) {
             __builtin_amdgcn_sched_barrier(0);
+            if constexpr (EXACT) {
+              if (g < NK) low[g] = low_frag(i + 1, g);
+              if (g + 1 < NK) kf[g + 1] = k_frag(i + 1, g + 1);
+              if (g == 0) next = mfma32<T16>(bf, q_half, next);
+            }
             if (g < NK) next = mfma32<T16>(kf[g], qf[g], next);
+            if constexpr (EXACT)
+              if (g < NK) next = mfma32<T16>(low[g], qf[g], next);
             if (g >= 4 && g - 4 < ND) pv(0, g - 4);
 #pragma unroll
             for (int e = g * ND / 2; e < (g + 1) * ND / 2; ++e) vt[e / ND][e % ND] = v_frag(i, e / ND, e % ND);
-            pf[g / 4][g % 4] = weights(sc, g);
+            if constexpr (EXACT) {
+              unsigned x;
+              pf[g / 4][g % 4] = weights2(sc, g, x);
+              pl[g / 4][g % 4] = x;
+            } else {
+              pf[g / 4][g % 4] = weights(sc, g);
+            }
           }
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -597,9 +715,14 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void tree4_wide_kernel(TreeAr
         issue(kDeep + 1, ahead[kDeep - 1]);
         meet();
         ta_f32x16 sa = {}, sb = {};
-        if (!idle)
+        if (!idle) {
 #pragma unroll
-          for (int kk = 0; kk < NK; ++kk) sa = mfma32<T16>(k_frag(0, kk), qf[kk], sa);
+          for (int kk = 0; kk < NK; ++kk) {
+            sa = mfma32<T16>(k_frag(0, kk), qf[kk], sa);
+            if constexpr (EXACT) sa = mfma32<T16>(low_frag(0, kk), qf[kk], sa);
+          }
+          if constexpr (EXACT) sa = mfma32<T16>(base_frag(0), q_half, sa);
+        }
         for (int i = 0; i < nb; i += 2) {
           turn(i, sa, sb, ahead[0]);
           if (i + 1 < nb) turn(i + 1, sb, sa, ahead[kDeep - 1]);
