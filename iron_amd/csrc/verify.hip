@@ -21,14 +21,15 @@
 namespace iron {
 namespace {
 
-constexpr int kChunk = 4096;  // logits of a workgroup
+constexpr int kSub = 1024;  // logits of a wave (with two such parts to a wave, one behind the other, whole calls took 1 % less to 3 % more)
+constexpr int kWalk = 4 * kSub;  // of a workgroup that sums the last weights
 constexpr int kMaxNodes = 1024;
 constexpr int kMaxSeqs = 8192;
 
-struct RowStat {  // of a row, or of a chunk of it
+struct RowStat {  // of a row, or of a part of it
   double z;       // sum of exp((l - m) / T)
   float m;        // the largest logit
-  int best;       // its first index
+  int best;       // its first index, -1 where no logit counts
 };
 
 struct Choice {  // what a sequence came to
@@ -51,55 +52,57 @@ struct VerifyArgs {
   int* rows;           // (num_nodes)
   int* row_starts;     // (num_seqs + 1)
   int* next;           // (num_seqs)
-  RowStat* part;       // workspace (num_nodes [x 2], chunks)
+  RowStat* part;       // workspace (num_nodes [x 2], subs)
   RowStat* stat;       // workspace (num_nodes [x 2])
-  double* chance;      // workspace (num_nodes, 2): p and q of the parent's row at the node's token
+  double2* chance;     // workspace (num_nodes): p and q of the parent's row at the node's token
   double2* ab;         // workspace (max_children, num_nodes): a_j, b_j
-  double* mass;        // workspace (max_children, num_nodes, chunks): parts of R_j
+  double* mass;        // workspace (max_children, num_nodes, subs): parts of R_j
   Choice* choice;      // workspace (num_seqs)
-  double* weight;      // workspace (num_seqs, chunks): parts of the last sum(w)
+  double* weight;      // workspace (num_seqs, subs): parts of the last sum(w)
   int* path;           // workspace (num_nodes): accepted rows, from each tree's first row on
-  int vocab, num_seqs, num_nodes, max_nodes, max_children, chunks;
+  int* tried;          // workspace (num_seqs, max_children): tokens that were not accepted at the last node
+  int vocab, num_seqs, num_nodes, max_nodes, max_children;
+  int subs;            // parts of kSub places in a row, made up to whole fours
 };
 
-// The tree of sequence s: its first row and its nodes, cut to the arrays.
-__device__ __forceinline__ void tree_of(const VerifyArgs& a, int s, int& first, int& nodes) {
-  first = min(max(a.starts[s], 0), a.num_nodes);
-  nodes = min(min(max(a.starts[s + 1], first), a.num_nodes) - first, a.max_nodes);
-}
+// The same value in every lane, in a scalar register.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-struct Place {
+// A tree: its sequence (-1: none), its first row and its nodes, cut to the arrays.
+struct Tree {
   int seq, first, nodes;
 };
 
-// The first sequence whose tree holds row n (seq -1: none). Every thread calls it.
-__device__ __forceinline__ Place place_of(const VerifyArgs& a, int n, int* shared) {
-  if (threadIdx.x == 0) *shared = a.num_seqs;
-  __syncthreads();
-  for (int s = threadIdx.x; s < a.num_seqs; s += blockDim.x) {
-    int first, nodes;
-    tree_of(a, s, first, nodes);
-    if (first <= n && n < first + nodes) atomicMin(shared, s);
-  }
-  __syncthreads();
-  Place p = {*shared, 0, 0};
-  if (p.seq == a.num_seqs)
-    p.seq = -1;
-  else
-    tree_of(a, p.seq, p.first, p.nodes);
-  return p;
+__device__ __forceinline__ Tree tree_of(const VerifyArgs& a, int s) {
+  const int first = min(max(a.starts[s], 0), a.num_nodes);
+  return {s, uniform(first), uniform(min(min(max(a.starts[s + 1], first), a.num_nodes) - first, a.max_nodes))};
 }
 
-// Children of node i of a tree (whole workgroup). A parent comes before its child.
-__device__ __forceinline__ int children_of(const VerifyArgs& a, const Place& p, int i, int* shared) {
-  __syncthreads();
-  if (threadIdx.x == 0) *shared = 0;
-  __syncthreads();
-  int mine = 0;
-  for (int c = i + 1 + threadIdx.x; c < p.nodes; c += blockDim.x) mine += a.parents[p.first + c] == i;
-  if (mine) atomicAdd(shared, mine);
-  __syncthreads();
-  return *shared;
+// The tree of row n, the last one that begins at or before it: 64 entries of starts
+// at a time, by every wave for itself.
+__device__ __forceinline__ Tree tree_with(const VerifyArgs& a, int n) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, count = a.num_seqs;  // the sequence is one of lo .. lo + count - 1
+  while (count > 1) {
+    const int step = (count + 63) / 64, at = lane * step;
+    const unsigned long long before = __ballot(at < count && a.starts[lo + min(at, count - 1)] <= n);
+    const int k = max(__popcll(before) - 1, 0);
+    lo += k * step;
+    count = min(step, count - k * step);
+  }
+  Tree t = tree_of(a, lo);
+  if (n < t.first || n >= t.first + t.nodes) t.seq = -1;
+  return t;
+}
+
+// Children of node i of a tree (a wave). A parent comes before its child.
+__device__ __forceinline__ int children_of(const VerifyArgs& a, const Tree& t, int i) {
+  int n = 0;
+  for (int c0 = i + 1; c0 < t.nodes; c0 += 64) {
+    const int c = c0 + (threadIdx.x & 63);
+    n += __popcll(__ballot(c < t.nodes && a.parents[t.first + min(c, t.nodes - 1)] == i));
+  }
+  return n;
 }
 
 // A temperature that is not above 0 stands for the likeliest token.
@@ -109,263 +112,466 @@ __device__ __forceinline__ bool greedy(float t) { return !(t > 0.f); }
 __device__ __forceinline__ float logit(float x) { return x != x ? -INFINITY : fminf(x, FLT_MAX); }
 
 template <typename T>
-__device__ __forceinline__ float load(const void* base, long long i) {
-  const T x = static_cast<const T*>(base)[i];
-  if constexpr (std::is_same_v<T, uint16_t>) return logit(bf16_to_f32(x));
-  else return logit(static_cast<float>(x));
+__device__ __forceinline__ float widen(T x) {
+  if constexpr (std::is_same_v<T, uint16_t>) return bf16_to_f32(x);
+  else return static_cast<float>(x);
 }
 
-__device__ __forceinline__ double boost(float l, float m, double inv_t) { return l == -INFINITY ? 0. : exp((static_cast<double>(l) - m) * inv_t); }
-
-__device__ __forceinline__ double wave_sum64(double x) {
-  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d, 64);
-  return x;
-}
-
-// Sum over the workgroup's 256 threads, in the same order every time. Every thread calls it.
-__device__ __forceinline__ double block_sum(double x, double* tmp) {
-  x = wave_sum64(x);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = x;
-  __syncthreads();
-  return (tmp[0] + tmp[1]) + (tmp[2] + tmp[3]);
-}
-
-// One chunk of a row of target or draft logits: its maximum and its sum.
+// Rows need no alignment but their elements': a row's places are counted from the
+// 16-byte boundary at or before it, so that the lanes of all rows load 16 bytes each;
+// place x holds token x - shift. What is fetched is made numbers only where it is
+// used, so that fetches stay in flight until then.
 template <typename T>
-__global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs a) {
-  __shared__ int si;
-  __shared__ double tmp[4];
-  __shared__ float top[4];
-  __shared__ int arg[4];
-  const int row = blockIdx.x / a.chunks, c = blockIdx.x - row * a.chunks;
-  const bool target = row < a.num_nodes;
-  const int n = target ? row : row - a.num_nodes;
-  const Place p = place_of(a, n, &si);
-  if (p.seq < 0) return;
-  const float temp = a.temps[p.seq];
-  if (!target && (greedy(temp) || children_of(a, p, n - p.first, &si) == 0)) return;
-  const void* base = target ? a.logits : a.draft;
-  const long long at = static_cast<long long>(n) * a.vocab;
-  const int lo = c * kChunk, hi = min(lo + kChunk, a.vocab);
-  float l[kChunk / 256];
-  float m = -INFINITY;
-  int best = INT_MAX;
+struct Row {
+  const T* base;
+  int shift, end;  // places [shift, end) are the row's
+  int limit;       // up to here a whole vector of 16 bytes is the buffer's
+  template <int N>
+  struct alignas(N * sizeof(T)) Vec {
+    T e[N];
+  };
+  __device__ __forceinline__ Row(const VerifyArgs& a, const void* logits, int n) {
+    const T* row = static_cast<const T*>(logits) + static_cast<long long>(n) * a.vocab;
+    shift = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15) / static_cast<int>(sizeof(T));
+    base = row - shift;
+    end = shift + a.vocab;
+    const long long left = static_cast<long long>(a.num_nodes - n) * a.vocab + shift;
+    limit = static_cast<int>(min(left, 1LL << 30)) - 16 / static_cast<int>(sizeof(T));
+  }
+  // N places from x on, a multiple of N; anything where they are not the row's
+  template <int N>
+  __device__ __forceinline__ Vec<N> fetch(int x) const {
+    if (limit < 0) return {};  // a buffer of less than 16 bytes
+    return *reinterpret_cast<const Vec<N>*>(base + min(x, limit / N * N));
+  }
+  // Their logits as they are, -inf outside the row; `inside`: all of them are the row's and the buffer has them whole
+  template <int N>
+  __device__ __forceinline__ void expand(int x, const Vec<N>& v, bool inside, float (&l)[N]) const {
 #pragma unroll
-  for (int i = 0; i < kChunk / 256; ++i) {
-    const int x = lo + i * 256 + static_cast<int>(threadIdx.x);
-    l[i] = x < hi ? load<T>(base, at + x) : -INFINITY;
-    if (l[i] > m) {
-      m = l[i];
-      best = x;
+    for (int i = 0; i < N; ++i) l[i] = widen(v.e[i]);
+    if (!inside) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) l[i] = x + i >= shift && x + i < end ? l[i] : -INFINITY;
+      if (x > limit && x < end)  // the last ones of the buffer
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (x + i >= shift && x + i < end) l[i] = widen(base[x + i]);
     }
   }
-  const float wm = wave_max(m);
-  int wb = m == wm ? best : INT_MAX;
-  for (int d = 32; d; d >>= 1) wb = min(wb, __shfl_xor(wb, d, 64));
-  if ((threadIdx.x & 63) == 0) {
-    top[threadIdx.x >> 6] = wm;
-    arg[threadIdx.x >> 6] = wb;
-  }
-  __syncthreads();
-  m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-  best = INT_MAX;
-  for (int w = 0; w < 4; ++w)
-    if (top[w] == m) best = min(best, arg[w]);
-  double z = 0.;
-  if (!greedy(temp)) {
-    const double inv = 1. / temp;
-#pragma unroll
-    for (int i = 0; i < kChunk / 256; ++i) z += boost(l[i], m, inv);
-    z = block_sum(z, tmp);
-  }
-  if (threadIdx.x == 0) a.part[static_cast<long long>(row) * a.chunks + c] = {z, m, best};
+  // Whether places [x, x + n) are all the row's and the buffer has their vectors whole.
+  __device__ __forceinline__ bool inside(int x, int n) const { return x >= shift && x + n <= min(end, limit); }
+  __device__ __forceinline__ float token(int x) const { return logit(widen(base[shift + x])); }
+};
+
+// The places of a lane in part `sub` of a row: kVecs loads of kVec.
+template <typename T>
+constexpr int kVec = 16 / sizeof(T);
+template <typename T>
+constexpr int kVecs = kSub / 64 / kVec<T>;
+template <typename T>
+__device__ __forceinline__ int place(int sub, int i) {
+  return sub * kSub + (i * 64 + static_cast<int>(threadIdx.x & 63)) * kVec<T>;
 }
 
-// The chunks of a row together (one wave).
-__device__ __forceinline__ RowStat merge(const VerifyArgs& a, int row, double inv) {
+// x moved across lanes by DPP control CTRL, 0 into lanes outside ROWMASK or without a source.
+template <int CTRL, int ROWMASK = 0xf>
+__device__ __forceinline__ double dpp64(double x) {
+  const long long b = __builtin_bit_cast(long long, x);
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(b), CTRL, ROWMASK, 0xf, false);
+  const unsigned hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(b >> 32), CTRL, ROWMASK, 0xf, false);
+  return __builtin_bit_cast(double, static_cast<long long>(hi) << 32 | lo);
+}
+
+__device__ __forceinline__ double lane64(double x, int lane) {
+  const long long b = __builtin_bit_cast(long long, x);
+  const unsigned lo = __builtin_amdgcn_readlane(static_cast<int>(b), lane), hi = __builtin_amdgcn_readlane(static_cast<int>(b >> 32), lane);
+  return __builtin_bit_cast(double, static_cast<long long>(hi) << 32 | lo);
+}
+
+// Inclusive sums over the wave's lanes, in the same order every time. All lanes are active.
+__device__ __forceinline__ double wave_scan64(double x) {
+  x += dpp64<0x111>(x);  // row_shr 1, 2, 4, 8, then the last lanes of rows into the rows behind
+  x += dpp64<0x112>(x);
+  x += dpp64<0x114>(x);
+  x += dpp64<0x118>(x);
+  x += dpp64<0x142, 0xa>(x);
+  x += dpp64<0x143, 0xc>(x);
+  return x;
+}
+__device__ __forceinline__ double wave_sum64(double x) { return lane64(wave_scan64(x), 63); }
+
+// log2(e) / T.
+__device__ __forceinline__ double rate_of(float temp) { return 1.4426950408889634 / temp; }
+
+// exp((l - m) / T) for l <= m, 0 for l = -inf: 2^t as 2^n 2^f with f in [-1/2, 1/2], the
+// series of 2^f to its 11th term (off by 2^-47 at most): 19 instructions of 5 cycles
+// each, where the library's exp takes some 40. The terms stand in scalar registers:
+// left to the compiler, each was moved into two vector registers before its use.
+struct Exp2 {
+  double k[12] = {1., 0x1.62e42fefa39efp-1, 0x1.ebfbdff82c58ep-3, 0x1.c6b08d704a0bfp-5, 0x1.3b2ab6fba4e77p-7, 0x1.5d87fe78a6730p-10, 0x1.430912f86c786p-13, 0x1.ffcbfc588b0c5p-17, 0x1.62c0223a5c822p-20, 0x1.b5253d395e7c1p-24, 0x1.e4cf5158b8ec7p-28, 0x1.e8cac7351bb22p-32};
+  __device__ __forceinline__ Exp2() {
+#pragma unroll
+    for (int i = 0; i < 12; ++i) asm("" : "+s"(k[i]));
+  }
+  __device__ __forceinline__ double operator()(float l, float m, double rate) const {
+    double t = (static_cast<double>(l) - m) * rate;
+    t = __builtin_fmax(t, -1100.);  // 2^-1100 is 0
+    const double n = rint(t), f = t - n;
+    double y = fma(k[11], f, k[10]);
+#pragma unroll
+    for (int i = 9; i >= 0; --i) y = fma(y, f, k[i]);
+    return __builtin_amdgcn_ldexp(y, static_cast<int>(n));
+  }
+  // Of N logits side by side: each step waits for the one before it, so a lone wave needs others in between.
+  template <int N>
+  __device__ __forceinline__ void operator()(const float (&l)[N], float m, double rate, double (&y)[N]) const {
+    double f[N];
+    int n[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const double t = __builtin_fmax((static_cast<double>(l[e]) - m) * rate, -1100.), r = rint(t);
+      f[e] = t - r;
+      n[e] = static_cast<int>(r);
+      y[e] = fma(k[11], f[e], k[10]);
+    }
+#pragma unroll
+    for (int i = 9; i >= 0; --i) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int e = 0; e < N; ++e) y[e] = fma(y[e], f[e], k[i]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int e = 0; e < N; ++e) y[e] = __builtin_amdgcn_ldexp(y[e], n[e]);
+  }
+};
+
+// The larger of three numbers; the compiler's own makes quiet NaN of its operands first, at an instruction each.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+// One part of a row of target or draft logits, by a wave: its maximum and its sum.
+// Bound by the fp64 instructions (30.7 M logits, 8 trees of 26 nodes: 34 us, 24 of
+// them these alone).
+template <typename T>
+__global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs a) {
   const int lane = threadIdx.x & 63;
-  const RowStat* part = a.part + static_cast<long long>(row) * a.chunks;
+  const int rows = a.draft ? 2 * a.num_nodes : a.num_nodes, id = uniform(blockIdx.x * 4 + (threadIdx.x >> 6));
+  const int row = id / a.subs, sub = id - row * a.subs;
+  if (row >= rows) return;
+  const bool target = row < a.num_nodes;
+  const int n = target ? row : row - a.num_nodes;
+  const Row<T> r(a, target ? a.logits : a.draft, n);
+  typename Row<T>::template Vec<kVec<T>> raw[kVecs<T>];
+  auto load = [&] {
+#pragma unroll
+    for (int i = 0; i < kVecs<T>; ++i) raw[i] = r.template fetch<kVec<T>>(place<T>(sub, i));
+  };
+  if (target) load();  // while the tree is looked up; of draft rows, many are not needed
+  const Tree t = tree_with(a, n);
+  if (t.seq < 0) return;
+  const float temp = a.temps[t.seq];
+  const bool top = greedy(temp);
+  if (!target) {
+    if (top || children_of(a, t, n - t.first) == 0) return;
+    load();
+  }
+  const double rate = top ? 0. : rate_of(temp);
+  const Exp2 boost;
+  float x[kVecs<T>][kVec<T>], m = -INFINITY;
+  const bool inside = r.inside(sub * kSub, kSub);
+#pragma unroll
+  for (int i = 0; i < kVecs<T>; ++i) r.expand(place<T>(sub, i), raw[i], inside, x[i]);
+  auto clean = [&] {  // NaN and infinities as they count
+    m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kVecs<T>; ++i)
+#pragma unroll
+      for (int e = 0; e < kVec<T>; ++e) m = fmaxf(m, x[i][e] = logit(x[i][e]));
+    m = wave_max(m);
+  };
+  auto sum = [&] {
+    double z = 0.;
+    if (m != -INFINITY)
+#pragma unroll
+      for (int i = 0; i < kVecs<T>; ++i) {
+        double y[kVec<T>];
+        boost(x[i], m, rate, y);
+#pragma unroll
+        for (int e = 0; e < kVec<T>; ++e) z += y[e];
+      }
+    return wave_sum64(z);
+  };
+  double z = 0.;
+  int best = INT_MAX;
+  if (top) {
+    clean();
+#pragma unroll
+    for (int i = kVecs<T> - 1; i >= 0; --i)
+#pragma unroll
+      for (int e = kVec<T> - 1; e >= 0; --e) best = x[i][e] == m ? place<T>(sub, i) + e - r.shift : best;
+    for (int d = 32; d; d >>= 1) best = min(best, __shfl_xor(best, d, 64));
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVecs<T>; ++i)
+#pragma unroll
+      for (int e = 0; e < kVec<T>; e += 2) m = max3(m, x[i][e], x[i][e + 1]);
+    m = wave_max(m);
+    z = m < INFINITY ? sum() : NAN;
+    if (!(z >= 0.)) {  // a NaN among them shows in the sum
+      clean();
+      z = sum();
+    }
+  }
+  if (lane == 0) a.part[static_cast<long long>(row) * a.subs + sub] = {z, m, best};
+}
+
+// The parts of a row together (one wave). The first 256 stay in registers.
+__device__ __forceinline__ RowStat merge(const VerifyArgs& a, int row, double rate) {
+  constexpr int kHeld = 4;
+  const int lane = threadIdx.x & 63;
+  const Exp2 boost;
+  const RowStat* part = a.part + static_cast<long long>(row) * a.subs;
+  RowStat held[kHeld];
   float m = -INFINITY;
-  for (int c = lane; c < a.chunks; c += 64) m = fmaxf(m, part[c].m);
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    held[i] = i * 64 + lane < a.subs ? part[i * 64 + lane] : RowStat{0., -INFINITY, INT_MAX};
+    m = fmaxf(m, held[i].m);
+  }
+  for (int c = kHeld * 64 + lane; c < a.subs; c += 64) m = fmaxf(m, part[c].m);
   m = wave_max(m);
   double z = 0.;
   int best = INT_MAX;
-  for (int c = lane; c < a.chunks; c += 64) {
-    const RowStat r = part[c];
-    z += r.z * boost(r.m, m, inv);
+  auto add = [&](const RowStat& r) {
+    z += r.z > 0. ? r.z * boost(r.m, m, rate) : 0.;
     if (r.m == m) best = min(best, r.best);
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) add(held[i]);
+  for (int c = kHeld * 64 + lane; c < a.subs; c += 64) add(part[c]);
   for (int d = 32; d; d >>= 1) best = min(best, __shfl_xor(best, d, 64));
   return {wave_sum64(z), m, m == -INFINITY ? -1 : best};
 }
 
-// One wave per node: its rows' sums, and the probabilities of its token in its parent's.
+// A workgroup per node, a wave each for its target row, its draft row, and its token's
+// probabilities in the two rows of its parent.
 template <typename T>
-__global__ __launch_bounds__(64) void verify_merge_kernel(VerifyArgs a) {
-  __shared__ int si;
-  const int n = blockIdx.x, lane = threadIdx.x;
-  const Place p = place_of(a, n, &si);
-  if (p.seq < 0) return;
-  const float temp = a.temps[p.seq];
-  const double inv = greedy(temp) ? 0. : 1. / temp;
-  const RowStat mine = merge(a, n, inv);
-  if (lane == 0) a.stat[n] = mine;
-  if (greedy(temp)) return;
-  if (a.draft && children_of(a, p, n - p.first, &si)) {
-    const RowStat q = merge(a, a.num_nodes + n, inv);
-    if (lane == 0) a.stat[a.num_nodes + n] = q;
+__global__ __launch_bounds__(256) void verify_merge_kernel(VerifyArgs a) {
+  const int n = blockIdx.x, lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6);
+  const int up = uniform(a.parents[n]), x = uniform(a.tokens[n]);
+  const Tree t = tree_with(a, n);
+  if (t.seq < 0) return;
+  const float temp = a.temps[t.seq];
+  if (w > 0 && greedy(temp)) return;
+  const double rate = greedy(temp) ? 0. : rate_of(temp);
+  if (w < 2) {
+    if (w == 1 && (!a.draft || children_of(a, t, n - t.first) == 0)) return;
+    const int row = w ? a.num_nodes + n : n;
+    const RowStat mine = merge(a, row, rate);
+    if (lane == 0) a.stat[row] = mine;
+    return;
   }
-  const int up = a.parents[n], x = a.tokens[n];
-  if (n == p.first || up < 0 || up >= n - p.first) return;
-  const int parent = p.first + up;
-  const bool real = static_cast<unsigned>(x) < static_cast<unsigned>(a.vocab);
-  const RowStat sp = merge(a, parent, inv);
-  double pc = real && sp.z > 0. ? boost(load<T>(a.logits, static_cast<long long>(parent) * a.vocab + x), sp.m, inv) / sp.z : 0., qc = 1.;
-  if (a.draft) {
-    const RowStat sq = merge(a, a.num_nodes + parent, inv);
-    qc = real && sq.z > 0. ? boost(load<T>(a.draft, static_cast<long long>(parent) * a.vocab + x), sq.m, inv) / sq.z : 0.;
+  if (n == t.first || up < 0 || up >= n - t.first) return;
+  const int parent = t.first + up;
+  double* chance = reinterpret_cast<double*>(a.chance + n) + (w - 2);
+  const void* logits = w == 2 ? a.logits : a.draft;
+  if (!logits) {
+    if (lane == 0) *chance = 1.;
+    return;
   }
-  if (lane == 0) {
-    a.chance[2 * n] = pc;
-    a.chance[2 * n + 1] = qc;
-  }
+  const float l = static_cast<unsigned>(x) < static_cast<unsigned>(a.vocab) ? Row<T>(a, logits, parent).token(x) : -INFINITY;
+  const Exp2 boost;
+  const RowStat all = merge(a, w == 2 ? parent : a.num_nodes + parent, rate);
+  if (lane == 0) *chance = all.z > 0. ? boost(l, all.m, rate) / all.z : 0.;
 }
 
 // R_j of a row from its parts (one wave, every lane returns it).
 __device__ __forceinline__ double mass_of(const VerifyArgs& a, int j, int n) {
   if (j == 0) return 1.;
   double r = 0.;
-  const double* part = a.mass + (static_cast<long long>(j) * a.num_nodes + n) * a.chunks;
-  for (int c = threadIdx.x & 63; c < a.chunks; c += 64) r += part[c];
+  const double* part = a.mass + (static_cast<long long>(j) * a.num_nodes + n) * a.subs;
+  for (int c = threadIdx.x & 63; c < a.subs; c += 64) r += part[c];
   return wave_sum64(r);
 }
 
-// The weight of logit x of row n for a_j, b_j.
+// The weight of a token of row n for a_j, b_j.
 struct Weigh {
-  double ka, kb, inv;  // a / sum, b / sum of p's and q's exponentials
+  double ka, kb, rate;  // a / sum, b / sum of p's and q's exponentials
   float mp, mq;
-  __device__ __forceinline__ double operator()(float lp, float lq) const {
+  Exp2 boost;
+  template <int N>
+  __device__ __forceinline__ void operator()(const float (&lp)[N], const float (&lq)[N], bool rival, double (&out)[N]) const {
 #pragma clang fp contract(off)  // equal rows of target and draft leave nothing at all
-    return fmax(ka * boost(lp, mp, inv) - kb * boost(lq, mq, inv), 0.);
+    boost(lp, mp, rate, out);
+    if (rival) {
+      double q[N];
+      boost(lq, mq, rate, q);
+#pragma unroll
+      for (int e = 0; e < N; ++e) out[e] = fmax(ka * out[e] - kb * q[e], 0.);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) out[e] *= ka;
+    }
   }
 };
 __device__ __forceinline__ Weigh weigh(const VerifyArgs& a, int n, double ca, double cb, float temp) {
   const RowStat p = a.stat[n];
-  Weigh w = {p.z > 0. ? ca / p.z : 0., 0., 1. / temp, p.m, 0.f};
+  Weigh w = {0., 0., rate_of(temp), 0.f, 0.f};
+  if (p.z > 0.) {
+    w.ka = ca / p.z;
+    w.mp = p.m;
+  }
   if (cb != 0.) {
     const RowStat q = a.stat[a.num_nodes + n];
-    w.kb = q.z > 0. ? cb / q.z : 0.;
-    w.mq = q.m;
+    if (q.z > 0.) {
+      w.kb = cb / q.z;
+      w.mq = q.m;
+    }
   }
   return w;
 }
 
-// R_j's part of a chunk, for rows with more than j children.
+// The weights of N places from x on of a row whose place `shift` is token 0: of its
+// target's logits and, where the drafter counts, the draft's; `gone` tokens have none.
+template <int N>
+__device__ __forceinline__ void weights(const Weigh& w, bool rival, const float (&lp)[N], const float (&lq)[N], int x, int shift, const int* gone, int num_gone, double (&out)[N]) {
+  float p[N], q[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    p[e] = logit(lp[e]);
+    q[e] = logit(lq[e]);
+  }
+  for (int k = 0; k < num_gone; ++k) {
+    const int at = gone[k] + shift - x;
+#pragma unroll
+    for (int e = 0; e < N; ++e) p[e] = at == e ? -INFINITY : p[e];
+  }
+  w(p, q, rival, out);
+}
+
+// R_j's part of kSub places, for rows with more than j children (a wave). The
+// logits are on their way while the rest is looked up.
 template <typename T>
 __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs a, int j) {
-  __shared__ int si;
-  __shared__ double tmp[4];
-  const int n = blockIdx.x / a.chunks, c = blockIdx.x - n * a.chunks;
-  const Place p = place_of(a, n, &si);
-  if (p.seq < 0) return;
-  const float temp = a.temps[p.seq];
-  if (greedy(temp) || children_of(a, p, n - p.first, &si) <= j) return;
+  const int lane = threadIdx.x & 63, id = uniform(blockIdx.x * 4 + (threadIdx.x >> 6));
+  const int n = id / a.subs, sub = id - n * a.subs;
+  if (n >= a.num_nodes) return;
+  const Tree t = tree_with(a, n);
+  if (t.seq < 0) return;
+  const float temp = a.temps[t.seq];
+  if (greedy(temp) || children_of(a, t, n - t.first) <= j) return;
+  const Row<T> rp(a, a.logits, n), rq(a, a.draft, n);
+  typename Row<T>::template Vec<kVec<T>> vp[kVecs<T>], vq[kVecs<T>];
+#pragma unroll
+  for (int i = 0; i < kVecs<T>; ++i) {
+    vp[i] = rp.template fetch<kVec<T>>(place<T>(sub, i));
+    vq[i] = rq.template fetch<kVec<T>>(place<T>(sub, i));
+  }
   const double r = mass_of(a, j - 1, n);
   const double2 was = j == 1 ? make_double2(1., 0.) : a.ab[static_cast<long long>(j - 1) * a.num_nodes + n];
   const double2 now = make_double2(was.x / r, was.y / r + 1.);
-  if (c == 0 && threadIdx.x == 0) a.ab[static_cast<long long>(j) * a.num_nodes + n] = now;
+  if (sub == 0 && lane == 0) a.ab[static_cast<long long>(j) * a.num_nodes + n] = now;
   const Weigh w = weigh(a, n, now.x, now.y, temp);
-  const long long at = static_cast<long long>(n) * a.vocab;
-  const int lo = c * kChunk, hi = min(lo + kChunk, a.vocab);
+  const bool inside = rp.inside(sub * kSub, kSub);
   double sum = 0.;
-  for (int x = lo + static_cast<int>(threadIdx.x); x < hi; x += 256) sum += w(load<T>(a.logits, at + x), load<T>(a.draft, at + x));
-  sum = block_sum(sum, tmp);
-  if (threadIdx.x == 0) a.mass[(static_cast<long long>(j) * a.num_nodes + n) * a.chunks + c] = sum;
+#pragma unroll
+  for (int i = 0; i < kVecs<T>; ++i) {
+    float lp[kVec<T>], lq[kVec<T>];
+    double x[kVec<T>];
+    rp.expand(place<T>(sub, i), vp[i], inside, lp);
+    rq.expand(place<T>(sub, i), vq[i], inside, lq);
+    weights(w, true, lp, lq, 0, 0, nullptr, 0, x);
+#pragma unroll
+    for (int e = 0; e < kVec<T>; ++e) sum += x[e];
+  }
+  sum = wave_sum64(sum);
+  if (lane == 0) a.mass[(static_cast<long long>(j) * a.num_nodes + n) * a.subs + sub] = sum;
 }
 
-// Down a tree: which rows are accepted, and what the next token is drawn from
-// (one wave, the same result in every workgroup that asks). path may be null.
-__device__ Choice walk(const VerifyArgs& a, const Place& p, float temp, int* path) {
+// Down a tree: which rows are accepted, and what the next token is drawn from (one
+// wave, the same result in every workgroup that asks). `write`: keeps the accepted
+// rows and the tokens that were not accepted at the last one. Lanes hold 64 nodes at a
+// time: one round trip for them, not one for each.
+__device__ Choice walk(const VerifyArgs& a, const Tree& t, float temp, bool write, int* gone) {
   const int lane = threadIdx.x & 63;
   Choice r = {1., 0., -1, 0, 0, 0};
-  if (p.nodes == 0) return r;
-  auto reach = [&](int i) {
-    if (path && lane == 0) path[r.count] = p.first + i;
+  if (t.nodes == 0) return r;
+  const bool top = greedy(temp);
+  int at = -1, best = -1;  // the current node within the tree; its likeliest token
+  double left = 1.;        // R of the next child's test
+  auto reach = [&](int i, int likeliest) {
+    at = i;
+    best = likeliest;
+    if (write && lane == 0) a.path[t.first + r.count] = t.first + i;
     r.count += 1;
-    r.node = p.first + i;
     r.a = 1.;
     r.b = 0.;
     r.tried = 0;
+    left = 1.;
   };
-  reach(0);
-  double left = 1.;  // R of the next child's test
-  for (int i0 = 1; i0 < p.nodes; i0 += 64) {
-    const int i = i0 + lane;
-    const int up = i < p.nodes ? a.parents[p.first + i] : -1;
-    int from = i0;
+  for (int i0 = 0; i0 < t.nodes; i0 += 64) {
+    const int i = min(i0 + lane, t.nodes - 1), n = t.first + i;
+    const int up = i0 + lane < t.nodes ? a.parents[n] : -1, token = a.tokens[n];
+    const float u = a.accept[n];
+    const int likeliest = top ? a.stat[n].best : -1;
+    const double2 chance = top ? make_double2(0., 0.) : a.chance[n];
+    if (i0 == 0) reach(0, __builtin_amdgcn_readlane(likeliest, 0));
+    int from = max(i0, 1);
     while (true) {  // the next child of the current node
-      const unsigned long long kids = __ballot(up == r.node - p.first && i >= from && i < p.nodes);
+      const unsigned long long kids = __ballot(up == at && i0 + lane >= from);
       if (!kids) break;
-      const int k = i0 + __ffsll(kids) - 1, n = p.first + k;
-      from = k + 1;
+      const int k = __ffsll(kids) - 1;
+      from = i0 + k + 1;
       if (r.tried >= a.max_children) continue;
+      const int x = __builtin_amdgcn_readlane(token, k);
       bool yes;
-      if (greedy(temp)) {
-        const int best = a.stat[r.node].best;
-        yes = best >= 0 && best == a.tokens[n];
+      if (top) {
+        yes = best >= 0 && best == x;
       } else {
-        const double pc = a.chance[2 * n], qc = a.chance[2 * n + 1];
+        const double pc = lane64(chance.x, k), qc = lane64(chance.y, k), uk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, u), k));
         if (a.draft) {
-          yes = static_cast<double>(a.accept[n]) * qc < fmax(r.a * pc - r.b * qc, 0.) / left;
+          yes = uk * qc < fmax(r.a * pc - r.b * qc, 0.) / left;
         } else {  // its token may have been tried before
           bool again = false;
-          for (int e = lane; e < k; e += 64) again |= a.parents[p.first + e] == r.node - p.first && e > r.node - p.first && a.tokens[p.first + e] == a.tokens[n];
-          again = __ballot(again) != 0;
-          yes = !again && static_cast<double>(a.accept[n]) < pc / left;
+          for (int e = 0; e < r.tried; ++e) again |= gone[e] == x;
+          yes = !again && uk < pc / left;
           if (!yes && !again) left -= pc;
         }
       }
       if (yes) {
-        reach(k);
-        left = 1.;
+        reach(i0 + k, __builtin_amdgcn_readlane(likeliest, k));
       } else {
+        if (lane == 0) gone[r.tried] = x;
+        __builtin_amdgcn_wave_barrier();
         r.tried += 1;
-        if (a.draft && !greedy(temp)) {
+        if (a.draft && !top) {
           r.a /= left;
           r.b = r.b / left + 1.;
-          left = r.tried < a.max_children ? mass_of(a, r.tried, r.node) : 1.;
+          left = r.tried < a.max_children ? mass_of(a, r.tried, t.first + at) : 1.;
           if (left == 0.) r.tried = a.max_children;  // nothing is left to accept
         }
       }
     }
   }
+  r.node = t.first + at;
   return r;
 }
 
-// The weight of a token without draft logits: 0 for those that were tried.
-__device__ __forceinline__ bool tried(const VerifyArgs& a, const Place& p, const Choice& r, int x) {
-  if (a.draft) return false;
-  int left = r.tried;
-  for (int k = r.node - p.first + 1; k < p.nodes && left; ++k)
-    if (a.parents[p.first + k] == r.node - p.first) {
-      if (a.tokens[p.first + k] == x) return true;
-      --left;
-    }
-  return false;
-}
-
-// Sequence s's walk, and a chunk of the sum that its next token is drawn by.
+// Sequence s's walk, and a part of the sum that its next token is drawn by.
 template <typename T>
 __global__ __launch_bounds__(256) void verify_walk_kernel(VerifyArgs a) {
   __shared__ Choice sr;
-  __shared__ double tmp[4];
-  const int s = blockIdx.x / a.chunks, c = blockIdx.x - s * a.chunks;
-  Place p = {s, 0, 0};
-  tree_of(a, s, p.first, p.nodes);
+  __shared__ int gone[64];
+  const int groups = a.subs / 4, s = blockIdx.x / groups, c = blockIdx.x - s * groups;
+  const int sub = 4 * c + uniform(threadIdx.x >> 6);
+  const Tree t = tree_of(a, s);
   const float temp = a.temps[s];
   if (threadIdx.x < 64) {
-    const Choice r = walk(a, p, temp, c == 0 ? a.path + p.first : nullptr);
+    const Choice r = walk(a, t, temp, c == 0, gone);
     if (threadIdx.x == 0) {
       sr = r;
       if (c == 0) a.choice[s] = r;
@@ -374,122 +580,167 @@ __global__ __launch_bounds__(256) void verify_walk_kernel(VerifyArgs a) {
   __syncthreads();
   const Choice r = sr;
   if (r.node < 0 || greedy(temp)) return;
+  const bool rival = r.b != 0.;
+  const Row<T> rp(a, a.logits, r.node), rq(a, rival ? a.draft : a.logits, r.node);
+  const bool inside = rp.inside(sub * kSub, kSub);
+  typename Row<T>::template Vec<kVec<T>> vp[kVecs<T>], vq[kVecs<T>];
+#pragma unroll
+  for (int i = 0; i < kVecs<T>; ++i) {
+    vp[i] = rp.template fetch<kVec<T>>(place<T>(sub, i));
+    vq[i] = rq.template fetch<kVec<T>>(place<T>(sub, i));  // where no drafter counts, the same again
+  }
+  const int num_gone = a.draft ? 0 : r.tried;
+  if (c == 0 && static_cast<int>(threadIdx.x) < num_gone) a.tried[s * a.max_children + threadIdx.x] = gone[threadIdx.x];
   const Weigh w = weigh(a, r.node, r.a, r.b, temp);
-  const long long at = static_cast<long long>(r.node) * a.vocab;
-  const int lo = c * kChunk, hi = min(lo + kChunk, a.vocab);
   double sum = 0.;
-  for (int x = lo + static_cast<int>(threadIdx.x); x < hi; x += 256)
-    if (!tried(a, p, r, x)) sum += w(load<T>(a.logits, at + x), r.b != 0. ? load<T>(a.draft, at + x) : -INFINITY);
-  sum = block_sum(sum, tmp);
-  if (threadIdx.x == 0) a.weight[static_cast<long long>(s) * a.chunks + c] = sum;
+#pragma unroll
+  for (int i = 0; i < kVecs<T>; ++i) {
+    double x[kVec<T>];
+    float lp[kVec<T>], lq[kVec<T>];
+    rp.expand(place<T>(sub, i), vp[i], inside, lp);
+    rq.expand(place<T>(sub, i), vq[i], inside, lq);
+    weights(w, rival, lp, lq, place<T>(sub, i), rp.shift, gone, num_gone, x);
+#pragma unroll
+    for (int e = 0; e < kVec<T>; ++e) sum += x[e];
+  }
+  sum = wave_sum64(sum);
+  if ((threadIdx.x & 63) == 0) a.weight[static_cast<long long>(s) * a.subs + sub] = sum;
+}
+
+// N numbers of each thread, in the threads' order: run[i] is the sum of all up to and
+// with its i-th. Returns the sum of all. Every thread calls it.
+template <int N>
+__device__ __forceinline__ double block_scan(const double (&x)[N], double (&run)[N], double* tmp) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  double mine = 0.;
+#pragma unroll
+  for (int i = 0; i < N; ++i) mine += x[i];
+  const double incl = wave_scan64(mine);
+  __syncthreads();  // tmp is free
+  if (lane == 63) tmp[w] = incl;
+  __syncthreads();
+  double before = 0., all = 0.;
+  for (int i = 0; i < 4; ++i) {
+    if (i < w) before += tmp[i];
+    all += tmp[i];
+  }
+  before += dpp64<0x138>(incl);  // of the lanes before this one (wave_shr 1)
+#pragma unroll
+  for (int i = 0; i < N; ++i) run[i] = before += x[i];
+  return all;
 }
 
 // One workgroup per sequence: its rows' place in the result, and its next token.
 template <typename T>
 __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs a) {
-  __shared__ int before, total, found, last;
-  __shared__ int at_chunk;
-  __shared__ double goal, base;
-  __shared__ double scan[256], tmp[4];
-  static_assert((1 << 20) / kChunk <= 256, "a thread to each chunk of the largest vocabulary");
-  const int s = blockIdx.x, tid = threadIdx.x;
-  if (tid == 0) before = total = 0;
-  __syncthreads();
-  int b = 0, t = 0;
-  for (int i = tid; i < a.num_seqs; i += 256) {
-    const int n = a.choice[i].count;
-    t += n;
-    if (i < s) b += n;
-  }
-  if (t) atomicAdd(&total, t);
-  if (b) atomicAdd(&before, b);
-  __syncthreads();
+  constexpr int kParts = 5;  // of a row, to a thread
+  static_assert(((1 << 20) / kWalk + 1) * (kWalk / kSub) <= kParts * 256, "the largest vocabulary's");
+  __shared__ int counts[8], found[4], last[4];
+  __shared__ double tmp[4], start;
+  const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  double x[kParts], run[kParts];
+#pragma unroll
+  for (int i = 0; i < kParts; ++i) x[i] = tid * kParts + i < a.subs ? a.weight[static_cast<long long>(s) * a.subs + tid * kParts + i] : 0.;
   Choice r = a.choice[s];
-  Place p = {s, 0, 0};
-  tree_of(a, s, p.first, p.nodes);
-  for (int i = tid; i < r.count && before + i < a.num_nodes; i += 256) a.rows[before + i] = a.path[p.first + i];
+  const Tree t = tree_of(a, s);
+  const float temp = a.temps[s], u = a.sample[s];
+  int b = 0, n = 0;
+  for (int i = tid; i < a.num_seqs; i += 256) {
+    const int count = a.choice[i].count;
+    n += count;
+    if (i < s) b += count;
+  }
+  for (int d = 32; d; d >>= 1) {
+    n += __shfl_xor(n, d, 64);
+    b += __shfl_xor(b, d, 64);
+  }
+  if (lane == 0) {
+    counts[wave] = b;
+    counts[4 + wave] = n;
+  }
+  __syncthreads();
+  const int before = counts[0] + counts[1] + counts[2] + counts[3], total = counts[4] + counts[5] + counts[6] + counts[7];
+  for (int i = tid; i < r.count && before + i < a.num_nodes; i += 256) a.rows[before + i] = a.path[t.first + i];
   for (long long i = total + s * 256LL + tid; i < a.num_nodes; i += a.num_seqs * 256LL) a.rows[i] = -1;
   if (tid == 0) {
     a.row_starts[s] = before;
     if (s == a.num_seqs - 1) a.row_starts[a.num_seqs] = total;
   }
-  const float temp = a.temps[s];
   if (r.node < 0 || greedy(temp)) {
     if (tid == 0) a.next[s] = r.node < 0 ? -1 : a.stat[r.node].best;
     return;
   }
-  const RowStat all = a.stat[r.node];
-  const double inv = 1. / temp;
-  // the chunks' weights; where nothing is left of p, p's own
-  double x = tid < a.chunks ? a.weight[static_cast<long long>(s) * a.chunks + tid] : 0.;
-  double sum = 0.;
-  const bool rest = block_sum(x, tmp) > 0.;
-  if (!rest) {
-    r.a = 1., r.b = 0., r.tried = 0;
-    if (tid < a.chunks) {
-      const RowStat part = a.part[static_cast<long long>(r.node) * a.chunks + tid];
-      x = all.z > 0. ? part.z * boost(part.m, all.m, inv) / all.z : 0.;
+  // The part of the row in which the sum passes u times all.
+  int num_gone = a.draft ? 0 : r.tried;
+  double sum = block_scan(x, run, tmp);
+  if (!(sum > 0.)) {  // nothing is left of p: p itself
+    const RowStat all = a.stat[r.node];
+    r.a = 1.;
+    r.b = 0.;
+    num_gone = 0;
+    const Exp2 boost;
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) {
+      const int c = tid * kParts + i;
+      const RowStat part = a.part[static_cast<long long>(r.node) * a.subs + min(c, a.subs - 1)];
+      x[i] = c < a.subs && part.z > 0. ? part.z * boost(part.m, all.m, rate_of(temp)) / all.z : 0.;
     }
+    sum = block_scan(x, run, tmp);
   }
-  scan[tid] = x;
-  __syncthreads();
-  if (tid == 0) {
-    sum = 0.;
-    for (int c = 0; c < a.chunks; ++c) sum += scan[c];
-    goal = a.sample[s] * sum;
-    double run = 0.;
-    int k = -1;
-    for (int c = 0; c < a.chunks; ++c) {
-      if (scan[c] > 0.) {
-        k = c;
-        base = run;
-        if (run + scan[c] > goal) break;
-      }
-      run += scan[c];
+  const double goal = u * sum;
+  // The first of all threads' numbers that has a weight and at which the sum is past the
+  // goal, else the last one with a weight, else -1. Numbers ascend with the threads.
+  int hit = INT_MAX, end = -1;
+  auto note = [&](int number, double weight, double upto) {
+    if (weight > 0.) {
+      if (upto > goal && hit == INT_MAX) hit = number;
+      end = number;
     }
-    at_chunk = k;
-    found = INT_MAX;
-    last = -1;
-  }
-  __syncthreads();
-  if (at_chunk < 0) {
+  };
+  auto first = [&] {
+    const unsigned long long hits = __ballot(hit != INT_MAX), ends = __ballot(end >= 0);
+    const int h = __shfl(hit, hits ? __ffsll(hits) - 1 : 0, 64), e = __shfl(end, ends ? 63 - __clzll(ends) : 0, 64);
+    __syncthreads();
+    if (lane == 0) {
+      found[wave] = h;
+      last[wave] = e;
+    }
+    __syncthreads();
+    hit = INT_MAX;
+    end = -1;
+    const int f = min(min(found[0], found[1]), min(found[2], found[3]));
+    return f != INT_MAX ? f : max(max(last[0], last[1]), max(last[2], last[3]));
+  };
+#pragma unroll
+  for (int i = 0; i < kParts; ++i) note(tid * kParts + i, x[i], run[i]);
+  const int part = first();
+  if (part < 0) {
     if (tid == 0) a.next[s] = -1;
     return;
   }
+#pragma unroll
+  for (int i = 0; i < kParts; ++i)
+    if (tid * kParts + i == part) start = run[i] - x[i];
+  __syncthreads();
+  // And the token there.
   const Weigh w = weigh(a, r.node, r.a, r.b, temp);
-  const long long at = static_cast<long long>(r.node) * a.vocab;
-  const int lo = at_chunk * kChunk + tid * (kChunk / 256), hi = min(lo + kChunk / 256, a.vocab);
-  double mine[kChunk / 256];
-  sum = 0.;
+  const bool rival = r.b != 0.;
+  const Row<T> rp(a, a.logits, r.node), rq(a, rival ? a.draft : a.logits, r.node);
+  const int p0 = part * kSub;
+  double y[4], upto[4];
+  float lp[4], lq[4];
+  rp.expand(p0 + tid * 4, rp.template fetch<4>(p0 + tid * 4), rp.inside(p0, kSub), lp);
+  rq.expand(p0 + tid * 4, rq.template fetch<4>(p0 + tid * 4), rp.inside(p0, kSub), lq);
+  weights(w, rival, lp, lq, p0 + tid * 4, rp.shift, a.tried + s * a.max_children, num_gone, y);
+  block_scan(y, upto, tmp);
 #pragma unroll
-  for (int i = 0; i < kChunk / 256; ++i) {
-    const int x = lo + i;
-    mine[i] = x < hi && !tried(a, p, r, x) ? w(load<T>(a.logits, at + x), r.b != 0. ? load<T>(a.draft, at + x) : -INFINITY) : 0.;
-    sum += mine[i];
-  }
-  scan[tid] = sum;
-  __syncthreads();
-  for (int d = 1; d < 256; d *= 2) {
-    const double y = tid >= d ? scan[tid - d] : 0.;
-    __syncthreads();
-    scan[tid] += y;
-    __syncthreads();
-  }
-  double run = base + (tid ? scan[tid - 1] : 0.);
-  int hit = INT_MAX, end = -1;
-#pragma unroll
-  for (int i = 0; i < kChunk / 256; ++i) {
-    run += mine[i];
-    if (mine[i] > 0.) {
-      end = lo + i;
-      if (hit == INT_MAX && run > goal) hit = lo + i;
-    }
-  }
-  if (hit != INT_MAX) atomicMin(&found, hit);
-  if (end >= 0) atomicMax(&last, end);
-  __syncthreads();
-  if (tid == 0) a.next[s] = found != INT_MAX ? found : last;
+  for (int i = 0; i < 4; ++i) note(p0 + tid * 4 + i, y[i], start + upto[i]);
+  const int at = first();
+  if (tid == 0) a.next[s] = at < 0 ? -1 : at - rp.shift;
 }
+
+// Parts of a row (places are counted from up to 7 elements before it), in whole fours.
+int subs_of(int vocab) { return (vocab + 7 + kWalk - 1) / kWalk * 4; }
 
 const char* check_shape(int vocab, int num_seqs, int num_nodes, int max_nodes, int max_children) {
   if (vocab < 1 || vocab > (1 << 20)) return "vocab outside [1, 2^20]";
@@ -497,8 +748,8 @@ const char* check_shape(int vocab, int num_seqs, int num_nodes, int max_nodes, i
   if (num_nodes < 1 || num_nodes > (1 << 20)) return "num_nodes outside [1, 2^20]";
   if (max_nodes < 1 || max_nodes > kMaxNodes) return "max_nodes outside [1, 1024]";
   if (max_children < 1 || max_children > 64) return "max_children outside [1, 64]";
-  const long long chunks = (vocab + kChunk - 1) / kChunk;
-  if (num_nodes * chunks >= (1LL << 23)) return "num_nodes * vocab: chunks of 4096 logits must count below 2^23";  // a launch has less than 2^32 threads
+  // a launch has less than 2^32 threads
+  if (num_nodes * (subs_of(vocab) / 4LL) >= (1LL << 23)) return "num_nodes * vocab: ceil((vocab + 7) / 4096) times num_nodes must be below 2^23";
   return nullptr;
 }
 
@@ -510,26 +761,28 @@ long long lay_out(VerifyArgs& a, bool draft, char* base) {
     at += (n * sizeof(*p) + 15) / 16 * 16;
   };
   const long long rows = (draft ? 2LL : 1LL) * a.num_nodes;
-  take(a.part, rows * a.chunks);
+  take(a.part, rows * a.subs);
   take(a.stat, rows);
-  take(a.chance, 2LL * a.num_nodes);
+  take(a.chance, a.num_nodes);
   take(a.choice, a.num_seqs);
-  take(a.weight, static_cast<long long>(a.num_seqs) * a.chunks);
+  take(a.weight, static_cast<long long>(a.num_seqs) * a.subs);
   take(a.path, a.num_nodes);
+  take(a.tried, static_cast<long long>(a.num_seqs) * a.max_children);
   const long long sums = draft && a.max_children > 1 ? static_cast<long long>(a.max_children) * a.num_nodes : 0;
   take(a.ab, sums);
-  take(a.mass, sums * a.chunks);
+  take(a.mass, sums * a.subs);
   return at;
 }
 
 template <typename T>
 void launch(const VerifyArgs& a, hipStream_t s) {
-  const int rows = (a.draft ? 2 : 1) * a.num_nodes;
-  IRON_LAUNCH((verify_stats_kernel<T>), dim3(rows * a.chunks), dim3(256), 0, s, a);
-  IRON_LAUNCH((verify_merge_kernel<T>), dim3(a.num_nodes), dim3(64), 0, s, a);
+  auto waves = [](long long n) { return dim3(static_cast<unsigned>((n + 3) / 4)); };  // in workgroups of four
+  const dim3 stats = waves((a.draft ? 2LL : 1LL) * a.num_nodes * a.subs), mass = waves(static_cast<long long>(a.num_nodes) * a.subs);
+  IRON_LAUNCH((verify_stats_kernel<T>), stats, dim3(256), 0, s, a);
+  IRON_LAUNCH((verify_merge_kernel<T>), dim3(a.num_nodes), dim3(256), 0, s, a);
   if (a.draft)
-    for (int j = 1; j < a.max_children; ++j) IRON_LAUNCH((verify_mass_kernel<T>), dim3(a.num_nodes * a.chunks), dim3(256), 0, s, a, j);
-  IRON_LAUNCH((verify_walk_kernel<T>), dim3(a.num_seqs * a.chunks), dim3(256), 0, s, a);
+    for (int j = 1; j < a.max_children; ++j) IRON_LAUNCH((verify_mass_kernel<T>), mass, dim3(256), 0, s, a, j);
+  IRON_LAUNCH((verify_walk_kernel<T>), dim3(a.num_seqs * (a.subs / 4)), dim3(256), 0, s, a);
   IRON_LAUNCH((verify_draw_kernel<T>), dim3(a.num_seqs), dim3(256), 0, s, a);
 }
 
@@ -545,7 +798,7 @@ extern "C" long long iron_draft_verify_workspace_bytes(int vocab, int num_seqs, 
   a.num_nodes = num_nodes;
   a.num_seqs = num_seqs;
   a.max_children = max_children;
-  a.chunks = (vocab + kChunk - 1) / kChunk;
+  a.subs = subs_of(vocab);
   return lay_out(a, draft != 0, nullptr);
 }
 
@@ -583,7 +836,7 @@ extern "C" int iron_draft_verify(const void* logits, const void* draft_logits, c
   a.num_nodes = num_nodes;
   a.max_nodes = max_nodes;
   a.max_children = max_children;
-  a.chunks = (vocab + kChunk - 1) / kChunk;
+  a.subs = subs_of(vocab);
   lay_out(a, draft_logits != nullptr, static_cast<char*>(workspace));
   hipStream_t s = static_cast<hipStream_t>(stream);
   dtype == 0 ? launch<uint16_t>(a, s) : dtype == 1 ? launch<_Float16>(a, s) : launch<float>(a, s);

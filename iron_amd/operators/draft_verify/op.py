@@ -59,8 +59,8 @@ class DraftVerify(PagedOperator):
 
     def __post_init__(self):
         self._check_counts(vocab=1 << 20, num_seqs=8192, num_nodes=1 << 20, max_nodes=1024, max_children=64)
-        if self.num_nodes * ((self.vocab + 4095) // 4096) >= 1 << 23:
-            raise ValueError(f"num_nodes={self.num_nodes}, vocab={self.vocab}: chunks of 4096 logits must count below 2**23")
+        if self.num_nodes * -(-(self.vocab + 7) // 4096) >= 1 << 23:
+            raise ValueError(f"num_nodes={self.num_nodes}, vocab={self.vocab}: num_nodes * ceil((vocab + 7) / 4096) must be below 2**23")
         if self.dtype not in _DTYPES:
             raise ValueError(f"dtype must be torch.bfloat16, torch.float16 or torch.float32, got {self.dtype!r}")
         PagedOperator.__init__(self, context=self.context)
