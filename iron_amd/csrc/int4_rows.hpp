@@ -69,45 +69,53 @@ __device__ __forceinline__ float int4_value(const void* row, int d) {
 // Half the largest range of a quarter whose b stays in fp16: b >= -(1 + 32 / 15) times it.
 constexpr float kInt4Most = 20480.f;
 
-// Quantizes N values (a quarter): the codes of x in words, and the pair. s is the
-// range by 15 and b the least value less 16 s, each rounded to fp16; a code is the
-// nearest for those, of two equally near ones the upper: how many of the borders
-// b + (k + 16.5) s, k = 0 .. 14, lie at or below x. The product is off by less than
-// half a code, and one comparison with the border next to it, which fp32 holds
-// exactly, decides. Values are cut to +-20480; a NaN makes the quarter NaN.
-template <int N>
-__device__ __forceinline__ unsigned int4_quantize(const float (&v)[N], unsigned (&words)[N / 8]) {
-  float x[N];
-  bool nan = false;
+// The least (largest) of a number over G lanes next to each other (2 or 4, aligned).
+template <int G>
+__device__ __forceinline__ float least_of(float x) {
+  auto turn = [&](int ctrl) { return __builtin_bit_cast(float, ctrl ? __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x4e, 0xf, 0xf, false)
+                                                                     : __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0xb1, 0xf, 0xf, false)); };
+  x = fminf(x, turn(0));  // quad_perm [1,0,3,2]
+  if constexpr (G == 4) x = fminf(x, turn(1));  // quad_perm [2,3,0,1]
+  return x;
+}
+
+// Quantizes a quarter of 8 G values, eight in each of G lanes: the codes of the
+// lane's eight in a word, and the pair. s is the range by 15 and b the least value
+// less 16 s, each rounded to fp16; a code is the nearest for those, of two equally
+// near ones the upper: how many of the borders b + (k + 16.5) s, k = 0 .. 14, lie at or
+// below x. The product is off by less than half a code, and one comparison with the
+// border next to it, which fp32 holds exactly, decides. Values are cut to +-20480; a
+// NaN makes the quarter NaN. All lanes of a quarter are active.
+template <int G>
+__device__ __forceinline__ unsigned int4_quantize(const float (&v)[8], unsigned& codes) {
+  float x[8], odd = 0.f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    nan |= v[i] != v[i];
+  for (int i = 0; i < 8; ++i) {
+    if (v[i] != v[i]) odd = -1.f;
     x[i] = fminf(fmaxf(v[i], -kInt4Most), kInt4Most);
   }
   float lo = x[0], hi = x[0];
 #pragma unroll
-  for (int i = 1; i < N; ++i) {
+  for (int i = 1; i < 8; ++i) {
     lo = fminf(lo, x[i]);
     hi = fmaxf(hi, x[i]);
   }
+  lo = least_of<G>(lo);
+  hi = -least_of<G>(-hi);
+  const bool nan = least_of<G>(odd) < 0.f;
   const _Float16 sh = static_cast<_Float16>((hi - lo) / 15.f);
   const float s = static_cast<float>(sh);
   const _Float16 bh = static_cast<_Float16>((lo - 16.f * s) + 0.f);  // of zeros of both signs, +0
   const float b = static_cast<float>(bh), inv = s > 0.f ? 1.f / s : 0.f;
+  codes = 0;
 #pragma unroll
-  for (int w = 0; w < N / 8; ++w) words[w] = 0;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
+  for (int i = 0; i < 8; ++i) {
     const float k = fminf(fmaxf(floorf((x[i] - b) * inv - 16.f), 0.f), 14.f);  // the border above code k
     const int code = static_cast<int>(k) + (s > 0.f && x[i] >= fmaf(k + 16.5f, s, b) ? 1 : 0);
-    words[i >> 3] |= static_cast<unsigned>(code) << (4 * ((i & 7) >> 1) + 16 * (i & 1));
+    codes |= static_cast<unsigned>(code) << (4 * (i >> 1) + 16 * (i & 1));
   }
-  if (nan) {
-#pragma unroll
-    for (int w = 0; w < N / 8; ++w) words[w] = 0;
-    return 0x7e000000u;
-  }
-  return __builtin_bit_cast(uint16_t, sh) | static_cast<unsigned>(__builtin_bit_cast(uint16_t, bh)) << 16;
+  if (nan) codes = 0;
+  return nan ? 0x7e000000u : __builtin_bit_cast(uint16_t, sh) | static_cast<unsigned>(__builtin_bit_cast(uint16_t, bh)) << 16;
 }
 
 }  // namespace iron

@@ -358,45 +358,51 @@ __device__ __forceinline__ float wide16(unsigned x) {
   return __uint_as_float(x << 16);
 }
 
-// 16 rows of the call, `items` of the (layer, K or V, head) planes to a workgroup:
-// a wave takes a plane, four lanes a row of it, so that neighbouring positions of a
-// page are written together.
+// 16 rows of the call, `items` of the (layer, K or V, head) planes to a workgroup: a
+// wave takes a plane, a lane eight values of a row at a time, so that both sides are
+// read and written in whole lines. The lanes of a quarter (2, or 4 with head_dim 128)
+// find its range together.
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void append4_rows_kernel(AppendArgs a, int items) {
-  constexpr int N = D / 4, kRow = kInt4Row<D>;
+  constexpr int kRow = kInt4Row<D>, L = D / 8, kTurns = kTile * L / 64;  // lanes of a row, rows of a lane
   __shared__ RowPlace place;
   const Pool& p = a.pool;
-  const int r0 = blockIdx.x * kTile, lane = threadIdx.x & 63, i = lane >> 2, part = lane & 3;
+  const int r0 = blockIdx.x * kTile, lane = threadIdx.x & 63, e = lane % L;
   place_rows(p, a.row_starts, a.num_rows, r0, place, [&](int s, int& begin) { return (begin = a.begin[s]) >= 0; }, [](int) { return INT_MAX; });
-  const int page = place.page[i], at = place.at[i];
-  if (place.owner[i] < 0 || page < 0) return;
-  const int src = a.rows[r0 + i];
-  const bool real = static_cast<unsigned>(src) < static_cast<unsigned>(a.num_nodes);
   const int H = p.n_kv_heads, planes = p.num_layers * 2 * H, stop = min(planes, (static_cast<int>(blockIdx.y) + 1) * items);
+  int page[kTurns], at[kTurns], src[kTurns];
+#pragma unroll
+  for (int i = 0; i < kTurns; ++i) {
+    const int r = i * (64 / L) + lane / L;
+    page[i] = place.owner[r] < 0 ? -1 : place.page[r];
+    at[i] = place.at[r];
+    src[i] = a.rows[min(r0 + r, a.num_rows - 1)];
+  }
   for (int x = blockIdx.y * items + (threadIdx.x >> 6); x < stop; x += 4) {
     const int lk = x / H, h = x - lk * H, l = lk >> 1;
-    float v[N] = {};
-    if (real) {
-      const uint4* from = (lk & 1 ? a.v_new : a.k_new) + ((static_cast<long long>(l) * a.num_nodes + src) * H + h) * (D / 8) + part * (N / 8);
+    uint4 y[kTurns];
 #pragma unroll
-      for (int e = 0; e < N / 8; ++e) {
-        const uint4 y = from[e];
-        const unsigned w[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[8 * e + 2 * j] = wide16<F16>(w[j] & 0xffffu);
-          v[8 * e + 2 * j + 1] = wide16<F16>(w[j] >> 16);
-        }
-      }
+    for (int i = 0; i < kTurns; ++i) {
+      const bool real = static_cast<unsigned>(src[i]) < static_cast<unsigned>(a.num_nodes);
+      y[i] = make_uint4(0, 0, 0, 0);
+      if (real) y[i] = (lk & 1 ? a.v_new : a.k_new)[((static_cast<long long>(l) * a.num_nodes + src[i]) * H + h) * L + e];
     }
-    unsigned codes[N / 8];
-    const unsigned pair = int4_quantize(v, codes);
-    unsigned char* to = (lk & 1 ? p.v : p.k) + (((static_cast<long long>(l) * p.num_pages + page) * H + h) * p.page_size + at) * kRow;
-    if constexpr (N == 16)
-      *reinterpret_cast<uint2*>(to + part * 8) = make_uint2(codes[0], codes[1]);
-    else
-      *reinterpret_cast<uint4*>(to + part * 16) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
-    *reinterpret_cast<unsigned*>(to + D / 2 + part * 4) = pair;
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+      const unsigned w[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[2 * j] = wide16<F16>(w[j] & 0xffffu);
+        v[2 * j + 1] = wide16<F16>(w[j] >> 16);
+      }
+      unsigned codes;
+      const unsigned pair = int4_quantize<L / 4>(v, codes);
+      if (page[i] < 0) continue;
+      unsigned char* to = (lk & 1 ? p.v : p.k) + (((static_cast<long long>(l) * p.num_pages + page[i]) * H + h) * p.page_size + at[i]) * kRow;
+      *reinterpret_cast<unsigned*>(to + e * 4) = codes;
+      if (e % (L / 4) == 0) *reinterpret_cast<unsigned*>(to + D / 2 + e / (L / 4) * 4) = pair;
+    }
   }
 }
 
@@ -412,42 +418,46 @@ struct GatherArgs {
 // The other way round: 16 rows of the result.
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void gather4_rows_kernel(GatherArgs a, int items) {
-  constexpr int N = D / 4, kRow = kInt4Row<D>;
+  constexpr int kRow = kInt4Row<D>, L = D / 8, kTurns = kTile * L / 64;
   __shared__ RowPlace place;
   const Pool& p = a.pool;
-  const int r0 = blockIdx.x * kTile, lane = threadIdx.x & 63, i = lane >> 2, part = lane & 3;
+  const int r0 = blockIdx.x * kTile, lane = threadIdx.x & 63, e = lane % L;
   place_rows(p, a.row_starts, a.num_rows, r0, place, [&](int s, int& begin) { return begin = a.begins[s], true; }, [&](int s) { return p.lens[s]; });
-  if (place.owner[i] < 0) return;
-  const int page = place.page[i], at = place.at[i];
   const int H = p.n_kv_heads, planes = p.num_layers * 2 * H, stop = min(planes, (static_cast<int>(blockIdx.y) + 1) * items);
+  int page[kTurns], at[kTurns];
+  bool mine[kTurns];
+#pragma unroll
+  for (int i = 0; i < kTurns; ++i) {
+    const int r = i * (64 / L) + lane / L;
+    mine[i] = place.owner[r] >= 0;
+    page[i] = place.page[r];
+    at[i] = place.at[r];
+  }
   for (int x = blockIdx.y * items + (threadIdx.x >> 6); x < stop; x += 4) {
     const int lk = x / H, h = x - lk * H, l = lk >> 1;
-    unsigned words[N / 8], pair = 0;
-    for (int e = 0; e < N / 8; ++e) words[e] = 0;
-    if (page >= 0) {
-      const unsigned char* from = (lk & 1 ? p.v : p.k) + (((static_cast<long long>(l) * p.num_pages + page) * H + h) * p.page_size + at) * kRow;
-      if constexpr (N == 16) {
-        const uint2 y = *reinterpret_cast<const uint2*>(from + part * 8);
-        words[0] = y.x, words[1] = y.y;
-      } else {
-        const uint4 y = *reinterpret_cast<const uint4*>(from + part * 16);
-        words[0] = y.x, words[1] = y.y, words[2] = y.z, words[3] = y.w;
-      }
-      pair = *reinterpret_cast<const unsigned*>(from + D / 2 + part * 4);
-    }
-    uint4* to = (lk & 1 ? a.v_out : a.k_out) + ((static_cast<long long>(l) * a.num_rows + r0 + i) * H + h) * (D / 8) + part * (N / 8);
+    unsigned codes[kTurns], pair[kTurns];
 #pragma unroll
-    for (int e = 0; e < N / 8; ++e) {
+    for (int i = 0; i < kTurns; ++i) {
+      codes[i] = pair[i] = 0;
+      if (page[i] >= 0) {
+        const unsigned char* from = (lk & 1 ? p.v : p.k) + (((static_cast<long long>(l) * p.num_pages + page[i]) * H + h) * p.page_size + at[i]) * kRow;
+        codes[i] = *reinterpret_cast<const unsigned*>(from + e * 4);
+        pair[i] = *reinterpret_cast<const unsigned*>(from + D / 2 + e / (L / 4) * 4);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
       unsigned y[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float lo = int4_dequant(pair, int4_code(words[e], 2 * j)), hi = int4_dequant(pair, int4_code(words[e], 2 * j + 1));
+        const float lo = int4_dequant(pair[i], int4_code(codes[i], 2 * j)), hi = int4_dequant(pair[i], int4_code(codes[i], 2 * j + 1));
         if constexpr (F16)
           y[j] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(lo)) | static_cast<unsigned>(__builtin_bit_cast(uint16_t, static_cast<_Float16>(hi))) << 16;
         else
           y[j] = cvt_pk_bf16(lo, hi);
       }
-      to[e] = make_uint4(y[0], y[1], y[2], y[3]);
+      const int r = r0 + i * (64 / L) + lane / L;
+      if (mine[i]) (lk & 1 ? a.v_out : a.k_out)[((static_cast<long long>(l) * a.num_rows + r) * H + h) * L + e] = make_uint4(y[0], y[1], y[2], y[3]);
     }
   }
 }
