@@ -69,49 +69,64 @@ __device__ __forceinline__ float int4_value(const void* row, int d) {
 // Half the largest range of a quarter whose b stays in fp16: b >= -(1 + 32 / 15) times it.
 constexpr float kInt4Most = 20480.f;
 
-// The least (largest) of a number over G lanes next to each other (2 or 4, aligned).
-template <int G>
-__device__ __forceinline__ float least_of(float x) {
-  auto turn = [&](int ctrl) { return __builtin_bit_cast(float, ctrl ? __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x4e, 0xf, 0xf, false)
-                                                                     : __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0xb1, 0xf, 0xf, false)); };
-  x = fminf(x, turn(0));  // quad_perm [1,0,3,2]
-  if constexpr (G == 4) x = fminf(x, turn(1));  // quad_perm [2,3,0,1]
-  return x;
+// The smallest, the largest of three numbers; the compiler's own makes quiet NaN of its operands first, at an instruction each.
+__device__ __forceinline__ float i4_min3(float a, float b, float c) {
+  float r;
+  asm("v_min3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+__device__ __forceinline__ float i4_max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
 }
 
-// Quantizes a quarter of 8 G values, eight in each of G lanes: the codes of the
-// lane's eight in a word, and the pair. s is the range by 15 and b the least value
-// less 16 s, each rounded to fp16; a code is the nearest for those, of two equally
-// near ones the upper: how many of the borders b + (k + 16.5) s, k = 0 .. 14, lie at or
-// below x. The product is off by less than half a code, and one comparison with the
-// border next to it, which fp32 holds exactly, decides. Values are cut to +-20480; a
-// NaN makes the quarter NaN. All lanes of a quarter are active.
+// A lane's neighbour's number (quad_perm [1,0,3,2]), and that of the other pair of four ([2,3,0,1]).
+__device__ __forceinline__ float i4_beside(float x) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0xb1, 0xf, 0xf, false)); }
+__device__ __forceinline__ float i4_across(float x) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x4e, 0xf, 0xf, false)); }
+
+// Quantizes a quarter of 8 G values (of a 16-bit type), eight in each of G lanes: the
+// codes of the lane's eight in a word, and the pair. s is the range by 15 and b the
+// least value less 16 s, each rounded to fp16; a code is the nearest for those, of two
+// equally near ones the upper: how many of the borders b + (k + 16.5) s, k = 0 .. 14, lie
+// at or below x. The product is off by less than half a code (by 2^-8: a range of 16-bit
+// values is 2^-11 of them or more), and one comparison with the border next to it, which
+// fp32 holds exactly, decides. Values are cut to +-20480; a NaN makes the quarter NaN.
+// All lanes of a quarter are active. 13 instructions a value.
 template <int G>
-__device__ __forceinline__ unsigned int4_quantize(const float (&v)[8], unsigned& codes) {
-  float x[8], odd = 0.f;
+__device__ __forceinline__ unsigned int4_quantize(float (&x)[8], unsigned& codes) {
+  bool nan = false;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (v[i] != v[i]) odd = -1.f;
-    x[i] = fminf(fmaxf(v[i], -kInt4Most), kInt4Most);
+  for (int i = 0; i < 8; i += 2) nan |= __builtin_isunordered(x[i], x[i + 1]);
+  float lo = i4_min3(x[0], x[1], x[2]), hi = i4_max3(x[0], x[1], x[2]);
+  lo = i4_min3(i4_min3(lo, x[3], x[4]), i4_min3(x[5], x[6], x[7]), lo);
+  hi = i4_max3(i4_max3(hi, x[3], x[4]), i4_max3(x[5], x[6], x[7]), hi);
+  lo = i4_min3(lo, i4_beside(lo), lo);
+  hi = i4_max3(hi, i4_beside(hi), hi);
+  if constexpr (G == 4) {
+    lo = i4_min3(lo, i4_across(lo), lo);
+    hi = i4_max3(hi, i4_across(hi), hi);
   }
-  float lo = x[0], hi = x[0];
+  // lanes of the wave with a NaN; those of this lane's quarter
+  const unsigned long long odd = __ballot(nan);
+  nan = (threadIdx.x & 32 ? static_cast<unsigned>(odd >> 32) : static_cast<unsigned>(odd)) >> (threadIdx.x & 31 & ~(G - 1)) & ((1u << G) - 1);
+  if (__ballot(!(lo >= -kInt4Most && hi <= kInt4Most))) {
+    auto cut = [](float y) { return fminf(fmaxf(y, -kInt4Most), kInt4Most); };
 #pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
+    for (int i = 0; i < 8; ++i) x[i] = cut(x[i]);
+    lo = cut(lo);
+    hi = cut(hi);
   }
-  lo = least_of<G>(lo);
-  hi = -least_of<G>(-hi);
-  const bool nan = least_of<G>(odd) < 0.f;
   const _Float16 sh = static_cast<_Float16>((hi - lo) / 15.f);
   const float s = static_cast<float>(sh);
   const _Float16 bh = static_cast<_Float16>((lo - 16.f * s) + 0.f);  // of zeros of both signs, +0
-  const float b = static_cast<float>(bh), inv = s > 0.f ? 1.f / s : 0.f;
+  const float b = static_cast<float>(bh), inv = s > 0.f ? 1.f / s : 0.f, first = -16.f - b * inv;
+  const float step = s > 0.f ? s : INFINITY;  // without a range every border is out of reach
   codes = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float k = fminf(fmaxf(floorf((x[i] - b) * inv - 16.f), 0.f), 14.f);  // the border above code k
-    const int code = static_cast<int>(k) + (s > 0.f && x[i] >= fmaf(k + 16.5f, s, b) ? 1 : 0);
+    const float k = __builtin_amdgcn_fmed3f(floorf(fmaf(x[i], inv, first)), 0.f, 14.f);  // the border above code k
+    const int code = static_cast<int>(k) + (x[i] >= fmaf(k + 16.5f, step, b) ? 1 : 0);
     codes |= static_cast<unsigned>(code) << (4 * (i >> 1) + 16 * (i & 1));
   }
   if (nan) codes = 0;
