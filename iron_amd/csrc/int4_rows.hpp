@@ -17,14 +17,21 @@ typedef _Float16 i4_f16x2 __attribute__((ext_vector_type(2)));
 template <int D>
 constexpr int kInt4Row = D / 2 + 16;  // bytes
 
+// (x & mask) | bits in one instruction, which takes one scalar operand only: the compiler makes two of it.
+__device__ __forceinline__ unsigned i4_pick(unsigned x, unsigned bits) {
+  unsigned r;
+  asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "s"(0x03c003c0u), "v"(bits));
+  return r;
+}
+
 // The fp16 pairs (0, 1), (2, 3), (4, 5), (6, 7) of a word of codes, each value
 // rounded once: half a step of fp16, an eighth of bf16's.
 __device__ __forceinline__ void int4_unpack8(unsigned codes, i4_f16x2 s, i4_f16x2 b, unsigned (&out)[4]) {
-  constexpr unsigned kMask = 0x03c003c0u, kSixteen = 0x4c004c00u;
+  constexpr unsigned kSixteen = 0x4c004c00u;
   const unsigned x[4] = {codes << 6, codes << 2, codes >> 2, codes >> 6};
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    out[i] = __builtin_bit_cast(unsigned, __builtin_elementwise_fma(__builtin_bit_cast(i4_f16x2, (x[i] & kMask) | kSixteen), s, b));
+    out[i] = __builtin_bit_cast(unsigned, __builtin_elementwise_fma(__builtin_bit_cast(i4_f16x2, i4_pick(x[i], kSixteen)), s, b));
 }
 
 // The same as sums of two fp16 numbers and b, without rounding: s has 11 bits and
@@ -32,11 +39,11 @@ __device__ __forceinline__ void int4_unpack8(unsigned codes, i4_f16x2 s, i4_f16x
 // fits fp16 (halved, the largest s does too; below 2^-13 the lower part may lose
 // its last bit, 2^-25). high + low + b / 2 is half the value.
 __device__ __forceinline__ void int4_split8(unsigned codes, i4_f16x2 s_high, i4_f16x2 s_low, unsigned (&high)[4], unsigned (&low)[4]) {
-  constexpr unsigned kMask = 0x03c003c0u, kEight = 0x48004800u;
+  constexpr unsigned kEight = 0x48004800u;
   const unsigned x[4] = {codes << 6, codes << 2, codes >> 2, codes >> 6};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const i4_f16x2 y = __builtin_bit_cast(i4_f16x2, (x[i] & kMask) | kEight);
+    const i4_f16x2 y = __builtin_bit_cast(i4_f16x2, i4_pick(x[i], kEight));
     high[i] = __builtin_bit_cast(unsigned, y * s_high);
     low[i] = __builtin_bit_cast(unsigned, y * s_low);
   }

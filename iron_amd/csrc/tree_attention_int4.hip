@@ -14,18 +14,31 @@ struct Quarter {
   unsigned pair;
 };
 
+// Buffer loads: the rows' address is the wave's, in scalar registers, a lane's offset
+// the same for all blocks (as global loads, each had its address computed in 64 bits).
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const unsigned char* rows) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(rows), 0, 0x7fffffff, kBufferFlags);
+}
 template <int D>
 __device__ __forceinline__ Quarter<D> load_quarter(const unsigned char* rows, unsigned at_codes, unsigned at_pair) {
+  const __amdgpu_buffer_rsrc_t rsrc = rows_at(rows);
   Quarter<D> x;
   if constexpr (D == 64) {
-    const ta_u32x2 v = *reinterpret_cast<const ta_u32x2*>(rows + at_codes);
+    const ta_u32x2 v = __builtin_bit_cast(ta_u32x2, __builtin_amdgcn_raw_buffer_load_b64(rsrc, at_codes, 0, 0));
     x.codes[0] = v.x, x.codes[1] = v.y;
   } else {
-    const ta_u32x4 v = *reinterpret_cast<const ta_u32x4*>(rows + at_codes);
+    const ta_u32x4 v = __builtin_bit_cast(ta_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at_codes, 0, 0));
     x.codes[0] = v.x, x.codes[1] = v.y, x.codes[2] = v.z, x.codes[3] = v.w;
   }
-  x.pair = *reinterpret_cast<const unsigned*>(rows + at_pair);
+  x.pair = __builtin_amdgcn_raw_buffer_load_b32(rsrc, at_pair, 0, 0);
   return x;
+}
+
+// The largest of three numbers; the compiler's own makes quiet NaN of its operands first, at an instruction each.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
 }
 
 // Eight values of a quarter (word kk) as the fp16 operand of a product.
@@ -81,6 +94,11 @@ __device__ __forceinline__ float to_fp16(ta_u32x4 (&q)[NK], float scale) {
   return factor == INFINITY ? NAN : factor;  // done over, too
 }
 
+// Workgroups of the kernels of few and of many rows that fit the 256 CUs at once, by
+// their registers.
+constexpr int few_resident(int D, int RT, bool F16) { return D == 64 ? (RT == 1 ? 1024 : 768) : RT == 1 && !F16 ? 768 : 512; }
+constexpr int wide_resident(int D, bool F16) { return D == 64 && !F16 ? 768 : 512; }
+
 // Few rows: a tile of 16 RT rows, a workgroup of 4 waves. Wave w has keys 16 w ..
 // + 15 of each block of 64 and all rows, so that nothing is shared until the end.
 // A lane has a quarter of a key's row, which it loads (kAhead blocks ahead, into
@@ -89,9 +107,9 @@ __device__ __forceinline__ float to_fp16(ta_u32x4 (&q)[NK], float scale) {
 // 16-bit rows in, V^T out by transposed reads. Two blocks make a step: the weights of
 // 2 x 4 keys, rounded to fp16, are the 8 elements of the B operand of O^T += V^T P^T.
 template <int D, bool F16, int RT>
-__global__ __launch_bounds__(256, 2) void tree4_kernel(TreeArgs a) {
+__global__ __launch_bounds__(256, few_resident(D, RT, F16) / 256) void tree4_kernel(TreeArgs a) {
   constexpr int R = 16 * RT, B = kBlock, kRow = kInt4Row<D>, kWide = D * 2;
-  constexpr int NK = D / 32, ND = D / 16, kAhead = D == 64 ? 8 : RT == 2 ? 2 : 4;
+  constexpr int NK = D / 32, ND = D / 16, kAhead = 2;
   constexpr int kOwn = 32 * kWide > R * D * 4 ? 32 * kWide : R * D * 4;  // LDS of a wave: V of two blocks, at the end its output
   __shared__ __attribute__((aligned(16))) unsigned char lds[4 * kOwn];
   __shared__ float stat_m[4][R], stat_l[4][R];
@@ -169,31 +187,16 @@ __global__ __launch_bounds__(256, 2) void tree4_kernel(TreeArgs a) {
       }
       // Q: the B operand of S^T = K Q^T (column: row 16 rt + c; dims D / 4 quad + 8 kk .. + 8)
       ta_u32x4 qf[RT][NK];
-      unsigned q_half[RT];  // fp16: half the sum of the lane's dims, in two parts, b's factor
       int node[RT];
-      float cs[RT];
-      auto load_q = [&](int rt) {
+      ta_f32x4 o[RT][ND];
+      float m[RT], off[RT], l[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
         const int r = min(row0 + 16 * rt + c, t.nodes * G - 1), in_tree = r / G;
         node[rt] = t.first + in_tree;
         const uint16_t* qp = a.q + (static_cast<long long>(node[rt]) * a.H + hk * G + (r - in_tree * G)) * D + quad * (D / 4);
 #pragma unroll
         for (int kk = 0; kk < NK; ++kk) qf[rt][kk] = *reinterpret_cast<const ta_u32x4*>(qp + 8 * kk);
-      };
-      ta_f32x4 o[RT][ND];
-      float m[RT], off[RT], l[RT];
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        load_q(rt);
-        cs[rt] = to_fp16<F16, false>(qf[rt], a.scale_log2);
-        if constexpr (F16) {
-          float sum = 0.f;
-#pragma unroll
-          for (int kk = 0; kk < NK; ++kk)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sum = add2<true>(qf[rt][kk][i], sum);
-          q_half[rt] = split_fp16(sum * 0.5f);
-          cs[rt] *= 2.f;
-        }
         m[rt] = -INFINITY;
         off[rt] = l[rt] = 0.f;
 #pragma unroll
@@ -222,6 +225,68 @@ __global__ __launch_bounds__(256, 2) void tree4_kernel(TreeArgs a) {
           }
         }
       };
+      // The tree's own keys first, while the cache's are on their way: 16-bit rows, weights
+      // in two parts (split4), V^T's 4 keys given twice.
+      for (int i = max(cached, 0); i < n; ++i) {
+        const int j0 = (blk0 + i - t.cached) * B + 16 * w, have = min(t.nodes - j0, 16);
+        if (have <= 0) continue;
+        const long long key = (static_cast<long long>(t.first + min(j0 + c, t.nodes - 1)) * a.Hkv + hk) * D + quad * (D / 4);
+        ta_f32x4 sc[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) sc[rt] = ta_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) {
+          const ta_u32x4 kf = *reinterpret_cast<const ta_u32x4*>(a.k_new + key + 8 * kk);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) sc[rt] = mfma<F16>(kf, qf[rt][kk], sc[rt]);
+          put_v(0, kk, *reinterpret_cast<const ta_u32x4*>(a.v_new + key + 8 * kk));
+        }
+        asm volatile("" ::: "memory");
+        float top[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const int word = a.mask[static_cast<long long>(node[rt]) * a.words + (j0 >> 5)] >> ((j0 & 31) + 4 * quad);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[rt][e] = 4 * quad + e < have && (word >> e & 1) ? sc[rt][e] : -INFINITY;
+          top[rt] = fmaxf(fmaxf(sc[rt][0], sc[rt][1]), fmaxf(sc[rt][2], sc[rt][3])) * a.scale_log2;
+        }
+        raise(top);
+        const unsigned m01 = keep01(have), m23 = keep23(have);
+        ta_u32x4 pf[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          float p[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(sc[rt][e], a.scale_log2, -off[rt]));
+          l[rt] += (p[0] + p[1]) + (p[2] + p[3]);
+          pf[rt] = split4<F16>(p);
+        }
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) {
+          ta_u32x2 vt = get_v(0, dt);
+          vt.x &= m01;
+          vt.y &= m23;
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) o[rt][dt] = mfma<F16>(ta_u32x4{vt.x, vt.y, vt.x, vt.y}, pf[rt], o[rt][dt]);
+        }
+        asm volatile("" ::: "memory");
+      }
+
+      float cs[RT];
+      unsigned q_half[RT];  // fp16: half the sum of the lane's dims, in two parts, b's factor
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        cs[rt] = to_fp16<F16, false>(qf[rt], a.scale_log2);
+        if constexpr (F16) {
+          float sum = 0.f;
+#pragma unroll
+          for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum = add2<true>(qf[rt][kk][i], sum);
+          q_half[rt] = split_fp16(sum * 0.5f);
+          cs[rt] *= 2.f;
+        }
+      }
       auto step = [&](int j) {  // the blocks in places j and j + 1
         if (valid[j] + valid[j + 1] == 0) return;
         ta_f32x4 sc[2][RT];
@@ -281,7 +346,7 @@ __global__ __launch_bounds__(256, 2) void tree4_kernel(TreeArgs a) {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
           const ta_f32x4 x = sc[0][rt], y = sc[1][rt];
-          top[rt] = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]))) * cs[rt];
+          top[rt] = max3(max3(max3(x[0], x[1], x[2]), x[3], y[0]), max3(y[1], y[2], y[3]), y[3]) * cs[rt];
         }
         raise(top);
         if constexpr (F16) {  // weights in two parts (split4), V^T's 4 keys given twice
@@ -325,55 +390,6 @@ __global__ __launch_bounds__(256, 2) void tree4_kernel(TreeArgs a) {
           page[0] = page_of(i + j + 2 + kAhead);
           page[1] = page_of(i + j + 3 + kAhead);
         }
-      }
-
-      // The tree's own keys, 16-bit rows: weights in two parts (split4), V^T's 4 keys given twice.
-      for (int i = max(cached, 0); i < n; ++i) {
-        const int j0 = (blk0 + i - t.cached) * B + 16 * w, have = min(t.nodes - j0, 16);
-        if (have <= 0) continue;
-        const long long key = (static_cast<long long>(t.first + min(j0 + c, t.nodes - 1)) * a.Hkv + hk) * D + quad * (D / 4);
-        ta_f32x4 sc[RT];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          sc[rt] = ta_f32x4{0.f, 0.f, 0.f, 0.f};
-          load_q(rt);
-        }
-#pragma unroll
-        for (int kk = 0; kk < NK; ++kk) {
-          const ta_u32x4 kf = *reinterpret_cast<const ta_u32x4*>(a.k_new + key + 8 * kk);
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) sc[rt] = mfma<F16>(kf, qf[rt][kk], sc[rt]);
-          put_v(0, kk, *reinterpret_cast<const ta_u32x4*>(a.v_new + key + 8 * kk));
-        }
-        asm volatile("" ::: "memory");
-        float top[RT];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          const int word = a.mask[static_cast<long long>(node[rt]) * a.words + (j0 >> 5)] >> ((j0 & 31) + 4 * quad);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[rt][e] = 4 * quad + e < have && (word >> e & 1) ? sc[rt][e] : -INFINITY;
-          top[rt] = fmaxf(fmaxf(sc[rt][0], sc[rt][1]), fmaxf(sc[rt][2], sc[rt][3])) * a.scale_log2;
-        }
-        raise(top);
-        const unsigned m01 = keep01(have), m23 = keep23(have);
-        ta_u32x4 pf[RT];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          float p[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(sc[rt][e], a.scale_log2, -off[rt]));
-          l[rt] += (p[0] + p[1]) + (p[2] + p[3]);
-          pf[rt] = split4<F16>(p);
-        }
-#pragma unroll
-        for (int dt = 0; dt < ND; ++dt) {
-          ta_u32x2 vt = get_v(0, dt);
-          vt.x &= m01;
-          vt.y &= m23;
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) o[rt][dt] = mfma<F16>(ta_u32x4{vt.x, vt.y, vt.x, vt.y}, pf[rt], o[rt][dt]);
-        }
-        asm volatile("" ::: "memory");
       }
 
       // The four waves' parts of the tile meet in LDS.
@@ -442,7 +458,7 @@ __global__ __launch_bounds__(256, 2) void tree4_kernel(TreeArgs a) {
 // block. The cache's blocks come first, with fp16 products, then the tree's, with
 // those of its type; a row's maximum, sum and output go on through both.
 template <int D, bool F16>
-__global__ __launch_bounds__(256, D == 64 && !F16 ? 3 : 2) void tree4_wide_kernel(TreeArgs a) {
+__global__ __launch_bounds__(256, wide_resident(D, F16) / 256) void tree4_wide_kernel(TreeArgs a) {
   constexpr int R = 128, B = kWideBlock, kRow = D * 2, kHalf = B * kRow, kRing = 3;
   constexpr int kStage = F16 ? 3 * kHalf : 2 * kHalf;  // K, V and, with fp16, K's lower parts; b's behind the ring
   constexpr int kRow4 = kInt4Row<D>, NW = D / 64;  // words of codes (16-byte chunks of 16-bit rows) of a lane and block
@@ -492,6 +508,7 @@ __global__ __launch_bounds__(256, D == 64 && !F16 ? 3 : 2) void tree4_wide_kerne
       // Blocks blk0 .. of the cache (CACHE) or of the tree.
       auto phase = [&](auto cache) {
         constexpr bool CACHE = decltype(cache)::value, T16 = CACHE || F16, EXACT = CACHE && F16;  // T16: fp16 operands
+        constexpr bool ONE = EXACT || (!CACHE && D == 128);  // K's fragments one ahead, not all at once: what registers there are
         const int nb = CACHE ? min(n, t.cached - blk0) : n - max(min(n, t.cached - blk0), 0);
         if (nb <= 0) return;
         const int first = CACHE ? blk0 : max(blk0 - t.cached, 0), have = CACHE ? t.len : t.nodes;
@@ -605,10 +622,10 @@ __global__ __launch_bounds__(256, D == 64 && !F16 ? 3 : 2) void tree4_wide_kerne
         };
         // The row's maximum, when scores pass it by more than 8 (in the log2 domain; cf. tree4_kernel).
         auto raise = [&](const ta_f32x16& sc) {
-          float mx = fmaxf(fmaxf(sc[0], sc[1]), sc[2]);
+          float mx = max3(sc[0], sc[1], sc[2]);
 #pragma unroll
-          for (int j = 3; j < 15; j += 2) mx = fmaxf(fmaxf(mx, sc[j]), sc[j + 1]);
-          mx = fmaxf(mx, sc[15]);
+          for (int j = 3; j < 15; j += 2) mx = max3(mx, sc[j], sc[j + 1]);
+          mx = max3(mx, sc[15], sc[15]);
           if (__builtin_amdgcn_ballot_w64(mx * cs > m + 8.f)) {
             float x, y;
             swap32(mx, x, y);
@@ -651,8 +668,8 @@ __global__ __launch_bounds__(256, D == 64 && !F16 ? 3 : 2) void tree4_wide_kerne
           }
           // K's fragments of block i + 1 (behind the last block: a stage that nothing writes, for scores that go unused)
           ta_u32x4 kf[NK], low[NK], bf;
-          if constexpr (EXACT) {
-            bf = base_frag(i + 1);
+          if constexpr (EXACT) bf = base_frag(i + 1);
+          if constexpr (ONE) {
             kf[0] = k_frag(i + 1, 0);
           } else {
 #pragma unroll
@@ -671,9 +688,10 @@ __global__ __launch_bounds__(256, D == 64 && !F16 ? 3 : 2) void tree4_wide_kerne
 #pragma unroll
           for (int g = 0; g < 8; ++g) {
             __builtin_amdgcn_sched_barrier(0);
+            if constexpr (ONE)
+              if (g + 1 < NK) kf[g + 1] = k_frag(i + 1, g + 1);
             if constexpr (EXACT) {
               if (g < NK) low[g] = low_frag(i + 1, g);
-              if (g + 1 < NK) kf[g + 1] = k_frag(i + 1, g + 1);
               if (g == 0) next = mfma32<T16>(bf, q_half, next);
             }
             if (g < NK) next = mfma32<T16>(kf[g], qf[g], next);
@@ -771,24 +789,22 @@ __global__ __launch_bounds__(256, D == 64 && !F16 ? 3 : 2) void tree4_wide_kerne
 }
 
 // Workgroups that fit the 256 CUs at once.
-int resident(int D, int R) { return D == 64 && R != 32 ? 768 : 512; }
+int resident(int D, int R) { return R < 128 ? few_resident(D, R / 16, false) : wide_resident(D, false); }
 
 template <int D, bool F16, int RT>
-void launch_few(const TreeArgs& a, hipStream_t s) {
+void launch_few(TreeArgs a, hipStream_t s) {
+  a.workgroups = std::min(a.workgroups, few_resident(D, RT, F16));
   IRON_LAUNCH((tree4_kernel<D, F16, RT>), dim3(a.workgroups), dim3(256), 0, s, a);
   IRON_LAUNCH((tree_join_kernel<D, F16, 16 * RT, kBlock, true>), dim3(a.num_nodes, (a.H + 3) / 4), dim3(256), 0, s, a);
 }
 
 template <int D, bool F16>
-void launch_rows(const TreeArgs& a, int R, hipStream_t s) {
-  if (R == 16)
-    launch_few<D, F16, 1>(a, s);
-  else if (R == 32)
-    launch_few<D, F16, 2>(a, s);
-  else {
-    IRON_LAUNCH((tree4_wide_kernel<D, F16>), dim3(a.workgroups), dim3(256), 0, s, a);
-    IRON_LAUNCH((tree_join_kernel<D, F16, 128, kWideBlock, true>), dim3(a.num_nodes, (a.H + 3) / 4), dim3(256), 0, s, a);
-  }
+void launch_rows(TreeArgs a, int R, hipStream_t s) {
+  if (R == 16) return launch_few<D, F16, 1>(a, s);
+  if (R == 32) return launch_few<D, F16, 2>(a, s);
+  a.workgroups = std::min(a.workgroups, wide_resident(D, F16));
+  IRON_LAUNCH((tree4_wide_kernel<D, F16>), dim3(a.workgroups), dim3(256), 0, s, a);
+  IRON_LAUNCH((tree_join_kernel<D, F16, 128, kWideBlock, true>), dim3(a.num_nodes, (a.H + 3) / 4), dim3(256), 0, s, a);
 }
 
 }  // namespace
