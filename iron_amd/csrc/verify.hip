@@ -55,7 +55,7 @@ struct VerifyArgs {
   RowStat* part;       // workspace (num_nodes [x 2], subs)
   RowStat* stat;       // workspace (num_nodes [x 2])
   double2* chance;     // workspace (num_nodes): p and q of the parent's row at the node's token
-  double2* ab;         // workspace (max_children, num_nodes): a_j, b_j
+  double2* ab;         // workspace (max_children, num_nodes): a_j, b_j; a_j below 0 where an earlier child is accepted
   double* mass;        // workspace (max_children, num_nodes, subs): parts of R_j
   Choice* choice;      // workspace (num_seqs)
   double* weight;      // workspace (num_seqs, subs): parts of the last sum(w)
@@ -398,6 +398,12 @@ __device__ __forceinline__ double mass_of(const VerifyArgs& a, int j, int n) {
   return wave_sum64(r);
 }
 
+// Whether a child is accepted: its number, its token's p and q, a_j and b_j, R_j.
+__device__ __forceinline__ bool passes(float u, double2 chance, double2 ab, double r) {
+#pragma clang fp contract(off)  // the same wherever it is asked
+  return u * chance.y < fmax(ab.x * chance.x - ab.y * chance.y, 0.) / r;
+}
+
 // The weight of a token of row n for a_j, b_j.
 struct Weigh {
   double ka, kb, rate;  // a / sum, b / sum of p's and q's exponentials
@@ -453,8 +459,20 @@ __device__ __forceinline__ void weights(const Weigh& w, bool rival, const float 
   w(p, q, rival, out);
 }
 
-// R_j's part of kSub places, for rows with more than j children (a wave). The
-// logits are on their way while the rest is looked up.
+// Child j of node i of a tree, -1 where it has fewer (a wave).
+__device__ __forceinline__ int child_of(const VerifyArgs& a, const Tree& t, int i, int j) {
+  for (int c0 = i + 1; c0 < t.nodes; c0 += 64) {
+    const int c = c0 + (threadIdx.x & 63);
+    unsigned long long kids = __ballot(c < t.nodes && a.parents[t.first + min(c, t.nodes - 1)] == i);
+    for (; kids && j; --j) kids &= kids - 1;
+    if (kids) return c0 + __ffsll(kids) - 1;
+  }
+  return -1;
+}
+
+// R_j's part of kSub places (a wave), for rows with more than j children of which the
+// first j are not accepted, wherever the walk may go: that a child is, the row's own
+// numbers say. The logits are on their way while the rest is looked up.
 template <typename T>
 __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs a, int j) {
   const int lane = threadIdx.x & 63, id = uniform(blockIdx.x * 4 + (threadIdx.x >> 6));
@@ -473,8 +491,11 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs a, int j) {
   }
   const double r = mass_of(a, j - 1, n);
   const double2 was = j == 1 ? make_double2(1., 0.) : a.ab[static_cast<long long>(j - 1) * a.num_nodes + n];
-  const double2 now = make_double2(was.x / r, was.y / r + 1.);
+  const int kid = t.first + child_of(a, t, n - t.first, j - 1);
+  const bool over = was.x < 0. || passes(a.accept[kid], a.chance[kid], was, r);
+  const double2 now = over ? make_double2(-1., 0.) : make_double2(was.x / r, was.y / r + 1.);
   if (sub == 0 && lane == 0) a.ab[static_cast<long long>(j) * a.num_nodes + n] = now;
+  if (over) return;
   const Weigh w = weigh(a, n, now.x, now.y, temp);
   const bool inside = rp.inside(sub * kSub, kSub);
   double sum = 0.;
@@ -534,7 +555,7 @@ __device__ Choice walk(const VerifyArgs& a, const Tree& t, float temp, bool writ
       } else {
         const double pc = lane64(chance.x, k), qc = lane64(chance.y, k), uk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, u), k));
         if (a.draft) {
-          yes = uk * qc < fmax(r.a * pc - r.b * qc, 0.) / left;
+          yes = passes(uk, make_double2(pc, qc), make_double2(r.a, r.b), left);
         } else {  // its token may have been tried before
           bool again = false;
           for (int e = 0; e < r.tried; ++e) again |= gone[e] == x;
