@@ -34,12 +34,23 @@ __device__ __forceinline__ Quarter<D> load_quarter(const unsigned char* rows, un
   return x;
 }
 
-// The largest of three numbers; the compiler's own makes quiet NaN of its operands first, at an instruction each.
+// The largest of three numbers; the compiler's own makes quiet NaN of its operands first,
+// at an instruction each. It does not see that this reads a product's result, which takes
+// 11 (16x16) or 19 (32x32) wait states: products go through settle() first.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
+
+template <int RT>
+__device__ __forceinline__ void settle(ta_f32x4 (&a)[2][RT]) {
+  if constexpr (RT == 1)
+    asm volatile("s_nop 10" : "+v"(a[0][0]), "+v"(a[1][0]));
+  else
+    asm volatile("s_nop 10" : "+v"(a[0][0]), "+v"(a[1][0]), "+v"(a[0][1]), "+v"(a[1][1]));
+}
+__device__ __forceinline__ void settle(ta_f32x16& a) { asm volatile("s_nop 15\n\ts_nop 2" : "+v"(a)); }
 
 // Eight values of a quarter (word kk) as the fp16 operand of a product.
 template <int D>
@@ -316,6 +327,7 @@ __global__ __launch_bounds__(256, few_resident(D, RT, F16) / 256) void tree4_ker
           }
         }
         asm volatile("" ::: "memory");
+        settle(sc);
         const bool some = valid[j] + valid[j + 1] < 32;  // keys that are none: no score, and values that cannot do harm
         if (some) {
 #pragma unroll
@@ -621,7 +633,8 @@ __global__ __launch_bounds__(256, wide_resident(D, F16) / 256) void tree4_wide_k
               ring + ((i % kRing * kStage + v_first) ^ (64 * db)) + 8 * q * kRow)));
         };
         // The row's maximum, when scores pass it by more than 8 (in the log2 domain; cf. tree4_kernel).
-        auto raise = [&](const ta_f32x16& sc) {
+        auto raise = [&](ta_f32x16& sc) {
+          settle(sc);
           float mx = max3(sc[0], sc[1], sc[2]);
 #pragma unroll
           for (int j = 3; j < 15; j += 2) mx = max3(mx, sc[j], sc[j + 1]);
