@@ -1,6 +1,17 @@
 // Attention of drafted trees over a paged KV cache of 4-bit rows (int4_rows.hpp):
 // tree_attention.hip's mathematics, tiles and shares of work; the cached keys and
 // values are b + s (16 + code), the tree's own are 16-bit rows.
+//
+// Roundings: in bf16 calls, cached keys, values and weights are rounded once to fp16,
+// an eighth of the result's own rounding each. In fp16 calls that would be 2.7 times
+// the result's own; there keys are not rounded (s in two parts, b by a product of
+// its own: S = K_high Q + K_low Q + b sum(q)) and weights go in two parts: 1.3 times.
+//
+// Measured (32 / 8 heads; a large copy moves 4.84 TB/s, a large library product does
+// 1.28-1.39 PFLOP/s): 64 sequences of 150-16384 positions, one token each, head_dim 64:
+// 48 us, the kernel 43 for 182 MB (with a 16-bit cache 94). One token behind 2047: 8.5 us
+// in a graph. 8 trees of 26 nodes behind 37-3968: 21 us. 2 trees of 64 nodes behind 20011
+// and 32768, head_dim 128, fp16: 143 us, 400 TFLOP/s of the mathematics' own products.
 #include "tree_common.hpp"
 
 namespace iron {
@@ -112,15 +123,17 @@ constexpr int wide_resident(int D, bool F16) { return D == 64 && !F16 ? 768 : 51
 
 // Few rows: a tile of 16 RT rows, a workgroup of 4 waves. Wave w has keys 16 w ..
 // + 15 of each block of 64 and all rows, so that nothing is shared until the end.
-// A lane has a quarter of a key's row, which it loads (kAhead blocks ahead, into
-// registers) and dequantizes itself. K's quarters are the A operand of S^T = K Q^T as
+// A lane has a quarter of a key's row, which it loads (a step ahead, into registers)
+// and dequantizes itself. K's quarters are the A operand of S^T = K Q^T as
 // they stand, with Q's dims in the same order; V's go through the wave's own LDS,
 // 16-bit rows in, V^T out by transposed reads. Two blocks make a step: the weights of
 // 2 x 4 keys, rounded to fp16, are the 8 elements of the B operand of O^T += V^T P^T.
+// Bound by memory, half of the waves' time waiting for it, at four waves to a SIMD: 2, 4,
+// 6 and 8 blocks ahead took 51, 55-61, 74 and 70 us for the batch above (registers, code).
 template <int D, bool F16, int RT>
 __global__ __launch_bounds__(256, few_resident(D, RT, F16) / 256) void tree4_kernel(TreeArgs a) {
   constexpr int R = 16 * RT, B = kBlock, kRow = kInt4Row<D>, kWide = D * 2;
-  constexpr int NK = D / 32, ND = D / 16, kAhead = 2;
+  constexpr int NK = D / 32, ND = D / 16;
   constexpr int kOwn = 32 * kWide > R * D * 4 ? 32 * kWide : R * D * 4;  // LDS of a wave: V of two blocks, at the end its output
   __shared__ __attribute__((aligned(16))) unsigned char lds[4 * kOwn];
   __shared__ float stat_m[4][R], stat_l[4][R];
@@ -174,27 +187,27 @@ __global__ __launch_bounds__(256, few_resident(D, RT, F16) / 256) void tree4_ker
         const bool real = static_cast<unsigned>(page) < static_cast<unsigned>(a.num_pages);
         return real && i < cached ? max(min(t.len - ((blk0 + i) * B + 16 * w), 16), 0) : 0;
       };
-      Quarter<D> kq[kAhead], vq[kAhead];
-      int valid[kAhead], page[2] = {0, 0};
-      auto issue = [&](int i, int j) {  // block i into place j
-        const long long at = rows_of(i, page[j & 1]);
-        valid[j] = valid_of(i, page[j & 1]);
-        kq[j] = load_quarter<D>(k_pages + at, at_codes, at_pair);
-        vq[j] = load_quarter<D>(v_pages + at, at_codes, at_pair);
+      // The two blocks of a step, loaded while the step before it is worked on; their
+      // pages are read a step earlier still.
+      Quarter<D> kq[2], vq[2];
+      int valid[2], page[2] = {0, 0};
+      auto read_pages = [&](int i) {
+        page[0] = page_of(i);
+        page[1] = page_of(i + 1);
+      };
+      auto issue = [&](int i) {  // blocks i and i + 1 (behind the last one: that one again, of which nothing counts)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const long long at = rows_of(i + j, page[j]);
+          valid[j] = valid_of(i + j, page[j]);
+          kq[j] = load_quarter<D>(k_pages + at, at_codes, at_pair);
+          vq[j] = load_quarter<D>(v_pages + at, at_codes, at_pair);
+        }
+        read_pages(i + 2);
       };
       if (cached > 0) {
-        int first[kAhead];
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) first[j] = page_of(j);
-        page[0] = page_of(kAhead);
-        page[1] = page_of(kAhead + 1);
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-          const int keep = page[j & 1];
-          page[j & 1] = first[j];
-          issue(j, j);
-          page[j & 1] = keep;
-        }
+        read_pages(0);
+        issue(0);
       }
       // Q: the B operand of S^T = K Q^T (column: row 16 rt + c; dims D / 4 quad + 8 kk .. + 8)
       ta_u32x4 qf[RT][NK];
@@ -298,51 +311,51 @@ __global__ __launch_bounds__(256, few_resident(D, RT, F16) / 256) void tree4_ker
           cs[rt] *= 2.f;
         }
       }
-      auto step = [&](int j) {  // the blocks in places j and j + 1
-        if (valid[j] + valid[j + 1] == 0) return;
+      auto step = [&] {
+        if (valid[0] + valid[1] == 0) return;
         ta_f32x4 sc[2][RT];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
 #pragma unroll
-          for (int kk = 0; kk < NK; ++kk) put_v(b, kk, unpack<D>(vq[j + b], kk));
+          for (int kk = 0; kk < NK; ++kk) put_v(b, kk, unpack<D>(vq[b], kk));
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) sc[b][rt] = ta_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int kk = 0; kk < NK; ++kk) {
             if constexpr (F16) {
               ta_u32x4 high, low;
-              unpack<D>(kq[j + b], kk, high, low);
+              unpack<D>(kq[b], kk, high, low);
 #pragma unroll
               for (int rt = 0; rt < RT; ++rt) sc[b][rt] = mfma<true>(low, qf[rt][kk], mfma<true>(high, qf[rt][kk], sc[b][rt]));
             } else {
-              const ta_u32x4 kf = unpack<D>(kq[j + b], kk);
+              const ta_u32x4 kf = unpack<D>(kq[b], kk);
 #pragma unroll
               for (int rt = 0; rt < RT; ++rt) sc[b][rt] = mfma<true>(kf, qf[rt][kk], sc[b][rt]);
             }
           }
           if constexpr (F16) {  // b, twice, times the two parts of the sum of the quarter's dims
-            const unsigned bb = __builtin_bit_cast(unsigned, int4_base(kq[j + b].pair));
+            const unsigned bb = __builtin_bit_cast(unsigned, int4_base(kq[b].pair));
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) sc[b][rt] = mfma<true>(ta_u32x4{bb, 0, 0, 0}, ta_u32x4{q_half[rt], 0, 0, 0}, sc[b][rt]);
           }
         }
         asm volatile("" ::: "memory");
         settle(sc);
-        const bool some = valid[j] + valid[j + 1] < 32;  // keys that are none: no score, and values that cannot do harm
+        const bool some = valid[0] + valid[1] < 32;  // keys that are none: no score, and values that cannot do harm
         if (some) {
 #pragma unroll
           for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
-              for (int rt = 0; rt < RT; ++rt) sc[b][rt][e] = 4 * quad + e < valid[j + b] ? sc[b][rt][e] : -INFINITY;
+              for (int rt = 0; rt < RT; ++rt) sc[b][rt][e] = 4 * quad + e < valid[b] ? sc[b][rt][e] : -INFINITY;
         }
         ta_u32x2 vt[2][ND];
         auto get = [&](int b) {
 #pragma unroll
           for (int dt = 0; dt < ND; ++dt) vt[b][dt] = get_v(b, dt);
           if (some) {
-            const unsigned m01 = keep01(valid[j + b]), m23 = keep23(valid[j + b]);
+            const unsigned m01 = keep01(valid[b]), m23 = keep23(valid[b]);
 #pragma unroll
             for (int dt = 0; dt < ND; ++dt) {
               vt[b][dt].x &= m01;
@@ -393,15 +406,9 @@ __global__ __launch_bounds__(256, few_resident(D, RT, F16) / 256) void tree4_ker
         }
         asm volatile("" ::: "memory");
       };
-      for (int i = 0; i < cached; i += kAhead) {
-#pragma unroll
-        for (int j = 0; j < kAhead; j += 2) {
-          step(j);
-          issue(i + j + kAhead, j);
-          issue(i + j + 1 + kAhead, j + 1);
-          page[0] = page_of(i + j + 2 + kAhead);
-          page[1] = page_of(i + j + 3 + kAhead);
-        }
+      for (int i = 0; i < cached; i += 2) {
+        step();
+        issue(i + 2);
       }
 
       // The four waves' parts of the tile meet in LDS.

@@ -254,7 +254,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // One part of a row of target or draft logits, by a wave: its maximum and its sum.
-// Bound by the fp64 instructions (30.7 M logits, 8 trees of 26 nodes: 34 us, 24 of
+// Bound by the fp64 instructions (30.7 M logits, 8 trees of 26 nodes: 36 us, 24 of
 // them these alone).
 template <typename T>
 __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs a) {

@@ -8,10 +8,12 @@ uint8 (num_pages, Hkv, page_size, D / 2 + 16), rows as PagedAppendInt4 writes th
 v_new have 16 bits. With D 64 a position takes 48 bytes instead of 128, with D 128
 80 instead of 256.
 
-A cached value b + s (16 + code) enters the products rounded once to fp16, in both
-types; so do the weights of cached positions (kept to 2^-30 of a row's largest).
-Tree rows have bf16 or fp16 weights: two parts of 16 bits, or, where a KV head has
-more than 32 rows (max_nodes times H / Hkv), one. Kernel: iron_tree_attention_int4.
+bf16 calls round cached keys, values and the weights of cached positions once to fp16,
+an eighth of the result's own rounding each (weights are kept to 2^-30 of a row's
+largest). fp16 calls take cached keys without rounding, values rounded once, and
+weights in two parts. Weights of the tree's rows are two parts of dtype, or, where a
+KV head has more than 32 rows (max_nodes times H / Hkv), one. Kernel:
+iron_tree_attention_int4.
 """
 
 from dataclasses import dataclass
