@@ -6,7 +6,8 @@ Requests, pages, lengths and status are PagedAppend's; k_pages and v_pages are
 uint8 (num_layers, num_pages, Hkv, page_size, D / 2 + 16). Each quarter of a row
 (D / 4 values from lo to hi) keeps s = fp16((hi - lo) / 15), b = fp16(lo - 16 s)
 and for each value the nearest of the 16 codes, of two equally near ones the upper:
-a cached value b + s (16 + code) is off by s / 2 and the rounding of b at most.
+a cached value b + s (16 + code) is off by s / 2, what rounding s takes off 15 s, and
+the rounding of b at most.
 Values are cut to +-20480 first; a NaN makes its quarter NaN. D 64 or 128,
 bf16 or fp16 (``dtype``: of k_new and v_new). Kernel: iron_paged_append_int4.
 """
