@@ -567,6 +567,7 @@ __device__ Choice walk(const VerifyArgs& a, const Tree& t, float temp, bool writ
         reach(i0 + k, __builtin_amdgcn_readlane(likeliest, k));
       } else {
         if (lane == 0) gone[r.tried] = x;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // other lanes read it
         __builtin_amdgcn_wave_barrier();
         r.tried += 1;
         if (a.draft && !top) {
