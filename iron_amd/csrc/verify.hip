@@ -246,7 +246,7 @@ struct Exp2 {
   }
 };
 
-// The larger of three numbers; the compiler's own makes quiet NaN of its operands first, at an instruction each.
+// The largest of three numbers, none of them NaN; the compiler's own makes quiet NaN of its operands first, at an instruction each.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
@@ -293,18 +293,6 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs a) {
       for (int e = 0; e < kVec<T>; ++e) m = fmaxf(m, x[i][e] = logit(x[i][e]));
     m = wave_max(m);
   };
-  auto sum = [&] {
-    double z = 0.;
-    if (m != -INFINITY)
-#pragma unroll
-      for (int i = 0; i < kVecs<T>; ++i) {
-        double y[kVec<T>];
-        boost(x[i], m, rate, y);
-#pragma unroll
-        for (int e = 0; e < kVec<T>; ++e) z += y[e];
-      }
-    return wave_sum64(z);
-  };
   double z = 0.;
   int best = INT_MAX;
   if (top) {
@@ -315,16 +303,26 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs a) {
       for (int e = kVec<T> - 1; e >= 0; --e) best = x[i][e] == m ? place<T>(sub, i) + e - r.shift : best;
     for (int d = 32; d; d >>= 1) best = min(best, __shfl_xor(best, d, 64));
   } else {
+    // A signalling NaN would make v_max3 forget what came before it, so NaN are looked for on their own.
+    bool nan = false;
 #pragma unroll
     for (int i = 0; i < kVecs<T>; ++i)
 #pragma unroll
-      for (int e = 0; e < kVec<T>; e += 2) m = max3(m, x[i][e], x[i][e + 1]);
+      for (int e = 0; e < kVec<T>; e += 2) {
+        nan |= __builtin_isunordered(x[i][e], x[i][e + 1]);
+        m = max3(m, x[i][e], x[i][e + 1]);
+      }
     m = wave_max(m);
-    z = m < INFINITY ? sum() : NAN;
-    if (!(z >= 0.)) {  // a NaN among them shows in the sum
-      clean();
-      z = sum();
-    }
+    if (__ballot(nan) || m == INFINITY) clean();
+    if (m != -INFINITY)
+#pragma unroll
+      for (int i = 0; i < kVecs<T>; ++i) {
+        double y[kVec<T>];
+        boost(x[i], m, rate, y);
+#pragma unroll
+        for (int e = 0; e < kVec<T>; ++e) z += y[e];
+      }
+    z = wave_sum64(z);
   }
   if (lane == 0) a.part[static_cast<long long>(row) * a.subs + sub] = {z, m, best};
 }

@@ -236,3 +236,29 @@ def test_streams_and_graphs(gpu):
             assert call(gpu, b, 9, 3, fn) == expect(b, 3)
             torch.cuda.synchronize()
             assert [o.tolist() for o in out] == expect(c, 3)
+
+
+@pytest.mark.parametrize("dtype,bits", [(torch.bfloat16, 0x7f81), (torch.float16, 0x7c01), (torch.float32, 0x7f800001)])
+@pytest.mark.parametrize("draft", [True, False])
+def test_signalling_nan(gpu, dtype, bits, draft):
+    """NaN whose quiet bit is not set count as -inf too, wherever they stand: beside the largest logit, among many, in a
+    row (or a part of one) without anything else."""
+    whole = torch.int32 if dtype == torch.float32 else torch.int16
+    for seed in range(4):
+        c = make(3000, [4, 3, 5, 1, 2], 2, dtype, draft, seed=30 + seed)
+        c["temps"] = torch.tensor([1.0, 0.03, 0.0, 0.03, 0.5])
+        g = torch.Generator().manual_seed(seed)
+        for name, shift in (("logits", 0), ("draft", 5)):
+            if c[name] is None:
+                continue
+            raw = c[name].view(whole)
+            for n in range(len(raw)):
+                top = (int(c["logits"][n].float().nan_to_num(-1e30).argmax()) + shift) % 3000
+                raw[n, torch.randint(0, 3000, (60,), generator=g)] = bits
+                raw[n, [i for i in range(top // 8 * 8, min(top // 8 * 8 + 8, 3000)) if i > top]] = bits
+                c[name][n, top] = 60.0  # far above the others at the smaller temperatures
+        last = len(c["logits"]) - 2
+        c["logits"][last - 1, 1:] = -math.inf  # one token, then nothing, in a part of the row
+        c["logits"].view(whole)[last - 1, [1, 3, 1024, 2500]] = bits
+        c["logits"].view(whole)[last] = bits  # nothing at all
+        assert call(gpu, c, 5, 2) == expect(c, 2)
