@@ -480,7 +480,7 @@ int iron_paged_gather_int4(const int* begins, const int* row_starts, const void*
  * is drawn from p. draft_logits of nodes without children are not read. Computed in
  * 64 bits. dtype 0: bf16, 1: fp16, 2: fp32 logits. vocab at most 2^20, num_nodes 2^20 and
  * below 2^23 / ceil((vocab + 7) / 4096), max_nodes 1024, max_children 64. node_starts must not decrease; trees are cut to max_nodes nodes and
- * to num_nodes rows. In the place of the sampling of
+ * to num_nodes rows. rows, row_starts and next_tokens overlap no other buffer of the call. In the place of the sampling of
  * iron/applications/llama_3.2_1b/llama_inference_harness.py:146-169. */
 long long iron_draft_verify_workspace_bytes(int vocab, int num_seqs, int num_nodes, int max_nodes, int max_children,
                                             int draft);

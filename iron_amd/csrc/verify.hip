@@ -839,6 +839,20 @@ extern "C" int iron_draft_verify(const void* logits, const void* draft_logits, c
   const long long need = iron_draft_verify_workspace_bytes(vocab, num_seqs, num_nodes, max_nodes, max_children, draft_logits != nullptr);
   IRON_REQUIRE(workspace && aligned16(workspace), "%s: the workspace must be given and 16-byte aligned", who);
   IRON_REQUIRE(workspace_bytes >= need, "%s: workspace of %lld bytes, %lld needed", who, workspace_bytes, need);
+  // The last launch reads while it writes the results, so these and the workspace lie apart from all else.
+  const long long elements = static_cast<long long>(num_nodes) * vocab * (dtype == 2 ? 4 : 2);
+  const struct {
+    const void* at;
+    long long bytes;
+  } spans[] = {{rows, 4LL * num_nodes}, {row_starts, 4LL * (num_seqs + 1)}, {next_tokens, 4LL * num_seqs}, {workspace, need},
+               {logits, elements}, {draft_logits, draft_logits ? elements : 0}, {tokens, 4LL * num_nodes}, {parents, 4LL * num_nodes},
+               {node_starts, 4LL * (num_seqs + 1)}, {temperatures, 4LL * num_seqs}, {accept_draws, 4LL * num_nodes}, {sample_draws, 4LL * num_seqs}};
+  for (int i = 0; i < 4; ++i)
+    for (int j = i + 1; j < 12; ++j) {
+      const uintptr_t x = reinterpret_cast<uintptr_t>(spans[i].at), y = reinterpret_cast<uintptr_t>(spans[j].at);
+      IRON_REQUIRE(x + spans[i].bytes <= y || y + spans[j].bytes <= x || !spans[j].bytes,
+                   "%s: rows, row_starts, next_tokens and the workspace must not overlap each other or an input", who);
+    }
   VerifyArgs a = {};
   a.logits = logits;
   a.draft = draft_logits;

@@ -29,7 +29,8 @@ node_starts (num_seqs + 1,) int32, temperatures (num_seqs,), accept_draws
 (num_nodes,), sample_draws (num_seqs,) fp32, uniform in [0, 1); out: rows
 (num_nodes,) int32, the accepted rows of all sequences from the first on, then -1;
 row_starts (num_seqs + 1,), where each sequence's begin; next_tokens (num_seqs,).
-bf16, fp16 or fp32 logits (``dtype``). Kernel: iron_draft_verify.
+bf16, fp16 or fp32 logits (``dtype``). The results are buffers of their own: one that
+overlaps another argument is refused. Kernel: iron_draft_verify.
 """
 
 from dataclasses import dataclass, field

@@ -154,3 +154,23 @@ def test_the_reference_rounds_to_the_nearest():
         bound = s.double() / 2 + 15 * s.double() * 2.0 ** -11 + (lo - 16 * s.double()).abs() * 2.0 ** -11 + 2.0 ** -24
         assert bool(((got.reshape(each.shape) - each).abs() <= bound[..., None]).all())
         assert bool((got[5] == 1.5).all())
+
+
+# bytes of each buffer of a call of 6 nodes and 100 bf16 logits
+SIZES = dict(logits=1200, draft_logits=1200, tokens=24, parents=24, node_starts=12, temperatures=8, accept_draws=24, sample_draws=8, rows=24, row_starts=12,
+             next_tokens=8, workspace=0)
+PLACES = {name: (1 + i) << 24 for i, name in enumerate(SIZES)}
+
+
+@pytest.mark.parametrize("other", list(SIZES))
+@pytest.mark.parametrize("out", ["rows", "row_starts", "next_tokens", "workspace"])
+def test_verify_refuses_results_over_other_buffers(out, other):
+    """The last launch reads trees, numbers, logits and the workspace while other workgroups of it write the results."""
+    sizes = {**SIZES, "workspace": _lib.query("iron_draft_verify_workspace_bytes", 100, 2, 6, 5, 2, 1)}
+    first, last = PLACES[other], PLACES[other] + (sizes[other] - 4) // 16 * 16
+    before = first - (sizes[out] - 4) // 16 * 16  # its last bytes lie there
+    for at in {first, last, before}:
+        if out != other:
+            where = {**PLACES, out: at}
+            with pytest.raises(_lib.IronHipError, match="overlap"):
+                _lib.call("iron_draft_verify", *[where[k] for k in SIZES if k != "workspace"], 0, 100, 2, 6, 5, 2, where["workspace"], sizes["workspace"], None)
