@@ -546,6 +546,13 @@ __device__ Choice walk(const VerifyArgs& a, const Tree& t, float temp, bool writ
       const int k = __ffsll(kids) - 1;
       from = i0 + k + 1;
       if (r.tried >= a.max_children) continue;
+      if (a.draft && !top && r.tried) {  // summed, as the node has more children than were tried
+        left = mass_of(a, r.tried, t.first + at);
+        if (left == 0.) {  // nothing is left to accept
+          r.tried = a.max_children;
+          continue;
+        }
+      }
       const int x = __builtin_amdgcn_readlane(token, k);
       bool yes;
       if (top) {
@@ -571,8 +578,6 @@ __device__ Choice walk(const VerifyArgs& a, const Tree& t, float temp, bool writ
         if (a.draft && !top) {
           r.a /= left;
           r.b = r.b / left + 1.;
-          left = r.tried < a.max_children ? mass_of(a, r.tried, t.first + at) : 1.;
-          if (left == 0.) r.tried = a.max_children;  // nothing is left to accept
         }
       }
     }

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import iron_amd.operators as ops
+from iron_amd import _lib
 from tests import int4_reference as ref
 
 pytestmark = pytest.mark.gpu
@@ -262,3 +263,21 @@ def test_signalling_nan(gpu, dtype, bits, draft):
         c["logits"].view(whole)[last - 1, [1, 3, 1024, 2500]] = bits
         c["logits"].view(whole)[last] = bits  # nothing at all
         assert call(gpu, c, 5, 2) == expect(c, 2)
+
+
+@pytest.mark.parametrize("draft", [True, False])
+@pytest.mark.parametrize("fill", [0x00, 0xff, 0x3f, 0x80])
+def test_what_the_workspace_held_does_not_matter(gpu, draft, fill):
+    """The entry point on a workspace full of zeros, NaN, ordinary and negative numbers: nothing is read that the call has
+    not written. The last nodes of the walk have no, one and more untried children, within and past max_children."""
+    for seed in range(4):
+        c = make(700, [9, 1, 12, 0, 70], 4, torch.float32, draft, greedy=0.2, seed=60 + seed, spare=2)
+        N, V = c["logits"].shape
+        for most in (1, 3, 4):
+            args = [c[k].to(gpu) if c[k] is not None else None for k in ("logits", "draft", "tokens", "parents", "starts", "temps", "accept", "sample")]
+            out = [torch.full((n,), 77, dtype=torch.int32, device=gpu) for n in (N, 6, 5)]
+            need = _lib.query("iron_draft_verify_workspace_bytes", V, 5, N, 70, most, int(draft))
+            ws = torch.full((need,), fill, dtype=torch.uint8, device=gpu)
+            _lib.call("iron_draft_verify", *[_lib.ptr(t) for t in args + out], 2, V, 5, N, 70, most, ws.data_ptr(), need,
+                      torch.cuda.current_stream().cuda_stream)
+            assert [o.tolist() for o in out] == expect(c, most)
