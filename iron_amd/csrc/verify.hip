@@ -55,8 +55,8 @@ struct VerifyArgs {
   RowStat* part;       // workspace (num_nodes [x 2], subs)
   RowStat* stat;       // workspace (num_nodes [x 2])
   double2* chance;     // workspace (num_nodes): p and q of the parent's row at the node's token
-  double2* ab;         // workspace (max_children, num_nodes): a_j, b_j; a_j below 0 where an earlier child is accepted
-  double* mass;        // workspace (max_children, num_nodes, subs): parts of R_j
+  double2* ab;         // workspace (max_children - 1, num_nodes): a_j, b_j from j = 1 on; a_j below 0 where an earlier child is accepted
+  double* mass;        // workspace (max_children - 1, num_nodes, subs): parts of R_j from j = 1 on
   Choice* choice;      // workspace (num_seqs)
   double* weight;      // workspace (num_seqs, subs): parts of the last sum(w)
   int* path;           // workspace (num_nodes): accepted rows, from each tree's first row on
@@ -391,7 +391,7 @@ __global__ __launch_bounds__(256) void verify_merge_kernel(VerifyArgs a) {
 __device__ __forceinline__ double mass_of(const VerifyArgs& a, int j, int n) {
   if (j == 0) return 1.;
   double r = 0.;
-  const double* part = a.mass + (static_cast<long long>(j) * a.num_nodes + n) * a.subs;
+  const double* part = a.mass + (static_cast<long long>(j - 1) * a.num_nodes + n) * a.subs;
   for (int c = threadIdx.x & 63; c < a.subs; c += 64) r += part[c];
   return wave_sum64(r);
 }
@@ -488,11 +488,11 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs a, int j) {
     vq[i] = rq.template fetch<kVec<T>>(place<T>(sub, i));
   }
   const double r = mass_of(a, j - 1, n);
-  const double2 was = j == 1 ? make_double2(1., 0.) : a.ab[static_cast<long long>(j - 1) * a.num_nodes + n];
+  const double2 was = j == 1 ? make_double2(1., 0.) : a.ab[static_cast<long long>(j - 2) * a.num_nodes + n];
   const int kid = t.first + child_of(a, t, n - t.first, j - 1);
   const bool over = was.x < 0. || passes(a.accept[kid], a.chance[kid], was, r);
   const double2 now = over ? make_double2(-1., 0.) : make_double2(was.x / r, was.y / r + 1.);
-  if (sub == 0 && lane == 0) a.ab[static_cast<long long>(j) * a.num_nodes + n] = now;
+  if (sub == 0 && lane == 0) a.ab[static_cast<long long>(j - 1) * a.num_nodes + n] = now;
   if (over) return;
   const Weigh w = weigh(a, n, now.x, now.y, temp);
   const bool inside = rp.inside(sub * kSub, kSub);
@@ -508,7 +508,7 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs a, int j) {
     for (int e = 0; e < kVec<T>; ++e) sum += x[e];
   }
   sum = wave_sum64(sum);
-  if (lane == 0) a.mass[(static_cast<long long>(j) * a.num_nodes + n) * a.subs + sub] = sum;
+  if (lane == 0) a.mass[(static_cast<long long>(j - 1) * a.num_nodes + n) * a.subs + sub] = sum;
 }
 
 // Down a tree: which rows are accepted, and what the next token is drawn from (one
@@ -793,7 +793,7 @@ long long lay_out(VerifyArgs& a, bool draft, char* base) {
   take(a.weight, static_cast<long long>(a.num_seqs) * a.subs);
   take(a.path, a.num_nodes);
   take(a.tried, static_cast<long long>(a.num_seqs) * a.max_children);
-  const long long sums = draft && a.max_children > 1 ? static_cast<long long>(a.max_children) * a.num_nodes : 0;
+  const long long sums = draft ? static_cast<long long>(a.max_children - 1) * a.num_nodes : 0;
   take(a.ab, sums);
   take(a.mass, sums * a.subs);
   return at;

@@ -174,3 +174,13 @@ def test_verify_refuses_results_over_other_buffers(out, other):
             where = {**PLACES, out: at}
             with pytest.raises(_lib.IronHipError, match="overlap"):
                 _lib.call("iron_draft_verify", *[where[k] for k in SIZES if k != "workspace"], 0, 100, 2, 6, 5, 2, where["workspace"], sizes["workspace"], None)
+
+
+@pytest.mark.parametrize("vocab,nodes", [(100, 6), (128256, 208)])
+def test_verify_workspace_holds_sums_behind_the_first_child_only(vocab, nodes):
+    """What is left after j children, j = 1 .. max_children - 1: two numbers to a row and a sum to each 1024 tokens of it."""
+    subs = (vocab + 7 + 4095) // 4096 * 4
+    sizes = [_lib.query("iron_draft_verify_workspace_bytes", vocab, 2, nodes, 5, k, 1) - 2 * k * 4 // 16 * 16 for k in (2, 4, 6)]
+    assert sizes[1] - sizes[0] == sizes[2] - sizes[1] == 2 * nodes * (16 + 8 * subs)
+    two, one = (_lib.query("iron_draft_verify_workspace_bytes", vocab, 2, nodes, 5, k, 1) for k in (2, 1))
+    assert two - one == nodes * (16 + 8 * subs)
