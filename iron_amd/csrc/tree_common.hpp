@@ -44,12 +44,6 @@ __device__ __forceinline__ uint16_t narrow(float x) {
   return f32_to_bf16(x);
 }
 
-// The tree of sequence s: its first row and its nodes, cut to the arrays.
-__device__ __forceinline__ void tree_of(const TreeArgs& a, int s, int& first, int& nodes) {
-  first = min(max(a.starts[s], 0), a.num_nodes);
-  nodes = min(min(max(a.starts[s + 1], first), a.num_nodes) - first, a.max_nodes);
-}
-
 typedef __bf16 ta_bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 ta_f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 ta_f16x2 __attribute__((ext_vector_type(2)));
