@@ -54,3 +54,41 @@ def test_few_rows_spill_nothing():
     sizes = re.findall(r"\.amdhsa_kernel (\S+)\n(?:(?!\.end_amdhsa_kernel).*\n)*?\s*\.amdhsa_private_segment_fixed_size (\d+)", asm)
     few = [int(n) for name, n in sizes if "tree4_kernel" in name]
     assert len(few) == 8 and not any(few)
+
+
+def scratch_by_kernel(asm):
+    return {name: int(n) for name, n in re.findall(r"\.amdhsa_kernel (\S+)\n(?:(?!\.end_amdhsa_kernel).*\n)*?\s*\.amdhsa_private_segment_fixed_size (\d+)", asm)}
+
+
+def scratch_depths(asm, kernel):
+    """How deep in loops each scratch access of a kernel lies, by what the compiler writes beside its blocks."""
+    body = asm[asm.index(f"\n{kernel}:"):]
+    depth, fresh, found = 0, False, []
+    for line in body[:body.index(".Lfunc_end")].splitlines():
+        if re.match(r"\.LBB|; %bb\.", line):
+            depth, fresh = 0, True
+        elif line.strip() and not line.strip().startswith(";"):
+            fresh = False
+        if fresh:
+            depth = max([depth, *map(int, re.findall(r"Depth=(\d+)", line))])
+        if line.strip().startswith("scratch_"):
+            found.append(depth)
+    return found
+
+
+def test_scratch_depths_are_found():
+    asm = "\nk:\n\tscratch_store_dword off, v3, off\n.LBB0_1: ; =>This Loop Header: Depth=1\n\tscratch_load_dword v3, off, off\n" \
+          ".LBB0_2: ;   Parent Loop BB0_1 Depth=1\n                                        ; =>  This Inner Loop Header: Depth=2\n\tscratch_load_dword v3, off, off\n" \
+          "; %bb.3: ;   in Loop: Header=BB0_1 Depth=1\n\tscratch_load_dword v3, off, off\n.Lfunc_end0:\n"
+    assert scratch_depths(asm, "k") == [0, 1, 2, 1]
+
+
+def test_many_rows_and_joins_spill_nothing_but_one_address():
+    """The kernel of many rows with fp16 and head_dim 128 has all 256 registers in use: one address is put away at its start and
+    fetched once a part (depth 1: the loop over parts), never in the loop over blocks. No other kernel spills."""
+    asm = contracts.device_asm(SOURCE)
+    sizes = scratch_by_kernel(asm)
+    full = [name for name in sizes if "tree4_wide_kernelILi128ELb1" in name]
+    assert len(full) == 1 and len(sizes) == 24
+    assert not [name for name, n in sizes.items() if n and name not in full]
+    assert sizes[full[0]] <= 8 and scratch_depths(asm, full[0]) in ([], [0, 1])
