@@ -30,6 +30,8 @@ def sequences(c):
     G = q.shape[1] // Hkv
     for s, n in enumerate(c["lens"]):
         a, b = c["starts"][s], c["starts"][s + 1]
+        if a == b:
+            continue
         t = torch.arange(n, device=q.device)
         page = c["table"][s].to(q.device).long()[t // ps]
         seen = torch.cat([torch.ones(b - a, n, dtype=torch.bool, device=q.device), c["sees"][a:b, :b - a].to(q.device)], 1)

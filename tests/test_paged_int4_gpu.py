@@ -321,3 +321,70 @@ def test_serving_steps(gpu, D, dtype):
         assert margin > 1e-12 and [rows.tolist(), row_starts.tolist(), nexts.tolist()] == [r, rs, nx]
         assert append_want(want, x[1], x[2], r, rs) == status.tolist() and all(want.same(dev))
     assert want.lens.sum() >= 4 * S + 101
+
+
+@pytest.mark.parametrize("dispatch", ["fused", "separate"])
+def test_in_an_operator_sequence(gpu, dispatch):
+    """Attention, verification, append and reading back as one runlist, called three times: the cache that a call leaves is
+    the next one's."""
+    from iron_amd.common import OperatorSequence
+
+    D, H, Hkv, ps, S, P, MP, V, N = 64, 4, 2, 16, 2, 12, 4, 50, 5
+    g = torch.Generator().manual_seed(31)
+    c = sane(cache_of(1, P, Hkv, ps, D, S, MP), D)
+    c.hold(0, 30, [7, 2])
+    c.hold(1, 5, [9])
+    starts, parents, begins = [0, 3, 5], [-1, 0, 1, -1, 0], [20, 0]
+    pool = dict(num_kv_heads=Hkv, head_dim=D, num_pages=P, page_size=ps, num_seqs=S, max_pages=MP)
+    attend = ops.TreeAttentionInt4(num_heads=H, num_nodes=N, max_nodes=3, **pool)
+    check = ops.DraftVerify(vocab=V, num_seqs=S, num_nodes=N, max_nodes=3, dtype=torch.float32)
+    put = ops.PagedAppendInt4(num_layers=1, num_nodes=N, num_rows=N, **pool)
+    read = ops.PagedGatherInt4(num_layers=1, num_rows=12, **pool)
+    cache = ("k_pages", "v_pages", "table", "lens")
+    numbers = ("tokens", "parents", "starts", "temps", "accept", "sample")
+    seq = OperatorSequence(name="int4_step", dispatch=dispatch,
+                           runlist=[(attend, "q", "k", "v", *cache, "starts", "mask", "out"),
+                                    (check, "logits", "draft", *numbers, "rows", "row_starts", "next"),
+                                    (put, "k", "v", "rows", "row_starts", *cache, "refs", "status"),
+                                    (read, "begins", "ranges", *cache, "k_out", "v_out")],
+                           input_args=["q", "k", "v", "mask", "logits", "draft", *numbers, "begins", "ranges", *cache, "refs"],
+                           output_args=["out", "rows", "row_starts", "next", "status", "k_out", "v_out"]).compile()
+    fn = seq.get_callable()
+    x = [torch.randn(N, n, D, generator=g).to(torch.bfloat16) for n in (H, Hkv, Hkv)]
+    sees = torch.tensor([[1, 0, 0], [1, 1, 0], [1, 1, 1], [1, 0, 0], [1, 1, 0]], dtype=torch.bool)
+    i32 = lambda v: torch.as_tensor(np.asarray(v), dtype=torch.int32)
+    step = dict(logits=torch.randn(N, V, generator=g), draft=torch.randn(N, V, generator=g), tokens=i32([0, 3, 5, 0, 9]), parents=i32(parents),
+                starts=i32(starts), temps=torch.tensor([0.8, 1.1]), accept=torch.rand(N, generator=g) * 0.1, sample=torch.rand(S, generator=g))
+    ranges = [0, 8, 12]
+    for name, value in dict(q=x[0], k=x[1], v=x[2], mask=attend.pack_mask(sees), begins=i32(begins), ranges=i32(ranges),
+                            k_pages=c.k, v_pages=c.v, table=i32(c.table), lens=i32(c.lens), refs=i32(c.refs), **step).items():
+        fn.get_buffer(name).torch_view(torch.uint8).copy_(value.contiguous().view(-1).view(torch.uint8))
+    want = c.copy()
+    rows, row_starts, nexts, margin = ref.verify(step["logits"], step["draft"], step["tokens"], parents, starts, step["temps"], step["accept"], step["sample"], 1)
+    assert margin > 1e-12 and max(row_starts) > 2
+    got = lambda name, dtype: fn.get_buffer(name).torch_view(dtype).cpu()
+    for _ in range(3):
+        fn()
+        torch.cuda.synchronize()
+        o, tol = ref.attention(*x, want.k[0], want.v[0], torch.from_numpy(want.table), want.lens.tolist(), starts, sees, 1 / math.sqrt(D), torch.zeros(N, H, D, dtype=torch.bfloat16), 3)
+        assert bool(((got("out", torch.bfloat16).view(N, H, D).double() - o).abs() <= tol).all())
+        assert [got(n, torch.int32).tolist() for n in ("rows", "row_starts", "next")] == [rows, row_starts, nexts]
+        assert append_want(want, x[1][None], x[2][None], rows, row_starts) == got("status", torch.int32).tolist()
+        zero = [torch.zeros(1, 12, Hkv, D, dtype=torch.bfloat16) for _ in range(2)]
+        for name, w in zip(("k_out", "v_out"), ref.gather(want.k, want.v, want.table, want.lens, begins, ranges, *zero, D)):
+            assert torch.equal(got(name, torch.bfloat16).view(w.shape), w)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype,bits", [(torch.bfloat16, 0x7f81), (torch.float16, 0x7c01)])
+def test_append_signalling_nan(gpu, D, dtype, bits):
+    """NaN whose quiet bit is not set make their quarter NaN too, and no other, at any place of it."""
+    k = torch.randn(1, D, 1, D, generator=torch.Generator().manual_seed(7)).to(dtype)
+    v = k.flip(3).contiguous()
+    for i in range(D):
+        k.view(torch.int16)[0, i, 0, i] = v.view(torch.int16)[0, i, 0, (7 * i) % D] = bits
+    c = cache_of(1, 9, 1, 16, D, 1, 8)
+    want = c.copy()
+    append_want(want, k, v, list(range(D)), [0, D])
+    dev, status = do_append(gpu, c, D, k, v, list(range(D)), [0, D])
+    assert status == [0] and all(want.same(dev))
