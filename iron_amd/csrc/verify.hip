@@ -4,10 +4,12 @@
 // node, with w_0 = p and R_0 = 1, its child j (in row order, token x, number u) is
 // accepted if u q(x) < w_j(x) / R_j; else w_{j+1} = max(w_j / R_j - q, 0) and
 // R_{j+1} is its sum. Where none is, the next token is drawn from w: the first x
-// whose cumulative sum passes r sum(w). Unrolled, w_j = max(a_j p - b_j q, 0) with
-// a_{j+1} = a_j / R_j and b_{j+1} = b_j / R_j + 1, so that a node's state is two
-// numbers and a sum over the vocabulary. Without draft logits q is 1 at the child's
-// token: w is p without the tokens tried, and no sums are needed on the way.
+// whose cumulative sum passes r sum(w). A node's state is the numbers 1 / R_i; every
+// token's w is taken through them step by step, two instructions each. (Unrolled it is
+// max(a p - b q, 0) with two numbers, but where little is left, a and b are large and
+// all of it cancels: rows with nearly all of their probability at one token came out wrong.)
+// Without draft logits q is 1 at the child's token: w is p without the tokens tried,
+// and no sums are needed on the way.
 //
 // Everything is in 64 bits: a vocabulary of 2^17 tokens of like probability puts
 // the borders of the cumulative sum 2^-17 apart, where sums of fp32 exponentials
@@ -33,11 +35,10 @@ struct RowStat {  // of a row, or of a part of it
 };
 
 struct Choice {  // what a sequence came to
-  double a, b;   // weights max(a p - b q, 0)
-  int node;      // the row whose distribution the next token is drawn from, -1 for an empty tree
-  int count;     // accepted rows
-  int tried;     // children that were not accepted there
-  int pad;
+  int node;   // the row whose distribution the next token is drawn from, -1 for an empty tree
+  int count;  // accepted rows
+  int tried;  // children that were not accepted there
+  int steps;  // with draft logits: how many of them were taken off p
 };
 
 struct VerifyArgs {
@@ -55,12 +56,13 @@ struct VerifyArgs {
   RowStat* part;       // workspace (num_nodes [x 2], subs)
   RowStat* stat;       // workspace (num_nodes [x 2])
   double2* chance;     // workspace (num_nodes): p and q of the parent's row at the node's token
-  double2* ab;         // workspace (max_children - 1, num_nodes): a_j, b_j from j = 1 on; a_j below 0 where an earlier child is accepted
+  double* scale;       // workspace (max_children - 1, num_nodes): 1 / R_j from j = 0 on; below 0 where a child up to the j-th is accepted
   double* mass;        // workspace (max_children - 1, num_nodes, subs): parts of R_j from j = 1 on
   Choice* choice;      // workspace (num_seqs)
   double* weight;      // workspace (num_seqs, subs): parts of the last sum(w)
   int* path;           // workspace (num_nodes): accepted rows, from each tree's first row on
   int* tried;          // workspace (num_seqs, max_children): tokens that were not accepted at the last node
+  double* last;        // workspace (num_seqs, max_children): 1 / R_j there
   int vocab, num_seqs, num_nodes, max_nodes, max_children;
   int subs;            // parts of kSub places in a row, made up to whole fours
 };
@@ -396,43 +398,63 @@ __device__ __forceinline__ double mass_of(const VerifyArgs& a, int j, int n) {
   return wave_sum64(r);
 }
 
-// Whether a child is accepted: its number, its token's p and q, a_j and b_j, R_j.
-__device__ __forceinline__ bool passes(float u, double2 chance, double2 ab, double r) {
-#pragma clang fp contract(off)  // the same wherever it is asked
-  return u * chance.y < fmax(ab.x * chance.x - ab.y * chance.y, 0.) / r;
+// What is left below this counts as nothing: its inverse may not be a number.
+constexpr double kLeast = 0x1p-1022;
+
+// p -> w_steps, steps >= 1; lane i has 1 / R_i (R_0 is 1).
+template <int N>
+__device__ __forceinline__ void take_off(double (&w)[N], const double (&q)[N], double inv, int steps) {
+#pragma clang fp contract(off)  // p - q of equal rows is nothing at all
+#pragma unroll
+  for (int e = 0; e < N; ++e) w[e] = fmax(w[e] - q[e], 0.);
+#pragma unroll 1
+  for (int i = 1; i < steps; ++i) {
+    const double v = lane64(inv, i);
+#pragma unroll
+    for (int e = 0; e < N; ++e) w[e] = fmax(fma(w[e], v, -q[e]), 0.);
+  }
 }
 
-// The weight of a token of row n for a_j, b_j.
+// Whether child j is accepted: its number, its token's p and q, 1 / R_i in lane i < j, 1 / R_j.
+__device__ __forceinline__ bool passes(float u, double2 chance, double inv, int j, double v) {
+  double w[1] = {chance.x};
+  if (j) take_off(w, {chance.y}, inv, j);
+  return u * chance.y < w[0] * v;
+}
+
+// The weight of a token of row n after `steps` children were taken off.
 struct Weigh {
-  double ka, kb, rate;  // a / sum, b / sum of p's and q's exponentials
+  double kp, kq, rate;  // 1 / sum of p's and of q's exponentials
   float mp, mq;
+  int steps;
+  double inv;  // lane i: 1 / R_i
   Exp2 boost;
   template <int N>
-  __device__ __forceinline__ void operator()(const float (&lp)[N], const float (&lq)[N], bool rival, double (&out)[N]) const {
-#pragma clang fp contract(off)  // equal rows of target and draft leave nothing at all
+  __device__ __forceinline__ void operator()(const float (&lp)[N], const float (&lq)[N], double (&out)[N]) const {
+#pragma clang fp contract(off)  // both rows are rounded alike
     boost(lp, mp, rate, out);
-    if (rival) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) out[e] *= kp;
+    if (steps) {
       double q[N];
       boost(lq, mq, rate, q);
 #pragma unroll
-      for (int e = 0; e < N; ++e) out[e] = fmax(ka * out[e] - kb * q[e], 0.);
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) out[e] *= ka;
+      for (int e = 0; e < N; ++e) q[e] *= kq;
+      take_off(out, q, inv, steps);
     }
   }
 };
-__device__ __forceinline__ Weigh weigh(const VerifyArgs& a, int n, double ca, double cb, float temp) {
+__device__ __forceinline__ Weigh weigh(const VerifyArgs& a, int n, int steps, double inv, float temp) {
   const RowStat p = a.stat[n];
-  Weigh w = {0., 0., rate_of(temp), 0.f, 0.f};
+  Weigh w = {0., 0., rate_of(temp), 0.f, 0.f, uniform(steps), inv};
   if (p.z > 0.) {
-    w.ka = ca / p.z;
+    w.kp = 1. / p.z;
     w.mp = p.m;
   }
-  if (cb != 0.) {
+  if (steps) {
     const RowStat q = a.stat[a.num_nodes + n];
     if (q.z > 0.) {
-      w.kb = cb / q.z;
+      w.kq = 1. / q.z;
       w.mq = q.m;
     }
   }
@@ -442,7 +464,7 @@ __device__ __forceinline__ Weigh weigh(const VerifyArgs& a, int n, double ca, do
 // The weights of N places from x on of a row whose place `shift` is token 0: of its
 // target's logits and, where the drafter counts, the draft's; `gone` tokens have none.
 template <int N>
-__device__ __forceinline__ void weights(const Weigh& w, bool rival, const float (&lp)[N], const float (&lq)[N], int x, int shift, const int* gone, int num_gone, double (&out)[N]) {
+__device__ __forceinline__ void weights(const Weigh& w, const float (&lp)[N], const float (&lq)[N], int x, int shift, const int* gone, int num_gone, double (&out)[N]) {
   float p[N], q[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) {
@@ -454,7 +476,7 @@ __device__ __forceinline__ void weights(const Weigh& w, bool rival, const float 
 #pragma unroll
     for (int e = 0; e < N; ++e) p[e] = at == e ? -INFINITY : p[e];
   }
-  w(p, q, rival, out);
+  w(p, q, out);
 }
 
 // Child j of node i of a tree, -1 where it has fewer (a wave).
@@ -487,14 +509,14 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs a, int j) {
     vp[i] = rp.template fetch<kVec<T>>(place<T>(sub, i));
     vq[i] = rq.template fetch<kVec<T>>(place<T>(sub, i));
   }
-  const double r = mass_of(a, j - 1, n);
-  const double2 was = j == 1 ? make_double2(1., 0.) : a.ab[static_cast<long long>(j - 2) * a.num_nodes + n];
+  double inv = lane < j - 1 ? a.scale[static_cast<long long>(lane) * a.num_nodes + n] : 0.;
+  const double v = 1. / mass_of(a, j - 1, n);
   const int kid = t.first + child_of(a, t, n - t.first, j - 1);
-  const bool over = was.x < 0. || passes(a.accept[kid], a.chance[kid], was, r);
-  const double2 now = over ? make_double2(-1., 0.) : make_double2(was.x / r, was.y / r + 1.);
-  if (sub == 0 && lane == 0) a.ab[static_cast<long long>(j - 1) * a.num_nodes + n] = now;
+  const bool over = (j > 1 && lane64(inv, j - 2) < 0.) || passes(a.accept[kid], a.chance[kid], inv, j - 1, v);
+  if (sub == 0 && lane == 0) a.scale[static_cast<long long>(j - 1) * a.num_nodes + n] = over ? -1. : v;
   if (over) return;
-  const Weigh w = weigh(a, n, now.x, now.y, temp);
+  if (lane == j - 1) inv = v;
+  const Weigh w = weigh(a, n, j, inv, temp);
   const bool inside = rp.inside(sub * kSub, kSub);
   double sum = 0.;
 #pragma unroll
@@ -503,7 +525,7 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs a, int j) {
     double x[kVec<T>];
     rp.expand(place<T>(sub, i), vp[i], inside, lp);
     rq.expand(place<T>(sub, i), vq[i], inside, lq);
-    weights(w, true, lp, lq, 0, 0, nullptr, 0, x);
+    weights(w, lp, lq, 0, 0, nullptr, 0, x);
 #pragma unroll
     for (int e = 0; e < kVec<T>; ++e) sum += x[e];
   }
@@ -513,23 +535,21 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs a, int j) {
 
 // Down a tree: which rows are accepted, and what the next token is drawn from (one
 // wave, the same result in every workgroup that asks). `write`: keeps the accepted
-// rows and the tokens that were not accepted at the last one. Lanes hold 64 nodes at a
-// time: one round trip for them, not one for each.
-__device__ Choice walk(const VerifyArgs& a, const Tree& t, float temp, bool write, int* gone) {
+// rows and the tokens that were not accepted at the last one. `inv`: lane i gets 1 / R_i
+// there. Lanes hold 64 nodes at a time: one round trip for them, not one for each.
+__device__ Choice walk(const VerifyArgs& a, const Tree& t, float temp, bool write, int* gone, double& inv) {
   const int lane = threadIdx.x & 63;
-  Choice r = {1., 0., -1, 0, 0, 0};
+  Choice r = {-1, 0, 0, 0};
   if (t.nodes == 0) return r;
   const bool top = greedy(temp);
   int at = -1, best = -1;  // the current node within the tree; its likeliest token
-  double left = 1.;        // R of the next child's test
+  double left = 1.;        // without draft logits: what the tokens tried leave of p; with them, 1 / R of the next child's test
   auto reach = [&](int i, int likeliest) {
     at = i;
     best = likeliest;
     if (write && lane == 0) a.path[t.first + r.count] = t.first + i;
     r.count += 1;
-    r.a = 1.;
-    r.b = 0.;
-    r.tried = 0;
+    r.tried = r.steps = 0;
     left = 1.;
   };
   for (int i0 = 0; i0 < t.nodes; i0 += 64) {
@@ -547,11 +567,12 @@ __device__ Choice walk(const VerifyArgs& a, const Tree& t, float temp, bool writ
       from = i0 + k + 1;
       if (r.tried >= a.max_children) continue;
       if (a.draft && !top && r.tried) {  // summed, as the node has more children than were tried
-        left = mass_of(a, r.tried, t.first + at);
-        if (left == 0.) {  // nothing is left to accept
+        const double sum = mass_of(a, r.tried, t.first + at);
+        if (!(sum >= kLeast)) {  // nothing is left to accept
           r.tried = a.max_children;
           continue;
         }
+        left = 1. / sum;
       }
       const int x = __builtin_amdgcn_readlane(token, k);
       bool yes;
@@ -560,7 +581,7 @@ __device__ Choice walk(const VerifyArgs& a, const Tree& t, float temp, bool writ
       } else {
         const double pc = lane64(chance.x, k), qc = lane64(chance.y, k), uk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, u), k));
         if (a.draft) {
-          yes = passes(uk, make_double2(pc, qc), make_double2(r.a, r.b), left);
+          yes = passes(uk, make_double2(pc, qc), inv, r.steps, left);
         } else {  // its token may have been tried before
           bool again = false;
           for (int e = 0; e < r.tried; ++e) again |= gone[e] == x;
@@ -576,8 +597,8 @@ __device__ Choice walk(const VerifyArgs& a, const Tree& t, float temp, bool writ
         __builtin_amdgcn_wave_barrier();
         r.tried += 1;
         if (a.draft && !top) {
-          r.a /= left;
-          r.b = r.b / left + 1.;
+          if (lane == r.steps) inv = left;
+          r.steps += 1;
         }
       }
     }
@@ -591,12 +612,15 @@ template <typename T>
 __global__ __launch_bounds__(256) void verify_walk_kernel(VerifyArgs a) {
   __shared__ Choice sr;
   __shared__ int gone[64];
+  __shared__ double scales[64];
   const int groups = a.subs / 4, s = blockIdx.x / groups, c = blockIdx.x - s * groups;
   const int sub = 4 * c + uniform(threadIdx.x >> 6);
   const Tree t = tree_of(a, s);
   const float temp = a.temps[s];
   if (threadIdx.x < 64) {
-    const Choice r = walk(a, t, temp, c == 0, gone);
+    double inv = 0.;
+    const Choice r = walk(a, t, temp, c == 0, gone, inv);
+    scales[threadIdx.x] = inv;
     if (threadIdx.x == 0) {
       sr = r;
       if (c == 0) a.choice[s] = r;
@@ -605,8 +629,7 @@ __global__ __launch_bounds__(256) void verify_walk_kernel(VerifyArgs a) {
   __syncthreads();
   const Choice r = sr;
   if (r.node < 0 || greedy(temp)) return;
-  const bool rival = r.b != 0.;
-  const Row<T> rp(a, a.logits, r.node), rq(a, rival ? a.draft : a.logits, r.node);
+  const Row<T> rp(a, a.logits, r.node), rq(a, r.steps ? a.draft : a.logits, r.node);
   const bool inside = rp.inside(sub * kSub, kSub);
   typename Row<T>::template Vec<kVec<T>> vp[kVecs<T>], vq[kVecs<T>];
 #pragma unroll
@@ -616,7 +639,8 @@ __global__ __launch_bounds__(256) void verify_walk_kernel(VerifyArgs a) {
   }
   const int num_gone = a.draft ? 0 : r.tried;
   if (c == 0 && static_cast<int>(threadIdx.x) < num_gone) a.tried[s * a.max_children + threadIdx.x] = gone[threadIdx.x];
-  const Weigh w = weigh(a, r.node, r.a, r.b, temp);
+  if (c == 0 && static_cast<int>(threadIdx.x) < r.steps) a.last[s * a.max_children + threadIdx.x] = scales[threadIdx.x];
+  const Weigh w = weigh(a, r.node, r.steps, scales[threadIdx.x & 63], temp);
   double sum = 0.;
 #pragma unroll
   for (int i = 0; i < kVecs<T>; ++i) {
@@ -624,7 +648,7 @@ __global__ __launch_bounds__(256) void verify_walk_kernel(VerifyArgs a) {
     float lp[kVec<T>], lq[kVec<T>];
     rp.expand(place<T>(sub, i), vp[i], inside, lp);
     rq.expand(place<T>(sub, i), vq[i], inside, lq);
-    weights(w, rival, lp, lq, place<T>(sub, i), rp.shift, gone, num_gone, x);
+    weights(w, lp, lq, place<T>(sub, i), rp.shift, gone, num_gone, x);
 #pragma unroll
     for (int e = 0; e < kVec<T>; ++e) sum += x[e];
   }
@@ -700,8 +724,7 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs a) {
   double sum = block_scan(x, run, tmp);
   if (!(sum > 0.)) {  // nothing is left of p: p itself
     const RowStat all = a.stat[r.node];
-    r.a = 1.;
-    r.b = 0.;
+    r.steps = 0;
     num_gone = 0;
     const Exp2 boost;
 #pragma unroll
@@ -748,15 +771,14 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs a) {
     if (tid * kParts + i == part) start = run[i] - x[i];
   __syncthreads();
   // And the token there.
-  const Weigh w = weigh(a, r.node, r.a, r.b, temp);
-  const bool rival = r.b != 0.;
-  const Row<T> rp(a, a.logits, r.node), rq(a, rival ? a.draft : a.logits, r.node);
+  const Weigh w = weigh(a, r.node, r.steps, lane < r.steps ? a.last[s * a.max_children + lane] : 0., temp);
+  const Row<T> rp(a, a.logits, r.node), rq(a, r.steps ? a.draft : a.logits, r.node);
   const int p0 = part * kSub;
   double y[4], upto[4];
   float lp[4], lq[4];
   rp.expand(p0 + tid * 4, rp.template fetch<4>(p0 + tid * 4), rp.inside(p0, kSub), lp);
   rq.expand(p0 + tid * 4, rq.template fetch<4>(p0 + tid * 4), rp.inside(p0, kSub), lq);
-  weights(w, rival, lp, lq, p0 + tid * 4, rp.shift, a.tried + s * a.max_children, num_gone, y);
+  weights(w, lp, lq, p0 + tid * 4, rp.shift, a.tried + s * a.max_children, num_gone, y);
   block_scan(y, upto, tmp);
 #pragma unroll
   for (int i = 0; i < 4; ++i) note(p0 + tid * 4 + i, y[i], start + upto[i]);
@@ -793,8 +815,9 @@ long long lay_out(VerifyArgs& a, bool draft, char* base) {
   take(a.weight, static_cast<long long>(a.num_seqs) * a.subs);
   take(a.path, a.num_nodes);
   take(a.tried, static_cast<long long>(a.num_seqs) * a.max_children);
+  take(a.last, draft ? static_cast<long long>(a.num_seqs) * a.max_children : 0);
   const long long sums = draft ? static_cast<long long>(a.max_children - 1) * a.num_nodes : 0;
-  take(a.ab, sums);
+  take(a.scale, sums);
   take(a.mass, sums * a.subs);
   return at;
 }

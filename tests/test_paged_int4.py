@@ -178,9 +178,9 @@ def test_verify_refuses_results_over_other_buffers(out, other):
 
 @pytest.mark.parametrize("vocab,nodes", [(100, 6), (128256, 208)])
 def test_verify_workspace_holds_sums_behind_the_first_child_only(vocab, nodes):
-    """What is left after j children, j = 1 .. max_children - 1: two numbers to a row and a sum to each 1024 tokens of it."""
+    """What is left after j children, j = 1 .. max_children - 1: a number to a row and a sum to each 1024 tokens of it."""
     subs = (vocab + 7 + 4095) // 4096 * 4
-    sizes = [_lib.query("iron_draft_verify_workspace_bytes", vocab, 2, nodes, 5, k, 1) - 2 * k * 4 // 16 * 16 for k in (2, 4, 6)]
-    assert sizes[1] - sizes[0] == sizes[2] - sizes[1] == 2 * nodes * (16 + 8 * subs)
+    sizes = [_lib.query("iron_draft_verify_workspace_bytes", vocab, 2, nodes, 5, k, 1) - 2 * k * (4 + 8) for k in (2, 4, 6)]
+    assert sizes[1] - sizes[0] == sizes[2] - sizes[1] == 2 * nodes * (8 + 8 * subs)
     two, one = (_lib.query("iron_draft_verify_workspace_bytes", vocab, 2, nodes, 5, k, 1) for k in (2, 1))
-    assert two - one == nodes * (16 + 8 * subs)
+    assert two - one == nodes * (8 + 8 * subs) + 2 * 8  # a sequence's tokens tried, 4 bytes each, fill up to 16
