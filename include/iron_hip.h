@@ -421,8 +421,9 @@ int iron_paged_append(const void* k_new, const void* v_new, const int* rows, con
  * bytes of codes, then four pairs (s, b) of fp16, one for each quarter of the row:
  * value = b + s (16 + code). A 32-bit word of codes holds eight consecutive values,
  * the even ones in the nibbles of its low half from the lowest up, the odd ones in
- * those of its high half. Rows of pages need no alignment but the pages' own (16
- * bytes). With dtype 0, cached keys, values and the weights of cached positions are
+ * those of its high half. A value past 65504, which no append makes, may count as
+ * infinite here. Rows of pages need no alignment but the pages' own (16 bytes).
+ * With dtype 0, cached keys, values and the weights of cached positions are
  * rounded once to fp16 (weights kept to 2^-30 of a row's largest); with dtype 1, keys
  * are not rounded, values once, and weights go in two parts. The tree's rows k_new
  * and v_new are dtype, and so are their weights: in two parts, or one where a KV head
@@ -478,9 +479,12 @@ int iron_paged_gather_int4(const int* begins, const int* row_starts, const void*
  * fp32; next_tokens[s] is -1 for an empty tree and for a row of -inf. Tokens outside
  * [0, vocab) are not accepted; where max(p - q, 0) is zero everywhere the next token
  * is drawn from p. draft_logits of nodes without children are not read. Computed in
- * 64 bits. dtype 0: bf16, 1: fp16, 2: fp32 logits. vocab at most 2^20, num_nodes 2^20 and
- * below 2^23 / ceil((vocab + 7) / 4096), max_nodes 1024, max_children 64. node_starts must not decrease; trees are cut to max_nodes nodes and
- * to num_nodes rows. rows, row_starts and next_tokens overlap no other buffer of the call. In the place of the sampling of
+ * 64 bits, exponentials off by up to 2^-46 (and 2^-52 of the argument). dtype 0: bf16,
+ * 1: fp16, 2: fp32 logits. vocab at most 2^20, num_nodes 2^20 and below
+ * 2^23 / ceil((vocab + 7) / 4096), max_nodes 1024, max_children 64. node_starts must
+ * not decrease; trees are cut to max_nodes nodes and to num_nodes rows. rows,
+ * row_starts and next_tokens overlap no other buffer of the call. In the place of the
+ * sampling of
  * iron/applications/llama_3.2_1b/llama_inference_harness.py:146-169. */
 long long iron_draft_verify_workspace_bytes(int vocab, int num_seqs, int num_nodes, int max_nodes, int max_children,
                                             int draft);

@@ -20,8 +20,9 @@ A temperature of 0 (or below, or NaN) takes the likeliest token, the lowest of e
 
 Logits of -inf (a filter's, or padding) and NaN have no probability, +inf counts as the
 largest fp32. A row without any gives next token -1; so does an empty tree. A token
-outside the vocabulary is not accepted, one without probability neither accepted nor drawn. Where max(p - q, 0) is zero everywhere, the
-next token is drawn from p. All of it is computed in 64 bits.
+outside the vocabulary is not accepted, one without probability neither accepted nor
+drawn. Where max(p - q, 0) is zero everywhere, the next token is drawn from p. All of
+it is computed in 64 bits, the exponentials to 2^-46 (and 2^-52 of their argument).
 
 Arg spec: logits (num_nodes, vocab), draft_logits (num_nodes, vocab; only with
 ``draft``; rows of nodes without children are not read), tokens, parents (num_nodes,),

@@ -4,7 +4,8 @@
 
 Everything is TreeAttention's but the pages: one layer's k_pages and v_pages are
 uint8 (num_pages, Hkv, page_size, D / 2 + 16), rows as PagedAppendInt4 writes them
-(``iron_amd.common.paging.int4_row_bytes`` says how). The tree's own rows k_new and
+(``iron_amd.common.paging.int4_row_bytes`` says how); a value past 65504, which
+PagedAppendInt4 does not make, may count as infinite. The tree's own rows k_new and
 v_new have 16 bits. With D 64 a position takes 48 bytes instead of 128, with D 128
 80 instead of 256.
 
