@@ -9,7 +9,7 @@
 // max(a p - b q, 0) with two numbers, but where little is left, a and b are large and
 // all of it cancels: rows with nearly all of their probability at one token came out wrong.)
 // Without draft logits q is 1 at the child's token: w is p without the tokens tried,
-// and no sums are needed on the way.
+// and no sums are needed on the way unless these have nearly all of p.
 //
 // Everything is in 64 bits: a vocabulary of 2^17 tokens of like probability puts
 // the borders of the cumulative sum 2^-17 apart, where sums of fp32 exponentials
@@ -399,6 +399,9 @@ __device__ __forceinline__ double mass_of(const VerifyArgs& a, int j, int n) {
   return wave_sum64(r);
 }
 
+// 1 less the probability of a token tried is off by 2^-53, at this size by 2^-45 of itself.
+constexpr double kCoarse = 0x1p-8;
+
 // What is left below this counts as nothing: its inverse may not be a number.
 constexpr double kLeast = 0x1p-1022;
 
@@ -534,10 +537,60 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs a, int j) {
   if (lane == 0) a.mass[(static_cast<long long>(j - 1) * a.num_nodes + n) * a.subs + sub] = sum;
 }
 
+// What the tokens tried leave of row n's p (one wave): the parts' sums, those that hold one of
+// the tokens made anew without them.
+template <typename T>
+__device__ double rest_of(const VerifyArgs& a, int n, double rate, const int* gone, int num_gone) {
+  const int lane = threadIdx.x & 63;
+  const RowStat all = a.stat[n];
+  const RowStat* part = a.part + static_cast<long long>(n) * a.subs;
+  const Row<T> r(a, a.logits, n);
+  const Exp2 boost;
+  auto part_of = [&](int k) {  // -1: no token of the row
+    const int x = uniform(gone[k]);
+    return static_cast<unsigned>(x) < static_cast<unsigned>(a.vocab) ? (x + r.shift) / kSub : -1;
+  };
+  double sum = 0.;
+#pragma unroll 1
+  for (int c = lane; c < a.subs; c += 64) {
+    const RowStat p = part[c];
+    bool whole = p.z > 0.;
+    for (int k = 0; k < num_gone; ++k) whole &= part_of(k) != c;
+    sum += whole ? p.z * boost(p.m, all.m, rate) : 0.;
+  }
+#pragma unroll 1
+  for (int k = 0; k < num_gone; ++k) {
+    const int c = part_of(k);
+    bool again = c < 0;
+    for (int e = 0; e < k; ++e) again |= part_of(e) == c;
+    if (again) continue;
+    const bool inside = r.inside(c * kSub, kSub);
+#pragma unroll 1
+    for (int i = 0; i < kVecs<T>; ++i) {
+      const int at = place<T>(c, i);
+      float l[kVec<T>];
+      double y[kVec<T>];
+      r.expand(at, r.template fetch<kVec<T>>(at), inside, l);
+#pragma unroll
+      for (int e = 0; e < kVec<T>; ++e) l[e] = logit(l[e]);
+      for (int x = 0; x < num_gone; ++x) {
+        const int hit = gone[x] + r.shift - at;
+#pragma unroll
+        for (int e = 0; e < kVec<T>; ++e) l[e] = hit == e ? -INFINITY : l[e];
+      }
+      boost(l, all.m, rate, y);
+#pragma unroll
+      for (int e = 0; e < kVec<T>; ++e) sum += y[e];
+    }
+  }
+  return wave_sum64(sum) / all.z;
+}
+
 // Down a tree: which rows are accepted, and what the next token is drawn from (one
 // wave, the same result in every workgroup that asks). `write`: keeps the accepted
 // rows and the tokens that were not accepted at the last one. `inv`: lane i gets 1 / R_i
 // there. Lanes hold 64 nodes at a time: one round trip for them, not one for each.
+template <typename T>
 __device__ Choice walk(const VerifyArgs& a, const Tree& t, float temp, bool write, int* gone, double& inv) {
   const int lane = threadIdx.x & 63;
   Choice r = {-1, 0, 0, 0};
@@ -545,6 +598,7 @@ __device__ Choice walk(const VerifyArgs& a, const Tree& t, float temp, bool writ
   const bool top = greedy(temp);
   int at = -1, best = -1;  // the current node within the tree; its likeliest token
   double left = 1.;        // without draft logits: what the tokens tried leave of p; with them, 1 / R of the next child's test
+  bool due = false;        // the tokens tried have nearly all of p: what they leave is summed for the next child
   auto reach = [&](int i, int likeliest) {
     at = i;
     best = likeliest;
@@ -552,6 +606,7 @@ __device__ Choice walk(const VerifyArgs& a, const Tree& t, float temp, bool writ
     r.count += 1;
     r.tried = r.steps = 0;
     left = 1.;
+    due = false;
   };
   for (int i0 = 0; i0 < t.nodes; i0 += 64) {
     const int i = min(i0 + lane, t.nodes - 1), n = t.first + i;
@@ -575,6 +630,8 @@ __device__ Choice walk(const VerifyArgs& a, const Tree& t, float temp, bool writ
         }
         left = 1. / sum;
       }
+      if (due) left = rest_of<T>(a, t.first + at, rate_of(temp), gone, r.tried);
+      due = false;
       const int x = __builtin_amdgcn_readlane(token, k);
       bool yes;
       if (top) {
@@ -587,7 +644,10 @@ __device__ Choice walk(const VerifyArgs& a, const Tree& t, float temp, bool writ
           bool again = false;
           for (int e = 0; e < r.tried; ++e) again |= gone[e] == x;
           yes = !again && uk < pc / left;
-          if (!yes && !again) left -= pc;
+          if (!yes && !again) {
+            left -= pc;
+            due = pc > 0. && left < kCoarse;
+          }
         }
       }
       if (yes) {
@@ -620,7 +680,7 @@ __global__ __launch_bounds__(256) void verify_walk_kernel(VerifyArgs a) {
   const float temp = a.temps[s];
   if (threadIdx.x < 64) {
     double inv = 0.;
-    const Choice r = walk(a, t, temp, c == 0, gone, inv);
+    const Choice r = walk<T>(a, t, temp, c == 0, gone, inv);
     scales[threadIdx.x] = inv;
     if (threadIdx.x == 0) {
       sr = r;

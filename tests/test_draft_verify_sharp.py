@@ -39,8 +39,9 @@ def walk(c, most, rows_of, unrolled=False):
         temp, node = float(c["temps"][s]), a
         while True:
             rows.append(node)
-            p, q = rows_of(c["logits"][node], temp), rows_of(c["draft"][node], temp)
+            p = rows_of(c["logits"][node], temp)
             one = p[0] * 0 + 1
+            q = rows_of(c["draft"][node], temp) if c["draft"] is not None else [one] * len(p)  # of the drafted token; others are not taken off
             left, at, bt, total, taken = p, one, one * 0, one, None
             for k in [i for i in range(node + 1, b) if int(c["parents"][i]) == node - a][:most]:
                 x = int(c["tokens"][k])
@@ -48,7 +49,9 @@ def walk(c, most, rows_of, unrolled=False):
                     taken = k
                     break
                 at, bt = at / total, bt / total + 1
-                if unrolled:
+                if c["draft"] is None:
+                    left = [one * 0 if i == x else u / total for i, u in enumerate(left)]
+                elif unrolled:
                     left = [max(at * u - bt * v, one * 0) for u, v in zip(p, q)]
                 else:
                     left = [max(u / total - v, one * 0) for u, v in zip(left, q)]
@@ -104,4 +107,37 @@ def test_unrolled_weights_would_not_do():
 def test_sharp_rows(gpu, dtype):
     for c, most, (rows, nexts) in cases(dtype, 150):
         got = calls.call(gpu, c, 9, most)
+        assert [r for r in got[0] if r >= 0] == rows and got[2] == nexts
+
+
+def lookups(dtype, V, want):
+    """Stars without draft logits: the likeliest tokens in order, or any, tried with numbers near 1, so that little is left."""
+    seed = 0
+    while want:
+        seed += 1
+        g = torch.Generator().manual_seed(seed)
+        pick = lambda values: values[int(torch.randint(0, len(values), (1,), generator=g))]
+        S, kids = 8, pick([2, 3, 5])
+        logits = (torch.randn(S * (kids + 1), V, generator=g) * pick([1, 3, 10])).to(dtype)
+        c = dict(logits=logits, draft=None, temps=torch.full((S,), pick([1.0, 0.5, 0.2, 0.05])), sample=torch.rand(S, generator=g),
+                 starts=torch.arange(0, S * (kids + 1) + 1, kids + 1, dtype=torch.int32), parents=torch.tensor(([-1] + [0] * kids) * S, dtype=torch.int32),
+                 tokens=torch.randint(0, V, (S * (kids + 1),), generator=g).to(torch.int32),
+                 accept=1 - 2.0 ** -torch.tensor([24.0, 23, 20, 10, 3])[torch.randint(0, 5, (S * (kids + 1),), generator=g)])
+        for s in range(0, S, 2):
+            top = torch.argsort(logits[s * (kids + 1)].float(), descending=True, stable=True)[:kids]
+            c["tokens"][s * (kids + 1) + 1:(s + 1) * (kids + 1)][:len(top)] = top.to(torch.int32)
+        exact = walk(c, kids, softmax60)
+        noise = np.random.default_rng(seed)
+        if all(walk(c, kids, lambda row, temp: softmax64(row, temp, r)) == exact for r in (None, *[noise] * 3)):
+            want -= 1
+            yield c, kids, exact
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V,want", [(2, 50), (9, 200), (2200, 4)])
+def test_sharp_rows_of_lookups(gpu, dtype, V, want):
+    """1 less the probabilities of the tokens tried has none of the digits of what they leave."""
+    for c, kids, (rows, nexts) in lookups(dtype, V, want):
+        got = calls.call(gpu, c, kids + 1, kids)
         assert [r for r in got[0] if r >= 0] == rows and got[2] == nexts
