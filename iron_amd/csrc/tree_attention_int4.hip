@@ -88,18 +88,29 @@ __device__ __forceinline__ unsigned split_fp16(float x) {
   return __builtin_bit_cast(unsigned, ta_f16x2{high, low});
 }
 
-// A row of q as the fp16 operand beside cached keys: bf16 rows are scaled by a power
-// of two that puts their largest element into [2^14, 2^15), so that none is cut and
-// those of 2^-29 of it and more stay exact; the scores get the inverse (factor).
+// A row of q as the fp16 operand beside cached keys, scaled by a power of two; the
+// scores get the inverse (factor). bf16: the largest element comes into [2^14, 2^15), so
+// that none is cut and those of 2^-29 of it and more stay exact. fp16: into [2^9, 2^10),
+// but by 2^24 at most, so that the sums of a quarter (32 elements at most), which b is
+// multiplied by, fit fp16 in two parts, those of subnormal rows too; elements of 2^-23 of
+// the largest and more stay exact.
 // A row with an infinity or NaN comes out with one, and is done over by the join.
 template <bool F16, bool WIDE, int NK>
 __device__ __forceinline__ float to_fp16(ta_u32x4 (&q)[NK], float scale) {
-  if constexpr (F16) return scale;
   float top = 0.f;
+  if constexpr (F16) {
+    ta_f16x2 most = {0, 0};
 #pragma unroll
-  for (int kk = 0; kk < NK; ++kk)
+    for (int kk = 0; kk < NK; ++kk)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(lo_bf16(q[kk][i])), fabsf(hi_bf16(q[kk][i]))));
+      for (int i = 0; i < 4; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(ta_f16x2, q[kk][i] & 0x7fff7fffu));
+    top = fmaxf(static_cast<float>(most[0]), static_cast<float>(most[1]));
+  } else {
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(lo_bf16(q[kk][i])), fabsf(hi_bf16(q[kk][i]))));
+  }
   if constexpr (WIDE) {  // two lanes have a row, or four
     float x, y;
     swap32(top, x, y);
@@ -107,12 +118,24 @@ __device__ __forceinline__ float to_fp16(ta_u32x4 (&q)[NK], float scale) {
   } else {
     top = row_max(top);
   }
-  const int e = 15 - __builtin_amdgcn_frexp_expf(top);
+  int e = (F16 ? 10 : 15) - __builtin_amdgcn_frexp_expf(top);
+  if constexpr (F16) {  // in two steps that fp16 has
+    e = min(e, 24);
+    const _Float16 a = static_cast<_Float16>(__builtin_amdgcn_ldexpf(1.f, e >> 1)), b = static_cast<_Float16>(__builtin_amdgcn_ldexpf(1.f, e - (e >> 1)));
 #pragma unroll
-  for (int kk = 0; kk < NK; ++kk)
+    for (int kk = 0; kk < NK; ++kk)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      q[kk][i] = pack2<true>(__builtin_amdgcn_ldexpf(lo_bf16(q[kk][i]), e), __builtin_amdgcn_ldexpf(hi_bf16(q[kk][i]), e));
+      for (int i = 0; i < 4; ++i) {
+        const unsigned x = q[kk][i];  // a bit cast of the vector's element itself takes its first one
+        q[kk][i] = __builtin_bit_cast(unsigned, __builtin_bit_cast(ta_f16x2, x) * ta_f16x2{a, a} * ta_f16x2{b, b});
+      }
+  } else {
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        q[kk][i] = pack2<true>(__builtin_amdgcn_ldexpf(lo_bf16(q[kk][i]), e), __builtin_amdgcn_ldexpf(hi_bf16(q[kk][i]), e));
+  }
   const float factor = __builtin_amdgcn_ldexpf(scale, -e);
   return factor == INFINITY ? NAN : factor;  // done over, too
 }

@@ -62,7 +62,8 @@ def bound(c, scale, exact_scores=False):
     - sums of n terms in fp32, 2^-23 of the terms' sizes each, with D terms; in fp16 calls 2 D + 8, of b + s (16 + code) apart
       (nothing, nor the next but one, where fp32 holds them: `exact_scores`);
     - bf16: a cached key's rounding to fp16, and q's elements far under the row's largest (2^-39 of that);
-    - fp16: the lower part of s (2^-24 of a code's value), b by sums of q in two parts: 2^-22 of the sum, D / 4 roundings of it;
+    - fp16: the lower part of s (2^-24 of a code's value), b by sums of q in two parts: 2^-22 of the sum, D / 4 roundings of it,
+      and like q's small elements 2^-33 of the row's largest;
     - the score times log2(e) less the maximum, 2^-22 of the largest score, the exponential and the parts' joining, 2^-21;
     - its rounding for the second product: fp16 (bf16 calls, cached), 2^-20 in two parts, half a step of dtype for nodes where a
       KV head has more than 32 rows; 2^-30 of a row's largest for weights under fp16's normal range.
@@ -87,7 +88,9 @@ def bound(c, scale, exact_scores=False):
                 b = pair[..., 1].abs()
                 apart = x.abs() @ (b + (k[:n] - pair[..., 1]).abs()).t().contiguous()
                 sums = x.unflatten(1, (4, -1)).sum(2).abs().repeat_interleave(D // 4, 1) / (D // 4)
-                off[:, :n] = scale * (2 * (2 * D + 10) * H32 * apart + 2.0 ** -24 * x.abs().sum(1)[:, None] + (2.0 ** -22 * sums + D / 4 * H32 * x.abs() + 2.0 ** -24) @ b.t().contiguous())
+                least = 2.0 ** -33 * x.abs().amax(1, keepdim=True)
+                off[:, :n] = scale * (2 * (2 * D + 10) * H32 * apart + 2.0 ** -24 * x.abs().sum(1)[:, None] + least * (k[:n] - pair[..., 1]).abs().sum(1)[None]
+                                      + (2.0 ** -22 * sums + D / 4 * H32 * x.abs() + least) @ b.t().contiguous())
             top = w.masked_fill(~seen, 0).abs().amax(1, keepdim=True)
             each = off + 2.0 ** -21 * (1 + 1.5 * top) + kr
             o, m = p @ v, p @ v.abs()

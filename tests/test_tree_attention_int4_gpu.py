@@ -331,3 +331,16 @@ def test_refusals(gpu):
         op.get_callable()(*args[:3], args[3].view(torch.int8), *args[4:])
     with pytest.raises(ValueError, match="elements"):
         op.get_callable()(*args[:3], args[3][1:], *args[4:])
+
+
+@pytest.mark.parametrize("counts", [[1, 2], [40, 3]])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_queries_at_the_ends_of_fp16(gpu, dtype, D, counts):
+    """Subnormal queries of fp16 with scales that make ordinary scores of them, and its largest ones."""
+    for q_size, scale in ((1e-6, 2e5), (1e-5, 2e4), (2.0 ** -24, 1e6), (3e4, 3e-6)):
+        c = case(gpu, 4, 2, D, dtype, [50, 100], counts, seed=31)
+        c["q"] = c["q"].float().clamp(-2, 2).mul(q_size).to(dtype)
+        check(c, run(gpu, c, scale), scale)
+    c["q"] = torch.full_like(c["q"], 6e4)  # sums of a quarter past fp16
+    check(c, run(gpu, c, 1e-6), 1e-6)
