@@ -425,7 +425,7 @@ int iron_paged_append(const void* k_new, const void* v_new, const int* rows, con
  * infinite here. Rows of pages need no alignment but the pages' own (16 bytes).
  * With dtype 0, cached keys, values and the weights of cached positions are
  * rounded once to fp16 (weights kept to 2^-30 of a row's largest); with dtype 1, keys
- * are not rounded, values once, and weights go in two parts. The tree's rows k_new
+ * are not rounded (but to 2^-24), values once, and weights go in two parts. The tree's rows k_new
  * and v_new are dtype, and so are their weights: in two parts, or one where a KV head
  * has more than 32 rows (max_nodes times G). Everything else is
  * iron_tree_attention's. iron_page_fork, iron_page_compact and iron_page_free take

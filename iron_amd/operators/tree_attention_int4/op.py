@@ -11,8 +11,8 @@ v_new have 16 bits. With D 64 a position takes 48 bytes instead of 128, with D 1
 
 bf16 calls round cached keys, values and the weights of cached positions once to fp16,
 an eighth of the result's own rounding each (weights are kept to 2^-30 of a row's
-largest). fp16 calls take cached keys without rounding, values rounded once, and
-weights in two parts. Weights of the tree's rows are two parts of dtype, or, where a
+largest). fp16 calls take cached keys without rounding (but to 2^-24), values rounded
+once, and weights in two parts. Weights of the tree's rows are two parts of dtype, or, where a
 KV head has more than 32 rows (max_nodes times H / Hkv), one. Kernel:
 iron_tree_attention_int4.
 """
